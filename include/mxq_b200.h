@@ -238,6 +238,84 @@ int mxq_block_lut_quantize_static(const float* V, float* P_lut, float* X, int64_
                                   int64_t block, const mxq_quant_spec* spec, int32_t group, int32_t max_iters,
                                   int32_t* status, void* stream);
 
+/* ------------------------------------------------------- the feed-forward on packed operands (no reference counterpart)
+ * Operands are the compact form with blocks of 32 along the last dimension: codes row-major (`pitch` bytes from row to
+ * row), scales E8M0 bytes, ceil(K / 32) per row. Indices are int32. */
+#define MXQ_ACT_NONE 0
+#define MXQ_ACT_RELU 1
+#define MXQ_ACT_GELU 2       /* with erf */
+#define MXQ_ACT_GELU_TANH 3
+#define MXQ_ACT_SILU 4
+#define MXQ_ACT_SWIGLU 5     /* silu(first half of the features) * second half */
+#define MXQ_ACT_GEGLU 6      /* gelu(first half) * second half */
+#define MXQ_OUT_F32 0
+#define MXQ_OUT_BF16 1
+#define MXQ_OUT_F16 2
+#define MXQ_OUT_PACKED 3
+typedef struct mxq_product_spec {
+  int32_t x_e, x_m, w_e, w_m;   /* element formats of the codes */
+  int32_t activation, out;      /* MXQ_ACT_*, MXQ_OUT_* */
+  int32_t out_e, out_m;         /* MXQ_OUT_PACKED: the element format of the output's codes */
+} mxq_product_spec;
+/* y[M, F] = act(x w^T + bias) (* up) + residual with x M x K and w N x K; F = N, or N / 2 for a gated activation. Sums in
+ * float32. bias: N float32 or NULL. residual: y's type, rows residual_stride elements apart, or NULL (not with a packed
+ * output). A packed output's scale is 2^(floor(log2 amax) - emax) per 32 columns, codes rounded to nearest even and
+ * saturated; a block with an Inf or a NaN gets the scale 0xFF and zero codes. Codes must be 8-bit (E4M3, E5M2) with base
+ * and pitch multiples of 16 bytes, or FP4 with base and pitch multiples of 32 bytes and K a multiple of 128
+ * (mxq_lay_codes brings any others to that). */
+int mxq_linear_packed(const uint8_t* x, const uint8_t* x_scales, int64_t x_pitch, int64_t M, const uint8_t* w,
+                      const uint8_t* w_scales, int64_t w_pitch, int64_t N, int64_t K, const mxq_product_spec* spec,
+                      const float* bias, const void* residual, int64_t residual_stride, void* out, uint8_t* out_scales,
+                      void* stream);
+/* The same product by expert: rows offsets[e] .. offsets[e + 1] - 1 of y (experts + 1 non-decreasing offsets, the last
+ * at most `slots`) are multiplied with expert e's N x K weights (w: experts x N x K, bias: experts x N). Row r of y takes
+ * row r of x (per 0), or row order[r] / per (per > 0). Rows from the last offset on are not written. At most 1024
+ * experts. */
+int mxq_experts_packed(const uint8_t* x, const uint8_t* x_scales, int64_t x_pitch, int64_t x_rows, const uint8_t* w,
+                       const uint8_t* w_scales, int64_t w_pitch, int64_t experts, int64_t N, int64_t K,
+                       const int32_t* offsets, const int32_t* order, int64_t slots, int64_t per,
+                       const mxq_product_spec* spec, const float* bias, void* out, uint8_t* out_scales, void* stream);
+/* rows x K codes of any MX element format (in_pitch bytes from row to row) as 8-bit codes at out_pitch: E4M3 and E5M2
+ * copied, FP6 and FP4 as the E4M3 codes of the same values. */
+int mxq_lay_codes(const uint8_t* codes, int64_t in_pitch, uint8_t* out, int64_t out_pitch, int64_t rows, int64_t K,
+                  int32_t e, int32_t m, void* stream);
+/* rows x K values (type MXQ_OUT_F32 / BF16 / F16, rows x_stride elements apart) packed as a packed output is; the codes
+ * 8-bit at out_pitch as mxq_lay_codes writes them. */
+int mxq_pack_rows(const void* x, int32_t type, int64_t x_stride, uint8_t* codes, int64_t out_pitch, uint8_t* scales,
+                  int64_t rows, int64_t K, int32_t e, int32_t m, void* stream);
+
+/* Routing. Scores s = softmax or sigmoid of the T x E logits (type MXQ_OUT_F32 / BF16 / F16, rows `stride` elements
+ * apart) in float32. An expert's choice value is its logit (bias NULL) or s + bias. groups > 1: the experts are `groups`
+ * equal runs, a run's value is its largest choice value, or (top2) the sum of its two largest, and only the `keep` best
+ * runs take part. experts[t, 0..k): the k largest choice values, descending; every tie goes to the lowest index.
+ * weights: their s, divided by (their sum + 1e-20) if renormalize, times scale. A logit of -Inf or NaN is never chosen; a
+ * place with nothing left to choose gets expert -1 and weight 0; the weights of a row with a NaN are NaN. At most 1024
+ * experts, k at most 32, at most 32 groups. */
+#define MXQ_SCORE_SOFTMAX 0
+#define MXQ_SCORE_SIGMOID 1
+typedef struct mxq_route_spec {
+  int32_t score, groups, keep, top2, renormalize;
+  float scale;
+} mxq_route_spec;
+int mxq_route(const void* logits, int32_t type, int64_t stride, const float* bias, float* weights, int32_t* experts,
+              int64_t T, int64_t E, int64_t k, const mxq_route_spec* spec, void* stream);
+/* d loss / d logits (their type, T x E) from grad = d loss / d weights (T x k) and the experts that mxq_route chose. */
+int mxq_route_backward(const float* grad, const void* logits, int32_t type, int64_t stride, const int32_t* experts,
+                       void* grad_logits, int64_t T, int64_t E, int64_t k, const mxq_route_spec* spec, void* stream);
+/* The slots (token-major, T x k flattened) in the order of their experts, each expert's in their own order: offsets
+ * (experts + 1), order[place] = slot, where[slot] = place. A slot whose expert is outside [0, experts) is left out: its
+ * where is -1 and the last places of order are -1. At most 1024 experts. */
+int mxq_dispatch(const int32_t* experts_of, int64_t slots, int64_t experts, int32_t* offsets, int32_t* order,
+                 int32_t* where, void* stream);
+/* y[t] = sum_j weights[t, j] z[where[t, j]] + residual[t], z slots x N, y T x N (one type); float32 sums in the order of
+ * j. A slot with where -1 adds weights * 0. residual: rows residual_stride apart, or NULL. */
+int mxq_combine(const void* z, int32_t type, const float* weights, const int32_t* where, const void* residual,
+                int64_t residual_stride, void* y, int64_t T, int64_t k, int64_t N, void* stream);
+/* dz[where[t, j]] = weights[t, j] dy[t] (rows of left-out places 0), dw[t, j] = dy[t] . z[where[t, j]] (left-out slots 0) */
+int mxq_combine_backward(const void* dy, int64_t dy_stride, const void* z, int32_t type, const float* weights,
+                         const int32_t* where, const int32_t* order, void* dz, float* dw, int64_t T, int64_t k, int64_t N,
+                         void* stream);
+
 /* ------------------------------------------------------------------------------------------ diagnostics */
 /* No reference counterpart: the number of bounded shared-memory waits (mbarrier) that gave up in the TMA-staged
  * kernels on the current device since the library was loaded. Always 0 in a correct run; synchronous. */

@@ -77,8 +77,8 @@ static PFN_cuTensorMapEncodeTiled_v12000 encode_fn() {
   return fn;
 }
 
-int encode_tmap_f32(CUtensorMap* map, const void* base, int rank, const uint64_t* dims, const uint64_t* strides,
-                    const uint32_t* box) {
+static int encode_tmap(CUtensorMap* map, CUtensorMapDataType type, CUtensorMapSwizzle swizzle, const void* base, int rank,
+                       const uint64_t* dims, const uint64_t* strides, const uint32_t* box) {
   auto fn = encode_fn();
   if (!fn) return set_error(MXQ_ERR_CUDA, "cuTensorMapEncodeTiled is not available from the driver");
   cuuint64_t d[5], s[4];
@@ -89,11 +89,23 @@ int encode_tmap_f32(CUtensorMap* map, const void* base, int rank, const uint64_t
     e[i] = 1;
     if (i > 0) s[i - 1] = strides[i - 1];
   }
-  CUresult r = fn(map, CU_TENSOR_MAP_DATA_TYPE_FLOAT32, (cuuint32_t)rank, const_cast<void*>(base), d, s, b, e,
-                  CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_NONE, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
-                  CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+  CUresult r = fn(map, type, (cuuint32_t)rank, const_cast<void*>(base), d, s, b, e, CU_TENSOR_MAP_INTERLEAVE_NONE,
+                  swizzle, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
   if (r != CUDA_SUCCESS) return set_error(MXQ_ERR_CUDA, "cuTensorMapEncodeTiled failed (%d)", (int)r);
   return MXQ_OK;
+}
+
+int encode_tmap_f32(CUtensorMap* map, const void* base, int rank, const uint64_t* dims, const uint64_t* strides,
+                    const uint32_t* box) {
+  return encode_tmap(map, CU_TENSOR_MAP_DATA_TYPE_FLOAT32, CU_TENSOR_MAP_SWIZZLE_NONE, base, rank, dims, strides, box);
+}
+
+int encode_tmap_codes(CUtensorMap* map, const void* base, bool nibbles, uint64_t rows, uint64_t cols, uint64_t pitch,
+                      uint32_t box_rows) {
+  const uint64_t dims[2] = {cols, rows}, strides[1] = {pitch};
+  const uint32_t box[2] = {128u, box_rows};
+  return encode_tmap(map, nibbles ? CU_TENSOR_MAP_DATA_TYPE_16U4_ALIGN16B : CU_TENSOR_MAP_DATA_TYPE_UINT8,
+                     CU_TENSOR_MAP_SWIZZLE_128B, base, 2, dims, strides, box);
 }
 
 unsigned* wait_status_word() {

@@ -1,0 +1,936 @@
+// Products of packed MX operands with their epilogue, dense and by expert:
+//
+//   acc[r, n] = sum_k x[r, k] w[n, k] 2^(sx[r, k/32] - 127) 2^(sw[n, k/32] - 127)        (float32, tensor cores)
+//   y = act(acc + bias) (* up) + residual,  written as float32 / bf16 / f16 or packed again (32 columns per scale)
+//
+// x and w are row-major codes with blocks of 32 along K, as block.*.quantize_packed(axis=-1) writes them. sm_100's
+// tcgen05.mma kind::mxf8f6f4 multiplies them as they are: codes and E8M0 bytes go from memory to shared memory to the
+// tensor core, nothing is dequantized. The products are exact and the sums are held in float32 in TMEM.
+//
+// Two kernels share the operand staging:
+//   k_mx_tile  128 rows of x by 256 rows of w per CTA, persistent, for many rows: the operations bound it.
+//   k_mx_rows  128 rows of w by 16-128 rows of x per CTA, K split over a cluster, for few rows: reading w bounds it.
+#include "common.cuh"
+#include "mx_codes.cuh"
+#include "tc.cuh"
+
+#include <cooperative_groups.h>
+
+namespace cg = cooperative_groups;
+using namespace mxq;
+
+namespace {
+
+enum { kActNone = 0, kActRelu, kActGelu, kActGeluTanh, kActSilu, kActSwiglu, kActGeglu };
+enum { kOutF32 = 0, kOutBf16, kOutF16, kOutPacked };
+
+struct Args {
+  const uint8_t *sx, *sw;      // E8M0 bytes, nb per row
+  int nb;
+  int vec;                     // scale bytes are read 16, 4 or 1 at a time (alignment and nb allow it)
+  const int32_t *offsets, *order;
+  int experts;                 // 0: dense
+  int per;                     // > 0: row r of the product is row order[r] / per of x
+  int rows, xrows;             // rows of the product, rows of x
+  int n, width;                // rows of w (per expert), columns of y
+  int kblocks;                 // steps of 128 along K
+  uint32_t idesc;
+  uint32_t xbytes, wbytes;     // what one row of a stage's tile counts on the barrier
+  const float* bias;
+  const void* residual;
+  int64_t residual_stride;
+  void* out;
+  uint8_t* out_scales;
+  int64_t out_pitch, out_nb;
+  int act, otype, ofmt;
+  int vec_out;                 // y's (and the residual's) rows take 16-byte accesses
+  unsigned* status;
+};
+
+// ------------------------------------------------------------------------------------------ epilogue values
+// exp and the division here are the fast ones (a few ulp of float32): y is rounded to 16 bits or fewer, or, as float32,
+// already carries the sum's own error of that size.
+__device__ __forceinline__ float over_one_plus_exp(float x, float t) { return __fdividef(x, __fadd_rn(1.0f, __expf(t))); }
+__device__ __forceinline__ float silu(float x) { return over_one_plus_exp(x, -x); }
+__device__ __forceinline__ float gelu(float x) { return 0.5f * x * (1.0f + erff(x * 0.70710678118654752f)); }
+// x (1 + tanh(u)) / 2 = x / (1 + exp(-2u)), u = sqrt(2 / pi) (x + 0.044715 x^3)
+__device__ __forceinline__ float gelu_tanh(float x) {
+  return over_one_plus_exp(x, -1.5957691216057308f * __fmaf_rn(0.044715f * x * x, x, x));
+}
+// a NaN stays one
+__device__ __forceinline__ float relu(float x) { return x < 0.0f ? 0.0f : x; }
+
+__device__ __forceinline__ float activate1(int act, float g) {
+  switch (act) {
+    case kActRelu: return relu(g);
+    case kActGelu:
+    case kActGeglu: return gelu(g);
+    case kActGeluTanh: return gelu_tanh(g);
+    case kActSilu:
+    case kActSwiglu: return silu(g);
+    default: return g;
+  }
+}
+// the switch outside the loop: one branch per 32 values
+template <int N>
+__device__ __forceinline__ void activate(int act, float (&v)[N]) {
+  switch (act) {
+    case kActRelu:
+#pragma unroll
+      for (int i = 0; i < N; i++) v[i] = relu(v[i]);
+      break;
+    case kActGelu:
+    case kActGeglu:
+#pragma unroll
+      for (int i = 0; i < N; i++) v[i] = gelu(v[i]);
+      break;
+    case kActGeluTanh:
+#pragma unroll
+      for (int i = 0; i < N; i++) v[i] = gelu_tanh(v[i]);
+      break;
+    case kActSilu:
+    case kActSwiglu:
+#pragma unroll
+      for (int i = 0; i < N; i++) v[i] = silu(v[i]);
+      break;
+    default: break;
+  }
+}
+
+// ------------------------------------------------------------------------------------------ operand staging
+constexpr int kTileBytes = 128 * 128;                 // 128 rows of one K step
+
+// 16 scale bytes of a row from K step 4g on (a step has 4): 0 beyond the row
+__device__ __forceinline__ uint4 load_scales(const uint8_t* row, int g, int nb, int vec) {
+  uint32_t w[4];
+  if (vec == 16) return __ldg(reinterpret_cast<const uint4*>(row + (int64_t)g * 16));
+#pragma unroll
+  for (int j = 0; j < 4; j++) {
+    const int at = g * 16 + j * 4;
+    w[j] = 0;
+    if (vec == 4) {
+      if (at < nb) w[j] = __ldg(reinterpret_cast<const uint32_t*>(row + at));
+    } else {
+#pragma unroll
+      for (int b = 0; b < 4; b++)
+        if (at + b < nb) w[j] |= (uint32_t)__ldg(row + at + b) << (8 * b);
+    }
+  }
+  return make_uint4(w[0], w[1], w[2], w[3]);
+}
+
+// place of row r's word in a stage's scale area (groups of 128 rows, 512 bytes each)
+__device__ __forceinline__ uint32_t scale_place(int r) { return (uint32_t)((r >> 7) * 512 + (r & 31) * 16 + ((r & 127) >> 5) * 4); }
+
+struct Ring {
+  int stage = 0;
+  unsigned phase = 0;
+  __device__ __forceinline__ void next(int stages) {
+    if (++stage == stages) {
+      stage = 0;
+      phase ^= 1u;
+    }
+  }
+};
+
+// One warp brings the scale words of its W rows per lane for K steps [k0, k1) into the ring: 16 bytes per row, that
+// is four steps, are read at once and the next four are on their way while these are stored.
+template <int W>
+__device__ __forceinline__ bool stage_scales(const uint8_t* const (&rows)[W], const uint32_t (&place)[W], int k0, int k1, const Args& a,
+                                             uint8_t* area, int pitch, uint64_t* full, uint64_t* empty, Ring& ring, int stages,
+                                             volatile int* abort) {
+  uint4 now[W], nxt[W];
+  int g = k0 >> 2;
+  const int last = (k1 - 1) >> 2;
+#pragma unroll
+  for (int i = 0; i < W; i++) now[i] = load_scales(rows[i], g, a.nb, a.vec);
+  for (; g <= last; g++) {
+    if (g < last) {
+#pragma unroll
+      for (int i = 0; i < W; i++) nxt[i] = load_scales(rows[i], g + 1, a.nb, a.vec);
+    }
+#pragma unroll
+    for (int j = 0; j < 4; j++) {
+      const int kb = g * 4 + j;
+      if (kb < k0 || kb >= k1) continue;
+      if (!tc::wait(&empty[ring.stage], ring.phase ^ 1u, abort, a.status)) return false;
+      uint8_t* to = area + (size_t)ring.stage * pitch;
+#pragma unroll
+      for (int i = 0; i < W; i++)
+        *reinterpret_cast<uint32_t*>(to + place[i]) = j == 0 ? now[i].x : j == 1 ? now[i].y : j == 2 ? now[i].z : now[i].w;
+      fence_proxy_async();
+      __syncwarp();
+      if ((threadIdx.x & 31) == 0) tc::mbar_arrive(&full[ring.stage]);
+      ring.next(stages);
+    }
+#pragma unroll
+    for (int i = 0; i < W; i++) now[i] = nxt[i];
+  }
+  return true;
+}
+
+// where expert e's rows begin, whatever the offsets hold within the product's rows
+__device__ __forceinline__ int row_begin(const Args& a, int e) { return min(max(a.offsets[e], 0), a.rows); }
+
+// The experts' tiles in order: first[e] = tiles before expert e. One warp.
+__device__ void count_tiles(int* first, const Args& a, int tile_rows, int per_row_tile) {
+  const int lane = threadIdx.x & 31;
+  int carry = 0;
+  for (int base = 0; base < a.experts; base += 32) {
+    const int e = base + lane;
+    int t = 0;
+    if (e < a.experts) {
+      const int c = row_begin(a, e + 1) - row_begin(a, e);
+      t = (c > 0 ? (c + tile_rows - 1) / tile_rows : 0) * per_row_tile;
+    }
+    int s = t;
+#pragma unroll
+    for (int d = 1; d < 32; d <<= 1) {
+      const int up = __shfl_up_sync(~0u, s, d);
+      if (lane >= d) s += up;
+    }
+    if (e < a.experts) first[e + 1] = carry + s;
+    carry += __shfl_sync(~0u, s, 31);
+  }
+  if (lane == 0) first[0] = 0;
+}
+
+struct Tile {
+  int expert;
+  int row0, rows;              // first row of the product, rows of it in this tile
+  int col;                     // column tile
+};
+
+// Tile t: by expert, then column tile, then row tile, so that the CTAs at work at one time share w's tiles. Dense: row
+// tiles in bands of 16 for the same reason. false: no such tile.
+__device__ __forceinline__ bool find_tile(int t, const Args& a, const int* first, int tile_rows, int col_tiles, Tile& o) {
+  if (a.experts == 0) {
+    const int row_tiles = (a.rows + tile_rows - 1) / tile_rows;
+    if (t >= row_tiles * col_tiles) return false;
+    const int band = t / (16 * col_tiles), in = t - band * 16 * col_tiles;
+    const int high = min(16, row_tiles - band * 16);
+    o.expert = 0;
+    o.col = in / high;
+    o.row0 = (band * 16 + in % high) * tile_rows;
+    o.rows = min(tile_rows, a.rows - o.row0);
+    return true;
+  }
+  if (t >= first[a.experts]) return false;
+  int lo = 0, hi = a.experts;                          // first[lo] <= t < first[hi]
+  while (hi - lo > 1) {
+    const int mid = (lo + hi) >> 1;
+    if (first[mid] <= t) lo = mid; else hi = mid;
+  }
+  const int in = t - first[lo], row_tiles = (first[lo + 1] - first[lo]) / col_tiles;
+  o.expert = lo;
+  o.col = in / row_tiles;
+  const int begin = row_begin(a, lo), end = row_begin(a, lo + 1);
+  o.row0 = begin + (in % row_tiles) * tile_rows;
+  o.rows = min(tile_rows, end - o.row0);
+  return true;
+}
+
+// the row of x that row r of the product is; a row beyond the tile stands for its last one and is never written
+__device__ __forceinline__ int x_row(const Args& a, const Tile& t, int r) {
+  r = t.row0 + min(r, t.rows - 1);
+  if (a.per > 0) r = a.order[r] / a.per;
+  return min(max(r, 0), a.xrows - 1);
+}
+__device__ __forceinline__ const uint8_t* w_scales(const Args& a, const Tile& t, int r) {
+  return a.sw + ((int64_t)t.expert * a.n + min(r, a.n - 1)) * a.nb;
+}
+
+// ------------------------------------------------------------------------------------------------ many rows
+constexpr int kStages = 4;
+constexpr int kStageBytes = 3 * kTileBytes;            // x 128 rows, w 256 rows
+constexpr int kStageScales = 3 * 512;
+
+struct TileShared {
+  uint64_t full[kStages], empty[kStages], acc_full, acc_free, last;
+  uint32_t tmem;
+  int abort;
+};
+constexpr int kTileSmem = 1024 + kStages * (kStageBytes + kStageScales) + (int)sizeof(TileShared);
+
+// 32 columns of one row of y: bias and activation are done; residual, rounding, store
+__device__ __forceinline__ void write_row(const Args& a, float (&y)[32], int64_t row, int col) {
+  const int left = a.width - col;
+  if (a.otype == kOutPacked) {
+    uint32_t top = 0;
+#pragma unroll
+    for (int i = 0; i < 32; i++) {
+      const uint32_t b = __float_as_uint(y[i]) & 0x7fffffffu;
+      if (i < left) top = max(top, b);
+    }
+    const uint32_t sb = scale_byte(top, a.ofmt);
+    const float inv = scale_inverse(sb);
+    a.out_scales[row * a.out_nb + (col >> 5)] = (uint8_t)sb;
+    uint32_t w[8];
+    const bool nib = a.ofmt == kFmtE2M1;
+    uint8_t* to = static_cast<uint8_t*>(a.out) + row * a.out_pitch + (nib ? col >> 1 : col);
+    if (nib) {
+#pragma unroll
+      for (int i = 0; i < 4; i++) {
+        w[i] = 0;
+#pragma unroll
+        for (int j = 0; j < 4; j++)
+          w[i] |= (encode2(kFmtE2M1, scaled(y[8 * i + 2 * j], inv), scaled(y[8 * i + 2 * j + 1], inv)) & 255u) << (8 * j);
+      }
+    } else {
+#pragma unroll
+      for (int i = 0; i < 8; i++)
+        w[i] = encode2(a.ofmt, scaled(y[4 * i], inv), scaled(y[4 * i + 1], inv)) |
+               encode2(a.ofmt, scaled(y[4 * i + 2], inv), scaled(y[4 * i + 3], inv)) << 16;
+    }
+    const int bytes = nib ? 16 : 32;
+    if (left >= 32 && a.vec_out) {
+      reinterpret_cast<uint4*>(to)[0] = make_uint4(w[0], w[1], w[2], w[3]);
+      if (!nib) reinterpret_cast<uint4*>(to)[1] = make_uint4(w[4], w[5], w[6], w[7]);
+    } else {
+      const int have = nib ? left >> 1 : left;
+#pragma unroll
+      for (int i = 0; i < 32; i++)
+        if (i < bytes && i < have) to[i] = (uint8_t)(w[i >> 2] >> (8 * (i & 3)));
+    }
+    return;
+  }
+  const bool whole = left >= 32 && a.vec_out;
+  if (a.otype == kOutF32) {
+    float* to = static_cast<float*>(a.out) + row * a.out_pitch + col;
+    const float* r = a.residual ? static_cast<const float*>(a.residual) + row * a.residual_stride + col : nullptr;
+    if (whole) {
+#pragma unroll
+      for (int i = 0; i < 8; i++) {
+        float4 v = make_float4(y[4 * i], y[4 * i + 1], y[4 * i + 2], y[4 * i + 3]);
+        if (r) {
+          const float4 q = __ldg(reinterpret_cast<const float4*>(r) + i);
+          v = make_float4(v.x + q.x, v.y + q.y, v.z + q.z, v.w + q.w);
+        }
+        reinterpret_cast<float4*>(to)[i] = v;
+      }
+    } else {
+#pragma unroll
+      for (int i = 0; i < 32; i++)
+        if (i < left) to[i] = r ? y[i] + r[i] : y[i];
+    }
+    return;
+  }
+  const bool bf = a.otype == kOutBf16;
+  uint16_t* to = static_cast<uint16_t*>(a.out) + row * a.out_pitch + col;
+  const uint16_t* r = a.residual ? static_cast<const uint16_t*>(a.residual) + row * a.residual_stride + col : nullptr;
+  auto widen = [bf](uint32_t h) {
+    return bf ? __uint_as_float(h << 16) : __half2float(__ushort_as_half((unsigned short)h));
+  };
+  auto pair = [bf](float lo, float hi) {
+    if (bf) {
+      const __nv_bfloat162 p = __floats2bfloat162_rn(lo, hi);
+      return *reinterpret_cast<const uint32_t*>(&p);
+    }
+    const __half2 p = __floats2half2_rn(lo, hi);
+    return *reinterpret_cast<const uint32_t*>(&p);
+  };
+  if (whole) {
+#pragma unroll
+    for (int i = 0; i < 4; i++) {
+      if (r) {
+        const uint4 q = __ldg(reinterpret_cast<const uint4*>(r) + i);
+        const uint32_t h[4] = {q.x, q.y, q.z, q.w};
+#pragma unroll
+        for (int j = 0; j < 4; j++) {
+          y[8 * i + 2 * j] += widen(h[j] & 0xffffu);
+          y[8 * i + 2 * j + 1] += widen(h[j] >> 16);
+        }
+      }
+      reinterpret_cast<uint4*>(to)[i] = make_uint4(pair(y[8 * i], y[8 * i + 1]), pair(y[8 * i + 2], y[8 * i + 3]),
+                                                   pair(y[8 * i + 4], y[8 * i + 5]), pair(y[8 * i + 6], y[8 * i + 7]));
+    }
+  } else {
+#pragma unroll
+    for (int i = 0; i < 32; i++)
+      if (i < left) to[i] = (uint16_t)(pair(r ? y[i] + widen(r[i]) : y[i], 0.0f) & 0xffffu);
+  }
+}
+
+// Warp 0 loads the codes, warp 1 issues the products, warps 2-3 bring the scales, warps 4-7 write y.
+//
+// TMEM (512 columns): two accumulators of 256 that share 64 columns, [0, 256) and [192, 448), and the stages' scale
+// words in [448, 512). The epilogue of a tile drains the shared columns first and then lets the next tile's products
+// start, so three quarters of it run beside them.
+template <bool GATED>
+__global__ void __launch_bounds__(256, 1) k_mx_tile(const __grid_constant__ CUtensorMap mx, const __grid_constant__ CUtensorMap mw,
+                                                    const __grid_constant__ Args a) {
+  extern __shared__ uint8_t raw[];
+  uint8_t* codes = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(raw) + 1023) & ~(uintptr_t)1023);
+  uint8_t* scales = codes + kStages * kStageBytes;
+  TileShared& sh = *reinterpret_cast<TileShared*>(scales + kStages * kStageScales);
+  int* first = reinterpret_cast<int*>(&sh + 1);
+  volatile int* abort = &sh.abort;
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  constexpr int kCols = GATED ? 128 : 256;             // columns of y per tile
+  const int col_tiles = (a.width + kCols - 1) / kCols;
+
+  if (threadIdx.x == 0) {
+    for (int i = 0; i < kStages; i++) {
+      mbar_init(&sh.full[i], 3);                       // the codes' bytes and the two scale warps
+      mbar_init(&sh.empty[i], 1);
+    }
+    mbar_init(&sh.acc_full, 1);
+    mbar_init(&sh.acc_free, 4);
+    mbar_init(&sh.last, 1);
+    sh.abort = 0;
+    fence_mbar_init();
+  }
+  if (warp == 1) tc::tmem_alloc(&sh.tmem, 512);
+  if (warp == 2 && a.experts) count_tiles(first, a, 128, col_tiles);
+  tc::fence_before();
+  __syncthreads();
+  tc::fence_after();
+  const uint32_t tmem = sh.tmem;
+  // the second half of a tile's w rows: the up projections, or the next 128 features
+  const int second = GATED ? a.width : 128;
+
+  if (warp == 0) {
+    Ring ring;
+    bool ok = true;
+    Tile t;
+    int sent = 0;
+    for (int i = blockIdx.x; ok && find_tile(i, a, first, 128, col_tiles, t); i += gridDim.x) {
+      int4 rows = make_int4(0, 0, 0, 0);
+      if (a.per > 0) rows = make_int4(x_row(a, t, 4 * lane), x_row(a, t, 4 * lane + 1), x_row(a, t, 4 * lane + 2), x_row(a, t, 4 * lane + 3));
+      const int w0 = t.expert * a.n + t.col * kCols;
+      for (int kb = 0; kb < a.kblocks; kb++) {
+        if (a.per > 0 || lane == 0) ok = tc::wait(&sh.empty[ring.stage], ring.phase ^ 1u, abort, a.status);
+        ok = __all_sync(~0u, ok);
+        if (!ok) break;
+        uint8_t* to = codes + ring.stage * kStageBytes;
+        uint64_t* bar = &sh.full[ring.stage];
+        if (lane == 0) {
+          mbar_expect_tx(bar, 128 * a.xbytes + 256 * a.wbytes);
+          if (a.per == 0) tma_load_2d(to, &mx, kb * 128, t.row0, bar);
+          tma_load_2d(to + kTileBytes, &mw, kb * 128, w0, bar);
+          tma_load_2d(to + 2 * kTileBytes, &mw, kb * 128, w0 + second, bar);
+        }
+        if (a.per > 0) tc::tma_gather4(to + lane * 512, &mx, kb * 128, rows, bar);
+        ring.next(kStages);
+        sent++;
+      }
+    }
+    if (!ok && lane == 0)                              // the loads under way land before the CTA leaves
+      for (int s = 0; s < kStages && s < sent; s++) {
+        ring.stage = ring.stage ? ring.stage - 1 : (ring.phase ^= 1u, kStages - 1);
+        tc::settle(&sh.full[ring.stage], ring.phase);
+      }
+  } else if (warp == 1) {
+    if (lane == 0) {
+      Ring ring;
+      bool ok = true;
+      Tile t;
+      int done = 0;
+      for (int i = blockIdx.x; ok && find_tile(i, a, first, 128, col_tiles, t); i += gridDim.x, done++) {
+        if (done) ok = tc::wait(&sh.acc_free, (done - 1) & 1, abort, a.status);
+        if (!ok) break;
+        tc::fence_after();
+        const uint32_t acc = tmem + (done & 1 ? 192 : 0);
+        for (int kb = 0; kb < a.kblocks; kb++) {
+          ok = tc::wait(&sh.full[ring.stage], ring.phase, abort, a.status);
+          if (!ok) break;
+          tc::fence_after();
+          const uint32_t at = smem_addr(codes + ring.stage * kStageBytes);
+          const uint32_t sc = smem_addr(scales + ring.stage * kStageScales);
+          const uint32_t ts = tmem + 448 + ring.stage * 12;
+#pragma unroll
+          for (int j = 0; j < 3; j++) tc::copy_scales(ts + 4 * j, tc::scale_desc(sc + 512 * j));
+          const uint64_t da = tc::operand_desc(at), db = tc::operand_desc(at + kTileBytes);
+#pragma unroll
+          for (int j = 0; j < 4; j++)                  // 32 codes further: 2 units of 16 bytes
+            tc::mma(acc, da + 2 * j, db + 2 * j, tc::mma_desc_step(a.idesc, j), ts, ts + 4, kb > 0 || j > 0);
+          tc::commit(&sh.empty[ring.stage]);
+          ring.next(kStages);
+        }
+        if (ok) tc::commit(&sh.acc_full);
+      }
+      if (!ok) {
+        tc::commit(&sh.last);
+        tc::settle(&sh.last, 0);
+      }
+    }
+  } else if (warp < 4) {
+    Ring ring;
+    Tile t;
+    // 384 rows of words, 12 per lane in two warps: x's 128, w's 256
+    const int half = warp - 2;
+    for (int i = blockIdx.x; find_tile(i, a, first, 128, col_tiles, t); i += gridDim.x) {
+      const uint8_t* rows[6];
+      uint32_t place[6];
+#pragma unroll
+      for (int j = 0; j < 6; j++) {
+        const int r = (j * 2 + half) * 32 + lane;
+        place[j] = scale_place(r);
+        if (r < 128)
+          rows[j] = a.sx + (int64_t)x_row(a, t, r) * a.nb;
+        else
+          rows[j] = w_scales(a, t, t.col * kCols + (r < 256 ? r - 128 : r - 256 + second));
+      }
+      if (!stage_scales<6>(rows, place, 0, a.kblocks, a, scales, kStageScales, sh.full, sh.empty, ring, kStages, abort)) break;
+    }
+  } else {
+    Tile t;
+    int done = 0;
+    const int q = warp - 4;
+    constexpr int kChunks = kCols / 32;
+    for (int i = blockIdx.x; find_tile(i, a, first, 128, col_tiles, t); i += gridDim.x, done++) {
+      const bool ok = tc::wait(&sh.acc_full, done & 1, abort, a.status);
+      __syncwarp();
+      tc::fence_after();
+      const uint32_t acc = tmem + (done & 1 ? 192 : 0) + ((uint32_t)(q * 32) << 16);
+      const int r = q * 32 + lane;
+      const float* bias = a.bias ? a.bias + (int64_t)t.expert * a.n : nullptr;
+#pragma unroll 1
+      for (int c = 0; c < kChunks; c++) {
+        // the columns shared with the other accumulator first: the first one's last 64, the second one's first 64
+        const int chunk = done & 1 ? c : (c + kChunks - 2) % kChunks;
+        const int col = t.col * kCols + chunk * 32;
+        float y[32];
+        tc::load32(acc + chunk * 32, y);
+        if (GATED) {
+          float up[32];
+          tc::load32(acc + 128 + chunk * 32, up);
+          if (bias) {
+#pragma unroll
+            for (int j = 0; j < 32; j++) {
+              const int n = min(col + j, a.width - 1);
+              y[j] += __ldg(bias + n);
+              up[j] += __ldg(bias + a.width + n);
+            }
+          }
+          activate(a.act, y);
+#pragma unroll
+          for (int j = 0; j < 32; j++) y[j] *= up[j];
+        } else {
+          if (bias) {
+#pragma unroll
+            for (int j = 0; j < 32; j++) y[j] += __ldg(bias + min(col + j, a.width - 1));
+          }
+          activate(a.act, y);
+        }
+        if (c == 1) {                                  // the next tile's products may start
+          tc::fence_before();
+          __syncwarp();
+          if (lane == 0) tc::mbar_arrive(&sh.acc_free);
+        }
+        if (!ok) {
+#pragma unroll
+          for (int j = 0; j < 32; j++) y[j] = __uint_as_float(0x7fc00000u);
+        }
+        if (r < t.rows && col < a.width) write_row(a, y, (int64_t)t.row0 + r, col);
+      }
+    }
+  }
+  __syncwarp();
+  tc::fence_before();
+  __syncthreads();
+  tc::fence_after();
+  if (warp == 1) tc::tmem_free(tmem, 512);
+}
+
+// ------------------------------------------------------------------------------------------------- few rows
+template <int BN>
+struct RowsShape {
+  static constexpr int kStageCodes = kTileBytes + BN * 128;
+  static constexpr int kStageScales = 1024;            // w's 128 rows, x's up to 128
+  static constexpr int kDepth = BN <= 32 ? 5 : BN == 64 ? 4 : 3;
+  static constexpr int kSmem = 1024 + kDepth * (kStageCodes + kStageScales) + 256;
+  static constexpr int kAcc = BN < 32 ? 32 : BN;       // accumulator columns
+  static constexpr int kTmem = kAcc + kDepth * 8 <= 64 ? 64 : kAcc + kDepth * 8 <= 128 ? 128 : 256;
+};
+
+struct RowsShared {
+  uint64_t full[5], empty[5], acc_full, last;
+  uint32_t tmem;
+  int abort;
+};
+static_assert(sizeof(RowsShared) <= 256, "barriers");
+
+// one column (token) of the transposed accumulator, this lane's feature: everything after bias and activation
+__device__ __forceinline__ void write_one(const Args& a, float y, int64_t row, int col) {
+  const bool in = col < a.width;
+  if (a.otype == kOutPacked) {
+    const uint32_t top = __reduce_max_sync(~0u, in ? __float_as_uint(y) & 0x7fffffffu : 0u);
+    const uint32_t sb = scale_byte(top, a.ofmt);
+    const float inv = scale_inverse(sb);
+    if ((threadIdx.x & 31) == 0 && in) a.out_scales[row * a.out_nb + (col >> 5)] = (uint8_t)sb;
+    const float z = scaled(y, inv);
+    const float next = __shfl_down_sync(~0u, z, 1);
+    uint8_t* to = static_cast<uint8_t*>(a.out) + row * a.out_pitch;
+    if (a.ofmt == kFmtE2M1) {
+      if (in && !(col & 1)) to[col >> 1] = (uint8_t)encode2(kFmtE2M1, z, next);
+    } else if (in) {
+      to[col] = (uint8_t)encode2(a.ofmt, z, 0.0f);
+    }
+    return;
+  }
+  if (!in) return;
+  if (a.otype == kOutF32) {
+    if (a.residual) y += static_cast<const float*>(a.residual)[row * a.residual_stride + col];
+    static_cast<float*>(a.out)[row * a.out_pitch + col] = y;
+  } else if (a.otype == kOutBf16) {
+    if (a.residual) y += __bfloat162float(static_cast<const __nv_bfloat16*>(a.residual)[row * a.residual_stride + col]);
+    static_cast<__nv_bfloat16*>(a.out)[row * a.out_pitch + col] = __float2bfloat16_rn(y);
+  } else {
+    if (a.residual) y += __half2float(static_cast<const __half*>(a.residual)[row * a.residual_stride + col]);
+    static_cast<__half*>(a.out)[row * a.out_pitch + col] = __float2half_rn(y);
+  }
+}
+
+// The cluster's CTAs each take a share of K; their partial sums meet in shared memory and are added in rank order (the
+// same sum on every run), each CTA finishing its share of the rows of x.
+template <int BN, bool GATED>
+__global__ void __launch_bounds__(128, 2) k_mx_rows(const __grid_constant__ CUtensorMap mx, const __grid_constant__ CUtensorMap mw,
+                                                 const __grid_constant__ Args a) {
+  using S = RowsShape<BN>;
+  extern __shared__ uint8_t raw[];
+  uint8_t* codes = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(raw) + 1023) & ~(uintptr_t)1023);
+  uint8_t* scales = codes + S::kDepth * S::kStageCodes;
+  RowsShared& sh = *reinterpret_cast<RowsShared*>(scales + S::kDepth * S::kStageScales);
+  int* first = reinterpret_cast<int*>(&sh + 1);
+  volatile int* abort = &sh.abort;
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  constexpr int kCols = GATED ? 64 : 128;              // columns of y per tile
+  const int col_tiles = (a.width + kCols - 1) / kCols;
+  cg::cluster_group cluster = cg::this_cluster();
+  const int split = (int)cluster.num_blocks(), rank = (int)cluster.block_rank();
+
+  if (threadIdx.x == 0) {
+    for (int i = 0; i < S::kDepth; i++) {
+      mbar_init(&sh.full[i], 3);
+      mbar_init(&sh.empty[i], 1);
+    }
+    mbar_init(&sh.acc_full, 1);
+    mbar_init(&sh.last, 1);
+    sh.abort = 0;
+    fence_mbar_init();
+  }
+  if (warp == 1) tc::tmem_alloc(&sh.tmem, S::kTmem);
+  if (warp == 2 && a.experts) count_tiles(first, a, BN, col_tiles);
+  tc::fence_before();
+  __syncthreads();
+  tc::fence_after();
+  const uint32_t tmem = sh.tmem;
+  Tile t;
+  const bool work = find_tile(blockIdx.x / split, a, first, BN, col_tiles, t);    // the same for the whole cluster
+  const int k0 = (int)((int64_t)a.kblocks * rank / split), k1 = (int)((int64_t)a.kblocks * (rank + 1) / split);
+  const bool busy = work && k1 > k0;
+
+  if (busy && warp == 0) {
+    Ring ring;
+    bool ok = true;
+    int sent = 0;
+    int4 rows = make_int4(0, 0, 0, 0);
+    if (a.per > 0 && lane < BN / 4)
+      rows = make_int4(x_row(a, t, 4 * lane), x_row(a, t, 4 * lane + 1), x_row(a, t, 4 * lane + 2), x_row(a, t, 4 * lane + 3));
+    const int w0 = t.expert * a.n + t.col * kCols;
+    for (int kb = k0; kb < k1; kb++) {
+      if (a.per > 0 || lane == 0) ok = tc::wait(&sh.empty[ring.stage], ring.phase ^ 1u, abort, a.status);
+      ok = __all_sync(~0u, ok);
+      if (!ok) break;
+      uint8_t* to = codes + ring.stage * S::kStageCodes;
+      uint64_t* bar = &sh.full[ring.stage];
+      if (lane == 0) {
+        mbar_expect_tx(bar, 128 * a.wbytes + BN * a.xbytes);
+        tma_load_2d(to, &mw, kb * 128, w0, bar);
+        if (GATED) tma_load_2d(to + kTileBytes / 2, &mw, kb * 128, w0 + a.width, bar);
+        if (a.per == 0) tma_load_2d(to + kTileBytes, &mx, kb * 128, t.row0, bar);
+      }
+      if (a.per > 0 && lane < BN / 4) tc::tma_gather4(to + kTileBytes + lane * 512, &mx, kb * 128, rows, bar);
+      ring.next(S::kDepth);
+      sent++;
+    }
+    if (!ok && lane == 0)
+      for (int s = 0; s < S::kDepth && s < sent; s++) {
+        ring.stage = ring.stage ? ring.stage - 1 : (ring.phase ^= 1u, S::kDepth - 1);
+        tc::settle(&sh.full[ring.stage], ring.phase);
+      }
+  } else if (busy && warp == 1) {
+    if (lane == 0) {
+      Ring ring;
+      bool ok = true;
+      for (int kb = k0; kb < k1; kb++) {
+        ok = tc::wait(&sh.full[ring.stage], ring.phase, abort, a.status);
+        if (!ok) break;
+        tc::fence_after();
+        const uint32_t at = smem_addr(codes + ring.stage * S::kStageCodes);
+        const uint32_t sc = smem_addr(scales + ring.stage * S::kStageScales);
+        const uint32_t ts = tmem + S::kAcc + ring.stage * 8;
+        tc::copy_scales(ts, tc::scale_desc(sc));
+        tc::copy_scales(ts + 4, tc::scale_desc(sc + 512));
+        const uint64_t da = tc::operand_desc(at), db = tc::operand_desc(at + kTileBytes);
+#pragma unroll
+        for (int j = 0; j < 4; j++)
+          tc::mma(tmem, da + 2 * j, db + 2 * j, tc::mma_desc_step(a.idesc, j), ts, ts + 4, kb > k0 || j > 0);
+        tc::commit(&sh.empty[ring.stage]);
+        ring.next(S::kDepth);
+      }
+      if (ok) {
+        tc::commit(&sh.acc_full);
+      } else {
+        tc::commit(&sh.last);
+        tc::settle(&sh.last, 0);
+      }
+    }
+  } else if (busy) {
+    constexpr int W = (128 + (BN < 32 ? 32 : BN) + 63) / 64;
+    const uint8_t* rows[W];
+    uint32_t place[W];
+#pragma unroll
+    for (int j = 0; j < W; j++) {
+      // rows of w, then of x; a lane with nothing left repeats w's last row in its own place
+      int r = (j * 2 + warp - 2) * 32 + lane;
+      if (r >= 128 + BN) r = 127;
+      place[j] = scale_place(r);
+      if (r >= 128)
+        rows[j] = a.sx + (int64_t)x_row(a, t, r - 128) * a.nb;
+      else
+        rows[j] = w_scales(a, t, t.col * kCols + (GATED && r >= 64 ? a.width + r - 64 : r));
+    }
+    Ring ring;
+    stage_scales<W>(rows, place, k0, k1, a, scales, S::kStageScales, sh.full, sh.empty, ring, S::kDepth, abort);
+  }
+  __syncwarp();
+
+  // partial sums, [row of x][feature], over the codes' stages, which are all consumed
+  float* part = reinterpret_cast<float*>(codes);
+  if (work) {
+    const bool ok = !busy || tc::wait(&sh.acc_full, 0, abort, a.status);
+    __syncwarp();
+    tc::fence_after();
+    const uint32_t acc = tmem + ((uint32_t)(warp * 32) << 16);
+#pragma unroll 1
+    for (int c = 0; c < BN; c += 16) {
+      float v[16];
+      tc::load16(acc + c, v);
+#pragma unroll
+      for (int j = 0; j < 16; j++)
+        part[(c + j) * 128 + warp * 32 + lane] = !busy ? 0.0f : ok ? v[j] : __uint_as_float(0x7fc00000u);
+    }
+  }
+  tc::fence_before();
+  if (split > 1) cluster.sync(); else __syncthreads();
+  tc::fence_after();
+  if (work) {
+    constexpr int kBlocks = kCols / 32;
+    const float* bias = a.bias ? a.bias + (int64_t)t.expert * a.n : nullptr;
+    const int pairs = t.rows * kBlocks;
+    for (int p = rank * 4 + warp; p < pairs; p += split * 4) {
+      const int r = p / kBlocks, f = (p % kBlocks) * 32 + lane, col = t.col * kCols + f;
+      float y = 0.0f, up = 0.0f;
+      for (int s = 0; s < split; s++) {
+        const float* from = split > 1 ? cluster.map_shared_rank(part, s) : part;
+        y += from[r * 128 + f];
+        if (GATED) up += from[r * 128 + 64 + f];
+      }
+      const int n = min(col, a.width - 1);
+      if (bias) y += __ldg(bias + n);
+      y = activate1(a.act, y);
+      if (GATED) {
+        if (bias) up += __ldg(bias + a.width + n);
+        y *= up;
+      }
+      if (t.col * kCols + (p % kBlocks) * 32 < a.width) write_one(a, y, (int64_t)t.row0 + r, col);
+    }
+  }
+  if (split > 1) cluster.sync(); else __syncthreads();  // the partial sums are read before their CTA leaves
+  if (warp == 1) tc::tmem_free(tmem, S::kTmem);
+}
+
+// --------------------------------------------------------------------------------------------------- host
+int set_smem(const void* f, int bytes) {
+  return check_cuda(cudaFuncSetAttribute(f, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes), "product: shared memory");
+}
+
+struct Operand {
+  const uint8_t* codes;
+  int64_t rows, pitch;
+  bool nibbles;
+};
+int map_of(CUtensorMap* m, const Operand& o, int64_t K, int box) {
+  return encode_tmap_codes(m, o.codes, o.nibbles, (uint64_t)o.rows, (uint64_t)K, (uint64_t)o.pitch, (uint32_t)box);
+}
+
+template <int BN, bool GATED>
+int launch_rows(Args& a, const Operand& x, const Operand& w, int64_t K, int64_t tiles, int split, int fx, int fw, cudaStream_t st) {
+  using S = RowsShape<BN>;
+  CUtensorMap mx, mw;
+  if (int rc = map_of(&mx, x, K, a.per > 0 ? 1 : BN)) return rc;
+  if (int rc = map_of(&mw, w, K, GATED ? 64 : 128)) return rc;
+  a.idesc = tc::mma_desc(fw, fx, 128, BN);
+  const int smem = S::kSmem + (a.experts ? 4 * (a.experts + 1) : 0);
+  auto f = k_mx_rows<BN, GATED>;
+  if (int rc = set_smem((const void*)f, smem)) return rc;
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3((unsigned)(tiles * split));
+  cfg.blockDim = dim3(128);
+  cfg.dynamicSmemBytes = smem;
+  cfg.stream = st;
+  cudaLaunchAttribute at[1];
+  at[0].id = cudaLaunchAttributeClusterDimension;
+  at[0].val.clusterDim.x = split;
+  at[0].val.clusterDim.y = at[0].val.clusterDim.z = 1;
+  cfg.attrs = at;
+  cfg.numAttrs = 1;
+  return check_cuda(cudaLaunchKernelEx(&cfg, f, mx, mw, a), "product (few rows)");
+}
+
+template <bool GATED>
+int launch_tile(Args& a, const Operand& x, const Operand& w, int64_t K, int64_t tiles, int fx, int fw, cudaStream_t st) {
+  CUtensorMap mx, mw;
+  if (int rc = map_of(&mx, x, K, a.per > 0 ? 1 : 128)) return rc;
+  if (int rc = map_of(&mw, w, K, 128)) return rc;
+  a.idesc = tc::mma_desc(fx, fw, 128, 256);
+  const int smem = kTileSmem + (a.experts ? 4 * (a.experts + 1) : 0);
+  auto f = k_mx_tile<GATED>;
+  if (int rc = set_smem((const void*)f, smem)) return rc;
+  const unsigned grid = (unsigned)(tiles < sm_count() ? tiles : sm_count());
+  f<<<grid, 256, smem, st>>>(mx, mw, a);
+  return MXQ_LAUNCH_CHECK("product");
+}
+
+int64_t up_div(int64_t a, int64_t b) { return (a + b - 1) / b; }
+
+template <bool GATED>
+int launch(Args& a, const Operand& x, const Operand& w, int64_t K, int fx, int fw, cudaStream_t st) {
+  // rows that share a tile of w: all of them, or an expert's share
+  const int64_t share = a.experts ? up_div(a.rows, a.experts) : a.rows;
+  const int64_t groups = a.experts ? (a.experts < a.rows ? a.experts : a.rows) : 1;
+  if (share > 128) {
+    const int64_t cols = up_div(a.width, GATED ? 128 : 256);
+    const int64_t tiles = (a.experts ? a.rows / 128 + groups : up_div(a.rows, 128)) * cols;
+    return launch_tile<GATED>(a, x, w, K, tiles, fx, fw, st);
+  }
+  const int bn = share <= 16 ? 16 : share <= 32 ? 32 : share <= 64 ? 64 : 128;
+  const int64_t cols = up_div(a.width, GATED ? 64 : 128);
+  const int64_t tiles = (a.experts ? a.rows / bn + groups : up_div(a.rows, bn)) * cols;
+  int split = 1;
+  while (split < 8 && tiles * split * 2 <= 2 * sm_count() && a.kblocks >= split * 4) split *= 2;
+  switch (bn) {
+    case 16: return launch_rows<16, GATED>(a, x, w, K, tiles, split, fx, fw, st);
+    case 32: return launch_rows<32, GATED>(a, x, w, K, tiles, split, fx, fw, st);
+    case 64: return launch_rows<64, GATED>(a, x, w, K, tiles, split, fx, fw, st);
+    default: return launch_rows<128, GATED>(a, x, w, K, tiles, split, fx, fw, st);
+  }
+}
+
+bool aligned(const void* p, int64_t n) { return reinterpret_cast<uintptr_t>(p) % (uintptr_t)n == 0; }
+
+int check_operand(const char* who, const char* what, const void* codes, int64_t pitch, int fmt, int64_t K, int* mma) {
+  MXQ_REQUIRE(fmt == kFmtE4M3 || fmt == kFmtE5M2 || fmt == kFmtE2M1, MXQ_ERR_UNSUPPORTED,
+              "%s: %s must be 8-bit or FP4 codes (mxq_lay_codes widens the others)", who, what);
+  if (fmt == kFmtE2M1) {
+    MXQ_REQUIRE(aligned(codes, 32) && pitch % 32 == 0 && K % 128 == 0 && pitch * 2 >= K, MXQ_ERR_VALUE,
+                "%s: FP4 %s needs a 32-byte aligned base and pitch and K a multiple of 128", who, what);
+    *mma = tc::kE2M1;
+  } else {
+    MXQ_REQUIRE(aligned(codes, 16) && pitch % 16 == 0 && pitch >= K, MXQ_ERR_VALUE,
+                "%s: %s needs a 16-byte aligned base and pitch", who, what);
+    *mma = fmt == kFmtE4M3 ? tc::kE4M3 : tc::kE5M2;
+  }
+  return MXQ_OK;
+}
+
+int product(const char* who, Args& a, const Operand& x, const Operand& w, int64_t K, const mxq_product_spec* s, cudaStream_t st) {
+  int fx = 0, fw = 0;
+  const int fmtx = format_of(s->x_e, s->x_m), fmtw = format_of(s->w_e, s->w_m);
+  if (int rc = check_operand(who, "x", x.codes, x.pitch, fmtx, K, &fx)) return rc;
+  if (int rc = check_operand(who, "w", w.codes, w.pitch, fmtw, K, &fw)) return rc;
+  MXQ_REQUIRE(s->activation >= kActNone && s->activation <= kActGeglu, MXQ_ERR_VALUE, "%s: activation %d", who, s->activation);
+  MXQ_REQUIRE(s->out >= kOutF32 && s->out <= kOutPacked, MXQ_ERR_VALUE, "%s: output type %d", who, s->out);
+  const bool gated = s->activation >= kActSwiglu;
+  MXQ_REQUIRE(!gated || a.n % 2 == 0, MXQ_ERR_VALUE, "%s: a gated activation needs an even number of rows of w, got %d", who, a.n);
+  a.width = gated ? a.n / 2 : a.n;
+  a.act = s->activation;
+  a.otype = s->out;
+  a.ofmt = kFmtE4M3;
+  a.out_pitch = a.width;
+  a.out_nb = up_div(a.width, 32);
+  if (s->out == kOutPacked) {
+    a.ofmt = format_of(s->out_e, s->out_m);
+    MXQ_REQUIRE(a.ofmt != kFmtNone, MXQ_ERR_VALUE, "%s: (e=%d, m=%d) is not an MX element format", who, s->out_e, s->out_m);
+    MXQ_REQUIRE(a.out_scales != nullptr && a.residual == nullptr, MXQ_ERR_VALUE, "%s: a packed output needs scales and takes no residual", who);
+    if (a.ofmt == kFmtE2M1) {
+      MXQ_REQUIRE(a.width % 2 == 0, MXQ_ERR_VALUE, "%s: packed FP4 needs an even width, got %d", who, a.width);
+      a.out_pitch = a.width / 2;
+    }
+  }
+  const int size = s->out == kOutF32 ? 4 : s->out == kOutPacked ? 1 : 2;
+  a.vec_out = a.out_pitch * size % 16 == 0 && aligned(a.out, 16) &&
+              (a.residual == nullptr || (a.residual_stride * size % 16 == 0 && aligned(a.residual, 16)));
+  a.nb = (int)up_div(K, 32);
+  a.kblocks = (int)up_div(K, 128);
+  a.vec = a.nb % 16 == 0 && aligned(a.sx, 16) && aligned(a.sw, 16) ? 16 : a.nb % 4 == 0 && aligned(a.sx, 4) && aligned(a.sw, 4) ? 4 : 1;
+  a.xbytes = 128;
+  a.wbytes = 128;
+  if (a.rows == 0 || a.width == 0) return MXQ_OK;
+  a.status = wait_status_word();
+  if (!a.status) return MXQ_ERR_CUDA;
+  return gated ? launch<true>(a, x, w, K, fx, fw, st) : launch<false>(a, x, w, K, fx, fw, st);
+}
+
+int check_sizes(const char* who, int64_t rows, int64_t N, int64_t K, int64_t experts) {
+  MXQ_REQUIRE(rows >= 0 && rows < (1ll << 30) && N >= 0 && K >= 1 && K < (1ll << 30) && experts >= 1 && experts * N < (1ll << 30),
+              MXQ_ERR_VALUE, "%s: bad sizes (rows %lld, N %lld, K %lld, experts %lld)", who, (long long)rows, (long long)N,
+              (long long)K, (long long)experts);
+  return MXQ_OK;
+}
+
+}  // namespace
+
+namespace mxq {
+unsigned product_wait_timeouts() { return read_wait_timeouts(); }
+}  // namespace mxq
+
+extern "C" int mxq_linear_packed(const uint8_t* x, const uint8_t* x_scales, int64_t x_pitch, int64_t M, const uint8_t* w,
+                                 const uint8_t* w_scales, int64_t w_pitch, int64_t N, int64_t K, const mxq_product_spec* spec,
+                                 const float* bias, const void* residual, int64_t residual_stride, void* out,
+                                 uint8_t* out_scales, void* stream) {
+  MXQ_REQUIRE(spec != nullptr, MXQ_ERR_VALUE, "linear_packed: no spec");
+  if (int rc = check_sizes("linear_packed", M, N, K, 1)) return rc;
+  Args a = {};
+  a.sx = x_scales;
+  a.sw = w_scales;
+  a.rows = a.xrows = (int)M;
+  a.n = (int)N;
+  a.bias = bias;
+  a.residual = residual;
+  a.residual_stride = residual_stride;
+  a.out = out;
+  a.out_scales = out_scales;
+  return product("linear_packed", a, {x, M, x_pitch, spec->x_e + spec->x_m == 3}, {w, N, w_pitch, spec->w_e + spec->w_m == 3}, K,
+                 spec, as_stream(stream));
+}
+
+extern "C" int mxq_experts_packed(const uint8_t* x, const uint8_t* x_scales, int64_t x_pitch, int64_t x_rows, const uint8_t* w,
+                                  const uint8_t* w_scales, int64_t w_pitch, int64_t experts, int64_t N, int64_t K,
+                                  const int32_t* offsets, const int32_t* order, int64_t slots, int64_t per,
+                                  const mxq_product_spec* spec, const float* bias, void* out, uint8_t* out_scales,
+                                  void* stream) {
+  MXQ_REQUIRE(spec != nullptr, MXQ_ERR_VALUE, "experts_packed: no spec");
+  if (int rc = check_sizes("experts_packed", slots, N, K, experts)) return rc;
+  MXQ_REQUIRE(experts <= 1024, MXQ_ERR_UNSUPPORTED, "experts_packed: at most 1024 experts, got %lld", (long long)experts);
+  MXQ_REQUIRE(per >= 0 && (slots == 0 || (x_rows >= 1 && x_rows < (1ll << 30) && (per == 0 ? x_rows >= slots : x_rows * per >= slots))),
+              MXQ_ERR_VALUE, "experts_packed: %lld rows of x do not serve %lld slots, %lld per row", (long long)x_rows,
+              (long long)slots, (long long)per);
+  Args a = {};
+  a.sx = x_scales;
+  a.sw = w_scales;
+  a.offsets = offsets;
+  a.order = order;
+  a.experts = (int)experts;
+  a.per = (int)per;
+  a.rows = (int)slots;
+  a.xrows = (int)x_rows;
+  a.n = (int)N;
+  a.bias = bias;
+  a.out = out;
+  a.out_scales = out_scales;
+  return product("experts_packed", a, {x, x_rows, x_pitch, spec->x_e + spec->x_m == 3},
+                 {w, experts * N, w_pitch, spec->w_e + spec->w_m == 3}, K, spec, as_stream(stream));
+}

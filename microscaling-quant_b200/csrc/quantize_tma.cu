@@ -646,8 +646,11 @@ extern "C" int mxq_testing_wait_timeout(const float* V, float* P, float* X, int6
 
 // Number of bounded shared-memory waits that gave up in the staged kernels since the library was loaded on the
 // current device (0 in every correct run); synchronous.
+namespace mxq {
+unsigned product_wait_timeouts();                      // mx_product.cu's count
+}
 extern "C" int mxq_device_timeouts(uint32_t* out) {
   if (!out) return mxq::set_error(MXQ_ERR_VALUE, "device_timeouts: null output");
-  *out = mxq::read_wait_timeouts();
+  *out = mxq::read_wait_timeouts() + mxq::product_wait_timeouts();
   return MXQ_OK;
 }

@@ -1,0 +1,622 @@
+// Routing to experts and back: the router's choice and its gradient, the slots in the order of their experts, and the
+// weighted sum of the experts' rows with its gradients. All of it is bound by the bytes it reads and writes or, for a few
+// tokens, by latency; scores and sums are float32.
+#include <cuda_bf16.h>
+#include <cuda_fp16.h>
+
+#include <cooperative_groups.h>
+
+#include "common.cuh"
+
+namespace cg = cooperative_groups;
+using namespace mxq;
+
+namespace {
+
+constexpr unsigned kAll = 0xffffffffu;
+constexpr int kMostExperts = 1024, kMostChosen = 32;
+constexpr float kEps = 1e-20f;
+
+template <typename T>
+__device__ __forceinline__ float to_float(T v);
+template <>
+__device__ __forceinline__ float to_float<float>(float v) { return v; }
+template <>
+__device__ __forceinline__ float to_float<__nv_bfloat16>(__nv_bfloat16 v) { return __bfloat162float(v); }
+template <>
+__device__ __forceinline__ float to_float<__half>(__half v) { return __half2float(v); }
+template <typename T>
+__device__ __forceinline__ T from_float(float v);
+template <>
+__device__ __forceinline__ float from_float<float>(float v) { return v; }
+template <>
+__device__ __forceinline__ __nv_bfloat16 from_float<__nv_bfloat16>(float v) { return __float2bfloat16_rn(v); }
+template <>
+__device__ __forceinline__ __half from_float<__half>(float v) { return __float2half_rn(v); }
+
+__device__ __forceinline__ float warp_sum(float v) {
+#pragma unroll
+  for (int d = 16; d; d >>= 1) v = __fadd_rn(v, __shfl_xor_sync(kAll, v, d));
+  return v;
+}
+__device__ __forceinline__ float warp_max(float v) {
+#pragma unroll
+  for (int d = 16; d; d >>= 1) v = fmaxf(v, __shfl_xor_sync(kAll, v, d));
+  return v;
+}
+
+// An order-preserving key of a choice value; 0 (below every other) for -Inf and NaN, which are never chosen; -0 as +0.
+__device__ __forceinline__ uint32_t key_of(float f) {
+  const uint32_t b = __float_as_uint(__fadd_rn(f, 0.0f));
+  if ((b & 0x7fffffffu) > 0x7f800000u || b == 0xff800000u) return 0u;
+  return b & 0x80000000u ? ~b : b | 0x80000000u;
+}
+__device__ __forceinline__ float value_of(uint32_t key) {
+  return __uint_as_float(key & 0x80000000u ? key & 0x7fffffffu : ~key);
+}
+__device__ __forceinline__ float sigmoid(float x) { return __fdiv_rn(1.0f, __fadd_rn(1.0f, expf(-x))); }
+__device__ __forceinline__ bool is_nan(float x) { return x != x; }
+
+struct RouteArgs {
+  int64_t stride;
+  int T, E, k, sigmoid, groups, keep, top2, renormalize;
+  float scale;
+};
+
+// A warp per token, V values per lane (expert i * 32 + lane). The k largest are taken one after the other: the warp's
+// largest key by one reduction, the lowest expert that has it by another.
+template <typename IN, int V>
+__global__ void __launch_bounds__(128) k_route(const IN* __restrict__ logits, const float* __restrict__ bias,
+                                               float* __restrict__ weights, int* __restrict__ experts, RouteArgs a) {
+  const int lane = threadIdx.x & 31;
+  const int64_t t = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 5);
+  if (t >= a.T) return;
+  float l[V], s[V];
+  bool bad = false;
+#pragma unroll
+  for (int i = 0; i < V; i++) {
+    const int e = i * 32 + lane;
+    l[i] = e < a.E ? to_float<IN>(logits[t * a.stride + e]) : -INFINITY;
+    bad |= is_nan(l[i]);
+  }
+  bad = __any_sync(kAll, bad);
+  float top = -INFINITY, sum = 1.0f;
+  if (!a.sigmoid) {
+#pragma unroll
+    for (int i = 0; i < V; i++) top = fmaxf(top, l[i]);
+    top = warp_max(top);
+    sum = 0.0f;
+#pragma unroll
+    for (int i = 0; i < V; i++) {
+      s[i] = l[i] == -INFINITY || is_nan(l[i]) ? 0.0f : expf(__fsub_rn(l[i], top));
+      sum = __fadd_rn(sum, s[i]);
+    }
+    sum = warp_sum(sum);
+#pragma unroll
+    for (int i = 0; i < V; i++) s[i] = __fdiv_rn(s[i], sum);
+  } else {
+#pragma unroll
+    for (int i = 0; i < V; i++) s[i] = sigmoid(l[i]);
+  }
+  uint32_t key[V];
+#pragma unroll
+  for (int i = 0; i < V; i++) {
+    const int e = i * 32 + lane;
+    const bool live = key_of(l[i]) != 0u;
+    key[i] = !live ? 0u : key_of(bias ? __fadd_rn(s[i], bias[e]) : l[i]);
+  }
+  if (a.groups > 1) {
+    const int run = a.E / a.groups;
+    uint32_t mine = 0u;                                // lane g: the key of group g's value
+    for (int g = 0; g < a.groups; g++) {
+      uint32_t best = 0u;
+      int at = 0;
+#pragma unroll
+      for (int i = 0; i < V; i++) {
+        const int e = i * 32 + lane;
+        if (e >= g * run && e < (g + 1) * run && key[i] > best) {
+          best = key[i];
+          at = e;
+        }
+      }
+      const uint32_t m = __reduce_max_sync(kAll, best);
+      uint32_t v = m;
+      if (a.top2 && m) {
+        const int first = __reduce_min_sync(kAll, best == m ? at : INT_MAX);
+        uint32_t second = 0u;
+#pragma unroll
+        for (int i = 0; i < V; i++) {
+          const int e = i * 32 + lane;
+          if (e >= g * run && e < (g + 1) * run && e != first) second = max(second, key[i]);
+        }
+        second = __reduce_max_sync(kAll, second);
+        if (second) v = key_of(__fadd_rn(value_of(m), value_of(second)));
+      }
+      if (lane == g) mine = v;
+    }
+    unsigned kept = 0u;
+    for (int j = 0; j < a.keep; j++) {
+      const uint32_t m = __reduce_max_sync(kAll, mine);
+      if (!m) break;
+      const int g = __ffs(__ballot_sync(kAll, mine == m)) - 1;
+      kept |= 1u << g;
+      if (lane == g) mine = 0u;
+    }
+#pragma unroll
+    for (int i = 0; i < V; i++) {
+      const int e = i * 32 + lane;
+      if (e < a.E && !(kept >> (e / run) & 1u)) key[i] = 0u;
+    }
+  }
+  int chosen = -1;                                     // lane j: the j-th choice
+  float w = 0.0f;
+  for (int j = 0; j < a.k; j++) {
+    uint32_t best = 0u;
+    int at = INT_MAX;
+    float sc = 0.0f;
+#pragma unroll
+    for (int i = 0; i < V; i++)
+      if (key[i] > best) {
+        best = key[i];
+        at = i * 32 + lane;
+        sc = s[i];
+      }
+    const uint32_t m = __reduce_max_sync(kAll, best);
+    if (!m) break;
+    const int e = __reduce_min_sync(kAll, best == m ? at : INT_MAX);
+    sc = __shfl_sync(kAll, sc, e & 31);
+#pragma unroll
+    for (int i = 0; i < V; i++)
+      if (i * 32 + lane == e) key[i] = 0u;
+    if (lane == j) {
+      chosen = e;
+      w = sc;
+    }
+  }
+  if (a.renormalize) w = __fdiv_rn(w, __fadd_rn(warp_sum(w), kEps));
+  w = bad ? __uint_as_float(0x7fc00000u) : __fmul_rn(w, a.scale);
+  if (lane < a.k) {
+    weights[t * a.k + lane] = w;
+    experts[t * a.k + lane] = chosen;
+  }
+}
+
+// A warp per token. Lane j holds choice j: g = grad scale, ds = (g - sum g s / S) / S when renormalized; softmax:
+// dl = p (ds - sum ds p), ds 0 where not chosen; sigmoid: dl = ds s (1 - s) at the chosen.
+template <typename IN, int V>
+__global__ void __launch_bounds__(128) k_route_backward(const float* __restrict__ grad, const IN* __restrict__ logits,
+                                                        const int* __restrict__ experts, IN* __restrict__ out, RouteArgs a) {
+  const int lane = threadIdx.x & 31;
+  const int64_t t = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 5);
+  if (t >= a.T) return;
+  const int e = lane < a.k ? experts[t * a.k + lane] : -1;
+  const bool live = e >= 0 && e < a.E;
+  const float le = live ? to_float<IN>(logits[t * a.stride + e]) : 0.0f;
+  float l[V], top = -INFINITY, sum = 0.0f;
+  bool bad = false;
+#pragma unroll
+  for (int i = 0; i < V; i++) {
+    const int x = i * 32 + lane;
+    l[i] = x < a.E ? to_float<IN>(logits[t * a.stride + x]) : -INFINITY;
+    bad |= is_nan(l[i]);
+    top = fmaxf(top, l[i]);
+  }
+  bad = __any_sync(kAll, bad);
+  float s;
+  if (a.sigmoid) {
+    s = live ? sigmoid(le) : 0.0f;
+  } else {
+    top = warp_max(top);
+#pragma unroll
+    for (int i = 0; i < V; i++) {
+      l[i] = l[i] == -INFINITY ? 0.0f : expf(__fsub_rn(l[i], top));
+      sum = __fadd_rn(sum, l[i]);
+    }
+    sum = warp_sum(sum);
+    s = live ? __fdiv_rn(expf(__fsub_rn(le, top)), sum) : 0.0f;
+  }
+  float ds = live ? __fmul_rn(grad[t * a.k + lane], a.scale) : 0.0f;
+  if (a.renormalize) {
+    const float total = __fadd_rn(warp_sum(s), kEps), dot = warp_sum(__fmul_rn(ds, s));
+    ds = live ? __fdiv_rn(__fsub_rn(ds, __fdiv_rn(dot, total)), total) : 0.0f;
+  }
+  const float nan = __uint_as_float(0x7fc00000u);
+  IN* row = out + t * a.E;
+  float d;
+  if (a.sigmoid) {
+    d = __fmul_rn(__fmul_rn(ds, s), __fsub_rn(1.0f, s));
+#pragma unroll
+    for (int i = 0; i < V; i++) {
+      const int x = i * 32 + lane;
+      if (x < a.E) row[x] = from_float<IN>(bad ? nan : 0.0f);
+    }
+  } else {
+    const float dot = warp_sum(__fmul_rn(ds, s));
+    d = __fmul_rn(s, __fsub_rn(ds, dot));
+    const float f = sum > 0.0f ? __fdiv_rn(-dot, sum) : 0.0f;
+#pragma unroll
+    for (int i = 0; i < V; i++) {
+      const int x = i * 32 + lane;
+      if (x < a.E) row[x] = from_float<IN>(bad ? nan : __fmul_rn(l[i], f));
+    }
+  }
+  __syncwarp();                                        // the chosen experts' values over the others
+  if (live && !bad) row[e] = from_float<IN>(d);
+}
+
+// ----------------------------------------------------------------------------------------------- dispatch
+// A stable counting sort in one launch. The slots are cut into a contiguous run per warp; each warp counts its run by
+// expert in shared memory, the counts are added up over the warps, the cluster's CTAs and the experts, and each warp
+// then walks its run again, 32 slots at a time in order, giving each slot the next place of its expert.
+constexpr int kDispatchWarps = 32;
+
+__global__ void __launch_bounds__(kDispatchWarps * 32) k_dispatch(const int* __restrict__ ids, int64_t S, int E,
+                                                                  int* __restrict__ offsets, int* __restrict__ order,
+                                                                  int* __restrict__ where) {
+  extern __shared__ int sm[];
+  int* count = sm;                                     // [warp][E]: counts, then the next place of each expert
+  int* total = sm + kDispatchWarps * E;                // [E] this CTA's
+  int* sums = total + E;                               // [32] of the scan over experts
+  cg::cluster_group cluster = cg::this_cluster();
+  const int ctas = (int)cluster.num_blocks(), rank = (int)cluster.block_rank();
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  for (int i = threadIdx.x; i < kDispatchWarps * E; i += blockDim.x) count[i] = 0;
+  __syncthreads();
+  const int64_t runs = (int64_t)ctas * kDispatchWarps, run = ((S + runs - 1) / runs + 31) / 32 * 32;
+  const int64_t begin = min(S, (rank * (int64_t)kDispatchWarps + warp) * run), end = min(S, begin + run);
+  int* mine = count + warp * E;
+  for (int64_t i = begin + lane; i < end; i += 32) {
+    const int e = ids[i];
+    if (e >= 0 && e < E) atomicAdd(mine + e, 1);
+  }
+  __syncthreads();
+  const int e = threadIdx.x;                           // a thread per expert: E <= 1024
+  int own = 0;
+  if (e < E) {
+    for (int w = 0; w < kDispatchWarps; w++) {
+      const int c = count[w * E + e];
+      count[w * E + e] = own;
+      own += c;
+    }
+    total[e] = own;
+  }
+  cluster.sync();
+  int all = 0, before = 0;
+  if (e < E)
+    for (int c = 0; c < ctas; c++) {
+      const int v = cluster.map_shared_rank(total, c)[e];
+      if (c < rank) before += v;
+      all += v;
+    }
+  int scan = all;                                      // over the experts: warps, then the warps' sums
+#pragma unroll
+  for (int d = 1; d < 32; d <<= 1) {
+    const int up = __shfl_up_sync(kAll, scan, d);
+    if (lane >= d) scan += up;
+  }
+  if (lane == 31) sums[warp] = scan;
+  __syncthreads();
+  int head = 0, live = 0;
+  for (int w = 0; w < kDispatchWarps; w++) {
+    const int v = sums[w];
+    if (w < warp) head += v;
+    live += v;
+  }
+  const int first = head + scan - all;
+  if (e < E) {
+    if (rank == 0) offsets[e] = first;
+    for (int w = 0; w < kDispatchWarps; w++) count[w * E + e] += first + before;
+  }
+  if (rank == 0 && threadIdx.x == 0) offsets[E] = live;
+  for (int64_t i = live + rank * (int64_t)blockDim.x + threadIdx.x; i < S; i += (int64_t)ctas * blockDim.x) order[i] = -1;
+  __syncthreads();
+  for (int64_t b = begin; b < end; b += 32) {
+    const int64_t i = b + lane;
+    int x = i < end ? ids[i] : -1;
+    if (x < 0 || x >= E) x = -1;
+    const unsigned same = __match_any_sync(kAll, x);
+    const int place = x >= 0 ? mine[x] + __popc(same & ((1u << lane) - 1u)) : -1;
+    __syncwarp();
+    if (x >= 0 && lane == __ffs(same) - 1) mine[x] += __popc(same);
+    __syncwarp();
+    if (i < end) {
+      where[i] = place;
+      if (place >= 0) order[place] = (int)i;
+    }
+  }
+  cluster.sync();                                      // the totals are read before their CTA leaves
+}
+
+// ------------------------------------------------------------------------------------------------ combine
+template <typename T>
+struct Vec {                                           // 16 bytes of T
+  static constexpr int N = 16 / sizeof(T);
+  uint4 raw;
+  __device__ __forceinline__ void get(float (&v)[N]) const {
+    const T* p = reinterpret_cast<const T*>(&raw);
+#pragma unroll
+    for (int i = 0; i < N; i++) v[i] = to_float<T>(p[i]);
+  }
+  __device__ __forceinline__ void set(const float (&v)[N]) {
+    T* p = reinterpret_cast<T*>(&raw);
+#pragma unroll
+    for (int i = 0; i < N; i++) p[i] = from_float<T>(v[i]);
+  }
+};
+// N values at column c of a row: one 16-byte access, or (VEC false) those within the row one by one
+template <typename T, bool VEC>
+__device__ __forceinline__ Vec<T> load_vec(const T* row, int64_t c, int64_t n) {
+  Vec<T> v;
+  if (VEC) {
+    v.raw = __ldg(reinterpret_cast<const uint4*>(row + c));
+  } else {
+    T* p = reinterpret_cast<T*>(&v.raw);
+#pragma unroll
+    for (int i = 0; i < Vec<T>::N; i++) p[i] = c + i < n ? row[c + i] : from_float<T>(0.0f);
+  }
+  return v;
+}
+template <typename T, bool VEC>
+__device__ __forceinline__ void store_vec(T* row, int64_t c, int64_t n, const Vec<T>& v) {
+  if (VEC) {
+    *reinterpret_cast<uint4*>(row + c) = v.raw;
+  } else {
+    const T* p = reinterpret_cast<const T*>(&v.raw);
+#pragma unroll
+    for (int i = 0; i < Vec<T>::N; i++)
+      if (c + i < n) row[c + i] = p[i];
+  }
+}
+
+// A CTA per token and stretch of columns, 16 bytes of y per thread; four of the experts' rows are on their way at once.
+template <typename T, bool VEC>
+__global__ void __launch_bounds__(256) k_combine(const T* __restrict__ z, const float* __restrict__ weights,
+                                                 const int* __restrict__ where, const T* __restrict__ residual,
+                                                 int64_t residual_stride, T* __restrict__ y, int k, int64_t n, int64_t rows) {
+  constexpr int N = Vec<T>::N;
+  const int64_t t = blockIdx.x, c = ((int64_t)blockIdx.y * blockDim.x + threadIdx.x) * N;
+  if (c >= n) return;
+  float acc[N], v[N];
+#pragma unroll
+  for (int i = 0; i < N; i++) acc[i] = 0.0f;
+  for (int j0 = 0; j0 < k; j0 += 4) {
+    Vec<T> r[4];
+    float w[4];
+    int at[4];
+#pragma unroll
+    for (int j = 0; j < 4; j++) {
+      at[j] = -1;
+      w[j] = 0.0f;
+      if (j0 + j < k) {
+        at[j] = where[t * k + j0 + j];
+        w[j] = weights[t * k + j0 + j];
+      }
+      if (at[j] >= 0 && at[j] < rows) r[j] = load_vec<T, VEC>(z + at[j] * n, c, n);
+      else r[j].raw = make_uint4(0, 0, 0, 0);
+    }
+#pragma unroll
+    for (int j = 0; j < 4; j++) {
+      if (j0 + j >= k) break;
+      r[j].get(v);
+#pragma unroll
+      for (int i = 0; i < N; i++) acc[i] = __fmaf_rn(w[j], v[i], acc[i]);
+    }
+  }
+  if (residual) {
+    load_vec<T, VEC>(residual + t * residual_stride, c, n).get(v);
+#pragma unroll
+    for (int i = 0; i < N; i++) acc[i] = __fadd_rn(acc[i], v[i]);
+  }
+  Vec<T> o;
+  o.set(acc);
+  store_vec<T, VEC>(y + t * n, c, n, o);
+}
+
+// A CTA per token: dy's row is read once per eight experts' rows; a thread's share of the dot products stays in
+// registers and is added up over the CTA in a fixed order.
+template <typename T, bool VEC>
+__global__ void __launch_bounds__(256) k_combine_backward(const T* __restrict__ dy, int64_t dy_stride, const T* __restrict__ z,
+                                                          const float* __restrict__ weights, const int* __restrict__ where,
+                                                          const int* __restrict__ order, T* __restrict__ dz,
+                                                          float* __restrict__ dw, int k, int64_t n, int64_t rows) {
+  constexpr int N = Vec<T>::N, J = 8;
+  __shared__ float part[8][J];
+  const int64_t t = blockIdx.x;
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, warps = blockDim.x >> 5;
+  for (int j0 = 0; j0 < k; j0 += J) {
+    int64_t at[J];
+    float w[J], dot[J];
+#pragma unroll
+    for (int j = 0; j < J; j++) {
+      const bool in = j0 + j < k;
+      at[j] = in ? where[t * k + j0 + j] : -1;
+      if (at[j] >= rows) at[j] = -1;
+      w[j] = in ? weights[t * k + j0 + j] : 0.0f;
+      dot[j] = 0.0f;
+    }
+    for (int64_t c = threadIdx.x * N; c < n; c += blockDim.x * N) {
+      float g[N], v[N], o[N];
+      load_vec<T, VEC>(dy + t * dy_stride, c, n).get(g);
+      Vec<T> r[J];
+#pragma unroll
+      for (int j = 0; j < J; j++)
+        if (at[j] >= 0) r[j] = load_vec<T, VEC>(z + at[j] * n, c, n);
+#pragma unroll
+      for (int j = 0; j < J; j++)
+        if (at[j] >= 0) {
+          r[j].get(v);
+#pragma unroll
+          for (int i = 0; i < N; i++) {
+            dot[j] = __fmaf_rn(g[i], v[i], dot[j]);
+            o[i] = __fmul_rn(w[j], g[i]);
+          }
+          Vec<T> q;
+          q.set(o);
+          store_vec<T, VEC>(dz + at[j] * n, c, n, q);
+        }
+    }
+#pragma unroll
+    for (int j = 0; j < J; j++) {
+      const float d = warp_sum(dot[j]);
+      if (lane == 0) part[warp][j] = d;
+    }
+    __syncthreads();
+    if (threadIdx.x < J && j0 + threadIdx.x < k) {
+      float d = 0.0f;
+      for (int i = 0; i < warps; i++) d = __fadd_rn(d, part[i][threadIdx.x]);
+      dw[t * k + j0 + threadIdx.x] = d;
+    }
+    __syncthreads();
+  }
+  for (int j = 0; j < k; j++) {                        // the rows that no slot has
+    if (order[t * k + j] >= 0) continue;
+    Vec<T> zero;
+    zero.raw = make_uint4(0, 0, 0, 0);
+    for (int64_t c = threadIdx.x * N; c < n; c += blockDim.x * N) store_vec<T, VEC>(dz + (t * k + j) * n, c, n, zero);
+  }
+}
+
+// --------------------------------------------------------------------------------------------------- host
+bool aligned16(const void* p) { return reinterpret_cast<uintptr_t>(p) % 16 == 0; }
+
+int check_route(const char* who, int64_t T, int64_t E, int64_t k, const mxq_route_spec* s, RouteArgs& a) {
+  MXQ_REQUIRE(s != nullptr, MXQ_ERR_VALUE, "%s: no spec", who);
+  MXQ_REQUIRE(T >= 0 && T < (1ll << 30) && E >= 1 && E <= kMostExperts, MXQ_ERR_VALUE, "%s: %lld tokens, %lld experts (at most %d)",
+              who, (long long)T, (long long)E, kMostExperts);
+  MXQ_REQUIRE(k >= 1 && k <= E && k <= kMostChosen, MXQ_ERR_VALUE, "%s: k must be in [1, min(experts, %d)], got %lld", who, kMostChosen,
+              (long long)k);
+  MXQ_REQUIRE(s->score == MXQ_SCORE_SOFTMAX || s->score == MXQ_SCORE_SIGMOID, MXQ_ERR_VALUE, "%s: score %d", who, s->score);
+  MXQ_REQUIRE(s->groups >= 1 && s->groups <= 32 && E % s->groups == 0 && s->keep >= 1 && s->keep <= s->groups, MXQ_ERR_VALUE,
+              "%s: %d of %d groups of %lld experts", who, s->keep, s->groups, (long long)E);
+  a.T = (int)T;
+  a.E = (int)E;
+  a.k = (int)k;
+  a.sigmoid = s->score == MXQ_SCORE_SIGMOID;
+  a.groups = s->groups;
+  a.keep = s->keep;
+  a.top2 = s->top2;
+  a.renormalize = s->renormalize;
+  a.scale = s->scale;
+  return MXQ_OK;
+}
+
+template <typename F>
+int by_type(const char* who, int32_t type, F f) {
+  switch (type) {
+    case MXQ_OUT_F32: return f(float{});
+    case MXQ_OUT_BF16: return f(__nv_bfloat16{});
+    case MXQ_OUT_F16: return f(__half{});
+    default: return set_error(MXQ_ERR_VALUE, "%s: type %d", who, type);
+  }
+}
+template <int N>
+struct Int { static constexpr int value = N; };
+template <typename F>
+void by_width(int E, F f) {
+  if (E <= 32) f(Int<1>{});
+  else if (E <= 64) f(Int<2>{});
+  else if (E <= 128) f(Int<4>{});
+  else if (E <= 256) f(Int<8>{});
+  else if (E <= 512) f(Int<16>{});
+  else f(Int<32>{});
+}
+
+}  // namespace
+
+extern "C" int mxq_route(const void* logits, int32_t type, int64_t stride, const float* bias, float* weights, int32_t* experts,
+                         int64_t T, int64_t E, int64_t k, const mxq_route_spec* spec, void* stream) {
+  RouteArgs a;
+  if (int rc = check_route("route", T, E, k, spec, a)) return rc;
+  a.stride = stride;
+  if (T == 0) return MXQ_OK;
+  return by_type("route", type, [&](auto zero) {
+    using IN = decltype(zero);
+    by_width(a.E, [&](auto v) {
+      k_route<IN, decltype(v)::value><<<(unsigned)((T + 3) / 4), 128, 0, as_stream(stream)>>>(static_cast<const IN*>(logits), bias, weights,
+                                                                                          experts, a);
+    });
+    return MXQ_LAUNCH_CHECK("route");
+  });
+}
+
+extern "C" int mxq_route_backward(const float* grad, const void* logits, int32_t type, int64_t stride, const int32_t* experts,
+                                  void* grad_logits, int64_t T, int64_t E, int64_t k, const mxq_route_spec* spec, void* stream) {
+  RouteArgs a;
+  if (int rc = check_route("route_backward", T, E, k, spec, a)) return rc;
+  a.stride = stride;
+  if (T == 0) return MXQ_OK;
+  return by_type("route_backward", type, [&](auto zero) {
+    using IN = decltype(zero);
+    by_width(a.E, [&](auto v) {
+      k_route_backward<IN, decltype(v)::value><<<(unsigned)((T + 3) / 4), 128, 0, as_stream(stream)>>>(
+          grad, static_cast<const IN*>(logits), experts, static_cast<IN*>(grad_logits), a);
+    });
+    return MXQ_LAUNCH_CHECK("route_backward");
+  });
+}
+
+extern "C" int mxq_dispatch(const int32_t* experts_of, int64_t slots, int64_t experts, int32_t* offsets, int32_t* order,
+                            int32_t* where, void* stream) {
+  MXQ_REQUIRE(slots >= 0 && slots < (1ll << 30) && experts >= 1 && experts <= kMostExperts, MXQ_ERR_VALUE,
+              "dispatch: %lld slots, %lld experts (at most %d)", (long long)slots, (long long)experts, kMostExperts);
+  // a CTA walks 4096 slots in four steps per warp; a cluster (at most 8 CTAs) shares more
+  int ctas = 1;
+  while (ctas < 8 && slots > 4096ll * ctas) ctas *= 2;
+  const int smem = (int)((kDispatchWarps + 1) * experts + 32) * 4;
+  if (int rc = check_cuda(cudaFuncSetAttribute(k_dispatch, cudaFuncAttributeMaxDynamicSharedMemorySize, smem), "dispatch: shared memory"))
+    return rc;
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3(ctas);
+  cfg.blockDim = dim3(kDispatchWarps * 32);
+  cfg.dynamicSmemBytes = smem;
+  cfg.stream = as_stream(stream);
+  cudaLaunchAttribute at[1];
+  at[0].id = cudaLaunchAttributeClusterDimension;
+  at[0].val.clusterDim.x = ctas;
+  at[0].val.clusterDim.y = at[0].val.clusterDim.z = 1;
+  cfg.attrs = at;
+  cfg.numAttrs = 1;
+  return check_cuda(cudaLaunchKernelEx(&cfg, k_dispatch, experts_of, slots, (int)experts, offsets, order, where), "dispatch");
+}
+
+static int check_combine(const char* who, int64_t T, int64_t k, int64_t N) {
+  MXQ_REQUIRE(T >= 0 && k >= 1 && N >= 0 && T * k < (1ll << 31), MXQ_ERR_VALUE, "%s: T %lld, k %lld, N %lld", who, (long long)T, (long long)k,
+              (long long)N);
+  return MXQ_OK;
+}
+
+extern "C" int mxq_combine(const void* z, int32_t type, const float* weights, const int32_t* where, const void* residual,
+                           int64_t residual_stride, void* y, int64_t T, int64_t k, int64_t N, void* stream) {
+  if (int rc = check_combine("combine", T, k, N)) return rc;
+  if (T == 0 || N == 0) return MXQ_OK;
+  return by_type("combine", type, [&](auto zero) {
+    using X = decltype(zero);
+    constexpr int V = Vec<X>::N;
+    const bool vec = N % V == 0 && aligned16(z) && aligned16(y) && (!residual || (aligned16(residual) && residual_stride % V == 0));
+    const int64_t threads = (N + V - 1) / V;
+    const int block = threads >= 256 ? 256 : threads > 128 ? 256 : threads > 64 ? 128 : 64;
+    const dim3 grid((unsigned)T, (unsigned)((threads + block - 1) / block));
+    auto f = vec ? k_combine<X, true> : k_combine<X, false>;
+    f<<<grid, block, 0, as_stream(stream)>>>(static_cast<const X*>(z), weights, where, static_cast<const X*>(residual), residual_stride,
+                                             static_cast<X*>(y), (int)k, N, T * k);
+    return MXQ_LAUNCH_CHECK("combine");
+  });
+}
+
+extern "C" int mxq_combine_backward(const void* dy, int64_t dy_stride, const void* z, int32_t type, const float* weights,
+                                    const int32_t* where, const int32_t* order, void* dz, float* dw, int64_t T, int64_t k, int64_t N,
+                                    void* stream) {
+  if (int rc = check_combine("combine_backward", T, k, N)) return rc;
+  if (T == 0) return MXQ_OK;
+  return by_type("combine_backward", type, [&](auto zero) {
+    using X = decltype(zero);
+    constexpr int V = Vec<X>::N;
+    const bool vec = N % V == 0 && aligned16(z) && aligned16(dz) && aligned16(dy) && dy_stride % V == 0;
+    const int64_t threads = (N + V - 1) / V;
+    const int block = threads > 128 ? 256 : threads > 64 ? 128 : 64;
+    auto f = vec ? k_combine_backward<X, true> : k_combine_backward<X, false>;
+    f<<<(unsigned)T, block, 0, as_stream(stream)>>>(static_cast<const X*>(dy), dy_stride, static_cast<const X*>(z), weights, where, order,
+                                                    static_cast<X*>(dz), dw, (int)k, N, T * k);
+    return MXQ_LAUNCH_CHECK("combine_backward");
+  });
+}

@@ -1,0 +1,135 @@
+// Fifth-generation tensor core plumbing for sm_100a: TMEM allocation and reads, the block-scaled matrix product
+// (tcgen05.mma kind::mxf8f6f4), the copies of its scales into TMEM, and waits that end.
+//
+// Every wait is bounded in time and also ends when another role of the CTA has given up: the first wait
+// that runs out raises the CTA's `abort` word in shared memory, every later wait returns false at once, and the roles
+// leave their loops together.
+#pragma once
+#include <cuda_bf16.h>
+#include <cuda_fp16.h>
+
+#include "tma.cuh"
+
+namespace mxq {
+namespace tc {
+
+// how long a wait may take: a correct one takes microseconds
+constexpr unsigned long long kWaitNs = 2000000000ull;
+
+__device__ __forceinline__ unsigned long long now_ns() {
+  unsigned long long t;
+  asm volatile("mov.u64 %0, %globaltimer;\n" : "=l"(t));
+  return t;
+}
+
+// false: gave up (this wait ran out, or another role's did)
+__device__ __forceinline__ bool wait(uint64_t* bar, unsigned parity, volatile int* abort, unsigned* status_word) {
+  if (mbar_try_wait_rounds(bar, parity, 4)) return true;
+  const unsigned long long begin = now_ns();
+  do {
+    if (mbar_try_wait_rounds(bar, parity, 4)) return true;
+    if (*abort) return false;
+  } while (now_ns() - begin < kWaitNs);
+  *abort = 1;
+  note_wait_timeout(status_word);
+  return false;
+}
+// the same for what a role that gave up has in flight towards shared memory or TMEM, without the abort word
+__device__ __forceinline__ void settle(uint64_t* bar, unsigned parity) {
+  const unsigned long long begin = now_ns();
+  while (!mbar_try_wait_rounds(bar, parity, 4) && now_ns() - begin < kWaitNs / 20) {
+  }
+}
+
+__device__ __forceinline__ void mbar_arrive(uint64_t* bar) {
+  asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];\n" ::"r"(smem_addr(bar)) : "memory");
+}
+
+__device__ __forceinline__ void fence_before() { asm volatile("tcgen05.fence::before_thread_sync;\n" ::: "memory"); }
+__device__ __forceinline__ void fence_after() { asm volatile("tcgen05.fence::after_thread_sync;\n" ::: "memory"); }
+
+// one whole warp; the address lands in shared memory
+__device__ __forceinline__ void tmem_alloc(uint32_t* where, uint32_t cols) {
+  asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;\n" ::"r"(smem_addr(where)), "r"(cols)
+               : "memory");
+  asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;\n");
+}
+__device__ __forceinline__ void tmem_free(uint32_t addr, uint32_t cols) {
+  asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;\n" ::"r"(addr), "r"(cols));
+}
+
+// K-major operand tile, rows of 128 bytes in the 128-byte swizzle: groups of 8 rows 1024 bytes apart
+__device__ __forceinline__ uint64_t operand_desc(uint32_t addr) {
+  return (uint64_t)((addr & 0x3ffffu) >> 4) | (1ull << 16) | (64ull << 32) | (1ull << 46) | (2ull << 61);
+}
+// 32 rows of 16 bytes, no swizzle: groups of 8 rows 128 bytes apart
+__device__ __forceinline__ uint64_t scale_desc(uint32_t addr) {
+  return (uint64_t)((addr & 0x3ffffu) >> 4) | (8ull << 32) | (1ull << 46);
+}
+
+// instruction descriptor of kind::mxf8f6f4 (K-major A and B, E8M0 scales): operand formats as mma_format() gives
+// them, tile m x n, the byte of each scale word that this K step of 32 reads
+enum { kE4M3 = 0, kE5M2 = 1, kE2M1 = 5 };
+__host__ __device__ constexpr uint32_t mma_desc(int fa, int fb, int m, int n) {
+  return ((uint32_t)fa << 7) | ((uint32_t)fb << 10) | ((uint32_t)(n >> 3) << 17) | (1u << 23) | ((uint32_t)(m >> 4) << 24);
+}
+__device__ __forceinline__ uint32_t mma_desc_step(uint32_t d, uint32_t byte) { return d | (byte << 4) | (byte << 29); }
+
+// 128 rows' scale words (4 E8M0 bytes each, shared memory (row % 32) * 16 + (row / 32) * 4) into 4 TMEM columns
+__device__ __forceinline__ void copy_scales(uint32_t tmem, uint64_t desc) {
+  asm volatile("tcgen05.cp.cta_group::1.32x128b.warpx4 [%0], %1;\n" ::"r"(tmem), "l"(desc) : "memory");
+}
+
+__device__ __forceinline__ void mma(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, uint32_t sa, uint32_t sb,
+                                    bool accumulate) {
+  asm volatile(
+      "{\n .reg .pred p;\n setp.ne.b32 p, %6, 0;\n"
+      " tcgen05.mma.cta_group::1.kind::mxf8f6f4.block_scale.scale_vec::1X [%0], %1, %2, %3, [%4], [%5], p;\n}\n" ::"r"(d),
+      "l"(a), "l"(b), "r"(idesc), "r"(sa), "r"(sb), "r"((unsigned)accumulate)
+      : "memory");
+}
+// the barrier arrives when every tcgen05 operation that this thread has issued is done
+__device__ __forceinline__ void commit(uint64_t* bar) {
+  asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];\n" ::"r"(smem_addr(bar))
+               : "memory");
+}
+
+// 32 columns of this warp's 32 lanes (the lane quarter warp % 4), one row per thread; the wait stands in the same
+// statement, so that nothing that uses the values can be moved above it
+__device__ __forceinline__ void load32(uint32_t addr, float (&v)[32]) {
+  uint32_t r[32];
+  asm volatile(
+      "tcgen05.ld.sync.aligned.32x32b.x32.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16,%17,%18,%19,"
+      "%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31}, [%32];\n tcgen05.wait::ld.sync.aligned;\n"
+      : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]),
+        "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15]), "=r"(r[16]),
+        "=r"(r[17]), "=r"(r[18]), "=r"(r[19]), "=r"(r[20]), "=r"(r[21]), "=r"(r[22]), "=r"(r[23]), "=r"(r[24]),
+        "=r"(r[25]), "=r"(r[26]), "=r"(r[27]), "=r"(r[28]), "=r"(r[29]), "=r"(r[30]), "=r"(r[31])
+      : "r"(addr)
+      : "memory");
+#pragma unroll
+  for (int i = 0; i < 32; i++) v[i] = __uint_as_float(r[i]);
+}
+__device__ __forceinline__ void load16(uint32_t addr, float (&v)[16]) {
+  uint32_t r[16];
+  asm volatile(
+      "tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15}, [%16];\n"
+      " tcgen05.wait::ld.sync.aligned;\n"
+      : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]),
+        "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15])
+      : "r"(addr)
+      : "memory");
+#pragma unroll
+  for (int i = 0; i < 16; i++) v[i] = __uint_as_float(r[i]);
+}
+// four rows of a tensor, 128 bytes each, one after the other in shared memory
+__device__ __forceinline__ void tma_gather4(void* dst, const CUtensorMap* map, int x, int4 rows, uint64_t* bar) {
+  asm volatile(
+      "cp.async.bulk.tensor.2d.shared::cta.global.tile::gather4.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4, %5, "
+      "%6}], [%7];\n" ::"r"(smem_addr(dst)),
+      "l"(map), "r"(x), "r"(rows.x), "r"(rows.y), "r"(rows.z), "r"(rows.w), "r"(smem_addr(bar))
+      : "memory");
+}
+
+}  // namespace tc
+}  // namespace mxq

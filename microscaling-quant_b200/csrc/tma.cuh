@@ -19,6 +19,13 @@ namespace mxq {
 int encode_tmap_f32(CUtensorMap* map, const void* base, int rank, const uint64_t* dims, const uint64_t* strides,
                     const uint32_t* box);
 
+// A map of a matrix of 8-bit codes (or FP4 codes, two per byte, spread to a code per byte place in shared memory: 8
+// bytes of codes and 8 of padding per 16 codes) in tiles of 128 codes x box_rows rows, in the 128-byte swizzle;
+// `pitch` bytes from row to row. Codes: base and pitch multiples of 16 bytes. FP4: base and pitch multiples of 32 bytes,
+// cols a multiple of 128.
+int encode_tmap_codes(CUtensorMap* map, const void* base, bool nibbles, uint64_t rows, uint64_t cols, uint64_t pitch,
+                      uint32_t box_rows);
+
 // The wait-status word: one 32-bit counter in pinned, mapped, portable host memory, allocated on first use (any
 // device; the same address serves every device), which a kernel whose bounded wait gave up increments with a
 // system-scope atomic. The host reads it with a plain load, so a caller can check it on every call without

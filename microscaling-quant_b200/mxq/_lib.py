@@ -43,6 +43,15 @@ class MxqAnchorSpec(ctypes.Structure):
                 ("emin", I32)]
 
 
+class MxqProductSpec(ctypes.Structure):
+    _fields_ = [("x_e", I32), ("x_m", I32), ("w_e", I32), ("w_m", I32), ("activation", I32), ("out", I32),
+                ("out_e", I32), ("out_m", I32)]
+
+
+class MxqRouteSpec(ctypes.Structure):
+    _fields_ = [("score", I32), ("groups", I32), ("keep", I32), ("top2", I32), ("renormalize", I32), ("scale", F32)]
+
+
 # entry point -> argument types (the return type of every entry point is int32 status)
 _SIGS = {
     "mxq_round_bits": [P, P, I32, P, I64, I32, P],
@@ -88,6 +97,16 @@ _SIGS = {
     "mxq_lut_decode": [P, P, I64, I32, I32, P, P],
     "mxq_lut_finder": [P, P, P, I64, I64, I32, I32, I32, P, P],
     "mxq_lut_format_tables": [I32, I32, P, P, P, P],
+    "mxq_linear_packed": [P, P, I64, I64, P, P, I64, I64, I64, ctypes.POINTER(MxqProductSpec), P, P, I64, P, P, P],
+    "mxq_experts_packed": [P, P, I64, I64, P, P, I64, I64, I64, I64, P, P, I64, I64, ctypes.POINTER(MxqProductSpec), P, P,
+                           P, P],
+    "mxq_lay_codes": [P, I64, P, I64, I64, I64, I32, I32, P],
+    "mxq_pack_rows": [P, I32, I64, P, I64, P, I64, I64, I32, I32, P],
+    "mxq_route": [P, I32, I64, P, P, P, I64, I64, I64, ctypes.POINTER(MxqRouteSpec), P],
+    "mxq_route_backward": [P, P, I32, I64, P, P, I64, I64, I64, ctypes.POINTER(MxqRouteSpec), P],
+    "mxq_dispatch": [P, I64, I64, P, P, P, P],
+    "mxq_combine": [P, I32, P, P, P, I64, P, I64, I64, I64, P],
+    "mxq_combine_backward": [P, I64, P, I32, P, P, P, P, P, I64, I64, I64, P],
     "mxq_device_timeouts": [P],
     "mxq_wait_status_word": [P],
     "mxq_testing_wait_timeout": [P, P, P, I64, I64, ctypes.c_uint32, P],

@@ -1,0 +1,273 @@
+"""Products of packed MX operands on the tensor cores, dense and by expert (no reference counterpart). Inference only.
+
+    y = linear_packed(x, w, "MXFP8_E4M3", bias=b, activation="silu", residual=r)       ... x K, N x K -> ... x F
+    z = experts_packed(x, w, "MXFP8_E4M3", plan, activation="swiglu", out="MXFP8_E4M3")
+
+An operand is a pair (codes, scales) as block.ocp.quantize_packed(V, fmt, axis=-1) gives it: uint8 codes (FP4 two per
+byte) and one E8M0 byte per 32 values of the last dimension. x may also be a float tensor: its rows are then packed to
+`x_fmt` within the call, by the rule of a packed output.
+
+    acc = sum_k x[.., k] w[n, k]            the values the codes stand for; products exact, sums float32
+    y   = act(acc + bias) [* up] + residual
+
+Activations: None, "relu", "gelu" (erf), "gelu_tanh", "silu", and the gated "swiglu" / "geglu", whose first N / 2 rows of
+w are the gate's and the others the up projection's (F = N / 2; else F = N). `out` is a float dtype or a format name; a
+packed output is a pair again: the scale 2^(floor(log2 amax) - emax) per 32 columns, codes rounded to nearest even and
+saturated, the scale of a block that holds an Inf or a NaN 0xFF (NaN).
+
+8-bit codes whose rows are multiples of 16 bytes, and FP4 codes with K a multiple of 128, are read as they are. Other
+codes (FP6, ragged or unaligned rows) are laid out as 8-bit codes first, in every call; `lay_packed` does it once for
+weights that are kept.
+"""
+from typing import NamedTuple, Optional, Tuple, Union
+
+import ctypes
+
+import torch
+
+from .. import _lib
+from ..block import BLOCK
+from ..element_quant.formats import Format, get
+
+__all__ = ["ACTIVATIONS", "Dispatch", "linear_packed", "experts_packed", "lay_packed"]
+
+ACTIVATIONS = (None, "relu", "gelu", "gelu_tanh", "silu", "swiglu", "geglu")
+GATED = ("swiglu", "geglu")
+FLOATS = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}
+PACKED = 3
+
+Pair = Tuple[torch.Tensor, torch.Tensor]
+
+
+class Dispatch(NamedTuple):
+    """The slots (token-major, T x k flattened) in the order of their experts, as nn.dispatch makes it (int32)."""
+    offsets: torch.Tensor   # (experts + 1): where each expert's places begin
+    order: torch.Tensor     # (slots): the slot at each place, -1 at the places beyond offsets[-1]
+    where: torch.Tensor     # (T, k): the place of each slot, -1 for a slot left out
+
+
+class _Operand(NamedTuple):
+    codes: torch.Tensor
+    scales: torch.Tensor
+    pitch: int              # bytes from row to row
+    e: int
+    m: int
+
+
+def _format(fmt, who: str) -> Format:
+    f = get(fmt)
+    if f is None:
+        raise ValueError(f"{who}: {fmt!r} is not an MX element format")
+    return f
+
+
+def _pair(v, f: Format, who: str, what: str):
+    """The checked (codes, scales) of an operand and its K."""
+    if not (isinstance(v, (tuple, list)) and len(v) == 2 and all(isinstance(t, torch.Tensor) for t in v)):
+        raise ValueError(f"{who}: {what} must be a pair (codes, scales) of uint8 tensors")
+    codes, scales = v
+    if codes.dtype != torch.uint8 or scales.dtype != torch.uint8 or codes.ndim < 1:
+        raise ValueError(f"{who}: {what} must be uint8 codes and scales, got {codes.dtype} and {scales.dtype}")
+    K = codes.shape[-1] * (2 if f.e + f.m == 3 else 1)
+    if K == 0:
+        raise ValueError(f"{who}: {what} has no values along its last dimension")
+    want = (*codes.shape[:-1], -(-K // BLOCK))
+    if tuple(scales.shape) != want:
+        raise ValueError(f"{who}: scales of {what} must have shape {want} for {f.name} codes {tuple(codes.shape)}, "
+                         f"got {tuple(scales.shape)}")
+    return codes, scales, K
+
+
+def _laid(codes: torch.Tensor, scales: torch.Tensor, f: Format, K: int, dev) -> _Operand:
+    """The operand as the kernels read it: as it is where its rows allow it, else laid out as 8-bit codes."""
+    codes, scales = codes.to(dev).contiguous(), scales.to(dev).contiguous()
+    bits = 1 + f.e + f.m
+    at = codes.data_ptr()
+    if bits == 8 and K % 16 == 0 and at % 16 == 0:
+        return _Operand(codes, scales, K, f.e, f.m)
+    if bits == 4 and K % 128 == 0 and at % 32 == 0:
+        return _Operand(codes, scales, K // 2, f.e, f.m)
+    rows = codes.numel() // codes.shape[-1]
+    pitch = -(-K // 16) * 16
+    wide = torch.empty((*codes.shape[:-1], pitch), dtype=torch.uint8, device=dev)
+    _lib.run("mxq_lay_codes", dev, _lib.ptr(codes), codes.shape[-1], _lib.ptr(wide), pitch, rows, K, f.e, f.m)
+    return _Operand(wide, scales, pitch, *((f.e, f.m) if bits == 8 else (4, 3)))
+
+
+def lay_packed(w: Pair, fmt: Union[str, Format]) -> Tuple[Pair, str]:
+    """(w, fmt) such that the products read w as it is, once for weights that are kept: FP6 codes, and FP4 codes with K
+    no multiple of 128, become the E4M3 codes of the same values. Rows of 8-bit codes that are no multiple of 16 bytes
+    cannot be kept so (the pair has no room between its rows) and come back unchanged."""
+    f = _format(fmt, "lay_packed")
+    codes, scales, K = _pair(w, f, "lay_packed", "w")
+    bits = 1 + f.e + f.m
+    if bits == 8 or K % 16 or (bits == 4 and K % 128 == 0):
+        return (codes, scales), f.name
+    dev = _lib.device_for(codes)
+    o = _laid(codes, scales, f, K, dev)
+    return (_lib.back(o.codes, codes.device), scales), "MXFP8_E4M3"
+
+
+def _x_operand(x, x_fmt, who: str, dev_of):
+    """(operand, leading shape, K, home) of x, a pair or a float tensor that is packed here."""
+    f = _format(x_fmt, who)
+    if isinstance(x, torch.Tensor):
+        if x.dtype not in FLOATS or x.ndim < 1:
+            raise ValueError(f"{who}: x must be a float32, bfloat16 or float16 tensor or a pair (codes, scales), got "
+                             f"{x.dtype}")
+        K = x.shape[-1]
+        if K == 0:
+            raise ValueError(f"{who}: x has no values along its last dimension")
+        dev = _lib.device_for(x, *dev_of)
+        v = x.detach().to(dev)
+        if v.ndim != 2:
+            v = v.reshape(-1, K)
+        if v.stride(1) != 1 or (v.shape[0] > 1 and v.stride(0) < K):
+            v = v.contiguous()
+        rows, pitch = v.shape[0], -(-K // 16) * 16
+        codes = torch.empty((rows, pitch), dtype=torch.uint8, device=dev)
+        scales = torch.empty((rows, -(-K // BLOCK)), dtype=torch.uint8, device=dev)
+        _lib.run("mxq_pack_rows", dev, _lib.ptr(v), FLOATS[v.dtype], v.stride(0) if rows > 1 else K, _lib.ptr(codes), pitch,
+                 _lib.ptr(scales), rows, K, f.e, f.m)
+        o = _Operand(codes, scales, pitch, *((f.e, f.m) if f.e + f.m == 7 else (4, 3)))
+        return o, x.shape[:-1], K, dev, x.device
+    codes, scales, K = _pair(x, f, who, "x")
+    dev = _lib.device_for(codes, *dev_of)
+    return _laid(codes, scales, f, K, dev), codes.shape[:-1], K, dev, codes.device
+
+
+def _make_spec(x_e, x_m, w_e, w_m, act, out, out_e, out_m):
+    return _lib.MxqProductSpec(x_e, x_m, w_e, w_m, act, out, out_e, out_m)
+
+
+_spec = _lib.cached(_make_spec)
+
+
+def _plan_output(out, activation, N: int, who: str):
+    """(activation code, output code, output Format or None, F)."""
+    if not (activation is None or isinstance(activation, str)) or activation not in ACTIVATIONS:
+        raise ValueError(f"{who}: activation must be one of {ACTIVATIONS}, got {activation!r}")
+    F = N
+    if activation in GATED:
+        if N % 2:
+            raise ValueError(f"{who}: {activation} needs an even number of rows of w, got {N}")
+        F = N // 2
+    if isinstance(out, torch.dtype):
+        if out not in FLOATS:
+            raise ValueError(f"{who}: out must be float32, bfloat16, float16 or an MX format, got {out}")
+        return ACTIVATIONS.index(activation), FLOATS[out], None, F
+    f = _format(out, who)
+    if f.e + f.m == 3 and F % 2:
+        raise ValueError(f"{who}: packed FP4 pairs up along the output, whose width is {F}")
+    return ACTIVATIONS.index(activation), PACKED, f, F
+
+
+def _outputs(lead, out, f, F: int, dev):
+    """The empty output: (tensor for the codes or values, scales or None)."""
+    if f is None:
+        return torch.empty((*lead, F), dtype=out, device=dev), None
+    return (torch.empty((*lead, F // 2 if f.e + f.m == 3 else F), dtype=torch.uint8, device=dev),
+            torch.empty((*lead, -(-F // BLOCK)), dtype=torch.uint8, device=dev))
+
+
+def _given(y, scales, home):
+    return _lib.back(y, home) if scales is None else (_lib.back(y, home), _lib.back(scales, home))
+
+
+def _product_ready():
+    if _lib._wait_word is None:                             # the kernel's wait-status word, checked by every call
+        _lib.wait_word()
+
+
+def linear_packed(x: Union[Pair, torch.Tensor], w: Pair, fmt: Union[str, Format], x_fmt: Union[str, Format] = "MXFP8_E4M3",
+                  bias: Optional[torch.Tensor] = None, activation: Optional[str] = None,
+                  residual: Optional[torch.Tensor] = None, out: Union[torch.dtype, str] = torch.bfloat16):
+    """y = act(x wᵀ + bias) [* up] + residual. x: (... x K) packed to x_fmt (a pair) or floats; w: an N x K pair of
+    `fmt`; bias: N values; residual: y's shape and dtype. Returns y (... x F) of dtype `out`, or its (codes, scales)."""
+    who = "linear_packed"
+    fw = _format(fmt, who)
+    wc, ws, K = _pair(w, fw, who, "w")
+    if wc.ndim != 2:
+        raise ValueError(f"{who}: w must be 2-D (N x K), got codes {tuple(wc.shape)}")
+    N = wc.shape[0]
+    act, otype, fo, F = _plan_output(out, activation, N, who)
+    if bias is not None and tuple(bias.shape) != (N,):
+        raise ValueError(f"{who}: bias must have shape {(N,)}, got {tuple(bias.shape)}")
+    _product_ready()
+    xo, lead, Kx, dev, home = _x_operand(x, x_fmt, who, (wc,))
+    if Kx != K:
+        raise ValueError(f"{who}: x has {Kx} values per row and w {K}")
+    M = xo.scales.numel() // xo.scales.shape[-1]
+    y, ys = _outputs(lead, out, fo, F, dev)
+    r, r_stride = None, 0
+    if residual is not None:
+        if fo is not None:
+            raise ValueError(f"{who}: a packed output takes no residual")
+        if residual.shape != y.shape or residual.dtype != out:
+            raise ValueError(f"{who}: residual must be {out} of shape {tuple(y.shape)}, got {residual.dtype} "
+                             f"{tuple(residual.shape)}")
+        r = residual.detach().to(dev).reshape(M, F)
+        if r.numel() and r.stride(1) != 1:
+            r = r.contiguous()
+        r_stride = r.stride(0) if M > 1 else F
+    if M == 0 or N == 0:
+        return _given(y, ys, home)
+    b = None if bias is None else _lib.on(bias, dev)
+    wo = _laid(wc, ws, fw, K, dev)
+    _lib.run("mxq_linear_packed", dev, _lib.ptr(xo.codes), _lib.ptr(xo.scales), xo.pitch, M, _lib.ptr(wo.codes),
+             _lib.ptr(wo.scales), wo.pitch, N, K,
+             ctypes.byref(_spec(xo.e, xo.m, wo.e, wo.m, act, otype, fo.e if fo else 0, fo.m if fo else 0)), _lib.ptr(b),
+             _lib.ptr(r), r_stride, _lib.ptr(y), _lib.ptr(ys))
+    return _given(y, ys, home)
+
+
+def _index(t: torch.Tensor, dev, who: str, what: str) -> torch.Tensor:
+    if not isinstance(t, torch.Tensor) or t.dtype != torch.int32:
+        raise ValueError(f"{who}: {what} must be an int32 tensor, got {getattr(t, 'dtype', type(t))}")
+    return t.to(dev).contiguous()
+
+
+def experts_packed(x: Union[Pair, torch.Tensor], w: Pair, fmt: Union[str, Format], plan: Dispatch, gather: bool = True,
+                   x_fmt: Union[str, Format] = "MXFP8_E4M3", bias: Optional[torch.Tensor] = None,
+                   activation: Optional[str] = None, out: Union[torch.dtype, str] = torch.bfloat16):
+    """linear_packed by expert: row r of the result belongs to the slot plan.order[r] and is multiplied with its expert's
+    weights. w: an E x N x K pair; bias: E x N. x: T x K, a row per token, read through the plan (gather), or
+    slots x K in the plan's order (not gather). Returns slots x F in the plan's order; the rows of places without a slot
+    (from offsets[-1] on) are not written."""
+    who = "experts_packed"
+    fw = _format(fmt, who)
+    wc, ws, K = _pair(w, fw, who, "w")
+    if wc.ndim != 3:
+        raise ValueError(f"{who}: w must be 3-D (experts x N x K), got codes {tuple(wc.shape)}")
+    E, N = wc.shape[0], wc.shape[1]
+    act, otype, fo, F = _plan_output(out, activation, N, who)
+    if plan.offsets.numel() != E + 1:
+        raise ValueError(f"{who}: the plan has {plan.offsets.numel() - 1} experts and w {E}")
+    if bias is not None and tuple(bias.shape) != (E, N):
+        raise ValueError(f"{who}: bias must have shape {(E, N)}, got {tuple(bias.shape)}")
+    _product_ready()
+    xo, lead, Kx, dev, home = _x_operand(x, x_fmt, who, (wc,))
+    if Kx != K:
+        raise ValueError(f"{who}: x has {Kx} values per row and w {K}")
+    if len(lead) != 1:
+        raise ValueError(f"{who}: x must be 2-D, got leading shape {tuple(lead)}")
+    slots, rows = plan.order.numel(), lead[0]
+    if gather:
+        if (slots == 0) != (rows == 0) or (rows and slots % rows):
+            raise ValueError(f"{who}: {slots} slots are no multiple of x's {rows} rows")
+        per = slots // rows if rows else 1
+    else:
+        if rows != slots:
+            raise ValueError(f"{who}: x has {rows} rows and the plan {slots} slots")
+        per = 0
+    y, ys = _outputs((slots,), out, fo, F, dev)
+    if slots == 0 or N == 0 or E == 0:
+        return _given(y, ys, home)
+    offsets, order = _index(plan.offsets, dev, who, "offsets"), _index(plan.order, dev, who, "order")
+    b = None if bias is None else _lib.on(bias, dev)
+    wo = _laid(wc, ws, fw, K, dev)
+    _lib.run("mxq_experts_packed", dev, _lib.ptr(xo.codes), _lib.ptr(xo.scales), xo.pitch, rows, _lib.ptr(wo.codes),
+             _lib.ptr(wo.scales), wo.pitch, E, N, K, _lib.ptr(offsets), _lib.ptr(order), slots, per,
+             ctypes.byref(_spec(xo.e, xo.m, wo.e, wo.m, act, otype, fo.e if fo else 0, fo.m if fo else 0)), _lib.ptr(b),
+             _lib.ptr(y), _lib.ptr(ys))
+    return _given(y, ys, home)
