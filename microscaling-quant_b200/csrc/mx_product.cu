@@ -866,8 +866,9 @@ int product(const char* who, Args& a, const Operand& x, const Operand& w, int64_
   a.nb = (int)up_div(K, 32);
   a.kblocks = (int)up_div(K, 128);
   a.vec = a.nb % 16 == 0 && aligned(a.sx, 16) && aligned(a.sw, 16) ? 16 : a.nb % 4 == 0 && aligned(a.sx, 4) && aligned(a.sw, 4) ? 4 : 1;
-  a.xbytes = 128;
-  a.wbytes = 128;
+  // a load of FP4 codes counts the bytes read, half of those that it fills
+  a.xbytes = fmtx == kFmtE2M1 ? 64 : 128;
+  a.wbytes = fmtw == kFmtE2M1 ? 64 : 128;
   if (a.rows == 0 || a.width == 0) return MXQ_OK;
   a.status = wait_status_word();
   if (!a.status) return MXQ_ERR_CUDA;
