@@ -16,6 +16,8 @@
 
 #include <cooperative_groups.h>
 
+#include <mutex>
+
 namespace cg = cooperative_groups;
 using namespace mxq;
 
@@ -98,6 +100,7 @@ __device__ __forceinline__ void activate(int act, float (&v)[N]) {
 }
 
 // ------------------------------------------------------------------------------------------ operand staging
+constexpr int kMostExperts = 1024;
 constexpr int kTileBytes = 128 * 128;                 // 128 rows of one K step
 
 // 16 scale bytes of a row from K step 4g on (a step has 4): 0 beyond the row
@@ -743,8 +746,23 @@ __global__ void __launch_bounds__(128, 2) k_mx_rows(const __grid_constant__ CUte
 }
 
 // --------------------------------------------------------------------------------------------------- host
-int set_smem(const void* f, int bytes) {
-  return check_cuda(cudaFuncSetAttribute(f, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes), "product: shared memory");
+// The kernel's largest shared memory, set once per kernel and context (a device, or a device after its reset)
+template <typename F>
+int set_smem(F f, int bytes) {
+  static std::mutex mu;
+  static F known[16];
+  static unsigned long long in[16];
+  const unsigned long long ctx = context_id();
+  std::lock_guard<std::mutex> lock(mu);
+  int i = 0;
+  for (; i < 16 && known[i] != nullptr; i++)
+    if (known[i] == f && in[i] == ctx && ctx != 0) return MXQ_OK;
+  const int rc = check_cuda(cudaFuncSetAttribute((const void*)f, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes), "product: shared memory");
+  if (rc == MXQ_OK && i < 16) {
+    known[i] = f;
+    in[i] = ctx;
+  }
+  return rc;
 }
 
 struct Operand {
@@ -765,7 +783,7 @@ int launch_rows(Args& a, const Operand& x, const Operand& w, int64_t K, int64_t 
   a.idesc = tc::mma_desc(fw, fx, 128, BN);
   const int smem = S::kSmem + (a.experts ? 4 * (a.experts + 1) : 0);
   auto f = k_mx_rows<BN, GATED>;
-  if (int rc = set_smem((const void*)f, smem)) return rc;
+  if (int rc = set_smem(f, S::kSmem + 4 * (kMostExperts + 1))) return rc;
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3((unsigned)(tiles * split));
   cfg.blockDim = dim3(128);
@@ -788,7 +806,7 @@ int launch_tile(Args& a, const Operand& x, const Operand& w, int64_t K, int64_t 
   a.idesc = tc::mma_desc(fx, fw, 128, 256);
   const int smem = kTileSmem + (a.experts ? 4 * (a.experts + 1) : 0);
   auto f = k_mx_tile<GATED>;
-  if (int rc = set_smem((const void*)f, smem)) return rc;
+  if (int rc = set_smem(f, kTileSmem + 4 * (kMostExperts + 1))) return rc;
   const unsigned grid = (unsigned)(tiles < sm_count() ? tiles : sm_count());
   f<<<grid, 256, smem, st>>>(mx, mw, a);
   return MXQ_LAUNCH_CHECK("product");
@@ -915,7 +933,8 @@ extern "C" int mxq_experts_packed(const uint8_t* x, const uint8_t* x_scales, int
                                   void* stream) {
   MXQ_REQUIRE(spec != nullptr, MXQ_ERR_VALUE, "experts_packed: no spec");
   if (int rc = check_sizes("experts_packed", slots, N, K, experts)) return rc;
-  MXQ_REQUIRE(experts <= 1024, MXQ_ERR_UNSUPPORTED, "experts_packed: at most 1024 experts, got %lld", (long long)experts);
+  MXQ_REQUIRE(experts <= kMostExperts, MXQ_ERR_UNSUPPORTED, "experts_packed: at most %d experts, got %lld", kMostExperts,
+              (long long)experts);
   MXQ_REQUIRE(per >= 0 && (slots == 0 || (x_rows >= 1 && x_rows < (1ll << 30) && (per == 0 ? x_rows >= slots : x_rows * per >= slots))),
               MXQ_ERR_VALUE, "experts_packed: %lld rows of x do not serve %lld slots, %lld per row", (long long)x_rows,
               (long long)slots, (long long)per);

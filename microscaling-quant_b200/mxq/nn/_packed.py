@@ -27,12 +27,13 @@ import torch
 
 from .. import _lib
 from ..block import BLOCK
-from ..element_quant.formats import Format, get
+from ..element_quant.formats import FORMATS, Format, get
 
 __all__ = ["ACTIVATIONS", "Dispatch", "linear_packed", "experts_packed", "lay_packed"]
 
 ACTIVATIONS = (None, "relu", "gelu", "gelu_tanh", "silu", "swiglu", "geglu")
 GATED = ("swiglu", "geglu")
+FIRST_GATED = 5
 FLOATS = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}
 PACKED = 3
 
@@ -46,94 +47,100 @@ class Dispatch(NamedTuple):
     where: torch.Tensor     # (T, k): the place of each slot, -1 for a slot left out
 
 
-class _Operand(NamedTuple):
-    codes: torch.Tensor
-    scales: torch.Tensor
-    pitch: int              # bytes from row to row
-    e: int
-    m: int
-
-
 def _format(fmt, who: str) -> Format:
-    f = get(fmt)
+    f = FORMATS.get(fmt) if type(fmt) is str else None
     if f is None:
-        raise ValueError(f"{who}: {fmt!r} is not an MX element format")
+        f = get(fmt)
+        if f is None:
+            raise ValueError(f"{who}: {fmt!r} is not an MX element format")
     return f
 
 
+def _here(t: torch.Tensor, dev) -> torch.Tensor:
+    """t on dev, contiguous."""
+    if t.device != dev:
+        t = t.detach().to(dev)
+    return t if t.is_contiguous() else t.detach().contiguous()
+
+
 def _pair(v, f: Format, who: str, what: str):
-    """The checked (codes, scales) of an operand and its K."""
-    if not (isinstance(v, (tuple, list)) and len(v) == 2 and all(isinstance(t, torch.Tensor) for t in v)):
+    """The checked codes and scales of an operand, the codes' shape and K."""
+    if not isinstance(v, (tuple, list)) or len(v) != 2 or not isinstance(v[0], torch.Tensor) or \
+            not isinstance(v[1], torch.Tensor):
         raise ValueError(f"{who}: {what} must be a pair (codes, scales) of uint8 tensors")
     codes, scales = v
-    if codes.dtype != torch.uint8 or scales.dtype != torch.uint8 or codes.ndim < 1:
+    shape, have = codes.shape, scales.shape
+    if codes.dtype is not torch.uint8 or scales.dtype is not torch.uint8 or not shape:
         raise ValueError(f"{who}: {what} must be uint8 codes and scales, got {codes.dtype} and {scales.dtype}")
-    K = codes.shape[-1] * (2 if f.e + f.m == 3 else 1)
+    K = shape[-1] * 2 if f.e + f.m == 3 else shape[-1]
     if K == 0:
         raise ValueError(f"{who}: {what} has no values along its last dimension")
-    want = (*codes.shape[:-1], -(-K // BLOCK))
-    if tuple(scales.shape) != want:
-        raise ValueError(f"{who}: scales of {what} must have shape {want} for {f.name} codes {tuple(codes.shape)}, "
-                         f"got {tuple(scales.shape)}")
-    return codes, scales, K
+    if len(have) != len(shape) or have[-1] != (K + BLOCK - 1) // BLOCK or have[:-1] != shape[:-1]:
+        raise ValueError(f"{who}: scales of {what} must have shape {(*shape[:-1], -(-K // BLOCK))} for {f.name} codes "
+                         f"{tuple(shape)}, got {tuple(have)}")
+    return codes, scales, shape, K
 
 
-def _laid(codes: torch.Tensor, scales: torch.Tensor, f: Format, K: int, dev) -> _Operand:
-    """The operand as the kernels read it: as it is where its rows allow it, else laid out as 8-bit codes."""
-    codes, scales = codes.to(dev).contiguous(), scales.to(dev).contiguous()
+def _laid(codes: torch.Tensor, scales: torch.Tensor, shape, f: Format, K: int, dev):
+    """The operand as the kernels read it, (codes, scales, bytes from row to row, e, m): as it is where its rows allow
+    it, else laid out as 8-bit codes."""
+    codes, scales = _here(codes, dev), _here(scales, dev)
     bits = 1 + f.e + f.m
-    at = codes.data_ptr()
-    if bits == 8 and K % 16 == 0 and at % 16 == 0:
-        return _Operand(codes, scales, K, f.e, f.m)
-    if bits == 4 and K % 128 == 0 and at % 32 == 0:
-        return _Operand(codes, scales, K // 2, f.e, f.m)
-    rows = codes.numel() // codes.shape[-1]
+    if bits == 8:
+        if K % 16 == 0 and codes.data_ptr() % 16 == 0:
+            return codes, scales, K, f.e, f.m
+    elif bits == 4 and K % 128 == 0 and codes.data_ptr() % 32 == 0:
+        return codes, scales, K // 2, f.e, f.m
+    rows = codes.numel() // shape[-1]
     pitch = -(-K // 16) * 16
-    wide = torch.empty((*codes.shape[:-1], pitch), dtype=torch.uint8, device=dev)
-    _lib.run("mxq_lay_codes", dev, _lib.ptr(codes), codes.shape[-1], _lib.ptr(wide), pitch, rows, K, f.e, f.m)
-    return _Operand(wide, scales, pitch, *((f.e, f.m) if bits == 8 else (4, 3)))
+    wide = torch.empty((*shape[:-1], pitch), dtype=torch.uint8, device=dev)
+    _lib.run("mxq_lay_codes", dev, codes.data_ptr(), shape[-1], wide.data_ptr(), pitch, rows, K, f.e, f.m)
+    return (wide, scales, pitch, f.e, f.m) if bits == 8 else (wide, scales, pitch, 4, 3)
 
 
 def lay_packed(w: Pair, fmt: Union[str, Format]) -> Tuple[Pair, str]:
     """(w, fmt) such that the products read w as it is, once for weights that are kept: FP6 codes, and FP4 codes with K
-    no multiple of 128, become the E4M3 codes of the same values. Rows of 8-bit codes that are no multiple of 16 bytes
-    cannot be kept so (the pair has no room between its rows) and come back unchanged."""
+    no multiple of 128, become the E4M3 codes of the same values. Rows that would not be multiples of 16 bytes cannot be
+    kept so (the pair has no room between its rows) and come back unchanged."""
     f = _format(fmt, "lay_packed")
-    codes, scales, K = _pair(w, f, "lay_packed", "w")
+    codes, scales, shape, K = _pair(w, f, "lay_packed", "w")
     bits = 1 + f.e + f.m
     if bits == 8 or K % 16 or (bits == 4 and K % 128 == 0):
         return (codes, scales), f.name
-    dev = _lib.device_for(codes)
-    o = _laid(codes, scales, f, K, dev)
-    return (_lib.back(o.codes, codes.device), scales), "MXFP8_E4M3"
+    wide = _laid(codes, scales, shape, f, K, _lib.device_for(codes))[0]
+    return (_lib.back(wide, codes.device), scales), "MXFP8_E4M3"
 
 
-def _x_operand(x, x_fmt, who: str, dev_of):
-    """(operand, leading shape, K, home) of x, a pair or a float tensor that is packed here."""
+def _x_operand(x, x_fmt, who: str, w: torch.Tensor):
+    """(operand, leading shape, K, device, home) of x, a pair or a float tensor that is packed here."""
     f = _format(x_fmt, who)
     if isinstance(x, torch.Tensor):
-        if x.dtype not in FLOATS or x.ndim < 1:
+        kind = FLOATS.get(x.dtype)
+        shape = x.shape
+        if kind is None or not shape:
             raise ValueError(f"{who}: x must be a float32, bfloat16 or float16 tensor or a pair (codes, scales), got "
                              f"{x.dtype}")
-        K = x.shape[-1]
+        K = shape[-1]
         if K == 0:
             raise ValueError(f"{who}: x has no values along its last dimension")
-        dev = _lib.device_for(x, *dev_of)
-        v = x.detach().to(dev)
-        if v.ndim != 2:
-            v = v.reshape(-1, K)
-        if v.stride(1) != 1 or (v.shape[0] > 1 and v.stride(0) < K):
-            v = v.contiguous()
-        rows, pitch = v.shape[0], -(-K // 16) * 16
+        dev = x.device if x.is_cuda else _lib.device_for(x, w)
+        v = x if x.device == dev else x.detach().to(dev)
+        if len(shape) != 2:
+            v = v.detach().reshape(-1, K)
+        rows, stride = v.shape[0], v.stride(0)
+        if v.stride(1) != 1 or (rows > 1 and stride < K):
+            v = v.detach().contiguous()
+            stride = K
+        pitch = -(-K // 16) * 16
         codes = torch.empty((rows, pitch), dtype=torch.uint8, device=dev)
         scales = torch.empty((rows, -(-K // BLOCK)), dtype=torch.uint8, device=dev)
-        _lib.run("mxq_pack_rows", dev, _lib.ptr(v), FLOATS[v.dtype], v.stride(0) if rows > 1 else K, _lib.ptr(codes), pitch,
-                 _lib.ptr(scales), rows, K, f.e, f.m)
-        o = _Operand(codes, scales, pitch, *((f.e, f.m) if f.e + f.m == 7 else (4, 3)))
-        return o, x.shape[:-1], K, dev, x.device
-    codes, scales, K = _pair(x, f, who, "x")
-    dev = _lib.device_for(codes, *dev_of)
-    return _laid(codes, scales, f, K, dev), codes.shape[:-1], K, dev, codes.device
+        _lib.run("mxq_pack_rows", dev, v.data_ptr(), kind, stride, codes.data_ptr(), pitch, scales.data_ptr(), rows, K, f.e,
+                 f.m)
+        e, m = (f.e, f.m) if f.e + f.m == 7 else (4, 3)
+        return (codes, scales, pitch, e, m), shape[:-1], K, dev, x.device
+    codes, scales, shape, K = _pair(x, f, who, "x")
+    dev = codes.device if codes.is_cuda else _lib.device_for(codes, w)
+    return _laid(codes, scales, shape, f, K, dev), shape[:-1], K, dev, codes.device
 
 
 def _make_spec(x_e, x_m, w_e, w_m, act, out, out_e, out_m):
@@ -145,21 +152,22 @@ _spec = _lib.cached(_make_spec)
 
 def _plan_output(out, activation, N: int, who: str):
     """(activation code, output code, output Format or None, F)."""
-    if not (activation is None or isinstance(activation, str)) or activation not in ACTIVATIONS:
+    if activation is not None and not (isinstance(activation, str) and activation in ACTIVATIONS):
         raise ValueError(f"{who}: activation must be one of {ACTIVATIONS}, got {activation!r}")
-    F = N
-    if activation in GATED:
+    act, F = ACTIVATIONS.index(activation), N
+    if act >= FIRST_GATED:
         if N % 2:
             raise ValueError(f"{who}: {activation} needs an even number of rows of w, got {N}")
         F = N // 2
     if isinstance(out, torch.dtype):
-        if out not in FLOATS:
+        kind = FLOATS.get(out)
+        if kind is None:
             raise ValueError(f"{who}: out must be float32, bfloat16, float16 or an MX format, got {out}")
-        return ACTIVATIONS.index(activation), FLOATS[out], None, F
+        return act, kind, None, F
     f = _format(out, who)
     if f.e + f.m == 3 and F % 2:
         raise ValueError(f"{who}: packed FP4 pairs up along the output, whose width is {F}")
-    return ACTIVATIONS.index(activation), PACKED, f, F
+    return act, PACKED, f, F
 
 
 def _outputs(lead, out, f, F: int, dev):
@@ -170,11 +178,13 @@ def _outputs(lead, out, f, F: int, dev):
             torch.empty((*lead, -(-F // BLOCK)), dtype=torch.uint8, device=dev))
 
 
-def _given(y, scales, home):
-    return _lib.back(y, home) if scales is None else (_lib.back(y, home), _lib.back(scales, home))
+def _given(y, scales, dev, home):
+    if home != dev:
+        y, scales = y.to(home), None if scales is None else scales.to(home)
+    return y if scales is None else (y, scales)
 
 
-def _product_ready():
+def _ready():
     if _lib._wait_word is None:                             # the kernel's wait-status word, checked by every call
         _lib.wait_word()
 
@@ -186,45 +196,49 @@ def linear_packed(x: Union[Pair, torch.Tensor], w: Pair, fmt: Union[str, Format]
     `fmt`; bias: N values; residual: y's shape and dtype. Returns y (... x F) of dtype `out`, or its (codes, scales)."""
     who = "linear_packed"
     fw = _format(fmt, who)
-    wc, ws, K = _pair(w, fw, who, "w")
-    if wc.ndim != 2:
-        raise ValueError(f"{who}: w must be 2-D (N x K), got codes {tuple(wc.shape)}")
-    N = wc.shape[0]
+    wc, ws, wshape, K = _pair(w, fw, who, "w")
+    if len(wshape) != 2:
+        raise ValueError(f"{who}: w must be 2-D (N x K), got codes {tuple(wshape)}")
+    N = wshape[0]
     act, otype, fo, F = _plan_output(out, activation, N, who)
     if bias is not None and tuple(bias.shape) != (N,):
         raise ValueError(f"{who}: bias must have shape {(N,)}, got {tuple(bias.shape)}")
-    _product_ready()
-    xo, lead, Kx, dev, home = _x_operand(x, x_fmt, who, (wc,))
+    _ready()
+    (xc, xs, xp, xe, xm), lead, Kx, dev, home = _x_operand(x, x_fmt, who, wc)
     if Kx != K:
         raise ValueError(f"{who}: x has {Kx} values per row and w {K}")
-    M = xo.scales.numel() // xo.scales.shape[-1]
     y, ys = _outputs(lead, out, fo, F, dev)
-    r, r_stride = None, 0
+    M = lead[0] if len(lead) == 1 else lead.numel()
+    r, r_at, r_stride = None, 0, 0
     if residual is not None:
         if fo is not None:
             raise ValueError(f"{who}: a packed output takes no residual")
-        if residual.shape != y.shape or residual.dtype != out:
+        if residual.shape != y.shape or residual.dtype is not out:
             raise ValueError(f"{who}: residual must be {out} of shape {tuple(y.shape)}, got {residual.dtype} "
                              f"{tuple(residual.shape)}")
-        r = residual.detach().to(dev).reshape(M, F)
-        if r.numel() and r.stride(1) != 1:
-            r = r.contiguous()
-        r_stride = r.stride(0) if M > 1 else F
+        r = residual if residual.device == dev else residual.detach().to(dev)
+        if len(lead) != 1:
+            r = r.detach().reshape(M, F)
+        r_stride = r.stride(0)
+        if F > 1 and r.stride(1) != 1:
+            r = r.detach().contiguous()
+            r_stride = F
+        r_at = r.data_ptr()
     if M == 0 or N == 0:
-        return _given(y, ys, home)
+        return _given(y, ys, dev, home)
     b = None if bias is None else _lib.on(bias, dev)
-    wo = _laid(wc, ws, fw, K, dev)
-    _lib.run("mxq_linear_packed", dev, _lib.ptr(xo.codes), _lib.ptr(xo.scales), xo.pitch, M, _lib.ptr(wo.codes),
-             _lib.ptr(wo.scales), wo.pitch, N, K,
-             ctypes.byref(_spec(xo.e, xo.m, wo.e, wo.m, act, otype, fo.e if fo else 0, fo.m if fo else 0)), _lib.ptr(b),
-             _lib.ptr(r), r_stride, _lib.ptr(y), _lib.ptr(ys))
-    return _given(y, ys, home)
+    wc, ws, wp, we, wm = _laid(wc, ws, wshape, fw, K, dev)
+    spec = _spec(xe, xm, we, wm, act, otype, fo.e if fo else 0, fo.m if fo else 0)
+    _lib.run("mxq_linear_packed", dev, xc.data_ptr(), xs.data_ptr(), xp, M, wc.data_ptr(), ws.data_ptr(), wp, N, K,
+             ctypes.byref(spec), None if b is None else b.data_ptr(), r_at, r_stride, y.data_ptr(),
+             None if ys is None else ys.data_ptr())
+    return _given(y, ys, dev, home)
 
 
 def _index(t: torch.Tensor, dev, who: str, what: str) -> torch.Tensor:
-    if not isinstance(t, torch.Tensor) or t.dtype != torch.int32:
+    if not isinstance(t, torch.Tensor) or t.dtype is not torch.int32:
         raise ValueError(f"{who}: {what} must be an int32 tensor, got {getattr(t, 'dtype', type(t))}")
-    return t.to(dev).contiguous()
+    return _here(t, dev)
 
 
 def experts_packed(x: Union[Pair, torch.Tensor], w: Pair, fmt: Union[str, Format], plan: Dispatch, gather: bool = True,
@@ -236,22 +250,23 @@ def experts_packed(x: Union[Pair, torch.Tensor], w: Pair, fmt: Union[str, Format
     (from offsets[-1] on) are not written."""
     who = "experts_packed"
     fw = _format(fmt, who)
-    wc, ws, K = _pair(w, fw, who, "w")
-    if wc.ndim != 3:
-        raise ValueError(f"{who}: w must be 3-D (experts x N x K), got codes {tuple(wc.shape)}")
-    E, N = wc.shape[0], wc.shape[1]
+    wc, ws, wshape, K = _pair(w, fw, who, "w")
+    if len(wshape) != 3:
+        raise ValueError(f"{who}: w must be 3-D (experts x N x K), got codes {tuple(wshape)}")
+    E, N = wshape[0], wshape[1]
     act, otype, fo, F = _plan_output(out, activation, N, who)
-    if plan.offsets.numel() != E + 1:
-        raise ValueError(f"{who}: the plan has {plan.offsets.numel() - 1} experts and w {E}")
+    offsets, order, _ = plan
+    if offsets.numel() != E + 1:
+        raise ValueError(f"{who}: the plan has {offsets.numel() - 1} experts and w {E}")
     if bias is not None and tuple(bias.shape) != (E, N):
         raise ValueError(f"{who}: bias must have shape {(E, N)}, got {tuple(bias.shape)}")
-    _product_ready()
-    xo, lead, Kx, dev, home = _x_operand(x, x_fmt, who, (wc,))
+    _ready()
+    (xc, xs, xp, xe, xm), lead, Kx, dev, home = _x_operand(x, x_fmt, who, wc)
     if Kx != K:
         raise ValueError(f"{who}: x has {Kx} values per row and w {K}")
     if len(lead) != 1:
         raise ValueError(f"{who}: x must be 2-D, got leading shape {tuple(lead)}")
-    slots, rows = plan.order.numel(), lead[0]
+    slots, rows = order.numel(), lead[0]
     if gather:
         if (slots == 0) != (rows == 0) or (rows and slots % rows):
             raise ValueError(f"{who}: {slots} slots are no multiple of x's {rows} rows")
@@ -262,12 +277,12 @@ def experts_packed(x: Union[Pair, torch.Tensor], w: Pair, fmt: Union[str, Format
         per = 0
     y, ys = _outputs((slots,), out, fo, F, dev)
     if slots == 0 or N == 0 or E == 0:
-        return _given(y, ys, home)
-    offsets, order = _index(plan.offsets, dev, who, "offsets"), _index(plan.order, dev, who, "order")
+        return _given(y, ys, dev, home)
+    offsets, order = _index(offsets, dev, who, "offsets"), _index(order, dev, who, "order")
     b = None if bias is None else _lib.on(bias, dev)
-    wo = _laid(wc, ws, fw, K, dev)
-    _lib.run("mxq_experts_packed", dev, _lib.ptr(xo.codes), _lib.ptr(xo.scales), xo.pitch, rows, _lib.ptr(wo.codes),
-             _lib.ptr(wo.scales), wo.pitch, E, N, K, _lib.ptr(offsets), _lib.ptr(order), slots, per,
-             ctypes.byref(_spec(xo.e, xo.m, wo.e, wo.m, act, otype, fo.e if fo else 0, fo.m if fo else 0)), _lib.ptr(b),
-             _lib.ptr(y), _lib.ptr(ys))
-    return _given(y, ys, home)
+    wc, ws, wp, we, wm = _laid(wc, ws, wshape, fw, K, dev)
+    spec = _spec(xe, xm, we, wm, act, otype, fo.e if fo else 0, fo.m if fo else 0)
+    _lib.run("mxq_experts_packed", dev, xc.data_ptr(), xs.data_ptr(), xp, rows, wc.data_ptr(), ws.data_ptr(), wp, E, N, K,
+             offsets.data_ptr(), order.data_ptr(), slots, per, ctypes.byref(spec), None if b is None else b.data_ptr(),
+             y.data_ptr(), None if ys is None else ys.data_ptr())
+    return _given(y, ys, dev, home)

@@ -24,7 +24,7 @@ import ctypes
 import torch
 
 from .. import _lib
-from ._packed import FLOATS, Dispatch, _index
+from ._packed import FLOATS, Dispatch, _here, _index
 
 __all__ = ["route", "route_backward", "dispatch", "combine", "combine_backward"]
 
@@ -40,9 +40,10 @@ _spec = _lib.cached(_make_spec)
 
 
 def _route_args(who, logits, k, score, groups, keep, group_score):
-    if not isinstance(logits, torch.Tensor) or logits.dtype not in FLOATS or logits.ndim != 2:
+    """(tokens, experts) of checked arguments."""
+    if not isinstance(logits, torch.Tensor) or logits.dtype not in FLOATS or logits.dim() != 2:
         raise ValueError(f"{who}: logits must be a 2-D float32, bfloat16 or float16 tensor (tokens x experts)")
-    E = logits.shape[1]
+    T, E = logits.shape
     if not isinstance(k, int) or not 1 <= k <= min(E, 32):
         raise ValueError(f"{who}: k must be in [1, min(experts, 32)], got {k!r} for {E} experts")
     if score not in SCORES or group_score not in GROUP_SCORES:
@@ -52,25 +53,33 @@ def _route_args(who, logits, k, score, groups, keep, group_score):
         raise ValueError(f"{who}: cannot keep {keep} of {groups} equal groups of {E} experts")
     if E > 1024:
         raise ValueError(f"{who}: at most 1024 experts, got {E}")
+    return T, E
 
 
 def _rows(t: torch.Tensor, dev) -> torch.Tensor:
-    """t on dev with its rows contiguous (any row stride)."""
-    t = t.detach().to(dev)
-    return t if t.stride(-1) == 1 or t.shape[-1] <= 1 and t.is_contiguous() else t.contiguous()
+    """t (2-D) on dev with its rows contiguous (any row stride)."""
+    if t.device != dev:
+        t = t.detach().to(dev)
+    return t if t.is_contiguous() or t.stride(1) == 1 else t.detach().contiguous()
+
+
+def _device(t: torch.Tensor):
+    return t.device if t.is_cuda else _lib.device_for(t)
 
 
 def _route(logits, k, score, bias, groups, keep, group_score, renormalize, scale):
     T, E = logits.shape
-    home, dev = logits.device, _lib.device_for(logits)
+    home, dev = logits.device, _device(logits)
     l = _rows(logits, dev)
     b = None if bias is None else _lib.on(bias, dev)
     weights = torch.empty((T, k), dtype=torch.float32, device=dev)
     experts = torch.empty((T, k), dtype=torch.int32, device=dev)
     s = _spec(SCORES.index(score), groups, keep, int(group_score == "top2"), int(bool(renormalize)), float(scale))
-    _lib.run("mxq_route", dev, _lib.ptr(l), FLOATS[l.dtype], l.stride(0), _lib.ptr(b), _lib.ptr(weights), _lib.ptr(experts),
-             T, E, k, ctypes.byref(s))
-    return _lib.back(weights, home), _lib.back(experts, home)
+    _lib.run("mxq_route", dev, l.data_ptr(), FLOATS[l.dtype], l.stride(0), None if b is None else b.data_ptr(),
+             weights.data_ptr(), experts.data_ptr(), T, E, k, ctypes.byref(s))
+    if home == dev:
+        return weights, experts
+    return weights.to(home), experts.to(home)
 
 
 class _Route(torch.autograd.Function):
@@ -94,9 +103,9 @@ def route(logits: torch.Tensor, k: int, score: str = "softmax", bias: Optional[t
           keep: int = 1, group_score: str = "max", renormalize: bool = False,
           scale: float = 1.0) -> Tuple[torch.Tensor, torch.Tensor]:
     """The k experts of each token: (weights T x k float32, experts T x k int32), as the module's text says."""
-    _route_args("route", logits, k, score, groups, keep, group_score)
-    if bias is not None and tuple(bias.shape) != (logits.shape[1],):
-        raise ValueError(f"route: bias must have shape {(logits.shape[1],)}, got {tuple(bias.shape)}")
+    _, E = _route_args("route", logits, k, score, groups, keep, group_score)
+    if bias is not None and tuple(bias.shape) != (E,):
+        raise ValueError(f"route: bias must have shape {(E,)}, got {tuple(bias.shape)}")
     if logits.requires_grad and torch.is_grad_enabled():
         return _Route.apply(logits, k, score, bias, groups, keep, group_score, renormalize, scale)
     return _route(logits, k, score, bias, groups, keep, group_score, renormalize, scale)
@@ -108,17 +117,16 @@ def route_backward(grad: torch.Tensor, logits: torch.Tensor, experts: torch.Tens
     who = "route_backward"
     if experts.ndim != 2:
         raise ValueError(f"{who}: experts must be 2-D (tokens x k), got {tuple(experts.shape)}")
-    _route_args(who, logits, experts.shape[1], score, 1, 1, "max")
-    T, E = logits.shape
     k = experts.shape[1]
+    T, E = _route_args(who, logits, k, score, 1, 1, "max")
     if experts.shape[0] != T or grad.shape != experts.shape:
         raise ValueError(f"{who}: grad {tuple(grad.shape)} and experts {tuple(experts.shape)} must be {T} x k")
-    home, dev = logits.device, _lib.device_for(logits)
+    home, dev = logits.device, _device(logits)
     l, g, e = _rows(logits, dev), _lib.on(grad, dev), _index(experts, dev, who, "experts")
     out = torch.empty((T, E), dtype=l.dtype, device=dev)
     s = _spec(SCORES.index(score), 1, 1, 0, int(bool(renormalize)), float(scale))
-    _lib.run("mxq_route_backward", dev, _lib.ptr(g), _lib.ptr(l), FLOATS[l.dtype], l.stride(0), _lib.ptr(e), _lib.ptr(out),
-             T, E, k, ctypes.byref(s))
+    _lib.run("mxq_route_backward", dev, g.data_ptr(), l.data_ptr(), FLOATS[l.dtype], l.stride(0), e.data_ptr(),
+             out.data_ptr(), T, E, k, ctypes.byref(s))
     return _lib.back(out, home)
 
 
@@ -127,36 +135,45 @@ def dispatch(experts: torch.Tensor, n_experts: int) -> Dispatch:
     expert is outside [0, n_experts) is left out."""
     if not isinstance(n_experts, int) or not 1 <= n_experts <= 1024:
         raise ValueError(f"dispatch: n_experts must be in [1, 1024], got {n_experts!r}")
-    home, dev = experts.device, _lib.device_for(experts)
+    home, dev = experts.device, _device(experts)
     e = _index(experts, dev, "dispatch", "experts")
-    offsets = torch.empty(n_experts + 1, dtype=torch.int32, device=dev)
-    order = torch.empty(e.numel(), dtype=torch.int32, device=dev)
-    where = torch.empty(e.shape, dtype=torch.int32, device=dev)
-    _lib.run("mxq_dispatch", dev, _lib.ptr(e), e.numel(), n_experts, _lib.ptr(offsets), _lib.ptr(order), _lib.ptr(where))
-    return Dispatch(_lib.back(offsets, home), _lib.back(order, home), _lib.back(where, home))
+    n = e.numel()
+    # one allocation: the three are made and kept together
+    offsets, order, where = torch.empty(2 * n + n_experts + 1, dtype=torch.int32, device=dev).split(
+        (n_experts + 1, n, n))
+    _lib.run("mxq_dispatch", dev, e.data_ptr(), n, n_experts, offsets.data_ptr(), order.data_ptr(), where.data_ptr())
+    where = where.view(e.shape)
+    if home != dev:
+        offsets, order, where = offsets.to(home), order.to(home), where.to(home)
+    return Dispatch(offsets, order, where)
 
 
 def _combine_args(who, z, weights, plan):
-    if not isinstance(z, torch.Tensor) or z.dtype not in FLOATS or z.ndim != 2:
+    """(T, k, N) of checked arguments."""
+    if not isinstance(z, torch.Tensor) or z.dtype not in FLOATS or z.dim() != 2:
         raise ValueError(f"{who}: z must be a 2-D float32, bfloat16 or float16 tensor (slots x N)")
-    if weights.ndim != 2 or weights.shape != plan.where.shape or plan.order.numel() != plan.where.numel():
-        raise ValueError(f"{who}: weights {tuple(weights.shape)} do not match the plan's {tuple(plan.where.shape)} slots")
-    if z.shape[0] != plan.where.numel():
-        raise ValueError(f"{who}: z has {z.shape[0]} rows and the plan {plan.where.numel()} slots")
+    _, order, where = plan
+    shape = where.shape
+    if len(shape) != 2 or weights.shape != shape or order.numel() != shape[0] * shape[1]:
+        raise ValueError(f"{who}: weights {tuple(weights.shape)} do not match the plan's {tuple(shape)} slots")
+    slots, N = z.shape
+    if slots != shape[0] * shape[1]:
+        raise ValueError(f"{who}: z has {slots} rows and the plan {shape[0] * shape[1]} slots")
+    return shape[0], shape[1], N
 
 
 def _combine(z, weights, where, residual):
     (T, k), N = where.shape, z.shape[1]
-    home, dev = z.device, _lib.device_for(z)
-    zc = z.detach().to(dev).contiguous()
-    w, at = _lib.on(weights, dev), _index(where, dev, "combine", "where")
+    home, dev = z.device, _device(z)
+    zc, w, at = _here(z, dev), _lib.on(weights, dev), _index(where, dev, "combine", "where")
     r = None if residual is None else _rows(residual, dev)
     y = torch.empty((T, N), dtype=z.dtype, device=dev)
     if k == 0:
-        return y.zero_() if residual is None else y.copy_(residual)
-    _lib.run("mxq_combine", dev, _lib.ptr(zc), FLOATS[zc.dtype], _lib.ptr(w), _lib.ptr(at), _lib.ptr(r),
-             r.stride(0) if r is not None else 0, _lib.ptr(y), T, k, N)
-    return _lib.back(y, home)
+        y = y.zero_() if r is None else y.copy_(r.detach())
+    else:
+        _lib.run("mxq_combine", dev, zc.data_ptr(), FLOATS[zc.dtype], w.data_ptr(), at.data_ptr(),
+                 None if r is None else r.data_ptr(), 0 if r is None else r.stride(0), y.data_ptr(), T, k, N)
+    return y if home == dev else y.to(home)
 
 
 class _Combine(torch.autograd.Function):
@@ -177,12 +194,12 @@ class _Combine(torch.autograd.Function):
 def combine(z: torch.Tensor, weights: torch.Tensor, plan: Dispatch, residual: Optional[torch.Tensor] = None) -> torch.Tensor:
     """y[t] = sum_j weights[t, j] z[plan.where[t, j]] (+ residual[t]), of z's dtype, summed in float32 in the order of j.
     z: slots x N in the plan's order. A slot left out adds its weight times 0."""
-    _combine_args("combine", z, weights, plan)
-    T, N = plan.where.shape[0], z.shape[1]
+    T, _, N = _combine_args("combine", z, weights, plan)
     if residual is not None and (tuple(residual.shape) != (T, N) or residual.dtype != z.dtype):
         raise ValueError(f"combine: residual must be {z.dtype} of shape {(T, N)}, got {residual.dtype} "
                          f"{tuple(residual.shape)}")
-    if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in (z, weights, residual)):
+    if torch.is_grad_enabled() and (z.requires_grad or weights.requires_grad or
+                                    (residual is not None and residual.requires_grad)):
         return _Combine.apply(z, weights, *plan, residual)
     return _combine(z, weights, plan.where, residual)
 
@@ -192,16 +209,17 @@ def combine_backward(dy: torch.Tensor, z: torch.Tensor, weights: torch.Tensor,
     """(dz, dw) of combine: dz[place] = weights[slot] dy[t] (0 at the places without a slot), dw[t, j] = dy[t] . z[place]
     in float32 (0 for a slot left out)."""
     who = "combine_backward"
-    _combine_args(who, z, weights, plan)
-    (T, k), N = plan.where.shape, z.shape[1]
+    T, k, N = _combine_args(who, z, weights, plan)
     if tuple(dy.shape) != (T, N) or dy.dtype != z.dtype:
         raise ValueError(f"{who}: dy must be {z.dtype} of shape {(T, N)}, got {dy.dtype} {tuple(dy.shape)}")
-    home, dev = z.device, _lib.device_for(z)
-    zc, g = z.detach().to(dev).contiguous(), _rows(dy, dev)
+    home, dev = z.device, _device(z)
+    zc, g = _here(z, dev), _rows(dy, dev)
     w, at, order = _lib.on(weights, dev), _index(plan.where, dev, who, "where"), _index(plan.order, dev, who, "order")
     dz = torch.empty((T * k, N), dtype=z.dtype, device=dev)
     dw = torch.empty((T, k), dtype=torch.float32, device=dev)
     if T and k:
-        _lib.run("mxq_combine_backward", dev, _lib.ptr(g), g.stride(0), _lib.ptr(zc), FLOATS[zc.dtype], _lib.ptr(w),
-                 _lib.ptr(at), _lib.ptr(order), _lib.ptr(dz), _lib.ptr(dw), T, k, N)
-    return _lib.back(dz, home), _lib.back(dw, home)
+        _lib.run("mxq_combine_backward", dev, g.data_ptr(), g.stride(0), zc.data_ptr(), FLOATS[zc.dtype], w.data_ptr(),
+                 at.data_ptr(), order.data_ptr(), dz.data_ptr(), dw.data_ptr(), T, k, N)
+    if home == dev:
+        return dz, dw
+    return dz.to(home), dw.to(home)
