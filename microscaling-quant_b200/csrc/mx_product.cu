@@ -8,7 +8,7 @@
 // tensor core, nothing is dequantized. The products are exact and the sums are held in float32 in TMEM.
 //
 // Two kernels share the operand staging:
-//   k_mx_tile  128 rows of x by 256 rows of w per CTA, persistent, for many rows: the operations bound it.
+//   k_mx_tile  256 rows of x by 256 rows of w per pair of CTAs, persistent, for many rows: the operations bound it.
 //   k_mx_rows  128 rows of w by 16-128 rows of x per CTA, K split over a cluster, for few rows: reading w bounds it.
 #include "common.cuh"
 #include "mx_codes.cuh"
@@ -137,10 +137,11 @@ struct Ring {
 };
 
 // One warp brings the scale words of its W rows per lane for K steps [k0, k1) into the ring: 16 bytes per row, that
-// is four steps, are read at once and the next four are on their way while these are stored.
+// is four steps, are read at once and the next four are on their way while these are stored. `full`: the stages'
+// barriers; far: their shared::cluster address where they are in another CTA, else 0.
 template <int W>
 __device__ __forceinline__ bool stage_scales(const uint8_t* const (&rows)[W], const uint32_t (&place)[W], int k0, int k1, const Args& a,
-                                             uint8_t* area, int pitch, uint64_t* full, uint64_t* empty, Ring& ring, int stages,
+                                             uint8_t* area, int pitch, uint64_t* full, uint32_t far, uint64_t* empty, Ring& ring, int stages,
                                              volatile int* abort) {
   uint4 now[W], nxt[W];
   int g = k0 >> 2;
@@ -163,7 +164,10 @@ __device__ __forceinline__ bool stage_scales(const uint8_t* const (&rows)[W], co
         *reinterpret_cast<uint32_t*>(to + place[i]) = j == 0 ? now[i].x : j == 1 ? now[i].y : j == 2 ? now[i].z : now[i].w;
       fence_proxy_async();
       __syncwarp();
-      if ((threadIdx.x & 31) == 0) tc::mbar_arrive(&full[ring.stage]);
+      if ((threadIdx.x & 31) == 0) {
+        if (far) tc::mbar_arrive_remote(far + 8u * ring.stage);
+        else tc::mbar_arrive(&full[ring.stage]);
+      }
       ring.next(stages);
     }
 #pragma unroll
@@ -244,151 +248,177 @@ __device__ __forceinline__ const uint8_t* w_scales(const Args& a, const Tile& t,
 }
 
 // ------------------------------------------------------------------------------------------------ many rows
-constexpr int kStages = 4;
-constexpr int kStageBytes = 3 * kTileBytes;            // x 128 rows, w 256 rows
-constexpr int kStageScales = 3 * 512;
+// A pair of CTAs (cta_group::2) makes 256 rows by 256 features at a time: each holds 128 rows of x and half of the
+// features of w, so that a stage brings 32 KB into each SM's shared memory and not the 48 KB of one CTA alone. Alone, the
+// stage's arrival and the tensor core's reads are 192 bytes a cycle at the full rate, the shared memory moves 128; as
+// a pair both are 128.
+constexpr int kStages = 5;
+constexpr int kStageBytes = 2 * kTileBytes;
+constexpr int kStageScales = 3 * 512;                  // x's 128 rows, all of w's 256
+constexpr int kWriters = 8;                            // epilogue warps
+constexpr int kPassBytes = 32 * 128;                   // what one of them stages: 32 rows of 128 bytes
 
 struct TileShared {
   uint64_t full[kStages], empty[kStages], acc_full, acc_free, last;
   uint32_t tmem;
   int abort;
 };
-constexpr int kTileSmem = 1024 + kStages * (kStageBytes + kStageScales) + (int)sizeof(TileShared);
+constexpr int kTileSmem = 1024 + kStages * (kStageBytes + kStageScales) + kWriters * kPassBytes + (int)sizeof(TileShared);
 
-// 32 columns of one row of y: bias and activation are done; residual, rounding, store
-__device__ __forceinline__ void write_row(const Args& a, float (&y)[32], int64_t row, int col) {
-  const int left = a.width - col;
-  if (a.otype == kOutPacked) {
-    uint32_t top = 0;
-#pragma unroll
-    for (int i = 0; i < 32; i++) {
-      const uint32_t b = __float_as_uint(y[i]) & 0x7fffffffu;
-      if (i < left) top = max(top, b);
-    }
-    const uint32_t sb = scale_byte(top, a.ofmt);
-    const float inv = scale_inverse(sb);
-    a.out_scales[row * a.out_nb + (col >> 5)] = (uint8_t)sb;
-    uint32_t w[8];
-    const bool nib = a.ofmt == kFmtE2M1;
-    uint8_t* to = static_cast<uint8_t*>(a.out) + row * a.out_pitch + (nib ? col >> 1 : col);
-    if (nib) {
-#pragma unroll
-      for (int i = 0; i < 4; i++) {
-        w[i] = 0;
-#pragma unroll
-        for (int j = 0; j < 4; j++)
-          w[i] |= (encode2(kFmtE2M1, scaled(y[8 * i + 2 * j], inv), scaled(y[8 * i + 2 * j + 1], inv)) & 255u) << (8 * j);
+// place of 16-byte piece j of a staged row: neighbouring rows in other banks
+__device__ __forceinline__ uint8_t* piece(uint8_t* stage, int row, int j) { return stage + row * 128 + ((j ^ (row & 7)) << 4); }
+
+// A warp's 32 rows between shared memory (128 bytes a row) and memory, each row's `bytes` (a multiple of 16 if vec) in one
+// run per row: rows below `rows` only.
+template <bool STORE>
+__device__ __forceinline__ void move_rows(uint8_t* stage, uint8_t* mem, int64_t pitch, int rows, int bytes, int width, int size, bool vec) {
+  const int lane = threadIdx.x & 31;
+  if (vec) {
+    const int sh = width == 128 ? 3 : width == 64 ? 2 : 1;       // pieces per row
+    for (int i = 0; i < (1 << sh); i++) {
+      const int r = (i * 32 + lane) >> sh, j = lane & ((1 << sh) - 1);
+      if (r < rows && j * 16 < bytes) {
+        uint4* s = reinterpret_cast<uint4*>(piece(stage, r, j));
+        uint4* m = reinterpret_cast<uint4*>(mem + r * pitch + j * 16);
+        if (STORE) *m = *s; else *s = *m;
       }
-    } else {
-#pragma unroll
-      for (int i = 0; i < 8; i++)
-        w[i] = encode2(a.ofmt, scaled(y[4 * i], inv), scaled(y[4 * i + 1], inv)) |
-               encode2(a.ofmt, scaled(y[4 * i + 2], inv), scaled(y[4 * i + 3], inv)) << 16;
-    }
-    const int bytes = nib ? 16 : 32;
-    if (left >= 32 && a.vec_out) {
-      reinterpret_cast<uint4*>(to)[0] = make_uint4(w[0], w[1], w[2], w[3]);
-      if (!nib) reinterpret_cast<uint4*>(to)[1] = make_uint4(w[4], w[5], w[6], w[7]);
-    } else {
-      const int have = nib ? left >> 1 : left;
-#pragma unroll
-      for (int i = 0; i < 32; i++)
-        if (i < bytes && i < have) to[i] = (uint8_t)(w[i >> 2] >> (8 * (i & 3)));
     }
     return;
   }
-  const bool whole = left >= 32 && a.vec_out;
-  if (a.otype == kOutF32) {
-    float* to = static_cast<float*>(a.out) + row * a.out_pitch + col;
-    const float* r = a.residual ? static_cast<const float*>(a.residual) + row * a.residual_stride + col : nullptr;
-    if (whole) {
-#pragma unroll
-      for (int i = 0; i < 8; i++) {
-        float4 v = make_float4(y[4 * i], y[4 * i + 1], y[4 * i + 2], y[4 * i + 3]);
-        if (r) {
-          const float4 q = __ldg(reinterpret_cast<const float4*>(r) + i);
-          v = make_float4(v.x + q.x, v.y + q.y, v.z + q.z, v.w + q.w);
-        }
-        reinterpret_cast<float4*>(to)[i] = v;
+  for (int r = 0; r < rows; r++)
+    for (int b = lane * size; b < bytes; b += 32 * size) {
+      uint8_t* s = piece(stage, r, b >> 4) + (b & 15);
+      uint8_t* m = mem + r * pitch + b;
+      if (size == 4) {
+        if (STORE) *reinterpret_cast<uint32_t*>(m) = *reinterpret_cast<uint32_t*>(s);
+        else *reinterpret_cast<uint32_t*>(s) = *reinterpret_cast<uint32_t*>(m);
+      } else if (size == 2) {
+        if (STORE) *reinterpret_cast<uint16_t*>(m) = *reinterpret_cast<uint16_t*>(s);
+        else *reinterpret_cast<uint16_t*>(s) = *reinterpret_cast<uint16_t*>(m);
+      } else {
+        *m = *s;
       }
-    } else {
+    }
+}
+
+__device__ __forceinline__ float widen16(uint32_t h, bool bf) {
+  return bf ? __uint_as_float(h << 16) : __half2float(__ushort_as_half((unsigned short)h));
+}
+__device__ __forceinline__ uint32_t narrow2(float lo, float hi, bool bf) {
+  if (bf) {
+    const __nv_bfloat162 p = __floats2bfloat162_rn(lo, hi);
+    return *reinterpret_cast<const uint32_t*>(&p);
+  }
+  const __half2 p = __floats2half2_rn(lo, hi);
+  return *reinterpret_cast<const uint32_t*>(&p);
+}
+
+// 32 columns of this lane's row into its staged row, at 16-byte piece j0 on; the residual's are there already
+__device__ __forceinline__ void stage_row(const Args& a, float (&y)[32], uint8_t* stage, int j0) {
+  const int lane = threadIdx.x & 31;
+  if (a.otype == kOutF32) {
 #pragma unroll
-      for (int i = 0; i < 32; i++)
-        if (i < left) to[i] = r ? y[i] + r[i] : y[i];
+    for (int i = 0; i < 8; i++) {
+      float4* to = reinterpret_cast<float4*>(piece(stage, lane, j0 + i));
+      float4 v = make_float4(y[4 * i], y[4 * i + 1], y[4 * i + 2], y[4 * i + 3]);
+      if (a.residual) {
+        const float4 q = *to;
+        v = make_float4(v.x + q.x, v.y + q.y, v.z + q.z, v.w + q.w);
+      }
+      *to = v;
     }
     return;
   }
   const bool bf = a.otype == kOutBf16;
-  uint16_t* to = static_cast<uint16_t*>(a.out) + row * a.out_pitch + col;
-  const uint16_t* r = a.residual ? static_cast<const uint16_t*>(a.residual) + row * a.residual_stride + col : nullptr;
-  auto widen = [bf](uint32_t h) {
-    return bf ? __uint_as_float(h << 16) : __half2float(__ushort_as_half((unsigned short)h));
-  };
-  auto pair = [bf](float lo, float hi) {
-    if (bf) {
-      const __nv_bfloat162 p = __floats2bfloat162_rn(lo, hi);
-      return *reinterpret_cast<const uint32_t*>(&p);
-    }
-    const __half2 p = __floats2half2_rn(lo, hi);
-    return *reinterpret_cast<const uint32_t*>(&p);
-  };
-  if (whole) {
 #pragma unroll
-    for (int i = 0; i < 4; i++) {
-      if (r) {
-        const uint4 q = __ldg(reinterpret_cast<const uint4*>(r) + i);
-        const uint32_t h[4] = {q.x, q.y, q.z, q.w};
+  for (int i = 0; i < 4; i++) {
+    uint4* to = reinterpret_cast<uint4*>(piece(stage, lane, j0 + i));
+    if (a.residual) {
+      const uint4 q = *to;
+      const uint32_t h[4] = {q.x, q.y, q.z, q.w};
 #pragma unroll
-        for (int j = 0; j < 4; j++) {
-          y[8 * i + 2 * j] += widen(h[j] & 0xffffu);
-          y[8 * i + 2 * j + 1] += widen(h[j] >> 16);
-        }
+      for (int j = 0; j < 4; j++) {
+        y[8 * i + 2 * j] += widen16(h[j] & 0xffffu, bf);
+        y[8 * i + 2 * j + 1] += widen16(h[j] >> 16, bf);
       }
-      reinterpret_cast<uint4*>(to)[i] = make_uint4(pair(y[8 * i], y[8 * i + 1]), pair(y[8 * i + 2], y[8 * i + 3]),
-                                                   pair(y[8 * i + 4], y[8 * i + 5]), pair(y[8 * i + 6], y[8 * i + 7]));
     }
-  } else {
-#pragma unroll
-    for (int i = 0; i < 32; i++)
-      if (i < left) to[i] = (uint16_t)(pair(r ? y[i] + widen(r[i]) : y[i], 0.0f) & 0xffffu);
+    *to = make_uint4(narrow2(y[8 * i], y[8 * i + 1], bf), narrow2(y[8 * i + 2], y[8 * i + 3], bf),
+                     narrow2(y[8 * i + 4], y[8 * i + 5], bf), narrow2(y[8 * i + 6], y[8 * i + 7], bf));
   }
 }
+// the same for a packed output: one block; returns its scale byte
+__device__ __forceinline__ uint32_t stage_block(const Args& a, const float (&y)[32], uint8_t* stage, int j0, int left) {
+  const int lane = threadIdx.x & 31;
+  uint32_t top = 0;
+#pragma unroll
+  for (int i = 0; i < 32; i++) {
+    const uint32_t b = __float_as_uint(y[i]) & 0x7fffffffu;
+    if (i < left) top = max(top, b);
+  }
+  const uint32_t sb = scale_byte(top, a.ofmt);
+  const float inv = scale_inverse(sb);
+  if (a.ofmt == kFmtE2M1) {
+    uint32_t w[4];
+#pragma unroll
+    for (int i = 0; i < 4; i++) {
+      w[i] = 0;
+#pragma unroll
+      for (int j = 0; j < 4; j++)
+        w[i] |= (encode2(kFmtE2M1, scaled(y[8 * i + 2 * j], inv), scaled(y[8 * i + 2 * j + 1], inv)) & 255u) << (8 * j);
+    }
+    *reinterpret_cast<uint4*>(piece(stage, lane, j0)) = make_uint4(w[0], w[1], w[2], w[3]);
+  } else {
+    uint32_t w[8];
+#pragma unroll
+    for (int i = 0; i < 8; i++)
+      w[i] = encode2(a.ofmt, scaled(y[4 * i], inv), scaled(y[4 * i + 1], inv)) |
+             encode2(a.ofmt, scaled(y[4 * i + 2], inv), scaled(y[4 * i + 3], inv)) << 16;
+    *reinterpret_cast<uint4*>(piece(stage, lane, j0)) = make_uint4(w[0], w[1], w[2], w[3]);
+    *reinterpret_cast<uint4*>(piece(stage, lane, j0 + 1)) = make_uint4(w[4], w[5], w[6], w[7]);
+  }
+  return sb;
+}
 
-// Warp 0 loads the codes, warp 1 issues the products, warps 2-3 bring the scales, warps 4-7 write y.
+// Warp 0 loads the codes, warp 1 of the pair's first CTA issues the products, warps 2-3 bring the scales, warps 4-11 write
+// y: two per lane quarter, each with units of 64 columns.
 //
-// TMEM (512 columns): two accumulators of 256 that share 64 columns, [0, 256) and [192, 448), and the stages' scale
-// words in [448, 512). The epilogue of a tile drains the shared columns first and then lets the next tile's products
-// start, so three quarters of it run beside them.
+// TMEM (512 columns, the same in both CTAs): two accumulators of 256 that share 64 columns, [0, 256) and [192, 448), and
+// the stages' scale words in [448, 508). The epilogue of a tile drains the shared columns first and then lets the next
+// tile's products start, so three quarters of it run beside them.
 template <bool GATED>
-__global__ void __launch_bounds__(256, 1) k_mx_tile(const __grid_constant__ CUtensorMap mx, const __grid_constant__ CUtensorMap mw,
-                                                    const __grid_constant__ Args a) {
+__global__ void __launch_bounds__(128 + 32 * kWriters, 1) __cluster_dims__(2, 1, 1)
+    k_mx_tile(const __grid_constant__ CUtensorMap mx, const __grid_constant__ CUtensorMap mw, const __grid_constant__ Args a) {
   extern __shared__ uint8_t raw[];
   uint8_t* codes = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(raw) + 1023) & ~(uintptr_t)1023);
   uint8_t* scales = codes + kStages * kStageBytes;
-  TileShared& sh = *reinterpret_cast<TileShared*>(scales + kStages * kStageScales);
+  uint8_t* passes = scales + kStages * kStageScales;
+  TileShared& sh = *reinterpret_cast<TileShared*>(passes + kWriters * kPassBytes);
   int* first = reinterpret_cast<int*>(&sh + 1);
   volatile int* abort = &sh.abort;
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int warp = __shfl_sync(~0u, threadIdx.x >> 5, 0), lane = threadIdx.x & 31;
   constexpr int kCols = GATED ? 128 : 256;             // columns of y per tile
   const int col_tiles = (a.width + kCols - 1) / kCols;
+  cg::cluster_group cluster = cg::this_cluster();
+  const int rank = (int)cluster.block_rank(), pair = blockIdx.x >> 1, pairs = gridDim.x >> 1;
 
   if (threadIdx.x == 0) {
     for (int i = 0; i < kStages; i++) {
-      mbar_init(&sh.full[i], 3);                       // the codes' bytes and the two scale warps
+      mbar_init(&sh.full[i], 5);                       // the first CTA's: the codes' bytes, both CTAs' scale warps
       mbar_init(&sh.empty[i], 1);
     }
     mbar_init(&sh.acc_full, 1);
-    mbar_init(&sh.acc_free, 4);
+    mbar_init(&sh.acc_free, 2 * kWriters);             // the first CTA's: both CTAs' epilogue warps
     mbar_init(&sh.last, 1);
     sh.abort = 0;
     fence_mbar_init();
   }
-  if (warp == 1) tc::tmem_alloc(&sh.tmem, 512);
-  if (warp == 2 && a.experts) count_tiles(first, a, 128, col_tiles);
+  if (warp == 1) tc::tmem_alloc<true>(&sh.tmem, 512);
+  if (warp == 2 && a.experts) count_tiles(first, a, 256, col_tiles);
   tc::fence_before();
-  __syncthreads();
+  cluster.sync();
   tc::fence_after();
   const uint32_t tmem = sh.tmem;
+  const uint32_t full = tc::remote(sh.full, 0);
   // the second half of a tile's w rows: the up projections, or the next 128 features
   const int second = GATED ? a.width : 128;
 
@@ -397,23 +427,23 @@ __global__ void __launch_bounds__(256, 1) k_mx_tile(const __grid_constant__ CUte
     bool ok = true;
     Tile t;
     int sent = 0;
-    for (int i = blockIdx.x; ok && find_tile(i, a, first, 128, col_tiles, t); i += gridDim.x) {
+    for (int i = pair; ok && find_tile(i, a, first, 256, col_tiles, t); i += pairs) {
       int4 rows = make_int4(0, 0, 0, 0);
-      if (a.per > 0) rows = make_int4(x_row(a, t, 4 * lane), x_row(a, t, 4 * lane + 1), x_row(a, t, 4 * lane + 2), x_row(a, t, 4 * lane + 3));
-      const int w0 = t.expert * a.n + t.col * kCols;
+      const int r0 = rank * 128 + 4 * lane;
+      if (a.per > 0) rows = make_int4(x_row(a, t, r0), x_row(a, t, r0 + 1), x_row(a, t, r0 + 2), x_row(a, t, r0 + 3));
+      const int w0 = t.expert * a.n + t.col * kCols + (rank ? second : 0);
       for (int kb = 0; kb < a.kblocks; kb++) {
-        if (a.per > 0 || lane == 0) ok = tc::wait(&sh.empty[ring.stage], ring.phase ^ 1u, abort, a.status);
-        ok = __all_sync(~0u, ok);
+        ok = tc::wait_warp(&sh.empty[ring.stage], ring.phase ^ 1u, abort, a.status);
         if (!ok) break;
         uint8_t* to = codes + ring.stage * kStageBytes;
-        uint64_t* bar = &sh.full[ring.stage];
-        if (lane == 0) {
-          mbar_expect_tx(bar, 128 * a.xbytes + 256 * a.wbytes);
-          if (a.per == 0) tma_load_2d(to, &mx, kb * 128, t.row0, bar);
-          tma_load_2d(to + kTileBytes, &mw, kb * 128, w0, bar);
-          tma_load_2d(to + 2 * kTileBytes, &mw, kb * 128, w0 + second, bar);
+        const uint32_t bar = full + 8u * ring.stage;
+        if (tc::elect()) {
+          if (rank == 0) mbar_expect_tx(&sh.full[ring.stage], 256 * (a.xbytes + a.wbytes));
+          if (a.per == 0) tc::tma_load_pair(to, &mx, kb * 128, t.row0 + rank * 128, bar);
+          tc::tma_load_pair(to + kTileBytes, &mw, kb * 128, w0, bar);
         }
-        if (a.per > 0) tc::tma_gather4(to + lane * 512, &mx, kb * 128, rows, bar);
+        __syncwarp();
+        if (a.per > 0) tc::tma_gather4_pair(to + lane * 512, &mx, kb * 128, rows, bar);
         ring.next(kStages);
         sent++;
       }
@@ -424,36 +454,38 @@ __global__ void __launch_bounds__(256, 1) k_mx_tile(const __grid_constant__ CUte
         tc::settle(&sh.full[ring.stage], ring.phase);
       }
   } else if (warp == 1) {
-    if (lane == 0) {
+    if (rank == 0) {
       Ring ring;
       bool ok = true;
       Tile t;
       int done = 0;
-      for (int i = blockIdx.x; ok && find_tile(i, a, first, 128, col_tiles, t); i += gridDim.x, done++) {
-        if (done) ok = tc::wait(&sh.acc_free, (done - 1) & 1, abort, a.status);
+      for (int i = pair; ok && find_tile(i, a, first, 256, col_tiles, t); i += pairs, done++) {
+        if (done) ok = tc::wait_warp(&sh.acc_free, (done - 1) & 1, abort, a.status);
         if (!ok) break;
-        tc::fence_after();
         const uint32_t acc = tmem + (done & 1 ? 192 : 0);
         for (int kb = 0; kb < a.kblocks; kb++) {
-          ok = tc::wait(&sh.full[ring.stage], ring.phase, abort, a.status);
+          ok = tc::wait_warp(&sh.full[ring.stage], ring.phase, abort, a.status);
           if (!ok) break;
           tc::fence_after();
           const uint32_t at = smem_addr(codes + ring.stage * kStageBytes);
           const uint32_t sc = smem_addr(scales + ring.stage * kStageScales);
           const uint32_t ts = tmem + 448 + ring.stage * 12;
-#pragma unroll
-          for (int j = 0; j < 3; j++) tc::copy_scales(ts + 4 * j, tc::scale_desc(sc + 512 * j));
           const uint64_t da = tc::operand_desc(at), db = tc::operand_desc(at + kTileBytes);
+          if (tc::elect()) {
 #pragma unroll
-          for (int j = 0; j < 4; j++)                  // 32 codes further: 2 units of 16 bytes
-            tc::mma(acc, da + 2 * j, db + 2 * j, tc::mma_desc_step(a.idesc, j), ts, ts + 4, kb > 0 || j > 0);
-          tc::commit(&sh.empty[ring.stage]);
+            for (int j = 0; j < 3; j++) tc::copy_scales<true>(ts + 4 * j, tc::scale_desc(sc + 512 * j));
+#pragma unroll
+            for (int j = 0; j < 4; j++)                // 32 codes further: 2 units of 16 bytes
+              tc::mma<true>(acc, da + 2 * j, db + 2 * j, tc::mma_desc_step(a.idesc, j), ts, ts + 4, kb > 0 || j > 0);
+            tc::commit<true>(&sh.empty[ring.stage]);
+            if (kb == a.kblocks - 1) tc::commit<true>(&sh.acc_full);
+          }
+          __syncwarp();
           ring.next(kStages);
         }
-        if (ok) tc::commit(&sh.acc_full);
       }
-      if (!ok) {
-        tc::commit(&sh.last);
+      if (!ok && tc::elect()) {
+        tc::commit<true>(&sh.last);
         tc::settle(&sh.last, 0);
       }
     }
@@ -462,7 +494,7 @@ __global__ void __launch_bounds__(256, 1) k_mx_tile(const __grid_constant__ CUte
     Tile t;
     // 384 rows of words, 12 per lane in two warps: x's 128, w's 256
     const int half = warp - 2;
-    for (int i = blockIdx.x; find_tile(i, a, first, 128, col_tiles, t); i += gridDim.x) {
+    for (int i = pair; find_tile(i, a, first, 256, col_tiles, t); i += pairs) {
       const uint8_t* rows[6];
       uint32_t place[6];
 #pragma unroll
@@ -470,70 +502,115 @@ __global__ void __launch_bounds__(256, 1) k_mx_tile(const __grid_constant__ CUte
         const int r = (j * 2 + half) * 32 + lane;
         place[j] = scale_place(r);
         if (r < 128)
-          rows[j] = a.sx + (int64_t)x_row(a, t, r) * a.nb;
+          rows[j] = a.sx + (int64_t)x_row(a, t, rank * 128 + r) * a.nb;
         else
           rows[j] = w_scales(a, t, t.col * kCols + (r < 256 ? r - 128 : r - 256 + second));
       }
-      if (!stage_scales<6>(rows, place, 0, a.kblocks, a, scales, kStageScales, sh.full, sh.empty, ring, kStages, abort)) break;
+      if (!stage_scales<6>(rows, place, 0, a.kblocks, a, scales, kStageScales, sh.full, rank ? full : 0u, sh.empty, ring, kStages, abort)) break;
     }
   } else {
     Tile t;
     int done = 0;
-    const int q = warp - 4;
-    constexpr int kChunks = kCols / 32;
-    for (int i = blockIdx.x; find_tile(i, a, first, 128, col_tiles, t); i += gridDim.x, done++) {
+    const int q = warp & 3, set = (warp - 4) >> 2;     // lane quarter; which of its two warps
+    uint8_t* stage = passes + (warp - 4) * kPassBytes;
+    const uint32_t acc_free = tc::remote(&sh.acc_free, 0);
+    constexpr int kUnits = kCols / 64;
+    const int size = a.otype == kOutF32 ? 4 : a.otype == kOutPacked ? 1 : 2;
+    const bool nib = a.otype == kOutPacked && a.ofmt == kFmtE2M1;
+    for (int i = pair; find_tile(i, a, first, 256, col_tiles, t); i += pairs, done++) {
       const bool ok = tc::wait(&sh.acc_full, done & 1, abort, a.status);
       __syncwarp();
       tc::fence_after();
+      // the second warps' word that they are through with the tile before; the first warps give theirs below
+      if (set == 1 && lane == 0) tc::mbar_arrive_remote(acc_free);
       const uint32_t acc = tmem + (done & 1 ? 192 : 0) + ((uint32_t)(q * 32) << 16);
-      const int r = q * 32 + lane;
+      const int row = t.row0 + rank * 128 + q * 32;    // the warp's first
+      const int rows = min(32, t.rows - rank * 128 - q * 32);
       const float* bias = a.bias ? a.bias + (int64_t)t.expert * a.n : nullptr;
 #pragma unroll 1
-      for (int c = 0; c < kChunks; c++) {
-        // the columns shared with the other accumulator first: the first one's last 64, the second one's first 64
-        const int chunk = done & 1 ? c : (c + kChunks - 2) % kChunks;
-        const int col = t.col * kCols + chunk * 32;
-        float y[32];
-        tc::load32(acc + chunk * 32, y);
-        if (GATED) {
-          float up[32];
-          tc::load32(acc + 128 + chunk * 32, up);
-          if (bias) {
+      for (int u = 0; u < kUnits / 2; u++) {
+        // units in turn from the columns that the accumulators share on: the first accumulator's last unit, the second's first
+        const int unit = ((done & 1 ? 0 : kUnits - 1) + 2 * u + set) % kUnits;
+        const int col0 = t.col * kCols + unit * 64;
+        const bool live = rows > 0 && col0 < a.width;
+        uint32_t sb = 0;
+#pragma unroll 1
+        for (int c = 0; c < 2; c++) {
+          const int col = col0 + c * 32, at = unit * 64 + c * 32;
+          if (live && a.residual && (c == 0 || size == 4) && col < a.width) {
+            const int w = size == 4 ? 32 : 64;
+            move_rows<false>(stage, const_cast<uint8_t*>(static_cast<const uint8_t*>(a.residual)) + (row * a.residual_stride + col) * size,
+                             a.residual_stride * size, rows, min(w, a.width - col) * size, 128, size, a.vec_out);
+            __syncwarp();
+          }
+          float y[32];
+          tc::load32(acc + at, y);
+          if (GATED) {
+            float up[32];
+            tc::load32(acc + 128 + at, up);
+            if (bias) {
 #pragma unroll
-            for (int j = 0; j < 32; j++) {
-              const int n = min(col + j, a.width - 1);
-              y[j] += __ldg(bias + n);
-              up[j] += __ldg(bias + a.width + n);
+              for (int j = 0; j < 32; j++) {
+                const int n = min(col + j, a.width - 1);
+                y[j] += __ldg(bias + n);
+                up[j] += __ldg(bias + a.width + n);
+              }
             }
-          }
-          activate(a.act, y);
+            activate(a.act, y);
 #pragma unroll
-          for (int j = 0; j < 32; j++) y[j] *= up[j];
+            for (int j = 0; j < 32; j++) y[j] *= up[j];
+          } else {
+            if (bias) {
+#pragma unroll
+              for (int j = 0; j < 32; j++) y[j] += __ldg(bias + min(col + j, a.width - 1));
+            }
+            activate(a.act, y);
+          }
+          if (set == 0 && u == 0 && c == 1) {          // the next tile's products may start
+            tc::fence_before();
+            __syncwarp();
+            if (lane == 0) tc::mbar_arrive_remote(acc_free);
+          }
+          if (!ok) {
+#pragma unroll
+            for (int j = 0; j < 32; j++) y[j] = __uint_as_float(0x7fc00000u);
+          }
+          if (!live) continue;
+          if (a.otype == kOutPacked)
+            sb |= stage_block(a, y, stage, nib ? c : 2 * c, a.width - col) << (8 * c);
+          else
+            stage_row(a, y, stage, size == 4 ? 0 : 4 * c);
+          if (size == 4 && col < a.width) {
+            __syncwarp();
+            move_rows<true>(stage, static_cast<uint8_t*>(a.out) + (row * a.out_pitch + col) * 4, a.out_pitch * 4, rows,
+                            min(32, a.width - col) * 4, 128, 4, a.vec_out);
+            __syncwarp();
+          }
+        }
+        if (!live || size == 4) continue;
+        __syncwarp();
+        const int left = min(64, a.width - col0);
+        if (a.otype == kOutPacked) {
+          move_rows<true>(stage, static_cast<uint8_t*>(a.out) + row * a.out_pitch + (nib ? col0 >> 1 : col0), a.out_pitch, rows,
+                          nib ? left >> 1 : left, nib ? 32 : 64, 1, a.vec_out);
+          if (lane < rows) {
+            uint8_t* to = a.out_scales + (row + lane) * a.out_nb + (col0 >> 5);
+            to[0] = (uint8_t)sb;
+            if (left > 32) to[1] = (uint8_t)(sb >> 8);
+          }
         } else {
-          if (bias) {
-#pragma unroll
-            for (int j = 0; j < 32; j++) y[j] += __ldg(bias + min(col + j, a.width - 1));
-          }
-          activate(a.act, y);
+          move_rows<true>(stage, static_cast<uint8_t*>(a.out) + (row * a.out_pitch + col0) * 2, a.out_pitch * 2, rows, left * 2, 128, 2,
+                          a.vec_out);
         }
-        if (c == 1) {                                  // the next tile's products may start
-          tc::fence_before();
-          __syncwarp();
-          if (lane == 0) tc::mbar_arrive(&sh.acc_free);
-        }
-        if (!ok) {
-#pragma unroll
-          for (int j = 0; j < 32; j++) y[j] = __uint_as_float(0x7fc00000u);
-        }
-        if (r < t.rows && col < a.width) write_row(a, y, (int64_t)t.row0 + r, col);
+        __syncwarp();
       }
     }
   }
   __syncwarp();
   tc::fence_before();
-  __syncthreads();
+  cluster.sync();
   tc::fence_after();
-  if (warp == 1) tc::tmem_free(tmem, 512);
+  if (warp == 1) tc::tmem_free<true>(tmem, 512);
 }
 
 // ------------------------------------------------------------------------------------------------- few rows
@@ -597,7 +674,7 @@ __global__ void __launch_bounds__(128, 2) k_mx_rows(const __grid_constant__ CUte
   RowsShared& sh = *reinterpret_cast<RowsShared*>(scales + S::kDepth * S::kStageScales);
   int* first = reinterpret_cast<int*>(&sh + 1);
   volatile int* abort = &sh.abort;
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int warp = __shfl_sync(~0u, threadIdx.x >> 5, 0), lane = threadIdx.x & 31;
   constexpr int kCols = GATED ? 64 : 128;              // columns of y per tile
   const int col_tiles = (a.width + kCols - 1) / kCols;
   cg::cluster_group cluster = cg::this_cluster();
@@ -613,7 +690,7 @@ __global__ void __launch_bounds__(128, 2) k_mx_rows(const __grid_constant__ CUte
     sh.abort = 0;
     fence_mbar_init();
   }
-  if (warp == 1) tc::tmem_alloc(&sh.tmem, S::kTmem);
+  if (warp == 1) tc::tmem_alloc<false>(&sh.tmem, S::kTmem);
   if (warp == 2 && a.experts) count_tiles(first, a, BN, col_tiles);
   tc::fence_before();
   __syncthreads();
@@ -633,17 +710,17 @@ __global__ void __launch_bounds__(128, 2) k_mx_rows(const __grid_constant__ CUte
       rows = make_int4(x_row(a, t, 4 * lane), x_row(a, t, 4 * lane + 1), x_row(a, t, 4 * lane + 2), x_row(a, t, 4 * lane + 3));
     const int w0 = t.expert * a.n + t.col * kCols;
     for (int kb = k0; kb < k1; kb++) {
-      if (a.per > 0 || lane == 0) ok = tc::wait(&sh.empty[ring.stage], ring.phase ^ 1u, abort, a.status);
-      ok = __all_sync(~0u, ok);
+      ok = tc::wait_warp(&sh.empty[ring.stage], ring.phase ^ 1u, abort, a.status);
       if (!ok) break;
       uint8_t* to = codes + ring.stage * S::kStageCodes;
       uint64_t* bar = &sh.full[ring.stage];
-      if (lane == 0) {
+      if (tc::elect()) {
         mbar_expect_tx(bar, 128 * a.wbytes + BN * a.xbytes);
         tma_load_2d(to, &mw, kb * 128, w0, bar);
         if (GATED) tma_load_2d(to + kTileBytes / 2, &mw, kb * 128, w0 + a.width, bar);
         if (a.per == 0) tma_load_2d(to + kTileBytes, &mx, kb * 128, t.row0, bar);
       }
+      __syncwarp();
       if (a.per > 0 && lane < BN / 4) tc::tma_gather4(to + kTileBytes + lane * 512, &mx, kb * 128, rows, bar);
       ring.next(S::kDepth);
       sent++;
@@ -654,31 +731,31 @@ __global__ void __launch_bounds__(128, 2) k_mx_rows(const __grid_constant__ CUte
         tc::settle(&sh.full[ring.stage], ring.phase);
       }
   } else if (busy && warp == 1) {
-    if (lane == 0) {
-      Ring ring;
-      bool ok = true;
-      for (int kb = k0; kb < k1; kb++) {
-        ok = tc::wait(&sh.full[ring.stage], ring.phase, abort, a.status);
-        if (!ok) break;
-        tc::fence_after();
-        const uint32_t at = smem_addr(codes + ring.stage * S::kStageCodes);
-        const uint32_t sc = smem_addr(scales + ring.stage * S::kStageScales);
-        const uint32_t ts = tmem + S::kAcc + ring.stage * 8;
-        tc::copy_scales(ts, tc::scale_desc(sc));
-        tc::copy_scales(ts + 4, tc::scale_desc(sc + 512));
-        const uint64_t da = tc::operand_desc(at), db = tc::operand_desc(at + kTileBytes);
+    Ring ring;
+    bool ok = true;
+    for (int kb = k0; kb < k1; kb++) {
+      ok = tc::wait_warp(&sh.full[ring.stage], ring.phase, abort, a.status);
+      if (!ok) break;
+      tc::fence_after();
+      const uint32_t at = smem_addr(codes + ring.stage * S::kStageCodes);
+      const uint32_t sc = smem_addr(scales + ring.stage * S::kStageScales);
+      const uint32_t ts = tmem + S::kAcc + ring.stage * 8;
+      const uint64_t da = tc::operand_desc(at), db = tc::operand_desc(at + kTileBytes);
+      if (tc::elect()) {
+        tc::copy_scales<false>(ts, tc::scale_desc(sc));
+        tc::copy_scales<false>(ts + 4, tc::scale_desc(sc + 512));
 #pragma unroll
         for (int j = 0; j < 4; j++)
-          tc::mma(tmem, da + 2 * j, db + 2 * j, tc::mma_desc_step(a.idesc, j), ts, ts + 4, kb > k0 || j > 0);
-        tc::commit(&sh.empty[ring.stage]);
-        ring.next(S::kDepth);
+          tc::mma<false>(tmem, da + 2 * j, db + 2 * j, tc::mma_desc_step(a.idesc, j), ts, ts + 4, kb > k0 || j > 0);
+        tc::commit<false>(&sh.empty[ring.stage]);
+        if (kb == k1 - 1) tc::commit<false>(&sh.acc_full);
       }
-      if (ok) {
-        tc::commit(&sh.acc_full);
-      } else {
-        tc::commit(&sh.last);
-        tc::settle(&sh.last, 0);
-      }
+      __syncwarp();
+      ring.next(S::kDepth);
+    }
+    if (!ok && tc::elect()) {
+      tc::commit<false>(&sh.last);
+      tc::settle(&sh.last, 0);
     }
   } else if (busy) {
     constexpr int W = (128 + (BN < 32 ? 32 : BN) + 63) / 64;
@@ -696,7 +773,7 @@ __global__ void __launch_bounds__(128, 2) k_mx_rows(const __grid_constant__ CUte
         rows[j] = w_scales(a, t, t.col * kCols + (GATED && r >= 64 ? a.width + r - 64 : r));
     }
     Ring ring;
-    stage_scales<W>(rows, place, k0, k1, a, scales, S::kStageScales, sh.full, sh.empty, ring, S::kDepth, abort);
+    stage_scales<W>(rows, place, k0, k1, a, scales, S::kStageScales, sh.full, 0u, sh.empty, ring, S::kDepth, abort);
   }
   __syncwarp();
 
@@ -742,7 +819,7 @@ __global__ void __launch_bounds__(128, 2) k_mx_rows(const __grid_constant__ CUte
     }
   }
   if (split > 1) cluster.sync(); else __syncthreads();  // the partial sums are read before their CTA leaves
-  if (warp == 1) tc::tmem_free(tmem, S::kTmem);
+  if (warp == 1) tc::tmem_free<false>(tmem, S::kTmem);
 }
 
 // --------------------------------------------------------------------------------------------------- host
@@ -803,12 +880,12 @@ int launch_tile(Args& a, const Operand& x, const Operand& w, int64_t K, int64_t 
   CUtensorMap mx, mw;
   if (int rc = map_of(&mx, x, K, a.per > 0 ? 1 : 128)) return rc;
   if (int rc = map_of(&mw, w, K, 128)) return rc;
-  a.idesc = tc::mma_desc(fx, fw, 128, 256);
+  a.idesc = tc::mma_desc(fx, fw, 256, 256);
   const int smem = kTileSmem + (a.experts ? 4 * (a.experts + 1) : 0);
   auto f = k_mx_tile<GATED>;
   if (int rc = set_smem(f, kTileSmem + 4 * (kMostExperts + 1))) return rc;
-  const unsigned grid = (unsigned)(tiles < sm_count() ? tiles : sm_count());
-  f<<<grid, 256, smem, st>>>(mx, mw, a);
+  const int64_t pairs = sm_count() / 2;
+  f<<<(unsigned)(2 * (tiles < pairs ? tiles : pairs)), 128 + 32 * kWriters, smem, st>>>(mx, mw, a);
   return MXQ_LAUNCH_CHECK("product");
 }
 
@@ -821,7 +898,7 @@ int launch(Args& a, const Operand& x, const Operand& w, int64_t K, int fx, int f
   const int64_t groups = a.experts ? (a.experts < a.rows ? a.experts : a.rows) : 1;
   if (share > 128) {
     const int64_t cols = up_div(a.width, GATED ? 128 : 256);
-    const int64_t tiles = (a.experts ? a.rows / 128 + groups : up_div(a.rows, 128)) * cols;
+    const int64_t tiles = (a.experts ? a.rows / 256 + groups : up_div(a.rows, 256)) * cols;
     return launch_tile<GATED>(a, x, w, K, tiles, fx, fw, st);
   }
   const int bn = share <= 16 ? 16 : share <= 32 ? 32 : share <= 64 ? 64 : 128;

@@ -13,31 +13,27 @@
 namespace mxq {
 namespace tc {
 
-// how long a wait may take: a correct one takes microseconds
-constexpr unsigned long long kWaitNs = 2000000000ull;
+// how many cycles a wait may take, about two seconds: a correct one takes microseconds
+constexpr long long kWaitCycles = 4000000000ll;
 
-__device__ __forceinline__ unsigned long long now_ns() {
-  unsigned long long t;
-  asm volatile("mov.u64 %0, %globaltimer;\n" : "=l"(t));
-  return t;
-}
+__device__ __forceinline__ bool try_wait(uint64_t* bar, unsigned parity) { return mbar_try_wait_rounds(bar, parity, 1); }
 
 // false: gave up (this wait ran out, or another role's did)
 __device__ __forceinline__ bool wait(uint64_t* bar, unsigned parity, volatile int* abort, unsigned* status_word) {
-  if (mbar_try_wait_rounds(bar, parity, 4)) return true;
-  const unsigned long long begin = now_ns();
+  if (try_wait(bar, parity) || try_wait(bar, parity)) return true;
+  const long long begin = clock64();
   do {
-    if (mbar_try_wait_rounds(bar, parity, 4)) return true;
+    if (try_wait(bar, parity) || try_wait(bar, parity)) return true;
     if (*abort) return false;
-  } while (now_ns() - begin < kWaitNs);
+  } while (clock64() - begin < kWaitCycles);
   *abort = 1;
   note_wait_timeout(status_word);
   return false;
 }
 // the same for what a role that gave up has in flight towards shared memory or TMEM, without the abort word
 __device__ __forceinline__ void settle(uint64_t* bar, unsigned parity) {
-  const unsigned long long begin = now_ns();
-  while (!mbar_try_wait_rounds(bar, parity, 4) && now_ns() - begin < kWaitNs / 20) {
+  const long long begin = clock64();
+  while (!try_wait(bar, parity) && clock64() - begin < kWaitCycles / 20) {
   }
 }
 
@@ -45,17 +41,52 @@ __device__ __forceinline__ void mbar_arrive(uint64_t* bar) {
   asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];\n" ::"r"(smem_addr(bar)) : "memory");
 }
 
+// wait() by a whole warp: the answer is the same in every lane, and the compiler knows it
+__device__ __forceinline__ bool wait_warp(uint64_t* bar, unsigned parity, volatile int* abort, unsigned* status_word) {
+  return __all_sync(0xffffffffu, wait(bar, parity, abort, status_word));
+}
+// one lane of a converged warp. The operands of what it issues have to be warp-uniform for the compiler (no lane index
+// in them, no branch on one around them): tcgen05 and TMA instructions take uniform registers, and from a branch on
+// the lane each of their operands is moved there one by one, about 65 cycles per instruction.
+__device__ __forceinline__ bool elect() {
+  unsigned yes;
+  asm volatile("{\n .reg .pred p;\n elect.sync _|p, 0xffffffff;\n selp.u32 %0, 1, 0, p;\n}\n" : "=r"(yes));
+  return yes;
+}
+
+// the same barrier in CTA `rank` of the cluster, and an arrival there
+__device__ __forceinline__ uint32_t remote(const void* p, uint32_t rank) {
+  uint32_t r;
+  asm volatile("mapa.shared::cluster.u32 %0, %1, %2;\n" : "=r"(r) : "r"(smem_addr(p)), "r"(rank));
+  return r;
+}
+// Its release reaches this CTA's threads only: what the other CTA's tensor core is to read has to be in shared memory
+// before (fence_proxy_async ends when it is). A release for the cluster here waits for everything that the SM has under
+// way, measured 1900 cycles a time.
+__device__ __forceinline__ void mbar_arrive_remote(uint32_t bar) {
+  asm volatile("mbarrier.arrive.shared::cluster.b64 _, [%0];\n" ::"r"(bar) : "memory");
+}
+
 __device__ __forceinline__ void fence_before() { asm volatile("tcgen05.fence::before_thread_sync;\n" ::: "memory"); }
 __device__ __forceinline__ void fence_after() { asm volatile("tcgen05.fence::after_thread_sync;\n" ::: "memory"); }
 
-// one whole warp; the address lands in shared memory
+// one whole warp (PAIR: one of each CTA of the pair); the address lands in shared memory
+template <bool PAIR>
 __device__ __forceinline__ void tmem_alloc(uint32_t* where, uint32_t cols) {
-  asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;\n" ::"r"(smem_addr(where)), "r"(cols)
-               : "memory");
-  asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;\n");
+  if (PAIR) {
+    asm volatile("tcgen05.alloc.cta_group::2.sync.aligned.shared::cta.b32 [%0], %1;\n" ::"r"(smem_addr(where)), "r"(cols) : "memory");
+    asm volatile("tcgen05.relinquish_alloc_permit.cta_group::2.sync.aligned;\n");
+  } else {
+    asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;\n" ::"r"(smem_addr(where)), "r"(cols) : "memory");
+    asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;\n");
+  }
 }
+template <bool PAIR>
 __device__ __forceinline__ void tmem_free(uint32_t addr, uint32_t cols) {
-  asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;\n" ::"r"(addr), "r"(cols));
+  if (PAIR)
+    asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, %1;\n" ::"r"(addr), "r"(cols));
+  else
+    asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;\n" ::"r"(addr), "r"(cols));
 }
 
 // K-major operand tile, rows of 128 bytes in the 128-byte swizzle: groups of 8 rows 1024 bytes apart
@@ -75,23 +106,43 @@ __host__ __device__ constexpr uint32_t mma_desc(int fa, int fb, int m, int n) {
 }
 __device__ __forceinline__ uint32_t mma_desc_step(uint32_t d, uint32_t byte) { return d | (byte << 4) | (byte << 29); }
 
-// 128 rows' scale words (4 E8M0 bytes each, shared memory (row % 32) * 16 + (row / 32) * 4) into 4 TMEM columns
+// 128 rows' scale words (4 E8M0 bytes each, shared memory (row % 32) * 16 + (row / 32) * 4) into 4 TMEM columns. PAIR:
+// in both CTAs, each from its own shared memory.
+template <bool PAIR>
 __device__ __forceinline__ void copy_scales(uint32_t tmem, uint64_t desc) {
-  asm volatile("tcgen05.cp.cta_group::1.32x128b.warpx4 [%0], %1;\n" ::"r"(tmem), "l"(desc) : "memory");
+  if (PAIR)
+    asm volatile("tcgen05.cp.cta_group::2.32x128b.warpx4 [%0], %1;\n" ::"r"(tmem), "l"(desc) : "memory");
+  else
+    asm volatile("tcgen05.cp.cta_group::1.32x128b.warpx4 [%0], %1;\n" ::"r"(tmem), "l"(desc) : "memory");
 }
 
+// PAIR: 256 rows of A, 128 in each CTA, which also holds half of B's rows; D's rows are in the CTA of their A rows
+template <bool PAIR>
 __device__ __forceinline__ void mma(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, uint32_t sa, uint32_t sb,
                                     bool accumulate) {
-  asm volatile(
-      "{\n .reg .pred p;\n setp.ne.b32 p, %6, 0;\n"
-      " tcgen05.mma.cta_group::1.kind::mxf8f6f4.block_scale.scale_vec::1X [%0], %1, %2, %3, [%4], [%5], p;\n}\n" ::"r"(d),
-      "l"(a), "l"(b), "r"(idesc), "r"(sa), "r"(sb), "r"((unsigned)accumulate)
-      : "memory");
+  if (PAIR)
+    asm volatile(
+        "{\n .reg .pred p;\n setp.ne.b32 p, %6, 0;\n"
+        " tcgen05.mma.cta_group::2.kind::mxf8f6f4.block_scale.scale_vec::1X [%0], %1, %2, %3, [%4], [%5], p;\n}\n" ::"r"(d),
+        "l"(a), "l"(b), "r"(idesc), "r"(sa), "r"(sb), "r"((unsigned)accumulate)
+        : "memory");
+  else
+    asm volatile(
+        "{\n .reg .pred p;\n setp.ne.b32 p, %6, 0;\n"
+        " tcgen05.mma.cta_group::1.kind::mxf8f6f4.block_scale.scale_vec::1X [%0], %1, %2, %3, [%4], [%5], p;\n}\n" ::"r"(d),
+        "l"(a), "l"(b), "r"(idesc), "r"(sa), "r"(sb), "r"((unsigned)accumulate)
+        : "memory");
 }
-// the barrier arrives when every tcgen05 operation that this thread has issued is done
+// the barrier (PAIR: of both CTAs) arrives when every tcgen05 operation that this thread has issued is done
+template <bool PAIR>
 __device__ __forceinline__ void commit(uint64_t* bar) {
-  asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];\n" ::"r"(smem_addr(bar))
-               : "memory");
+  if (PAIR)
+    asm volatile("tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.multicast::cluster.b64 [%0], %1;\n" ::"r"(
+                     smem_addr(bar)),
+                 "h"((uint16_t)3)
+                 : "memory");
+  else
+    asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];\n" ::"r"(smem_addr(bar)) : "memory");
 }
 
 // 32 columns of this warp's 32 lanes (the lane quarter warp % 4), one row per thread; the wait stands in the same
@@ -122,12 +173,27 @@ __device__ __forceinline__ void load16(uint32_t addr, float (&v)[16]) {
 #pragma unroll
   for (int i = 0; i < 16; i++) v[i] = __uint_as_float(r[i]);
 }
+// loads whose barrier (a shared::cluster address) may be in the other CTA of the pair
+__device__ __forceinline__ void tma_load_pair(void* dst, const CUtensorMap* map, int x, int y, uint32_t bar) {
+  asm volatile(
+      "cp.async.bulk.tensor.2d.cta_group::2.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3}], [%4];\n" ::
+          "r"(smem_addr(dst)),
+      "l"(map), "r"(x), "r"(y), "r"(bar)
+      : "memory");
+}
 // four rows of a tensor, 128 bytes each, one after the other in shared memory
 __device__ __forceinline__ void tma_gather4(void* dst, const CUtensorMap* map, int x, int4 rows, uint64_t* bar) {
   asm volatile(
       "cp.async.bulk.tensor.2d.shared::cta.global.tile::gather4.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4, %5, "
       "%6}], [%7];\n" ::"r"(smem_addr(dst)),
       "l"(map), "r"(x), "r"(rows.x), "r"(rows.y), "r"(rows.z), "r"(rows.w), "r"(smem_addr(bar))
+      : "memory");
+}
+__device__ __forceinline__ void tma_gather4_pair(void* dst, const CUtensorMap* map, int x, int4 rows, uint32_t bar) {
+  asm volatile(
+      "cp.async.bulk.tensor.2d.cta_group::2.shared::cluster.global.tile::gather4.mbarrier::complete_tx::bytes [%0], [%1, {%2, "
+      "%3, %4, %5, %6}], [%7];\n" ::"r"(smem_addr(dst)),
+      "l"(map), "r"(x), "r"(rows.x), "r"(rows.y), "r"(rows.z), "r"(rows.w), "r"(bar)
       : "memory");
 }
 
