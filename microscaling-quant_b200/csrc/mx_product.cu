@@ -46,15 +46,35 @@ struct Args {
   int64_t out_pitch, out_nb;
   int act, otype, ofmt;
   int vec_out;                 // y's (and the residual's) rows take 16-byte accesses
+  int vec_bias;                // so do the biases
   unsigned* status;
 };
 
 // ------------------------------------------------------------------------------------------ epilogue values
-// exp and the division here are the fast ones (a few ulp of float32): y is rounded to 16 bits or fewer, or, as float32,
-// already carries the sum's own error of that size.
-__device__ __forceinline__ float over_one_plus_exp(float x, float t) { return __fdividef(x, __fadd_rn(1.0f, __expf(t))); }
+// x / (1 + exp(t)) by the hardware's exp2 and reciprocal (a few ulp of float32, subnormal intermediates flushed): y is
+// rounded to 16 bits or fewer, or, as float32, already carries the sum's own error of that size.
+__device__ __forceinline__ float over_one_plus_exp(float x, float t) {
+  float e, r;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(e) : "f"(__fmul_rn(t, 1.4426950408889634f)));
+  asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(__fadd_rn(1.0f, e)));
+  return __fmul_rn(x, r);
+}
 __device__ __forceinline__ float silu(float x) { return over_one_plus_exp(x, -x); }
-__device__ __forceinline__ float gelu(float x) { return 0.5f * x * (1.0f + erff(x * 0.70710678118654752f)); }
+// x Phi(x), Phi by Abramowitz and Stegun's 7.1.26 for erfc (absolute error 1.5e-7): for z = |x| / sqrt(2), t = 1 / (1 + 0.3275911 z),
+// erfc(z) = (a1 t + .. + a5 t^5) exp(-z^2), and Phi is half of that below zero and one minus half of it above. A dozen
+// instructions where erff takes about forty: the epilogue's code has to stay in the instruction cache.
+__device__ __forceinline__ float gelu(float x) {
+  const float z = fabsf(x) * 0.70710678118654752f;
+  float t, e;
+  asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(t) : "f"(__fmaf_rn(0.3275911f, z, 1.0f)));
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(e) : "f"(__fmul_rn(z * z, -1.4426950408889634f)));
+  float h = __fmaf_rn(t, 0.5f * 1.061405429f, 0.5f * -1.453152027f);
+  h = __fmaf_rn(t, h, 0.5f * 1.421413741f);
+  h = __fmaf_rn(t, h, 0.5f * -0.284496736f);
+  h = __fmaf_rn(t, h, 0.5f * 0.254829592f);
+  h = h * t * e;
+  return x * (x < 0.0f ? h : 1.0f - h);
+}
 // x (1 + tanh(u)) / 2 = x / (1 + exp(-2u)), u = sqrt(2 / pi) (x + 0.044715 x^3)
 __device__ __forceinline__ float gelu_tanh(float x) {
   return over_one_plus_exp(x, -1.5957691216057308f * __fmaf_rn(0.044715f * x * x, x, x));
@@ -105,25 +125,35 @@ constexpr int kTileBytes = 128 * 128;                 // 128 rows of one K step
 
 // 16 scale bytes of a row from K step 4g on (a step has 4): 0 beyond the row
 __device__ __forceinline__ uint4 load_scales(const uint8_t* row, int g, int nb, int vec) {
+  if (vec == 16) {                                     // the line and its neighbour come to L2 at the first touch
+    uint4 v;
+    asm volatile("ld.global.nc.L2::256B.v4.u32 {%0, %1, %2, %3}, [%4];"
+                 : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w)
+                 : "l"(row + (int64_t)g * 16));
+    return v;
+  }
   uint32_t w[4];
-  if (vec == 16) return __ldg(reinterpret_cast<const uint4*>(row + (int64_t)g * 16));
+  if (vec == 4) {
+#pragma unroll
+    for (int j = 0; j < 4; j++) w[j] = g * 16 + j * 4 < nb ? __ldg(reinterpret_cast<const uint32_t*>(row + g * 16 + j * 4)) : 0u;
+    return make_uint4(w[0], w[1], w[2], w[3]);
+  }
+  // rows at any byte: the aligned words that hold a byte of the row, shifted together; what is beyond the row is cleared
+  // (a scale of the next row could be a NaN's)
+  const uint8_t* from = row + (int64_t)g * 16;
+  const int left = nb - g * 16, off = (int)(reinterpret_cast<uintptr_t>(from) & 3u);
+  const uint32_t* words = reinterpret_cast<const uint32_t*>(from - off);
+  uint32_t q[5];
+#pragma unroll
+  for (int j = 0; j < 5; j++) q[j] = 4 * j - off < left && 4 * j - off < 16 ? __ldg(words + j) : 0u;
 #pragma unroll
   for (int j = 0; j < 4; j++) {
-    const int at = g * 16 + j * 4;
-    w[j] = 0;
-    if (vec == 4) {
-      if (at < nb) w[j] = __ldg(reinterpret_cast<const uint32_t*>(row + at));
-    } else {
-#pragma unroll
-      for (int b = 0; b < 4; b++)
-        if (at + b < nb) w[j] |= (uint32_t)__ldg(row + at + b) << (8 * b);
-    }
+    w[j] = __funnelshift_r(q[j], q[j + 1], 8 * off);
+    const int have = left - 4 * j;
+    if (have < 4) w[j] = have <= 0 ? 0u : w[j] & ((1u << (8 * have)) - 1u);
   }
   return make_uint4(w[0], w[1], w[2], w[3]);
 }
-
-// place of row r's word in a stage's scale area (groups of 128 rows, 512 bytes each)
-__device__ __forceinline__ uint32_t scale_place(int r) { return (uint32_t)((r >> 7) * 512 + (r & 31) * 16 + ((r & 127) >> 5) * 4); }
 
 struct Ring {
   int stage = 0;
@@ -136,59 +166,69 @@ struct Ring {
   }
 };
 
-// One warp brings the scale words of its W rows per lane for K steps [k0, k1) into the ring: 16 bytes per row, that
-// is four steps, are read at once and the next four are on their way while these are stored. `full`: the stages'
-// barriers; far: their shared::cluster address where they are in another CTA, else 0.
-template <int W>
-__device__ __forceinline__ bool stage_scales(const uint8_t* const (&rows)[W], const uint32_t (&place)[W], int k0, int k1, const Args& a,
-                                             uint8_t* area, int pitch, uint64_t* full, uint32_t far, uint64_t* empty, Ring& ring, int stages,
-                                             volatile int* abort) {
-  uint4 now[W], nxt[W];
-  int g = k0 >> 2;
-  const int last = (k1 - 1) >> 2;
+// Scales on their way to a stage. The loader warp's lane holds, for each of G groups of 128 rows, the four rows lane, 32 +
+// lane, 64 + lane and 96 + lane: their words stand side by side in the layout that copy_scales takes, so a step costs one
+// 16-byte store per group.
+template <int G>
+struct ScaleRows {
+  const uint8_t* row[4 * G];
+  __device__ __forceinline__ void load(uint4 (&v)[4 * G], int g, const Args& a) const {
 #pragma unroll
-  for (int i = 0; i < W; i++) now[i] = load_scales(rows[i], g, a.nb, a.vec);
-  for (; g <= last; g++) {
-    if (g < last) {
-#pragma unroll
-      for (int i = 0; i < W; i++) nxt[i] = load_scales(rows[i], g + 1, a.nb, a.vec);
-    }
-#pragma unroll
-    for (int j = 0; j < 4; j++) {
-      const int kb = g * 4 + j;
-      if (kb < k0 || kb >= k1) continue;
-      if (!tc::wait(&empty[ring.stage], ring.phase ^ 1u, abort, a.status)) return false;
-      uint8_t* to = area + (size_t)ring.stage * pitch;
-#pragma unroll
-      for (int i = 0; i < W; i++)
-        *reinterpret_cast<uint32_t*>(to + place[i]) = j == 0 ? now[i].x : j == 1 ? now[i].y : j == 2 ? now[i].z : now[i].w;
-      fence_proxy_async();
-      __syncwarp();
-      if ((threadIdx.x & 31) == 0) {
-        if (far) tc::mbar_arrive_remote(far + 8u * ring.stage);
-        else tc::mbar_arrive(&full[ring.stage]);
-      }
-      ring.next(stages);
-    }
-#pragma unroll
-    for (int i = 0; i < W; i++) now[i] = nxt[i];
+    for (int i = 0; i < 4 * G; i++) v[i] = load_scales(row[i], g, a.nb, a.vec);
   }
+};
+// step j of the four that v holds, into the ring's next stage
+template <int G>
+__device__ __forceinline__ bool store_scales(const uint4 (&v)[4 * G], int j, const Args& a, uint8_t* area, int pitch, uint64_t* ready,
+                                             uint64_t* empty, Ring& ring, int stages, volatile int* abort) {
+  if (!tc::wait_warp(&empty[ring.stage], ring.phase ^ 1u, abort, a.status)) return false;
+  uint8_t* to = area + (size_t)ring.stage * pitch + (threadIdx.x & 31) * 16;
+  auto word = [j](const uint4& q) { return j == 0 ? q.x : j == 1 ? q.y : j == 2 ? q.z : q.w; };
+#pragma unroll
+  for (int i = 0; i < G; i++)
+    *reinterpret_cast<uint4*>(to + 512 * i) = make_uint4(word(v[4 * i]), word(v[4 * i + 1]), word(v[4 * i + 2]), word(v[4 * i + 3]));
+  __syncwarp();
+  if (tc::elect()) tc::mbar_arrive(&ready[ring.stage]);
+  ring.next(stages);
+  return true;
+}
+// The words' way from the loader to the tensor core's view of shared memory, in a warp of its own: the fence waits for all
+// that its thread has under way, and the loader has the next loads under way. far: the full barriers' shared::cluster
+// address where they are in another CTA, else 0.
+__device__ __forceinline__ bool forward_scales(const Args& a, uint64_t* ready, uint64_t* full, uint32_t far, Ring& ring, int stages,
+                                               volatile int* abort) {
+  if (!tc::wait_warp(&ready[ring.stage], ring.phase, abort, a.status)) return false;
+  if (tc::elect()) {
+    fence_proxy_async();
+    if (far) tc::mbar_arrive_remote(far + 8u * ring.stage);
+    else tc::mbar_arrive(&full[ring.stage]);
+  }
+  __syncwarp();
+  ring.next(stages);
   return true;
 }
 
 // where expert e's rows begin, whatever the offsets hold within the product's rows
 __device__ __forceinline__ int row_begin(const Args& a, int e) { return min(max(a.offsets[e], 0), a.rows); }
 
-// The experts' tiles in order: first[e] = tiles before expert e. One warp.
-__device__ void count_tiles(int* first, const Args& a, int tile_rows, int per_row_tile) {
+// The experts' tiles in order, in shared memory: first[e] tiles are before expert e, whose rows begin at begin[e].
+struct Table {
+  int *first, *begin;
+  __device__ __forceinline__ Table(void* at, int experts) : first(static_cast<int*>(at)), begin(first + experts + 1) {}
+};
+constexpr int table_bytes(int experts) { return 8 * (experts + 1); }
+
+// one warp
+__device__ void count_tiles(const Table& tab, const Args& a, int tile_rows, int per_row_tile) {
   const int lane = threadIdx.x & 31;
   int carry = 0;
   for (int base = 0; base < a.experts; base += 32) {
     const int e = base + lane;
     int t = 0;
     if (e < a.experts) {
-      const int c = row_begin(a, e + 1) - row_begin(a, e);
+      const int b = row_begin(a, e), c = row_begin(a, e + 1) - b;
       t = (c > 0 ? (c + tile_rows - 1) / tile_rows : 0) * per_row_tile;
+      tab.begin[e] = b;
     }
     int s = t;
 #pragma unroll
@@ -196,45 +236,41 @@ __device__ void count_tiles(int* first, const Args& a, int tile_rows, int per_ro
       const int up = __shfl_up_sync(~0u, s, d);
       if (lane >= d) s += up;
     }
-    if (e < a.experts) first[e + 1] = carry + s;
+    if (e < a.experts) tab.first[e + 1] = carry + s;
     carry += __shfl_sync(~0u, s, 31);
   }
-  if (lane == 0) first[0] = 0;
+  if (lane == 0) {
+    tab.first[0] = 0;
+    tab.begin[a.experts] = row_begin(a, a.experts);
+  }
 }
 
+// Tile t: by expert, then column tile, then row tile, so that the CTAs at work at one time share w's tiles. Dense: row
+// tiles in bands of 8 for the same reason. Callers ask for rising t below tile_count().
 struct Tile {
-  int expert;
+  int expert = 0;
   int row0, rows;              // first row of the product, rows of it in this tile
   int col;                     // column tile
+  __device__ __forceinline__ void find(int t, const Args& a, const Table& tab, int tile_rows, int col_tiles) {
+    if (a.experts == 0) {
+      const int row_tiles = (a.rows + tile_rows - 1) / tile_rows;
+      const int band = t / (kBand * col_tiles), in = t - band * kBand * col_tiles;
+      const int high = min(kBand, row_tiles - band * kBand);
+      col = in / high;
+      row0 = (band * kBand + in % high) * tile_rows;
+      rows = min(tile_rows, a.rows - row0);
+      return;
+    }
+    while (t >= tab.first[expert + 1]) expert++;
+    const int in = t - tab.first[expert], row_tiles = (tab.first[expert + 1] - tab.first[expert]) / col_tiles;
+    col = in / row_tiles;
+    row0 = tab.begin[expert] + (in - col * row_tiles) * tile_rows;
+    rows = min(tile_rows, tab.begin[expert + 1] - row0);
+  }
+  static constexpr int kBand = 8;
 };
-
-// Tile t: by expert, then column tile, then row tile, so that the CTAs at work at one time share w's tiles. Dense: row
-// tiles in bands of 16 for the same reason. false: no such tile.
-__device__ __forceinline__ bool find_tile(int t, const Args& a, const int* first, int tile_rows, int col_tiles, Tile& o) {
-  if (a.experts == 0) {
-    const int row_tiles = (a.rows + tile_rows - 1) / tile_rows;
-    if (t >= row_tiles * col_tiles) return false;
-    const int band = t / (16 * col_tiles), in = t - band * 16 * col_tiles;
-    const int high = min(16, row_tiles - band * 16);
-    o.expert = 0;
-    o.col = in / high;
-    o.row0 = (band * 16 + in % high) * tile_rows;
-    o.rows = min(tile_rows, a.rows - o.row0);
-    return true;
-  }
-  if (t >= first[a.experts]) return false;
-  int lo = 0, hi = a.experts;                          // first[lo] <= t < first[hi]
-  while (hi - lo > 1) {
-    const int mid = (lo + hi) >> 1;
-    if (first[mid] <= t) lo = mid; else hi = mid;
-  }
-  const int in = t - first[lo], row_tiles = (first[lo + 1] - first[lo]) / col_tiles;
-  o.expert = lo;
-  o.col = in / row_tiles;
-  const int begin = row_begin(a, lo), end = row_begin(a, lo + 1);
-  o.row0 = begin + (in % row_tiles) * tile_rows;
-  o.rows = min(tile_rows, end - o.row0);
-  return true;
+__device__ __forceinline__ int tile_count(const Args& a, const Table& tab, int tile_rows, int col_tiles) {
+  return a.experts ? tab.first[a.experts] : (a.rows + tile_rows - 1) / tile_rows * col_tiles;
 }
 
 // the row of x that row r of the product is; a row beyond the tile stands for its last one and is never written
@@ -259,7 +295,7 @@ constexpr int kWriters = 8;                            // epilogue warps
 constexpr int kPassBytes = 32 * 128;                   // what one of them stages: 32 rows of 128 bytes
 
 struct TileShared {
-  uint64_t full[kStages], empty[kStages], acc_full, acc_free, last;
+  uint64_t full[kStages], empty[kStages], ready[kStages], acc_full, acc_free, last;
   uint32_t tmem;
   int abort;
 };
@@ -268,44 +304,61 @@ constexpr int kTileSmem = 1024 + kStages * (kStageBytes + kStageScales) + kWrite
 // place of 16-byte piece j of a staged row: neighbouring rows in other banks
 __device__ __forceinline__ uint8_t* piece(uint8_t* stage, int row, int j) { return stage + row * 128 + ((j ^ (row & 7)) << 4); }
 
-// A warp's 32 rows between shared memory (128 bytes a row) and memory, each row's `bytes` (a multiple of 16 if vec) in one
-// run per row: rows below `rows` only.
-template <bool STORE>
-__device__ __forceinline__ void move_rows(uint8_t* stage, uint8_t* mem, int64_t pitch, int rows, int bytes, int width, int size, bool vec) {
+// A warp's 32 staged rows to memory, `bytes` of each of the first `rows`. P: 16-byte pieces per staged row; vec: memory takes
+// 16-byte accesses (then bytes is a multiple of 16), else it is written in elements of `size` bytes.
+template <int P>
+__device__ __forceinline__ void put_rows(uint8_t* stage, uint8_t* mem, int64_t pitch, int rows, int bytes, int size, bool vec) {
   const int lane = threadIdx.x & 31;
   if (vec) {
-    const int sh = width == 128 ? 3 : width == 64 ? 2 : 1;       // pieces per row
-    for (int i = 0; i < (1 << sh); i++) {
-      const int r = (i * 32 + lane) >> sh, j = lane & ((1 << sh) - 1);
-      if (r < rows && j * 16 < bytes) {
-        uint4* s = reinterpret_cast<uint4*>(piece(stage, r, j));
-        uint4* m = reinterpret_cast<uint4*>(mem + r * pitch + j * 16);
-        if (STORE) *m = *s; else *s = *m;
-      }
+    const int j = lane % P, r0 = lane / P;
+    uint8_t* to = mem + r0 * pitch + j * 16;
+    uint4 v[P];
+#pragma unroll
+    for (int i = 0; i < P; i++) v[i] = *reinterpret_cast<const uint4*>(piece(stage, i * (32 / P) + r0, j));
+#pragma unroll
+    for (int i = 0; i < P; i++)
+      if (i * (32 / P) + r0 < rows && j * 16 < bytes) *reinterpret_cast<uint4*>(to + i * (32 / P) * pitch) = v[i];
+    return;
+  }
+  for (int r = 0; r < rows; r++)
+    for (int b = lane * size; b < bytes; b += 32 * size) {
+      const uint8_t* from = piece(stage, r, b >> 4) + (b & 15);
+      uint8_t* to = mem + r * pitch + b;
+      if (size == 4) *reinterpret_cast<uint32_t*>(to) = *reinterpret_cast<const uint32_t*>(from);
+      else if (size == 2) *reinterpret_cast<uint16_t*>(to) = *reinterpret_cast<const uint16_t*>(from);
+      else *to = *from;
+    }
+}
+// the other way, 128 bytes a row: under way when it returns (vec), to be waited for with cp.async.wait_all
+__device__ __forceinline__ void get_rows(uint8_t* stage, const uint8_t* mem, int64_t pitch, int rows, int bytes, int size, bool vec) {
+  const int lane = threadIdx.x & 31;
+  if (vec) {
+    const int j = lane & 7, r0 = lane >> 3;
+#pragma unroll
+    for (int i = 0; i < 8; i++) {
+      const int r = i * 4 + r0;
+      if (r < rows && j * 16 < bytes)
+        asm volatile("cp.async.cg.shared.global [%0], [%1], 16;\n" ::"r"(smem_addr(piece(stage, r, j))), "l"(mem + r * pitch + j * 16)
+                     : "memory");
     }
     return;
   }
   for (int r = 0; r < rows; r++)
     for (int b = lane * size; b < bytes; b += 32 * size) {
-      uint8_t* s = piece(stage, r, b >> 4) + (b & 15);
-      uint8_t* m = mem + r * pitch + b;
-      if (size == 4) {
-        if (STORE) *reinterpret_cast<uint32_t*>(m) = *reinterpret_cast<uint32_t*>(s);
-        else *reinterpret_cast<uint32_t*>(s) = *reinterpret_cast<uint32_t*>(m);
-      } else if (size == 2) {
-        if (STORE) *reinterpret_cast<uint16_t*>(m) = *reinterpret_cast<uint16_t*>(s);
-        else *reinterpret_cast<uint16_t*>(s) = *reinterpret_cast<uint16_t*>(m);
-      } else {
-        *m = *s;
-      }
+      uint8_t* to = piece(stage, r, b >> 4) + (b & 15);
+      const uint8_t* from = mem + r * pitch + b;
+      if (size == 4) *reinterpret_cast<uint32_t*>(to) = *reinterpret_cast<const uint32_t*>(from);
+      else *reinterpret_cast<uint16_t*>(to) = *reinterpret_cast<const uint16_t*>(from);
     }
 }
 
-__device__ __forceinline__ float widen16(uint32_t h, bool bf) {
-  return bf ? __uint_as_float(h << 16) : __half2float(__ushort_as_half((unsigned short)h));
+template <int OUT>
+__device__ __forceinline__ float widen16(uint32_t h) {
+  return OUT == kOutBf16 ? __uint_as_float(h << 16) : __half2float(__ushort_as_half((unsigned short)h));
 }
-__device__ __forceinline__ uint32_t narrow2(float lo, float hi, bool bf) {
-  if (bf) {
+template <int OUT>
+__device__ __forceinline__ uint32_t narrow2(float lo, float hi) {
+  if (OUT == kOutBf16) {
     const __nv_bfloat162 p = __floats2bfloat162_rn(lo, hi);
     return *reinterpret_cast<const uint32_t*>(&p);
   }
@@ -314,78 +367,116 @@ __device__ __forceinline__ uint32_t narrow2(float lo, float hi, bool bf) {
 }
 
 // 32 columns of this lane's row into its staged row, at 16-byte piece j0 on; the residual's are there already
-__device__ __forceinline__ void stage_row(const Args& a, float (&y)[32], uint8_t* stage, int j0) {
+template <int OUT>
+__device__ __forceinline__ void stage_row(bool residual, float (&y)[32], uint8_t* stage, int j0) {
   const int lane = threadIdx.x & 31;
-  if (a.otype == kOutF32) {
+  if (OUT == kOutF32) {
+    if (residual) {
 #pragma unroll
-    for (int i = 0; i < 8; i++) {
-      float4* to = reinterpret_cast<float4*>(piece(stage, lane, j0 + i));
-      float4 v = make_float4(y[4 * i], y[4 * i + 1], y[4 * i + 2], y[4 * i + 3]);
-      if (a.residual) {
-        const float4 q = *to;
-        v = make_float4(v.x + q.x, v.y + q.y, v.z + q.z, v.w + q.w);
+      for (int i = 0; i < 8; i++) {
+        const float4 q = *reinterpret_cast<const float4*>(piece(stage, lane, j0 + i));
+        y[4 * i] += q.x;
+        y[4 * i + 1] += q.y;
+        y[4 * i + 2] += q.z;
+        y[4 * i + 3] += q.w;
       }
-      *to = v;
     }
+#pragma unroll
+    for (int i = 0; i < 8; i++)
+      *reinterpret_cast<float4*>(piece(stage, lane, j0 + i)) = make_float4(y[4 * i], y[4 * i + 1], y[4 * i + 2], y[4 * i + 3]);
     return;
   }
-  const bool bf = a.otype == kOutBf16;
+  if (residual) {
 #pragma unroll
-  for (int i = 0; i < 4; i++) {
-    uint4* to = reinterpret_cast<uint4*>(piece(stage, lane, j0 + i));
-    if (a.residual) {
-      const uint4 q = *to;
+    for (int i = 0; i < 4; i++) {
+      const uint4 q = *reinterpret_cast<const uint4*>(piece(stage, lane, j0 + i));
       const uint32_t h[4] = {q.x, q.y, q.z, q.w};
 #pragma unroll
       for (int j = 0; j < 4; j++) {
-        y[8 * i + 2 * j] += widen16(h[j] & 0xffffu, bf);
-        y[8 * i + 2 * j + 1] += widen16(h[j] >> 16, bf);
+        y[8 * i + 2 * j] += widen16<OUT>(h[j] & 0xffffu);
+        y[8 * i + 2 * j + 1] += widen16<OUT>(h[j] >> 16);
       }
     }
-    *to = make_uint4(narrow2(y[8 * i], y[8 * i + 1], bf), narrow2(y[8 * i + 2], y[8 * i + 3], bf),
-                     narrow2(y[8 * i + 4], y[8 * i + 5], bf), narrow2(y[8 * i + 6], y[8 * i + 7], bf));
   }
+#pragma unroll
+  for (int i = 0; i < 4; i++)
+    *reinterpret_cast<uint4*>(piece(stage, lane, j0 + i)) =
+        make_uint4(narrow2<OUT>(y[8 * i], y[8 * i + 1]), narrow2<OUT>(y[8 * i + 2], y[8 * i + 3]),
+                   narrow2<OUT>(y[8 * i + 4], y[8 * i + 5]), narrow2<OUT>(y[8 * i + 6], y[8 * i + 7]));
 }
-// the same for a packed output: one block; returns its scale byte
-__device__ __forceinline__ uint32_t stage_block(const Args& a, const float (&y)[32], uint8_t* stage, int j0, int left) {
+// the same for a packed output: one block, of which `left` columns exist; returns its scale byte
+template <int FMT>
+__device__ __forceinline__ uint32_t stage_block(float (&y)[32], uint8_t* stage, int c, int left) {
   const int lane = threadIdx.x & 31;
+  if (left < 32) {                                     // columns that do not exist
+#pragma unroll
+    for (int i = 0; i < 32; i++)
+      if (i >= left) y[i] = 0.0f;
+  }
   uint32_t top = 0;
 #pragma unroll
-  for (int i = 0; i < 32; i++) {
-    const uint32_t b = __float_as_uint(y[i]) & 0x7fffffffu;
-    if (i < left) top = max(top, b);
-  }
-  const uint32_t sb = scale_byte(top, a.ofmt);
+  for (int i = 0; i < 32; i++) top = max(top, __float_as_uint(y[i]) & 0x7fffffffu);
+  const uint32_t sb = scale_byte(top, FMT);
   const float inv = scale_inverse(sb);
-  if (a.ofmt == kFmtE2M1) {
+  if (sb == 255u) {
+#pragma unroll
+    for (int i = 0; i < 32; i++) y[i] = 0.0f;
+  }
+#pragma unroll
+  for (int i = 0; i < 32; i++) y[i] = __fmul_rn(y[i], inv);
+  if (FMT == kFmtE2M1) {
     uint32_t w[4];
 #pragma unroll
     for (int i = 0; i < 4; i++) {
       w[i] = 0;
 #pragma unroll
-      for (int j = 0; j < 4; j++)
-        w[i] |= (encode2(kFmtE2M1, scaled(y[8 * i + 2 * j], inv), scaled(y[8 * i + 2 * j + 1], inv)) & 255u) << (8 * j);
+      for (int j = 0; j < 4; j++) w[i] |= (encode2(FMT, y[8 * i + 2 * j], y[8 * i + 2 * j + 1]) & 255u) << (8 * j);
     }
-    *reinterpret_cast<uint4*>(piece(stage, lane, j0)) = make_uint4(w[0], w[1], w[2], w[3]);
+    *reinterpret_cast<uint4*>(piece(stage, lane, c)) = make_uint4(w[0], w[1], w[2], w[3]);
   } else {
     uint32_t w[8];
 #pragma unroll
     for (int i = 0; i < 8; i++)
-      w[i] = encode2(a.ofmt, scaled(y[4 * i], inv), scaled(y[4 * i + 1], inv)) |
-             encode2(a.ofmt, scaled(y[4 * i + 2], inv), scaled(y[4 * i + 3], inv)) << 16;
-    *reinterpret_cast<uint4*>(piece(stage, lane, j0)) = make_uint4(w[0], w[1], w[2], w[3]);
-    *reinterpret_cast<uint4*>(piece(stage, lane, j0 + 1)) = make_uint4(w[4], w[5], w[6], w[7]);
+      w[i] = encode2(FMT, y[4 * i], y[4 * i + 1]) | encode2(FMT, y[4 * i + 2], y[4 * i + 3]) << 16;
+    *reinterpret_cast<uint4*>(piece(stage, lane, 2 * c)) = make_uint4(w[0], w[1], w[2], w[3]);
+    *reinterpret_cast<uint4*>(piece(stage, lane, 2 * c + 1)) = make_uint4(w[4], w[5], w[6], w[7]);
   }
   return sb;
 }
+__device__ __forceinline__ uint32_t stage_block(int fmt, float (&y)[32], uint8_t* stage, int c, int left) {
+  switch (fmt) {
+    case kFmtE4M3: return stage_block<kFmtE4M3>(y, stage, c, left);
+    case kFmtE5M2: return stage_block<kFmtE5M2>(y, stage, c, left);
+    case kFmtE3M2: return stage_block<kFmtE3M2>(y, stage, c, left);
+    case kFmtE2M3: return stage_block<kFmtE2M3>(y, stage, c, left);
+    default: return stage_block<kFmtE2M1>(y, stage, c, left);
+  }
+}
 
-// Warp 0 loads the codes, warp 1 of the pair's first CTA issues the products, warps 2-3 bring the scales, warps 4-11 write
+// y += 32 biases from column col on
+__device__ __forceinline__ void add_bias(const Args& a, const float* bias, int col, float (&y)[32]) {
+  if (a.vec_bias && col + 32 <= a.width) {
+#pragma unroll
+    for (int i = 0; i < 8; i++) {
+      const float4 b = __ldg(reinterpret_cast<const float4*>(bias + col) + i);
+      y[4 * i] += b.x;
+      y[4 * i + 1] += b.y;
+      y[4 * i + 2] += b.z;
+      y[4 * i + 3] += b.w;
+    }
+  } else {
+#pragma unroll
+    for (int j = 0; j < 32; j++) y[j] += __ldg(bias + min(col + j, a.width - 1));
+  }
+}
+
+// Warp 0 loads the codes, warp 1 of the pair's first CTA issues the products, warps 2 and 3 bring the scales, warps 4-11 write
 // y: two per lane quarter, each with units of 64 columns.
 //
 // TMEM (512 columns, the same in both CTAs): two accumulators of 256 that share 64 columns, [0, 256) and [192, 448), and
 // the stages' scale words in [448, 508). The epilogue of a tile drains the shared columns first and then lets the next
 // tile's products start, so three quarters of it run beside them.
-template <bool GATED>
+template <bool GATED, int OUT>
 __global__ void __launch_bounds__(128 + 32 * kWriters, 1) __cluster_dims__(2, 1, 1)
     k_mx_tile(const __grid_constant__ CUtensorMap mx, const __grid_constant__ CUtensorMap mw, const __grid_constant__ Args a) {
   extern __shared__ uint8_t raw[];
@@ -393,7 +484,7 @@ __global__ void __launch_bounds__(128 + 32 * kWriters, 1) __cluster_dims__(2, 1,
   uint8_t* scales = codes + kStages * kStageBytes;
   uint8_t* passes = scales + kStages * kStageScales;
   TileShared& sh = *reinterpret_cast<TileShared*>(passes + kWriters * kPassBytes);
-  int* first = reinterpret_cast<int*>(&sh + 1);
+  const Table tab(&sh + 1, a.experts);
   volatile int* abort = &sh.abort;
   const int warp = __shfl_sync(~0u, threadIdx.x >> 5, 0), lane = threadIdx.x & 31;
   constexpr int kCols = GATED ? 128 : 256;             // columns of y per tile
@@ -403,8 +494,9 @@ __global__ void __launch_bounds__(128 + 32 * kWriters, 1) __cluster_dims__(2, 1,
 
   if (threadIdx.x == 0) {
     for (int i = 0; i < kStages; i++) {
-      mbar_init(&sh.full[i], 5);                       // the first CTA's: the codes' bytes, both CTAs' scale warps
+      mbar_init(&sh.full[i], 3);                       // the first CTA's: the codes' bytes, both CTAs' scales
       mbar_init(&sh.empty[i], 1);
+      mbar_init(&sh.ready[i], 1);
     }
     mbar_init(&sh.acc_full, 1);
     mbar_init(&sh.acc_free, 2 * kWriters);             // the first CTA's: both CTAs' epilogue warps
@@ -413,12 +505,13 @@ __global__ void __launch_bounds__(128 + 32 * kWriters, 1) __cluster_dims__(2, 1,
     fence_mbar_init();
   }
   if (warp == 1) tc::tmem_alloc<true>(&sh.tmem, 512);
-  if (warp == 2 && a.experts) count_tiles(first, a, 256, col_tiles);
+  if (warp == 2 && a.experts) count_tiles(tab, a, 256, col_tiles);
   tc::fence_before();
   cluster.sync();
   tc::fence_after();
   const uint32_t tmem = sh.tmem;
   const uint32_t full = tc::remote(sh.full, 0);
+  const int tiles = tile_count(a, tab, 256, col_tiles);
   // the second half of a tile's w rows: the up projections, or the next 128 features
   const int second = GATED ? a.width : 128;
 
@@ -427,7 +520,8 @@ __global__ void __launch_bounds__(128 + 32 * kWriters, 1) __cluster_dims__(2, 1,
     bool ok = true;
     Tile t;
     int sent = 0;
-    for (int i = pair; ok && find_tile(i, a, first, 256, col_tiles, t); i += pairs) {
+    for (int i = pair; ok && i < tiles; i += pairs) {
+      t.find(i, a, tab, 256, col_tiles);
       int4 rows = make_int4(0, 0, 0, 0);
       const int r0 = rank * 128 + 4 * lane;
       if (a.per > 0) rows = make_int4(x_row(a, t, r0), x_row(a, t, r0 + 1), x_row(a, t, r0 + 2), x_row(a, t, r0 + 3));
@@ -457,9 +551,8 @@ __global__ void __launch_bounds__(128 + 32 * kWriters, 1) __cluster_dims__(2, 1,
     if (rank == 0) {
       Ring ring;
       bool ok = true;
-      Tile t;
       int done = 0;
-      for (int i = pair; ok && find_tile(i, a, first, 256, col_tiles, t); i += pairs, done++) {
+      for (int i = pair; ok && i < tiles; i += pairs, done++) {
         if (done) ok = tc::wait_warp(&sh.acc_free, (done - 1) & 1, abort, a.status);
         if (!ok) break;
         const uint32_t acc = tmem + (done & 1 ? 192 : 0);
@@ -489,25 +582,48 @@ __global__ void __launch_bounds__(128 + 32 * kWriters, 1) __cluster_dims__(2, 1,
         tc::settle(&sh.last, 0);
       }
     }
-  } else if (warp < 4) {
+  } else if (warp == 2) {
+    // x's 128 rows and w's 256. The next four steps' words are on their way while these are stored, over the ends of the
+    // tiles too.
+    const int groups = (a.kblocks + 3) >> 2;
+    ScaleRows<3> rows;
+    uint4 now[12], nxt[12];
     Ring ring;
     Tile t;
-    // 384 rows of words, 12 per lane in two warps: x's 128, w's 256
-    const int half = warp - 2;
-    for (int i = pair; find_tile(i, a, first, 256, col_tiles, t); i += pairs) {
-      const uint8_t* rows[6];
-      uint32_t place[6];
+    int i = pair, g = 0;
+    auto aim = [&] {                                   // the rows of tile i
+      if (i >= tiles) return false;
+      t.find(i, a, tab, 256, col_tiles);
 #pragma unroll
-      for (int j = 0; j < 6; j++) {
-        const int r = (j * 2 + half) * 32 + lane;
-        place[j] = scale_place(r);
-        if (r < 128)
-          rows[j] = a.sx + (int64_t)x_row(a, t, rank * 128 + r) * a.nb;
-        else
-          rows[j] = w_scales(a, t, t.col * kCols + (r < 256 ? r - 128 : r - 256 + second));
+      for (int j = 0; j < 4; j++) {
+        const int r = j * 32 + lane;
+        rows.row[j] = a.sx + (int64_t)x_row(a, t, rank * 128 + r) * a.nb;
+        rows.row[4 + j] = w_scales(a, t, t.col * kCols + r);
+        rows.row[8 + j] = w_scales(a, t, t.col * kCols + r + second);
       }
-      if (!stage_scales<6>(rows, place, 0, a.kblocks, a, scales, kStageScales, sh.full, rank ? full : 0u, sh.empty, ring, kStages, abort)) break;
+      return true;
+    };
+    bool more = aim(), ok = true;
+    if (more) rows.load(now, 0, a);
+    while (more && ok) {
+      const int steps = min(4, a.kblocks - 4 * g);
+      if (++g == groups) {
+        g = 0;
+        i += pairs;
+        more = aim();
+      }
+      if (more) rows.load(nxt, g, a);
+#pragma unroll
+      for (int j = 0; j < 4; j++)
+        if (j < steps && ok) ok = store_scales<3>(now, j, a, scales, kStageScales, sh.ready, sh.empty, ring, kStages, abort);
+#pragma unroll
+      for (int j = 0; j < 12; j++) now[j] = nxt[j];
     }
+  } else if (warp == 3) {
+    Ring ring;
+    bool ok = true;
+    for (int i = pair; ok && i < tiles; i += pairs)
+      for (int kb = 0; kb < a.kblocks && ok; kb++) ok = forward_scales(a, sh.ready, sh.full, rank ? full : 0u, ring, kStages, abort);
   } else {
     Tile t;
     int done = 0;
@@ -515,92 +631,106 @@ __global__ void __launch_bounds__(128 + 32 * kWriters, 1) __cluster_dims__(2, 1,
     uint8_t* stage = passes + (warp - 4) * kPassBytes;
     const uint32_t acc_free = tc::remote(&sh.acc_free, 0);
     constexpr int kUnits = kCols / 64;
-    const int size = a.otype == kOutF32 ? 4 : a.otype == kOutPacked ? 1 : 2;
-    const bool nib = a.otype == kOutPacked && a.ofmt == kFmtE2M1;
-    for (int i = pair; find_tile(i, a, first, 256, col_tiles, t); i += pairs, done++) {
+    constexpr int size = OUT == kOutF32 ? 4 : OUT == kOutPacked ? 1 : 2;
+    const bool nib = OUT == kOutPacked && a.ofmt == kFmtE2M1;
+    for (int i = pair; i < tiles; i += pairs, done++) {
+      t.find(i, a, tab, 256, col_tiles);
+      const int row = t.row0 + rank * 128 + q * 32;    // the warp's first
+      const int rows = min(32, t.rows - rank * 128 - q * 32);
+      // units in turn from the columns that the accumulators share on: the first accumulator's last unit, the second's first
+      auto unit_of = [&](int u) { return ((done & 1 ? 0 : kUnits - 1) + 2 * u + set) % kUnits; };
+      // the residual's columns from col on go to the stage while the products and the activation are at work
+      auto fetch = [&](int col) {
+        if (a.residual && rows > 0 && col < a.width)
+          get_rows(stage, static_cast<const uint8_t*>(a.residual) + (row * a.residual_stride + col) * size, a.residual_stride * size,
+                   rows, min(128, (a.width - col) * size), size, a.vec_out);
+      };
+      fetch(t.col * kCols + unit_of(0) * 64);
       const bool ok = tc::wait(&sh.acc_full, done & 1, abort, a.status);
       __syncwarp();
       tc::fence_after();
       // the second warps' word that they are through with the tile before; the first warps give theirs below
       if (set == 1 && lane == 0) tc::mbar_arrive_remote(acc_free);
       const uint32_t acc = tmem + (done & 1 ? 192 : 0) + ((uint32_t)(q * 32) << 16);
-      const int row = t.row0 + rank * 128 + q * 32;    // the warp's first
-      const int rows = min(32, t.rows - rank * 128 - q * 32);
       const float* bias = a.bias ? a.bias + (int64_t)t.expert * a.n : nullptr;
 #pragma unroll 1
       for (int u = 0; u < kUnits / 2; u++) {
-        // units in turn from the columns that the accumulators share on: the first accumulator's last unit, the second's first
-        const int unit = ((done & 1 ? 0 : kUnits - 1) + 2 * u + set) % kUnits;
-        const int col0 = t.col * kCols + unit * 64;
+        const int unit = unit_of(u), col0 = t.col * kCols + unit * 64;
         const bool live = rows > 0 && col0 < a.width;
-        uint32_t sb = 0;
+        if (u > 0) fetch(col0);
+        // The accumulator's shared columns leave TMEM before anything is done with them: of a gated tile's first unit
+        // these are the gates' (second accumulator) or the ups'.
+        const bool ups = GATED && !(done & 1);
+        float y[32], next[32];
+        tc::load32(acc + unit * 64 + (ups ? 128 : 0), y);
+        tc::load32(acc + unit * 64 + (ups ? 160 : 32), next);
+        if (set == 0 && u == 0) {                      // the next tile's products may start
+          tc::fence_before();
+          __syncwarp();
+          if (lane == 0) tc::mbar_arrive_remote(acc_free);
+        }
+        // One body for both halves, not unrolled: straight-line code for 64 columns ran from the instruction cache's second
+        // level, at 4 to 5 cycles an instruction.
 #pragma unroll 1
         for (int c = 0; c < 2; c++) {
-          const int col = col0 + c * 32, at = unit * 64 + c * 32;
-          if (live && a.residual && (c == 0 || size == 4) && col < a.width) {
-            const int w = size == 4 ? 32 : 64;
-            move_rows<false>(stage, const_cast<uint8_t*>(static_cast<const uint8_t*>(a.residual)) + (row * a.residual_stride + col) * size,
-                             a.residual_stride * size, rows, min(w, a.width - col) * size, 128, size, a.vec_out);
-            __syncwarp();
-          }
-          float y[32];
-          tc::load32(acc + at, y);
+          const int col = col0 + c * 32, left = a.width - col;
           if (GATED) {
-            float up[32];
-            tc::load32(acc + 128 + at, up);
-            if (bias) {
+            float late[32];
+            tc::load32(acc + (ups ? 0 : 128) + unit * 64 + c * 32, late);
+            if (ups) {
 #pragma unroll
               for (int j = 0; j < 32; j++) {
-                const int n = min(col + j, a.width - 1);
-                y[j] += __ldg(bias + n);
-                up[j] += __ldg(bias + a.width + n);
+                const float up = y[j];
+                y[j] = late[j];
+                late[j] = up;
               }
             }
-            activate(a.act, y);
-#pragma unroll
-            for (int j = 0; j < 32; j++) y[j] *= up[j];
-          } else {
             if (bias) {
-#pragma unroll
-              for (int j = 0; j < 32; j++) y[j] += __ldg(bias + min(col + j, a.width - 1));
+              add_bias(a, bias, col, y);
+              add_bias(a, bias + a.width, col, late);
             }
             activate(a.act, y);
-          }
-          if (set == 0 && u == 0 && c == 1) {          // the next tile's products may start
-            tc::fence_before();
-            __syncwarp();
-            if (lane == 0) tc::mbar_arrive_remote(acc_free);
+#pragma unroll
+            for (int j = 0; j < 32; j++) y[j] *= late[j];
+          } else {
+            if (bias) add_bias(a, bias, col, y);
+            activate(a.act, y);
           }
           if (!ok) {
 #pragma unroll
             for (int j = 0; j < 32; j++) y[j] = __uint_as_float(0x7fc00000u);
           }
-          if (!live) continue;
-          if (a.otype == kOutPacked)
-            sb |= stage_block(a, y, stage, nib ? c : 2 * c, a.width - col) << (8 * c);
-          else
-            stage_row(a, y, stage, size == 4 ? 0 : 4 * c);
-          if (size == 4 && col < a.width) {
-            __syncwarp();
-            move_rows<true>(stage, static_cast<uint8_t*>(a.out) + (row * a.out_pitch + col) * 4, a.out_pitch * 4, rows,
-                            min(32, a.width - col) * 4, 128, 4, a.vec_out);
-            __syncwarp();
+          if (live && left > 0) {
+            if (OUT == kOutPacked) {
+              const uint32_t sb = stage_block(a.ofmt, y, stage, c, left);
+              if (lane < rows) a.out_scales[(row + lane) * a.out_nb + (col >> 5)] = (uint8_t)sb;
+            } else {
+              if (a.residual && (c == 0 || OUT == kOutF32)) {
+                asm volatile("cp.async.wait_all;\n" ::: "memory");
+                __syncwarp();
+              }
+              stage_row<OUT>(a.residual != nullptr, y, stage, OUT == kOutF32 ? 0 : 4 * c);
+              if (OUT == kOutF32) {                    // 32 columns fill the stage
+                __syncwarp();
+                put_rows<8>(stage, static_cast<uint8_t*>(a.out) + (row * a.out_pitch + col) * 4, a.out_pitch * 4, rows,
+                            min(32, left) * 4, 4, a.vec_out);
+                __syncwarp();
+                if (c == 0) fetch(col + 32);
+              }
+            }
           }
+#pragma unroll
+          for (int j = 0; j < 32; j++) y[j] = next[j];
         }
-        if (!live || size == 4) continue;
-        __syncwarp();
+        if (OUT == kOutF32 || !live) continue;
         const int left = min(64, a.width - col0);
-        if (a.otype == kOutPacked) {
-          move_rows<true>(stage, static_cast<uint8_t*>(a.out) + row * a.out_pitch + (nib ? col0 >> 1 : col0), a.out_pitch, rows,
-                          nib ? left >> 1 : left, nib ? 32 : 64, 1, a.vec_out);
-          if (lane < rows) {
-            uint8_t* to = a.out_scales + (row + lane) * a.out_nb + (col0 >> 5);
-            to[0] = (uint8_t)sb;
-            if (left > 32) to[1] = (uint8_t)(sb >> 8);
-          }
+        __syncwarp();
+        if (OUT == kOutPacked) {
+          uint8_t* out = static_cast<uint8_t*>(a.out) + row * a.out_pitch;
+          if (nib) put_rows<2>(stage, out + (col0 >> 1), a.out_pitch, rows, left >> 1, 1, a.vec_out);
+          else put_rows<4>(stage, out + col0, a.out_pitch, rows, left, 1, a.vec_out);
         } else {
-          move_rows<true>(stage, static_cast<uint8_t*>(a.out) + (row * a.out_pitch + col0) * 2, a.out_pitch * 2, rows, left * 2, 128, 2,
-                          a.vec_out);
+          put_rows<8>(stage, static_cast<uint8_t*>(a.out) + (row * a.out_pitch + col0) * 2, a.out_pitch * 2, rows, left * 2, 2, a.vec_out);
         }
         __syncwarp();
       }
@@ -625,7 +755,7 @@ struct RowsShape {
 };
 
 struct RowsShared {
-  uint64_t full[5], empty[5], acc_full, last;
+  uint64_t full[5], empty[5], ready[5], acc_full, last;
   uint32_t tmem;
   int abort;
 };
@@ -672,7 +802,7 @@ __global__ void __launch_bounds__(128, 2) k_mx_rows(const __grid_constant__ CUte
   uint8_t* codes = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(raw) + 1023) & ~(uintptr_t)1023);
   uint8_t* scales = codes + S::kDepth * S::kStageCodes;
   RowsShared& sh = *reinterpret_cast<RowsShared*>(scales + S::kDepth * S::kStageScales);
-  int* first = reinterpret_cast<int*>(&sh + 1);
+  const Table tab(&sh + 1, a.experts);
   volatile int* abort = &sh.abort;
   const int warp = __shfl_sync(~0u, threadIdx.x >> 5, 0), lane = threadIdx.x & 31;
   constexpr int kCols = GATED ? 64 : 128;              // columns of y per tile
@@ -682,8 +812,9 @@ __global__ void __launch_bounds__(128, 2) k_mx_rows(const __grid_constant__ CUte
 
   if (threadIdx.x == 0) {
     for (int i = 0; i < S::kDepth; i++) {
-      mbar_init(&sh.full[i], 3);
+      mbar_init(&sh.full[i], 2);                       // the codes' bytes and the scales
       mbar_init(&sh.empty[i], 1);
+      mbar_init(&sh.ready[i], 1);
     }
     mbar_init(&sh.acc_full, 1);
     mbar_init(&sh.last, 1);
@@ -691,13 +822,14 @@ __global__ void __launch_bounds__(128, 2) k_mx_rows(const __grid_constant__ CUte
     fence_mbar_init();
   }
   if (warp == 1) tc::tmem_alloc<false>(&sh.tmem, S::kTmem);
-  if (warp == 2 && a.experts) count_tiles(first, a, BN, col_tiles);
+  if (warp == 2 && a.experts) count_tiles(tab, a, BN, col_tiles);
   tc::fence_before();
   __syncthreads();
   tc::fence_after();
   const uint32_t tmem = sh.tmem;
   Tile t;
-  const bool work = find_tile(blockIdx.x / split, a, first, BN, col_tiles, t);    // the same for the whole cluster
+  const bool work = (int)blockIdx.x / split < tile_count(a, tab, BN, col_tiles);  // the same for the whole cluster
+  if (work) t.find(blockIdx.x / split, a, tab, BN, col_tiles);
   const int k0 = (int)((int64_t)a.kblocks * rank / split), k1 = (int)((int64_t)a.kblocks * (rank + 1) / split);
   const bool busy = work && k1 > k0;
 
@@ -757,23 +889,33 @@ __global__ void __launch_bounds__(128, 2) k_mx_rows(const __grid_constant__ CUte
       tc::commit<false>(&sh.last);
       tc::settle(&sh.last, 0);
     }
-  } else if (busy) {
-    constexpr int W = (128 + (BN < 32 ? 32 : BN) + 63) / 64;
-    const uint8_t* rows[W];
-    uint32_t place[W];
+  } else if (busy && warp == 2) {
+    ScaleRows<2> rows;                                 // w's 128 rows; x's, the last repeated up to 128
 #pragma unroll
-    for (int j = 0; j < W; j++) {
-      // rows of w, then of x; a lane with nothing left repeats w's last row in its own place
-      int r = (j * 2 + warp - 2) * 32 + lane;
-      if (r >= 128 + BN) r = 127;
-      place[j] = scale_place(r);
-      if (r >= 128)
-        rows[j] = a.sx + (int64_t)x_row(a, t, r - 128) * a.nb;
-      else
-        rows[j] = w_scales(a, t, t.col * kCols + (GATED && r >= 64 ? a.width + r - 64 : r));
+    for (int j = 0; j < 4; j++) {
+      const int r = j * 32 + lane;
+      rows.row[j] = w_scales(a, t, t.col * kCols + (GATED && r >= 64 ? a.width + r - 64 : r));
+      rows.row[4 + j] = a.sx + (int64_t)x_row(a, t, r) * a.nb;
     }
     Ring ring;
-    stage_scales<W>(rows, place, k0, k1, a, scales, S::kStageScales, sh.full, 0u, sh.empty, ring, S::kDepth, abort);
+    uint4 now[8], nxt[8];
+    int g = k0 >> 2;
+    const int last = (k1 - 1) >> 2;
+    bool ok = true;
+    rows.load(now, g, a);
+    for (; g <= last && ok; g++) {
+      if (g < last) rows.load(nxt, g + 1, a);
+#pragma unroll
+      for (int j = 0; j < 4; j++)
+        if (g * 4 + j >= k0 && g * 4 + j < k1 && ok)
+          ok = store_scales<2>(now, j, a, scales, S::kStageScales, sh.ready, sh.empty, ring, S::kDepth, abort);
+#pragma unroll
+      for (int i = 0; i < 8; i++) now[i] = nxt[i];
+    }
+  } else if (busy) {
+    Ring ring;
+    bool ok = true;
+    for (int kb = k0; kb < k1 && ok; kb++) ok = forward_scales(a, sh.ready, sh.full, 0u, ring, S::kDepth, abort);
   }
   __syncwarp();
 
@@ -827,15 +969,15 @@ __global__ void __launch_bounds__(128, 2) k_mx_rows(const __grid_constant__ CUte
 template <typename F>
 int set_smem(F f, int bytes) {
   static std::mutex mu;
-  static F known[16];
-  static unsigned long long in[16];
+  static F known[32];
+  static unsigned long long in[32];
   const unsigned long long ctx = context_id();
   std::lock_guard<std::mutex> lock(mu);
   int i = 0;
-  for (; i < 16 && known[i] != nullptr; i++)
+  for (; i < 32 && known[i] != nullptr; i++)
     if (known[i] == f && in[i] == ctx && ctx != 0) return MXQ_OK;
   const int rc = check_cuda(cudaFuncSetAttribute((const void*)f, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes), "product: shared memory");
-  if (rc == MXQ_OK && i < 16) {
+  if (rc == MXQ_OK && i < 32) {
     known[i] = f;
     in[i] = ctx;
   }
@@ -858,9 +1000,9 @@ int launch_rows(Args& a, const Operand& x, const Operand& w, int64_t K, int64_t 
   if (int rc = map_of(&mx, x, K, a.per > 0 ? 1 : BN)) return rc;
   if (int rc = map_of(&mw, w, K, GATED ? 64 : 128)) return rc;
   a.idesc = tc::mma_desc(fw, fx, 128, BN);
-  const int smem = S::kSmem + (a.experts ? 4 * (a.experts + 1) : 0);
+  const int smem = S::kSmem + (a.experts ? table_bytes(a.experts) : 0);
   auto f = k_mx_rows<BN, GATED>;
-  if (int rc = set_smem(f, S::kSmem + 4 * (kMostExperts + 1))) return rc;
+  if (int rc = set_smem(f, S::kSmem + table_bytes(kMostExperts))) return rc;
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3((unsigned)(tiles * split));
   cfg.blockDim = dim3(128);
@@ -875,15 +1017,15 @@ int launch_rows(Args& a, const Operand& x, const Operand& w, int64_t K, int64_t 
   return check_cuda(cudaLaunchKernelEx(&cfg, f, mx, mw, a), "product (few rows)");
 }
 
-template <bool GATED>
+template <bool GATED, int OUT>
 int launch_tile(Args& a, const Operand& x, const Operand& w, int64_t K, int64_t tiles, int fx, int fw, cudaStream_t st) {
   CUtensorMap mx, mw;
   if (int rc = map_of(&mx, x, K, a.per > 0 ? 1 : 128)) return rc;
   if (int rc = map_of(&mw, w, K, 128)) return rc;
   a.idesc = tc::mma_desc(fx, fw, 256, 256);
-  const int smem = kTileSmem + (a.experts ? 4 * (a.experts + 1) : 0);
-  auto f = k_mx_tile<GATED>;
-  if (int rc = set_smem(f, kTileSmem + 4 * (kMostExperts + 1))) return rc;
+  const int smem = kTileSmem + (a.experts ? table_bytes(a.experts) : 0);
+  auto f = k_mx_tile<GATED, OUT>;
+  if (int rc = set_smem(f, kTileSmem + table_bytes(kMostExperts))) return rc;
   const int64_t pairs = sm_count() / 2;
   f<<<(unsigned)(2 * (tiles < pairs ? tiles : pairs)), 128 + 32 * kWriters, smem, st>>>(mx, mw, a);
   return MXQ_LAUNCH_CHECK("product");
@@ -899,7 +1041,12 @@ int launch(Args& a, const Operand& x, const Operand& w, int64_t K, int fx, int f
   if (share > 128) {
     const int64_t cols = up_div(a.width, GATED ? 128 : 256);
     const int64_t tiles = (a.experts ? a.rows / 256 + groups : up_div(a.rows, 256)) * cols;
-    return launch_tile<GATED>(a, x, w, K, tiles, fx, fw, st);
+    switch (a.otype) {
+      case kOutF32: return launch_tile<GATED, kOutF32>(a, x, w, K, tiles, fx, fw, st);
+      case kOutBf16: return launch_tile<GATED, kOutBf16>(a, x, w, K, tiles, fx, fw, st);
+      case kOutF16: return launch_tile<GATED, kOutF16>(a, x, w, K, tiles, fx, fw, st);
+      default: return launch_tile<GATED, kOutPacked>(a, x, w, K, tiles, fx, fw, st);
+    }
   }
   const int bn = share <= 16 ? 16 : share <= 32 ? 32 : share <= 64 ? 64 : 128;
   const int64_t cols = up_div(a.width, GATED ? 64 : 128);
@@ -958,6 +1105,7 @@ int product(const char* who, Args& a, const Operand& x, const Operand& w, int64_
   const int size = s->out == kOutF32 ? 4 : s->out == kOutPacked ? 1 : 2;
   a.vec_out = a.out_pitch * size % 16 == 0 && aligned(a.out, 16) &&
               (a.residual == nullptr || (a.residual_stride * size % 16 == 0 && aligned(a.residual, 16)));
+  a.vec_bias = a.width % 4 == 0 && aligned(a.bias, 16);
   a.nb = (int)up_div(K, 32);
   a.kblocks = (int)up_div(K, 128);
   a.vec = a.nb % 16 == 0 && aligned(a.sx, 16) && aligned(a.sw, 16) ? 16 : a.nb % 4 == 0 && aligned(a.sx, 4) && aligned(a.sw, 4) ? 4 : 1;
