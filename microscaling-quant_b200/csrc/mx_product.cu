@@ -46,7 +46,6 @@ struct Args {
   int64_t out_pitch, out_nb;
   int act, otype, ofmt;
   int vec_out;                 // y's (and the residual's) rows take 16-byte accesses
-  int vec_bias;                // so do the biases
   unsigned* status;
 };
 
@@ -246,28 +245,51 @@ __device__ void count_tiles(const Table& tab, const Args& a, int tile_rows, int 
 }
 
 // Tile t: by expert, then column tile, then row tile, so that the CTAs at work at one time share w's tiles. Dense: row
-// tiles in bands of 8 for the same reason. Callers ask for rising t below tile_count().
+// tiles in bands of 8 for the same reason.
 struct Tile {
-  int expert = 0;
-  int row0, rows;              // first row of the product, rows of it in this tile
+  int expert, row0, rows;              // its expert; first row of the product, rows of it in this tile
   int col;                     // column tile
   __device__ __forceinline__ void find(int t, const Args& a, const Table& tab, int tile_rows, int col_tiles) {
     if (a.experts == 0) {
       const int row_tiles = (a.rows + tile_rows - 1) / tile_rows;
       const int band = t / (kBand * col_tiles), in = t - band * kBand * col_tiles;
       const int high = min(kBand, row_tiles - band * kBand);
+      expert = 0;
       col = in / high;
       row0 = (band * kBand + in % high) * tile_rows;
       rows = min(tile_rows, a.rows - row0);
       return;
     }
-    while (t >= tab.first[expert + 1]) expert++;
-    const int in = t - tab.first[expert], row_tiles = (tab.first[expert + 1] - tab.first[expert]) / col_tiles;
+    int lo = 0, hi = a.experts;                        // first[lo] <= t < first[hi]
+    while (hi - lo > 1) {
+      const int mid = (lo + hi) >> 1;
+      if (tab.first[mid] <= t) lo = mid; else hi = mid;
+    }
+    const int in = t - tab.first[lo], row_tiles = (tab.first[lo + 1] - tab.first[lo]) / col_tiles;
+    expert = lo;
     col = in / row_tiles;
-    row0 = tab.begin[expert] + (in - col * row_tiles) * tile_rows;
-    rows = min(tile_rows, tab.begin[expert + 1] - row0);
+    row0 = tab.begin[lo] + (in - col * row_tiles) * tile_rows;
+    rows = min(tile_rows, tab.begin[lo + 1] - row0);
   }
   static constexpr int kBand = 8;
+};
+// A warp's tiles one after the other: each lane finds one of the next 32, since a search takes about 1000 cycles
+struct Tiles {
+  Tile mine = {0, 0, 0, 0};
+  int at = 0;
+  // the tile `step` after the last one (the first: tile `from`), which exists
+  __device__ __forceinline__ Tile next(int from, int step, int tiles, const Args& a, const Table& tab, int tile_rows, int col_tiles) {
+    const int lane = threadIdx.x & 31;
+    if (at == 0 && from + step * lane < tiles) mine.find(from + step * lane, a, tab, tile_rows, col_tiles);
+    __syncwarp();
+    Tile t;
+    t.expert = __shfl_sync(~0u, mine.expert, at);
+    t.row0 = __shfl_sync(~0u, mine.row0, at);
+    t.rows = __shfl_sync(~0u, mine.rows, at);
+    t.col = __shfl_sync(~0u, mine.col, at);
+    at = (at + 1) & 31;
+    return t;
+  }
 };
 __device__ __forceinline__ int tile_count(const Args& a, const Table& tab, int tile_rows, int col_tiles) {
   return a.experts ? tab.first[a.experts] : (a.rows + tile_rows - 1) / tile_rows * col_tiles;
@@ -315,9 +337,12 @@ __device__ __forceinline__ void put_rows(uint8_t* stage, uint8_t* mem, int64_t p
     uint4 v[P];
 #pragma unroll
     for (int i = 0; i < P; i++) v[i] = *reinterpret_cast<const uint4*>(piece(stage, i * (32 / P) + r0, j));
+    if (j * 16 < bytes) {
+      pitch *= 32 / P;
 #pragma unroll
-    for (int i = 0; i < P; i++)
-      if (i * (32 / P) + r0 < rows && j * 16 < bytes) *reinterpret_cast<uint4*>(to + i * (32 / P) * pitch) = v[i];
+      for (int i = 0; i < P; i++, to += pitch)
+        if (i * (32 / P) + r0 < rows) *reinterpret_cast<uint4*>(to) = v[i];
+    }
     return;
   }
   for (int r = 0; r < rows; r++)
@@ -453,21 +478,10 @@ __device__ __forceinline__ uint32_t stage_block(int fmt, float (&y)[32], uint8_t
   }
 }
 
-// y += 32 biases from column col on
-__device__ __forceinline__ void add_bias(const Args& a, const float* bias, int col, float (&y)[32]) {
-  if (a.vec_bias && col + 32 <= a.width) {
+// y += the biases of 32 columns, lane j's for column j
+__device__ __forceinline__ void add_bias(float mine, float (&y)[32]) {
 #pragma unroll
-    for (int i = 0; i < 8; i++) {
-      const float4 b = __ldg(reinterpret_cast<const float4*>(bias + col) + i);
-      y[4 * i] += b.x;
-      y[4 * i + 1] += b.y;
-      y[4 * i + 2] += b.z;
-      y[4 * i + 3] += b.w;
-    }
-  } else {
-#pragma unroll
-    for (int j = 0; j < 32; j++) y[j] += __ldg(bias + min(col + j, a.width - 1));
-  }
+  for (int j = 0; j < 32; j++) y[j] += __shfl_sync(~0u, mine, j);
 }
 
 // Warp 0 loads the codes, warp 1 of the pair's first CTA issues the products, warps 2 and 3 bring the scales, warps 4-11 write
@@ -518,10 +532,10 @@ __global__ void __launch_bounds__(128 + 32 * kWriters, 1) __cluster_dims__(2, 1,
   if (warp == 0) {
     Ring ring;
     bool ok = true;
-    Tile t;
+    Tiles list;
     int sent = 0;
     for (int i = pair; ok && i < tiles; i += pairs) {
-      t.find(i, a, tab, 256, col_tiles);
+      const Tile t = list.next(i, pairs, tiles, a, tab, 256, col_tiles);
       int4 rows = make_int4(0, 0, 0, 0);
       const int r0 = rank * 128 + 4 * lane;
       if (a.per > 0) rows = make_int4(x_row(a, t, r0), x_row(a, t, r0 + 1), x_row(a, t, r0 + 2), x_row(a, t, r0 + 3));
@@ -589,11 +603,11 @@ __global__ void __launch_bounds__(128 + 32 * kWriters, 1) __cluster_dims__(2, 1,
     ScaleRows<3> rows;
     uint4 now[12], nxt[12];
     Ring ring;
-    Tile t;
+    Tiles list;
     int i = pair, g = 0;
     auto aim = [&] {                                   // the rows of tile i
       if (i >= tiles) return false;
-      t.find(i, a, tab, 256, col_tiles);
+      const Tile t = list.next(i, pairs, tiles, a, tab, 256, col_tiles);
 #pragma unroll
       for (int j = 0; j < 4; j++) {
         const int r = j * 32 + lane;
@@ -625,7 +639,7 @@ __global__ void __launch_bounds__(128 + 32 * kWriters, 1) __cluster_dims__(2, 1,
     for (int i = pair; ok && i < tiles; i += pairs)
       for (int kb = 0; kb < a.kblocks && ok; kb++) ok = forward_scales(a, sh.ready, sh.full, rank ? full : 0u, ring, kStages, abort);
   } else {
-    Tile t;
+    Tiles list;
     int done = 0;
     const int q = warp & 3, set = (warp - 4) >> 2;     // lane quarter; which of its two warps
     uint8_t* stage = passes + (warp - 4) * kPassBytes;
@@ -634,7 +648,7 @@ __global__ void __launch_bounds__(128 + 32 * kWriters, 1) __cluster_dims__(2, 1,
     constexpr int size = OUT == kOutF32 ? 4 : OUT == kOutPacked ? 1 : 2;
     const bool nib = OUT == kOutPacked && a.ofmt == kFmtE2M1;
     for (int i = pair; i < tiles; i += pairs, done++) {
-      t.find(i, a, tab, 256, col_tiles);
+      const Tile t = list.next(i, pairs, tiles, a, tab, 256, col_tiles);
       const int row = t.row0 + rank * 128 + q * 32;    // the warp's first
       const int rows = min(32, t.rows - rank * 128 - q * 32);
       // units in turn from the columns that the accumulators share on: the first accumulator's last unit, the second's first
@@ -645,19 +659,34 @@ __global__ void __launch_bounds__(128 + 32 * kWriters, 1) __cluster_dims__(2, 1,
           get_rows(stage, static_cast<const uint8_t*>(a.residual) + (row * a.residual_stride + col) * size, a.residual_stride * size,
                    rows, min(128, (a.width - col) * size), size, a.vec_out);
       };
+      // a unit's biases: column lane and column 32 + lane, of the gates and of the ups
+      const float* bias = a.bias ? a.bias + (int64_t)t.expert * a.n : nullptr;
+      float b[2] = {0.0f, 0.0f}, b_up[2] = {0.0f, 0.0f};
+      auto fetch_bias = [&](int col) {
+        if (!bias) return;
+#pragma unroll
+        for (int c = 0; c < 2; c++) {
+          const int n = min(col + 32 * c + lane, a.width - 1);
+          b[c] = __ldg(bias + n);
+          if (GATED) b_up[c] = __ldg(bias + a.width + n);
+        }
+      };
       fetch(t.col * kCols + unit_of(0) * 64);
+      fetch_bias(t.col * kCols + unit_of(0) * 64);
       const bool ok = tc::wait(&sh.acc_full, done & 1, abort, a.status);
       __syncwarp();
       tc::fence_after();
       // the second warps' word that they are through with the tile before; the first warps give theirs below
       if (set == 1 && lane == 0) tc::mbar_arrive_remote(acc_free);
       const uint32_t acc = tmem + (done & 1 ? 192 : 0) + ((uint32_t)(q * 32) << 16);
-      const float* bias = a.bias ? a.bias + (int64_t)t.expert * a.n : nullptr;
 #pragma unroll 1
       for (int u = 0; u < kUnits / 2; u++) {
         const int unit = unit_of(u), col0 = t.col * kCols + unit * 64;
         const bool live = rows > 0 && col0 < a.width;
-        if (u > 0) fetch(col0);
+        if (u > 0) {
+          fetch(col0);
+          fetch_bias(col0);
+        }
         // The accumulator's shared columns leave TMEM before anything is done with them: of a gated tile's first unit
         // these are the gates' (second accumulator) or the ups'.
         const bool ups = GATED && !(done & 1);
@@ -686,14 +715,14 @@ __global__ void __launch_bounds__(128 + 32 * kWriters, 1) __cluster_dims__(2, 1,
               }
             }
             if (bias) {
-              add_bias(a, bias, col, y);
-              add_bias(a, bias + a.width, col, late);
+              add_bias(c ? b[1] : b[0], y);
+              add_bias(c ? b_up[1] : b_up[0], late);
             }
             activate(a.act, y);
 #pragma unroll
             for (int j = 0; j < 32; j++) y[j] *= late[j];
           } else {
-            if (bias) add_bias(a, bias, col, y);
+            if (bias) add_bias(c ? b[1] : b[0], y);
             activate(a.act, y);
           }
           if (!ok) {
@@ -1105,7 +1134,6 @@ int product(const char* who, Args& a, const Operand& x, const Operand& w, int64_
   const int size = s->out == kOutF32 ? 4 : s->out == kOutPacked ? 1 : 2;
   a.vec_out = a.out_pitch * size % 16 == 0 && aligned(a.out, 16) &&
               (a.residual == nullptr || (a.residual_stride * size % 16 == 0 && aligned(a.residual, 16)));
-  a.vec_bias = a.width % 4 == 0 && aligned(a.bias, 16);
   a.nb = (int)up_div(K, 32);
   a.kblocks = (int)up_div(K, 128);
   a.vec = a.nb % 16 == 0 && aligned(a.sx, 16) && aligned(a.sw, 16) ? 16 : a.nb % 4 == 0 && aligned(a.sx, 4) && aligned(a.sw, 4) ? 4 : 1;
