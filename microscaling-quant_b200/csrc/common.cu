@@ -64,6 +64,24 @@ unsigned long long context_id() {
   return id;
 }
 
+int allow_smem(const void* kernel, int bytes) {
+  constexpr int kMost = 64;
+  static std::mutex mu;
+  static const void* known[kMost];
+  static unsigned long long in[kMost];
+  static int n = 0;
+  const unsigned long long ctx = context_id();
+  std::lock_guard<std::mutex> lock(mu);
+  for (int i = 0; i < n; i++)
+    if (known[i] == kernel && in[i] == ctx && ctx != 0) return MXQ_OK;
+  const int rc = check_cuda(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes), "shared memory of a kernel");
+  if (rc == MXQ_OK && n < kMost) {
+    known[n] = kernel;
+    in[n++] = ctx;
+  }
+  return rc;
+}
+
 static PFN_cuTensorMapEncodeTiled_v12000 encode_fn() {
   static std::once_flag once;
   static PFN_cuTensorMapEncodeTiled_v12000 fn = nullptr;

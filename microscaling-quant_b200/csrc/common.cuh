@@ -21,6 +21,10 @@ int sm_count();
 // 0 when the driver cannot say.
 unsigned long long context_id();
 
+// Lets `kernel` be launched with up to `bytes` of dynamic shared memory on the current device: one call to the runtime per
+// kernel and context, always with the same `bytes`.
+int allow_smem(const void* kernel, int bytes);
+
 inline cudaStream_t as_stream(void* s) { return reinterpret_cast<cudaStream_t>(s); }
 
 // Grid size for a grid-stride loop over n items: enough CTAs to fill every SM `per_sm` times, never more than the

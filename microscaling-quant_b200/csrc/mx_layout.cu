@@ -11,6 +11,10 @@ using namespace mxq;
 
 namespace {
 
+// The product that comes next on the stream may be launched while this grid is at work (it waits for its end before it
+// reads anything).
+__device__ __forceinline__ void start_next_grid() { asm volatile("griddepcontrol.launch_dependents;\n" ::: "memory"); }
+
 // four codes of one row -> one 32-bit word of 8-bit codes; `in` points at the row, c is a multiple of 4
 __device__ __forceinline__ uint32_t lay4(const uint8_t* in, int64_t c, int64_t K, int fmt) {
   uint32_t w = 0;
@@ -28,6 +32,7 @@ __device__ __forceinline__ uint32_t lay4(const uint8_t* in, int64_t c, int64_t K
 // a thread per 16 codes of the output; its place beyond K is written as zeros (the tensor map never reads it)
 __global__ void __launch_bounds__(256) k_lay_codes(const uint8_t* __restrict__ in, int64_t in_pitch, uint8_t* __restrict__ out,
                                                    int64_t out_pitch, int64_t rows, int64_t K, int fmt, int vec) {
+  start_next_grid();
   const int64_t per = out_pitch >> 4, n = rows * per, stride = (int64_t)gridDim.x * blockDim.x;
   for (int64_t i = (int64_t)blockIdx.x * blockDim.x + threadIdx.x; i < n; i += stride) {
     const int64_t r = i / per, c = (i - r * per) << 4;
@@ -72,6 +77,7 @@ __device__ __forceinline__ float to_float<__half>(__half v) { return __half2floa
 template <typename T, bool VEC>
 __global__ void __launch_bounds__(256) k_pack_rows(const T* __restrict__ x, int64_t x_stride, uint8_t* __restrict__ codes,
                                                    int64_t out_pitch, uint8_t* __restrict__ scales, int64_t rows, int64_t K, int fmt) {
+  start_next_grid();
   const int64_t nb = (K + 31) / 32, n = rows * nb * 4, stride = (int64_t)gridDim.x * blockDim.x;
   const int64_t n32 = (n + 31) / 32 * 32;              // whole warps stay for the shuffles
   for (int64_t i = (int64_t)blockIdx.x * blockDim.x + threadIdx.x; i < n32; i += stride) {

@@ -16,8 +16,6 @@
 
 #include <cooperative_groups.h>
 
-#include <mutex>
-
 namespace cg = cooperative_groups;
 using namespace mxq;
 
@@ -81,18 +79,7 @@ __device__ __forceinline__ float gelu_tanh(float x) {
 // a NaN stays one
 __device__ __forceinline__ float relu(float x) { return x < 0.0f ? 0.0f : x; }
 
-__device__ __forceinline__ float activate1(int act, float g) {
-  switch (act) {
-    case kActRelu: return relu(g);
-    case kActGelu:
-    case kActGeglu: return gelu(g);
-    case kActGeluTanh: return gelu_tanh(g);
-    case kActSilu:
-    case kActSwiglu: return silu(g);
-    default: return g;
-  }
-}
-// the switch outside the loop: one branch per 32 values
+// the switch outside the loop: one branch for all values
 template <int N>
 __device__ __forceinline__ void activate(int act, float (&v)[N]) {
   switch (act) {
@@ -518,7 +505,12 @@ __global__ void __launch_bounds__(128 + 32 * kWriters, 1) __cluster_dims__(2, 1,
     sh.abort = 0;
     fence_mbar_init();
   }
+  if (warp == 0 && tc::elect()) {
+    tc::prefetch_map(&mw);
+    tc::prefetch_map(&mx);
+  }
   if (warp == 1) tc::tmem_alloc<true>(&sh.tmem, 512);
+  tc::wait_for_prior_grid();
   if (warp == 2 && a.experts) count_tiles(tab, a, 256, col_tiles);
   tc::fence_before();
   cluster.sync();
@@ -790,34 +782,78 @@ struct RowsShared {
 };
 static_assert(sizeof(RowsShared) <= 256, "barriers");
 
-// one column (token) of the transposed accumulator, this lane's feature: everything after bias and activation
-__device__ __forceinline__ void write_one(const Args& a, float y, int64_t row, int col) {
-  const bool in = col < a.width;
-  if (a.otype == kOutPacked) {
-    const uint32_t top = __reduce_max_sync(~0u, in ? __float_as_uint(y) & 0x7fffffffu : 0u);
+// four columns of a row of y from column col on, all but the store's rounding done
+__device__ __forceinline__ void write_four(const Args& a, float (&y)[4], int64_t row, int col, bool valid) {
+  const int left = valid ? a.width - col : 0;
+  if (a.otype == kOutPacked) {                         // eight lanes hold a block
+    uint32_t top = 0;
+#pragma unroll
+    for (int i = 0; i < 4; i++) top = max(top, i < left ? __float_as_uint(y[i]) & 0x7fffffffu : 0u);
+#pragma unroll
+    for (int d = 1; d < 8; d <<= 1) top = max(top, __shfl_xor_sync(~0u, top, d));
     const uint32_t sb = scale_byte(top, a.ofmt);
     const float inv = scale_inverse(sb);
-    if ((threadIdx.x & 31) == 0 && in) a.out_scales[row * a.out_nb + (col >> 5)] = (uint8_t)sb;
-    const float z = scaled(y, inv);
-    const float next = __shfl_down_sync(~0u, z, 1);
+    if (left <= 0) return;
+    if ((threadIdx.x & 7) == 0) a.out_scales[row * a.out_nb + (col >> 5)] = (uint8_t)sb;
+#pragma unroll
+    for (int i = 0; i < 4; i++) y[i] = i < left ? scaled(y[i], inv) : 0.0f;
+    uint32_t lo = encode2(a.ofmt, y[0], y[1]), hi = encode2(a.ofmt, y[2], y[3]);
     uint8_t* to = static_cast<uint8_t*>(a.out) + row * a.out_pitch;
-    if (a.ofmt == kFmtE2M1) {
-      if (in && !(col & 1)) to[col >> 1] = (uint8_t)encode2(kFmtE2M1, z, next);
-    } else if (in) {
-      to[col] = (uint8_t)encode2(a.ofmt, z, 0.0f);
+    if (a.ofmt == kFmtE2M1) {                          // the width is even
+      to[col >> 1] = (uint8_t)lo;
+      if (left > 2) to[(col >> 1) + 1] = (uint8_t)hi;
+    } else if (left >= 4 && a.vec_out) {
+      *reinterpret_cast<uint32_t*>(to + col) = lo | hi << 16;
+    } else {
+      lo |= hi << 16;
+#pragma unroll
+      for (int i = 0; i < 4; i++)
+        if (i < left) to[col + i] = (uint8_t)(lo >> (8 * i));
     }
     return;
   }
-  if (!in) return;
+  if (left <= 0) return;
+  const int64_t at = row * a.out_pitch + col, from = row * a.residual_stride + col;
   if (a.otype == kOutF32) {
-    if (a.residual) y += static_cast<const float*>(a.residual)[row * a.residual_stride + col];
-    static_cast<float*>(a.out)[row * a.out_pitch + col] = y;
-  } else if (a.otype == kOutBf16) {
-    if (a.residual) y += __bfloat162float(static_cast<const __nv_bfloat16*>(a.residual)[row * a.residual_stride + col]);
-    static_cast<__nv_bfloat16*>(a.out)[row * a.out_pitch + col] = __float2bfloat16_rn(y);
+    float* to = static_cast<float*>(a.out) + at;
+    const float* r = a.residual ? static_cast<const float*>(a.residual) + from : nullptr;
+    if (left >= 4 && a.vec_out) {
+      float4 v = make_float4(y[0], y[1], y[2], y[3]);
+      if (r) {
+        const float4 q = *reinterpret_cast<const float4*>(r);
+        v = make_float4(v.x + q.x, v.y + q.y, v.z + q.z, v.w + q.w);
+      }
+      *reinterpret_cast<float4*>(to) = v;
+    } else {
+#pragma unroll
+      for (int i = 0; i < 4; i++)
+        if (i < left) to[i] = r ? y[i] + r[i] : y[i];
+    }
+    return;
+  }
+  uint16_t* to = static_cast<uint16_t*>(a.out) + at;
+  const uint16_t* r = a.residual ? static_cast<const uint16_t*>(a.residual) + from : nullptr;
+  const bool bf = a.otype == kOutBf16, four = left >= 4 && a.vec_out;
+  if (r) {
+    uint16_t h[4] = {0, 0, 0, 0};
+    if (four) {
+      *reinterpret_cast<uint2*>(h) = *reinterpret_cast<const uint2*>(r);
+    } else {
+#pragma unroll
+      for (int i = 0; i < 4; i++)
+        if (i < left) h[i] = r[i];
+    }
+#pragma unroll
+    for (int i = 0; i < 4; i++) y[i] += bf ? widen16<kOutBf16>(h[i]) : widen16<kOutF16>(h[i]);
+  }
+  const uint32_t lo = bf ? narrow2<kOutBf16>(y[0], y[1]) : narrow2<kOutF16>(y[0], y[1]);
+  const uint32_t hi = bf ? narrow2<kOutBf16>(y[2], y[3]) : narrow2<kOutF16>(y[2], y[3]);
+  if (four) {
+    *reinterpret_cast<uint2*>(to) = make_uint2(lo, hi);
   } else {
-    if (a.residual) y += __half2float(static_cast<const __half*>(a.residual)[row * a.residual_stride + col]);
-    static_cast<__half*>(a.out)[row * a.out_pitch + col] = __float2half_rn(y);
+#pragma unroll
+    for (int i = 0; i < 4; i++)
+      if (i < left) to[i] = (uint16_t)((i < 2 ? lo : hi) >> (16 * (i & 1)));
   }
 }
 
@@ -850,7 +886,12 @@ __global__ void __launch_bounds__(128, 2) k_mx_rows(const __grid_constant__ CUte
     sh.abort = 0;
     fence_mbar_init();
   }
+  if (warp == 0 && tc::elect()) {
+    tc::prefetch_map(&mw);
+    tc::prefetch_map(&mx);
+  }
   if (warp == 1) tc::tmem_alloc<false>(&sh.tmem, S::kTmem);
+  tc::wait_for_prior_grid();
   if (warp == 2 && a.experts) count_tiles(tab, a, BN, col_tiles);
   tc::fence_before();
   __syncthreads();
@@ -968,25 +1009,46 @@ __global__ void __launch_bounds__(128, 2) k_mx_rows(const __grid_constant__ CUte
   if (split > 1) cluster.sync(); else __syncthreads();
   tc::fence_after();
   if (work) {
-    constexpr int kBlocks = kCols / 32;
+    // a row of kCols columns by kCols / 4 lanes, rows dealt out to the cluster's warps
+    constexpr int kLanes = kCols / 4, kRows = 32 / kLanes;
     const float* bias = a.bias ? a.bias + (int64_t)t.expert * a.n : nullptr;
-    const int pairs = t.rows * kBlocks;
-    for (int p = rank * 4 + warp; p < pairs; p += split * 4) {
-      const int r = p / kBlocks, f = (p % kBlocks) * 32 + lane, col = t.col * kCols + f;
-      float y = 0.0f, up = 0.0f;
+    const int f = lane % kLanes * 4, col = t.col * kCols + f;
+    float b[4] = {0.0f, 0.0f, 0.0f, 0.0f}, b_up[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+    if (bias) {
+#pragma unroll
+      for (int i = 0; i < 4; i++) {
+        const int n = min(col + i, a.width - 1);
+        b[i] = __ldg(bias + n);
+        if (GATED) b_up[i] = __ldg(bias + a.width + n);
+      }
+    }
+    for (int base = (rank * 4 + warp) * kRows; base < t.rows; base += split * 4 * kRows) {
+      const int r = base + lane / kLanes, at = min(r, t.rows - 1) * 128 + f;
+      float y[4] = {0.0f, 0.0f, 0.0f, 0.0f}, up[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll 4
       for (int s = 0; s < split; s++) {
         const float* from = split > 1 ? cluster.map_shared_rank(part, s) : part;
-        y += from[r * 128 + f];
-        if (GATED) up += from[r * 128 + 64 + f];
+        const float4 v = *reinterpret_cast<const float4*>(from + at);
+        y[0] += v.x;
+        y[1] += v.y;
+        y[2] += v.z;
+        y[3] += v.w;
+        if (GATED) {
+          const float4 u = *reinterpret_cast<const float4*>(from + at + 64);
+          up[0] += u.x;
+          up[1] += u.y;
+          up[2] += u.z;
+          up[3] += u.w;
+        }
       }
-      const int n = min(col, a.width - 1);
-      if (bias) y += __ldg(bias + n);
-      y = activate1(a.act, y);
+#pragma unroll
+      for (int i = 0; i < 4; i++) y[i] += b[i];
+      activate(a.act, y);
       if (GATED) {
-        if (bias) up += __ldg(bias + a.width + n);
-        y *= up;
+#pragma unroll
+        for (int i = 0; i < 4; i++) y[i] *= up[i] + b_up[i];
       }
-      if (t.col * kCols + (p % kBlocks) * 32 < a.width) write_one(a, y, (int64_t)t.row0 + r, col);
+      write_four(a, y, (int64_t)t.row0 + r, col, r < t.rows);
     }
   }
   if (split > 1) cluster.sync(); else __syncthreads();  // the partial sums are read before their CTA leaves
@@ -994,25 +1056,6 @@ __global__ void __launch_bounds__(128, 2) k_mx_rows(const __grid_constant__ CUte
 }
 
 // --------------------------------------------------------------------------------------------------- host
-// The kernel's largest shared memory, set once per kernel and context (a device, or a device after its reset)
-template <typename F>
-int set_smem(F f, int bytes) {
-  static std::mutex mu;
-  static F known[32];
-  static unsigned long long in[32];
-  const unsigned long long ctx = context_id();
-  std::lock_guard<std::mutex> lock(mu);
-  int i = 0;
-  for (; i < 32 && known[i] != nullptr; i++)
-    if (known[i] == f && in[i] == ctx && ctx != 0) return MXQ_OK;
-  const int rc = check_cuda(cudaFuncSetAttribute((const void*)f, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes), "product: shared memory");
-  if (rc == MXQ_OK && i < 32) {
-    known[i] = f;
-    in[i] = ctx;
-  }
-  return rc;
-}
-
 struct Operand {
   const uint8_t* codes;
   int64_t rows, pitch;
@@ -1031,18 +1074,20 @@ int launch_rows(Args& a, const Operand& x, const Operand& w, int64_t K, int64_t 
   a.idesc = tc::mma_desc(fw, fx, 128, BN);
   const int smem = S::kSmem + (a.experts ? table_bytes(a.experts) : 0);
   auto f = k_mx_rows<BN, GATED>;
-  if (int rc = set_smem(f, S::kSmem + table_bytes(kMostExperts))) return rc;
+  if (int rc = allow_smem((const void*)f, S::kSmem + table_bytes(kMostExperts))) return rc;
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3((unsigned)(tiles * split));
   cfg.blockDim = dim3(128);
   cfg.dynamicSmemBytes = smem;
   cfg.stream = st;
-  cudaLaunchAttribute at[1];
-  at[0].id = cudaLaunchAttributeClusterDimension;
-  at[0].val.clusterDim.x = split;
-  at[0].val.clusterDim.y = at[0].val.clusterDim.z = 1;
+  cudaLaunchAttribute at[2];
+  at[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  at[0].val.programmaticStreamSerializationAllowed = 1;
+  at[1].id = cudaLaunchAttributeClusterDimension;
+  at[1].val.clusterDim.x = split;
+  at[1].val.clusterDim.y = at[1].val.clusterDim.z = 1;
   cfg.attrs = at;
-  cfg.numAttrs = 1;
+  cfg.numAttrs = 2;
   return check_cuda(cudaLaunchKernelEx(&cfg, f, mx, mw, a), "product (few rows)");
 }
 
@@ -1054,10 +1099,19 @@ int launch_tile(Args& a, const Operand& x, const Operand& w, int64_t K, int64_t 
   a.idesc = tc::mma_desc(fx, fw, 256, 256);
   const int smem = kTileSmem + (a.experts ? table_bytes(a.experts) : 0);
   auto f = k_mx_tile<GATED, OUT>;
-  if (int rc = set_smem(f, kTileSmem + table_bytes(kMostExperts))) return rc;
+  if (int rc = allow_smem((const void*)f, kTileSmem + table_bytes(kMostExperts))) return rc;
   const int64_t pairs = sm_count() / 2;
-  f<<<(unsigned)(2 * (tiles < pairs ? tiles : pairs)), 128 + 32 * kWriters, smem, st>>>(mx, mw, a);
-  return MXQ_LAUNCH_CHECK("product");
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3((unsigned)(2 * (tiles < pairs ? tiles : pairs)));
+  cfg.blockDim = dim3(128 + 32 * kWriters);
+  cfg.dynamicSmemBytes = smem;
+  cfg.stream = st;
+  cudaLaunchAttribute at[1];
+  at[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  at[0].val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = at;
+  cfg.numAttrs = 1;
+  return check_cuda(cudaLaunchKernelEx(&cfg, f, mx, mw, a), "product");
 }
 
 int64_t up_div(int64_t a, int64_t b) { return (a + b - 1) / b; }

@@ -563,8 +563,7 @@ extern "C" int mxq_dispatch(const int32_t* experts_of, int64_t slots, int64_t ex
   int ctas = 1;
   while (ctas < 8 && slots > 4096ll * ctas) ctas *= 2;
   const int smem = (int)((kDispatchWarps + 1) * experts + 32) * 4;
-  if (int rc = check_cuda(cudaFuncSetAttribute(k_dispatch, cudaFuncAttributeMaxDynamicSharedMemorySize, smem), "dispatch: shared memory"))
-    return rc;
+  if (int rc = allow_smem((const void*)k_dispatch, ((kDispatchWarps + 1) * kMostExperts + 32) * 4)) return rc;
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3(ctas);
   cfg.blockDim = dim3(kDispatchWarps * 32);

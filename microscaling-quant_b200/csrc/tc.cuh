@@ -89,6 +89,15 @@ __device__ __forceinline__ void tmem_free(uint32_t addr, uint32_t cols) {
     asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;\n" ::"r"(addr), "r"(cols));
 }
 
+// Programmatic dependent launch: the kernel was launched while the one before it on the stream was still at work; what that
+// one (or any before it) wrote may be read after this. Nothing of it before, and no TMEM that it may still want is held
+// back from it: the grid before either holds its own already or needs none (only kernels without TMEM start their
+// successor early).
+__device__ __forceinline__ void wait_for_prior_grid() { asm volatile("griddepcontrol.wait;\n" ::: "memory"); }
+__device__ __forceinline__ void prefetch_map(const CUtensorMap* map) {
+  asm volatile("prefetch.tensormap [%0];\n" ::"l"(map) : "memory");
+}
+
 // K-major operand tile, rows of 128 bytes in the 128-byte swizzle: groups of 8 rows 1024 bytes apart
 __device__ __forceinline__ uint64_t operand_desc(uint32_t addr) {
   return (uint64_t)((addr & 0x3ffffu) >> 4) | (1ull << 16) | (64ull << 32) | (1ull << 46) | (2ull << 61);

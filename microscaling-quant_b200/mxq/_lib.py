@@ -137,16 +137,20 @@ def lib():
 
 def call(name, *args):
     """Call entry point `name`; a nonzero status raises the matching exception with the library's message."""
-    rc = getattr(lib(), name)(*args)
+    rc = getattr(_lib or lib(), name)(*args)
     if rc != OK:
-        msg = lib().mxq_last_error().decode()
-        if rc == ERR_VALUE:
-            raise ValueError(msg)
-        if rc == ERR_INDEX:
-            raise IndexError(msg)
-        if rc == ERR_UNSUPPORTED:
-            raise NotImplementedError(f"mxq_b200: {msg}")
-        raise RuntimeError(f"mxq_b200: {msg}")
+        _raise(rc)
+
+
+def _raise(rc):
+    msg = lib().mxq_last_error().decode()
+    if rc == ERR_VALUE:
+        raise ValueError(msg)
+    if rc == ERR_INDEX:
+        raise IndexError(msg)
+    if rc == ERR_UNSUPPORTED:
+        raise NotImplementedError(f"mxq_b200: {msg}")
+    raise RuntimeError(f"mxq_b200: {msg}")
 
 
 # ------------------------------------------------------------------------------------------------ devices
@@ -183,8 +187,8 @@ _raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None)
 def _stream_of(index):
     """The current stream of device `index` as a cudaStream_t (torch's raw getter when it has one)."""
     if _raw_stream is not None:
-        return ctypes.c_void_p(_raw_stream(index))
-    return ctypes.c_void_p(torch.cuda.current_stream(index).cuda_stream)
+        return _raw_stream(index)
+    return torch.cuda.current_stream(index).cuda_stream
 
 
 def back(t, like_device):
@@ -218,13 +222,18 @@ def run(name, device, *args):
     """call() with `device` current; the last argument of every entry point is the stream, appended here. Raises
     RuntimeError if a bounded wait of an earlier kernel has given up (check_waits)."""
     cur = torch.cuda.current_device()
-    idx = device.index if device.index is not None else cur
+    idx = device.index
+    if idx is None:
+        idx = cur
     if idx == cur:                                          # the usual case: no device switch
-        call(name, *args, _stream_of(idx))
+        rc = getattr(_lib or lib(), name)(*args, _stream_of(idx))
+        if rc != OK:
+            _raise(rc)
     else:
         with torch.cuda.device(device):
             call(name, *args, _stream_of(idx))
-    check_waits()
+    if _wait_word is not None and _wait_word.value:
+        check_waits()
 
 
 # ------------------------------------------------------------------------------------------ wait status

@@ -93,7 +93,7 @@ def _laid(codes: torch.Tensor, scales: torch.Tensor, shape, f: Format, K: int, d
         return codes, scales, K // 2, f.e, f.m
     rows = codes.numel() // shape[-1]
     pitch = -(-K // 16) * 16
-    wide = torch.empty((*shape[:-1], pitch), dtype=torch.uint8, device=dev)
+    wide = torch.empty(*shape[:-1], pitch, dtype=torch.uint8, device=dev)
     _lib.run("mxq_lay_codes", dev, codes.data_ptr(), shape[-1], wide.data_ptr(), pitch, rows, K, f.e, f.m)
     return (wide, scales, pitch, f.e, f.m) if bits == 8 else (wide, scales, pitch, 4, 3)
 
@@ -132,8 +132,8 @@ def _x_operand(x, x_fmt, who: str, w: torch.Tensor):
             v = v.detach().contiguous()
             stride = K
         pitch = -(-K // 16) * 16
-        codes = torch.empty((rows, pitch), dtype=torch.uint8, device=dev)
-        scales = torch.empty((rows, -(-K // BLOCK)), dtype=torch.uint8, device=dev)
+        codes = torch.empty(rows, pitch, dtype=torch.uint8, device=dev)
+        scales = torch.empty(rows, -(-K // BLOCK), dtype=torch.uint8, device=dev)
         _lib.run("mxq_pack_rows", dev, v.data_ptr(), kind, stride, codes.data_ptr(), pitch, scales.data_ptr(), rows, K, f.e,
                  f.m)
         e, m = (f.e, f.m) if f.e + f.m == 7 else (4, 3)
@@ -173,9 +173,9 @@ def _plan_output(out, activation, N: int, who: str):
 def _outputs(lead, out, f, F: int, dev):
     """The empty output: (tensor for the codes or values, scales or None)."""
     if f is None:
-        return torch.empty((*lead, F), dtype=out, device=dev), None
-    return (torch.empty((*lead, F // 2 if f.e + f.m == 3 else F), dtype=torch.uint8, device=dev),
-            torch.empty((*lead, -(-F // BLOCK)), dtype=torch.uint8, device=dev))
+        return torch.empty(*lead, F, dtype=out, device=dev), None
+    return (torch.empty(*lead, F // 2 if f.e + f.m == 3 else F, dtype=torch.uint8, device=dev),
+            torch.empty(*lead, -(-F // BLOCK), dtype=torch.uint8, device=dev))
 
 
 def _given(y, scales, dev, home):

@@ -72,8 +72,8 @@ def _route(logits, k, score, bias, groups, keep, group_score, renormalize, scale
     home, dev = logits.device, _device(logits)
     l = _rows(logits, dev)
     b = None if bias is None else _lib.on(bias, dev)
-    weights = torch.empty((T, k), dtype=torch.float32, device=dev)
-    experts = torch.empty((T, k), dtype=torch.int32, device=dev)
+    weights = torch.empty(T, k, dtype=torch.float32, device=dev)
+    experts = torch.empty(T, k, dtype=torch.int32, device=dev)
     s = _spec(SCORES.index(score), groups, keep, int(group_score == "top2"), int(bool(renormalize)), float(scale))
     _lib.run("mxq_route", dev, l.data_ptr(), FLOATS[l.dtype], l.stride(0), None if b is None else b.data_ptr(),
              weights.data_ptr(), experts.data_ptr(), T, E, k, ctypes.byref(s))
@@ -123,7 +123,7 @@ def route_backward(grad: torch.Tensor, logits: torch.Tensor, experts: torch.Tens
         raise ValueError(f"{who}: grad {tuple(grad.shape)} and experts {tuple(experts.shape)} must be {T} x k")
     home, dev = logits.device, _device(logits)
     l, g, e = _rows(logits, dev), _lib.on(grad, dev), _index(experts, dev, who, "experts")
-    out = torch.empty((T, E), dtype=l.dtype, device=dev)
+    out = torch.empty(T, E, dtype=l.dtype, device=dev)
     s = _spec(SCORES.index(score), 1, 1, 0, int(bool(renormalize)), float(scale))
     _lib.run("mxq_route_backward", dev, g.data_ptr(), l.data_ptr(), FLOATS[l.dtype], l.stride(0), e.data_ptr(),
              out.data_ptr(), T, E, k, ctypes.byref(s))
@@ -138,11 +138,10 @@ def dispatch(experts: torch.Tensor, n_experts: int) -> Dispatch:
     home, dev = experts.device, _device(experts)
     e = _index(experts, dev, "dispatch", "experts")
     n = e.numel()
-    # one allocation: the three are made and kept together
-    offsets, order, where = torch.empty(2 * n + n_experts + 1, dtype=torch.int32, device=dev).split(
-        (n_experts + 1, n, n))
+    offsets = torch.empty(n_experts + 1, dtype=torch.int32, device=dev)
+    order = torch.empty(n, dtype=torch.int32, device=dev)
+    where = torch.empty_like(e)
     _lib.run("mxq_dispatch", dev, e.data_ptr(), n, n_experts, offsets.data_ptr(), order.data_ptr(), where.data_ptr())
-    where = where.view(e.shape)
     if home != dev:
         offsets, order, where = offsets.to(home), order.to(home), where.to(home)
     return Dispatch(offsets, order, where)
@@ -167,7 +166,7 @@ def _combine(z, weights, where, residual):
     home, dev = z.device, _device(z)
     zc, w, at = _here(z, dev), _lib.on(weights, dev), _index(where, dev, "combine", "where")
     r = None if residual is None else _rows(residual, dev)
-    y = torch.empty((T, N), dtype=z.dtype, device=dev)
+    y = torch.empty(T, N, dtype=z.dtype, device=dev)
     if k == 0:
         y = y.zero_() if r is None else y.copy_(r.detach())
     else:
@@ -215,8 +214,8 @@ def combine_backward(dy: torch.Tensor, z: torch.Tensor, weights: torch.Tensor,
     home, dev = z.device, _device(z)
     zc, g = _here(z, dev), _rows(dy, dev)
     w, at, order = _lib.on(weights, dev), _index(plan.where, dev, who, "where"), _index(plan.order, dev, who, "order")
-    dz = torch.empty((T * k, N), dtype=z.dtype, device=dev)
-    dw = torch.empty((T, k), dtype=torch.float32, device=dev)
+    dz = torch.empty(T * k, N, dtype=z.dtype, device=dev)
+    dw = torch.empty(T, k, dtype=torch.float32, device=dev)
     if T and k:
         _lib.run("mxq_combine_backward", dev, g.data_ptr(), g.stride(0), zc.data_ptr(), FLOATS[zc.dtype], w.data_ptr(),
                  at.data_ptr(), order.data_ptr(), dz.data_ptr(), dw.data_ptr(), T, k, N)
