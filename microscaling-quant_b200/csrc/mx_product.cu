@@ -1121,26 +1121,32 @@ int launch(Args& a, const Operand& x, const Operand& w, int64_t K, int fx, int f
   // rows that share a tile of w: all of them, or an expert's share
   const int64_t share = a.experts ? up_div(a.rows, a.experts) : a.rows;
   const int64_t groups = a.experts ? (a.experts < a.rows ? a.experts : a.rows) : 1;
-  if (share > 128) {
-    const int64_t cols = up_div(a.width, GATED ? 128 : 256);
-    const int64_t tiles = (a.experts ? a.rows / 256 + groups : up_div(a.rows, 256)) * cols;
+  const int64_t cols = up_div(a.width, GATED ? 64 : 128);
+  // Tiles of few rows: as many as there are; by expert several times the mean, since the longest expert's second tile would
+  // read w again (64 experts of 2048 x 1024 with 8 rows each at random: 37 us with tiles of 16, 33 with 32 and 64).
+  const int bn = a.experts ? (share <= 2 ? 16 : share <= 8 ? 32 : 64) : share <= 16 ? 16 : share <= 32 ? 32 : 64;
+  const int64_t tiles = (a.experts ? a.rows / bn + groups : up_div(a.rows, bn)) * cols;
+  // Which kernel, measured on E4M3: dense 4096 x 4096, M = 256: 15.9 us by few rows, 17.8 by many, M = 384: 19.7 and 18.7;
+  // 2048 x 2048, M = 512: 13.2 and 13.1; 8192 x 2048, M = 128: 13.4 and 13.8, M = 256: 15.1 and 13.9. By expert, 64 experts
+  // 2048 x 1024: 8 rows each 33 and 35, 12 rows 44 and 39; 8 experts 4096 x 2048, 32 rows: 16 and 23.
+  const bool few = a.experts ? share <= 8 || tiles <= 4 * sm_count() : tiles <= sm_count();
+  if (!few) {
+    const int64_t wide = up_div(a.width, GATED ? 128 : 256);
+    const int64_t big = (a.experts ? a.rows / 256 + groups : up_div(a.rows, 256)) * wide;
     switch (a.otype) {
-      case kOutF32: return launch_tile<GATED, kOutF32>(a, x, w, K, tiles, fx, fw, st);
-      case kOutBf16: return launch_tile<GATED, kOutBf16>(a, x, w, K, tiles, fx, fw, st);
-      case kOutF16: return launch_tile<GATED, kOutF16>(a, x, w, K, tiles, fx, fw, st);
-      default: return launch_tile<GATED, kOutPacked>(a, x, w, K, tiles, fx, fw, st);
+      case kOutF32: return launch_tile<GATED, kOutF32>(a, x, w, K, big, fx, fw, st);
+      case kOutBf16: return launch_tile<GATED, kOutBf16>(a, x, w, K, big, fx, fw, st);
+      case kOutF16: return launch_tile<GATED, kOutF16>(a, x, w, K, big, fx, fw, st);
+      default: return launch_tile<GATED, kOutPacked>(a, x, w, K, big, fx, fw, st);
     }
   }
-  const int bn = share <= 16 ? 16 : share <= 32 ? 32 : share <= 64 ? 64 : 128;
-  const int64_t cols = up_div(a.width, GATED ? 64 : 128);
-  const int64_t tiles = (a.experts ? a.rows / bn + groups : up_div(a.rows, bn)) * cols;
+  // K split over a cluster while that gives every SM two CTAs at most and each CTA two steps at least
   int split = 1;
   while (split < 8 && tiles * split * 2 <= 2 * sm_count() && a.kblocks >= split * 4) split *= 2;
   switch (bn) {
     case 16: return launch_rows<16, GATED>(a, x, w, K, tiles, split, fx, fw, st);
     case 32: return launch_rows<32, GATED>(a, x, w, K, tiles, split, fx, fw, st);
-    case 64: return launch_rows<64, GATED>(a, x, w, K, tiles, split, fx, fw, st);
-    default: return launch_rows<128, GATED>(a, x, w, K, tiles, split, fx, fw, st);
+    default: return launch_rows<64, GATED>(a, x, w, K, tiles, split, fx, fw, st);
   }
 }
 

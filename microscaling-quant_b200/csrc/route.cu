@@ -54,31 +54,55 @@ __device__ __forceinline__ uint32_t key_of(float f) {
 __device__ __forceinline__ float value_of(uint32_t key) {
   return __uint_as_float(key & 0x80000000u ? key & 0x7fffffffu : ~key);
 }
-__device__ __forceinline__ float sigmoid(float x) { return __fdiv_rn(1.0f, __fadd_rn(1.0f, expf(-x))); }
+__device__ __forceinline__ float sigmoid(float x) { return __frcp_rn(__fadd_rn(1.0f, expf(-x))); }
 __device__ __forceinline__ bool is_nan(float x) { return x != x; }
 
 struct RouteArgs {
   int64_t stride;
   int T, E, k, sigmoid, groups, keep, top2, renormalize;
+  int vec;                     // every lane's values are whole 16-byte pieces of the row, and there
   float scale;
 };
 
-// A warp per token, V values per lane (expert i * 32 + lane). The k largest are taken one after the other: the warp's
-// largest key by one reduction, the lowest expert that has it by another.
+// V neighbouring values of a row: 16-byte loads where the row allows them
+template <typename IN, int V>
+__device__ __forceinline__ void load_row(const IN* row, int e0, int E, bool vec, float (&l)[V]) {
+  constexpr int N = 16 / sizeof(IN);
+  if (V >= N && vec) {
+#pragma unroll
+    for (int i = 0; i < V / N; i++) {
+      const uint4 q = __ldg(reinterpret_cast<const uint4*>(row + e0) + i);
+      const IN* p = reinterpret_cast<const IN*>(&q);
+#pragma unroll
+      for (int j = 0; j < N; j++) l[(V >= N ? i * N + j : 0)] = to_float<IN>(p[j]);
+    }
+    return;
+  }
+#pragma unroll
+  for (int i = 0; i < V; i++) l[i] = e0 + i < E ? to_float<IN>(row[e0 + i]) : -INFINITY;
+}
+
+// Two largest of two pairs
+__device__ __forceinline__ void merge2(uint32_t& a, uint32_t& b, uint32_t c, uint32_t d) {
+  b = max(min(a, c), max(b, d));
+  a = max(a, c);
+}
+
+// A warp per token, V neighbouring experts per lane (lane V on), so that the lowest lane holds the lowest experts and a
+// tie is the first lane of a ballot. The k largest are taken one after the other: the lanes' best by one warp reduction,
+// and the lane that had it looks for its next. Groups whose runs are whole lanes, a power of two of them (every usual
+// shape), are ranked by shuffles, all at once; others one by one.
 template <typename IN, int V>
 __global__ void __launch_bounds__(128) k_route(const IN* __restrict__ logits, const float* __restrict__ bias,
                                                float* __restrict__ weights, int* __restrict__ experts, RouteArgs a) {
-  const int lane = threadIdx.x & 31;
+  const int lane = threadIdx.x & 31, e0 = lane * V;
   const int64_t t = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 5);
   if (t >= a.T) return;
   float l[V], s[V];
+  load_row<IN, V>(logits + t * a.stride, e0, a.E, a.vec, l);
   bool bad = false;
 #pragma unroll
-  for (int i = 0; i < V; i++) {
-    const int e = i * 32 + lane;
-    l[i] = e < a.E ? to_float<IN>(logits[t * a.stride + e]) : -INFINITY;
-    bad |= is_nan(l[i]);
-  }
+  for (int i = 0; i < V; i++) bad |= is_nan(l[i]);
   bad = __any_sync(kAll, bad);
   float top = -INFINITY, sum = 1.0f;
   if (!a.sigmoid) {
@@ -92,8 +116,6 @@ __global__ void __launch_bounds__(128) k_route(const IN* __restrict__ logits, co
       sum = __fadd_rn(sum, s[i]);
     }
     sum = warp_sum(sum);
-#pragma unroll
-    for (int i = 0; i < V; i++) s[i] = __fdiv_rn(s[i], sum);
   } else {
 #pragma unroll
     for (int i = 0; i < V; i++) s[i] = sigmoid(l[i]);
@@ -101,78 +123,91 @@ __global__ void __launch_bounds__(128) k_route(const IN* __restrict__ logits, co
   uint32_t key[V];
 #pragma unroll
   for (int i = 0; i < V; i++) {
-    const int e = i * 32 + lane;
-    const bool live = key_of(l[i]) != 0u;
-    key[i] = !live ? 0u : key_of(bias ? __fadd_rn(s[i], bias[e]) : l[i]);
+    key[i] = key_of(l[i]);
+    if (bias) {
+      if (!a.sigmoid) s[i] = __fdiv_rn(s[i], sum);
+      key[i] = key[i] ? key_of(__fadd_rn(s[i], e0 + i < a.E ? __ldg(bias + e0 + i) : 0.0f)) : 0u;
+    }
   }
   if (a.groups > 1) {
-    const int run = a.E / a.groups;
-    uint32_t mine = 0u;                                // lane g: the key of group g's value
-    for (int g = 0; g < a.groups; g++) {
-      uint32_t best = 0u;
-      int at = 0;
+    const int run = a.E / a.groups, width = run / V;
+    if (run % V == 0 && (width & (width - 1)) == 0) {
+      uint32_t best = 0u, second = 0u;
 #pragma unroll
-      for (int i = 0; i < V; i++) {
-        const int e = i * 32 + lane;
-        if (e >= g * run && e < (g + 1) * run && key[i] > best) {
-          best = key[i];
-          at = e;
-        }
+      for (int i = 0; i < V; i++) merge2(best, second, key[i], 0u);
+      for (int d = 1; d < width; d <<= 1) merge2(best, second, __shfl_xor_sync(kAll, best, d), __shfl_xor_sync(kAll, second, d));
+      if (a.top2 && second) best = key_of(__fadd_rn(value_of(best), value_of(second)));
+      const int g = lane / width;
+      int ahead = 0;                                   // groups that come before this lane's
+      for (int o = 0; o < a.groups; o++) {
+        const uint32_t v = __shfl_sync(kAll, best, o * width);
+        ahead += v > best || (v == best && o < g);
       }
-      const uint32_t m = __reduce_max_sync(kAll, best);
-      uint32_t v = m;
-      if (a.top2 && m) {
-        const int first = __reduce_min_sync(kAll, best == m ? at : INT_MAX);
-        uint32_t second = 0u;
+      if (ahead >= a.keep) {
+#pragma unroll
+        for (int i = 0; i < V; i++) key[i] = 0u;
+      }
+    } else {
+      uint32_t mine = 0u;                              // lane g: the key of group g's value
+      for (int g = 0; g < a.groups; g++) {
+        uint32_t best = 0u, second = 0u;
 #pragma unroll
         for (int i = 0; i < V; i++) {
-          const int e = i * 32 + lane;
-          if (e >= g * run && e < (g + 1) * run && e != first) second = max(second, key[i]);
+          const bool in = e0 + i >= g * run && e0 + i < (g + 1) * run;
+          merge2(best, second, in ? key[i] : 0u, 0u);
         }
-        second = __reduce_max_sync(kAll, second);
-        if (second) v = key_of(__fadd_rn(value_of(m), value_of(second)));
+        for (int d = 1; d < 32; d <<= 1) merge2(best, second, __shfl_xor_sync(kAll, best, d), __shfl_xor_sync(kAll, second, d));
+        if (a.top2 && second) best = key_of(__fadd_rn(value_of(best), value_of(second)));
+        if (lane == g) mine = best;
       }
-      if (lane == g) mine = v;
-    }
-    unsigned kept = 0u;
-    for (int j = 0; j < a.keep; j++) {
-      const uint32_t m = __reduce_max_sync(kAll, mine);
-      if (!m) break;
-      const int g = __ffs(__ballot_sync(kAll, mine == m)) - 1;
-      kept |= 1u << g;
-      if (lane == g) mine = 0u;
-    }
+      unsigned kept = 0u;
+      for (int j = 0; j < a.keep; j++) {
+        const uint32_t m = __reduce_max_sync(kAll, mine);
+        if (!m) break;
+        const int g = __ffs(__ballot_sync(kAll, mine == m)) - 1;
+        kept |= 1u << g;
+        if (lane == g) mine = 0u;
+      }
 #pragma unroll
-    for (int i = 0; i < V; i++) {
-      const int e = i * 32 + lane;
-      if (e < a.E && !(kept >> (e / run) & 1u)) key[i] = 0u;
+      for (int i = 0; i < V; i++)
+        if (e0 + i < a.E && !(kept >> ((e0 + i) / run) & 1u)) key[i] = 0u;
     }
   }
-  int chosen = -1;                                     // lane j: the j-th choice
-  float w = 0.0f;
-  for (int j = 0; j < a.k; j++) {
-    uint32_t best = 0u;
-    int at = INT_MAX;
-    float sc = 0.0f;
+  uint32_t best = 0u;                                  // this lane's best, its place among the V, its score
+  int at = 0;
+  float sc = 0.0f;
+  auto look = [&] {
+    best = 0u;
 #pragma unroll
     for (int i = 0; i < V; i++)
       if (key[i] > best) {
         best = key[i];
-        at = i * 32 + lane;
+        at = i;
         sc = s[i];
       }
+  };
+  look();
+  int chosen = -1;                                     // lane j: the j-th choice
+  float w = 0.0f;
+  for (int j = 0; j < a.k; j++) {
     const uint32_t m = __reduce_max_sync(kAll, best);
     if (!m) break;
-    const int e = __reduce_min_sync(kAll, best == m ? at : INT_MAX);
-    sc = __shfl_sync(kAll, sc, e & 31);
-#pragma unroll
-    for (int i = 0; i < V; i++)
-      if (i * 32 + lane == e) key[i] = 0u;
+    const int win = __ffs(__ballot_sync(kAll, best == m)) - 1;
+    const int e = __shfl_sync(kAll, e0 + at, win);
+    const float v = __shfl_sync(kAll, sc, win);
     if (lane == j) {
       chosen = e;
-      w = sc;
+      w = v;
+    }
+    if (lane == win) {
+#pragma unroll
+      for (int i = 0; i < V; i++)
+        if (i == at) key[i] = 0u;
+      look();
     }
   }
+  if (!a.sigmoid && !bias) w = __fdiv_rn(w, sum);
+  if (chosen < 0) w = 0.0f;
   if (a.renormalize) w = __fdiv_rn(w, __fadd_rn(warp_sum(w), kEps));
   w = bad ? __uint_as_float(0x7fc00000u) : __fmul_rn(w, a.scale);
   if (lane < a.k) {
@@ -256,7 +291,8 @@ __global__ void __launch_bounds__(kDispatchWarps * 32) k_dispatch(const int* __r
   extern __shared__ int sm[];
   int* count = sm;                                     // [warp][E]: counts, then the next place of each expert
   int* total = sm + kDispatchWarps * E;                // [E] this CTA's
-  int* sums = total + E;                               // [32] of the scan over experts
+  int* start = total + E;                              // [E] the first place of this CTA's
+  int* sums = start + E;                               // [32] of the scan over experts
   cg::cluster_group cluster = cg::this_cluster();
   const int ctas = (int)cluster.num_blocks(), rank = (int)cluster.block_rank();
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
@@ -265,7 +301,16 @@ __global__ void __launch_bounds__(kDispatchWarps * 32) k_dispatch(const int* __r
   const int64_t runs = (int64_t)ctas * kDispatchWarps, run = ((S + runs - 1) / runs + 31) / 32 * 32;
   const int64_t begin = min(S, (rank * (int64_t)kDispatchWarps + warp) * run), end = min(S, begin + run);
   int* mine = count + warp * E;
-  for (int64_t i = begin + lane; i < end; i += 32) {
+  // the run's first 256 slots stay in registers for the second walk
+  constexpr int kHeld = 8;
+  int held[kHeld];
+#pragma unroll
+  for (int h = 0; h < kHeld; h++) held[h] = begin + h * 32 + lane < end ? ids[begin + h * 32 + lane] : -1;
+#pragma unroll
+  for (int h = 0; h < kHeld; h++)
+    if (held[h] >= 0 && held[h] < E) atomicAdd(mine + held[h], 1);
+#pragma unroll 4
+  for (int64_t i = begin + kHeld * 32 + lane; i < end; i += 32) {
     const int e = ids[i];
     if (e >= 0 && e < E) atomicAdd(mine + e, 1);
   }
@@ -273,6 +318,7 @@ __global__ void __launch_bounds__(kDispatchWarps * 32) k_dispatch(const int* __r
   const int e = threadIdx.x;                           // a thread per expert: E <= 1024
   int own = 0;
   if (e < E) {
+#pragma unroll 16
     for (int w = 0; w < kDispatchWarps; w++) {
       const int c = count[w * E + e];
       count[w * E + e] = own;
@@ -305,17 +351,15 @@ __global__ void __launch_bounds__(kDispatchWarps * 32) k_dispatch(const int* __r
   const int first = head + scan - all;
   if (e < E) {
     if (rank == 0) offsets[e] = first;
-    for (int w = 0; w < kDispatchWarps; w++) count[w * E + e] += first + before;
+    start[e] = first + before;
   }
   if (rank == 0 && threadIdx.x == 0) offsets[E] = live;
   for (int64_t i = live + rank * (int64_t)blockDim.x + threadIdx.x; i < S; i += (int64_t)ctas * blockDim.x) order[i] = -1;
   __syncthreads();
-  for (int64_t b = begin; b < end; b += 32) {
-    const int64_t i = b + lane;
-    int x = i < end ? ids[i] : -1;
+  auto place32 = [&](int64_t i, int x) {
     if (x < 0 || x >= E) x = -1;
     const unsigned same = __match_any_sync(kAll, x);
-    const int place = x >= 0 ? mine[x] + __popc(same & ((1u << lane) - 1u)) : -1;
+    const int place = x >= 0 ? start[x] + mine[x] + __popc(same & ((1u << lane) - 1u)) : -1;
     __syncwarp();
     if (x >= 0 && lane == __ffs(same) - 1) mine[x] += __popc(same);
     __syncwarp();
@@ -323,7 +367,11 @@ __global__ void __launch_bounds__(kDispatchWarps * 32) k_dispatch(const int* __r
       where[i] = place;
       if (place >= 0) order[place] = (int)i;
     }
-  }
+  };
+#pragma unroll
+  for (int h = 0; h < kHeld; h++)
+    if (begin + h * 32 < end) place32(begin + h * 32 + lane, held[h]);
+  for (int64_t b = begin + kHeld * 32; b < end; b += 32) place32(b + lane, b + lane < end ? ids[b + lane] : -1);
   cluster.sync();                                      // the totals are read before their CTA leaves
 }
 
@@ -412,48 +460,53 @@ __global__ void __launch_bounds__(256) k_combine(const T* __restrict__ z, const 
   store_vec<T, VEC>(y + t * n, c, n, o);
 }
 
-// A CTA per token: dy's row is read once per eight experts' rows; a thread's share of the dot products stays in
-// registers and is added up over the CTA in a fixed order.
-template <typename T, bool VEC>
+// A CTA per token. J experts' rows (all of them up to 8) at a time: dy's piece is read once for them, their pieces of z are
+// on their way together, and a thread's share of the dot products stays in registers and is added up over the CTA in a
+// fixed order.
+template <typename T, bool VEC, int J>
 __global__ void __launch_bounds__(256) k_combine_backward(const T* __restrict__ dy, int64_t dy_stride, const T* __restrict__ z,
                                                           const float* __restrict__ weights, const int* __restrict__ where,
                                                           const int* __restrict__ order, T* __restrict__ dz,
-                                                          float* __restrict__ dw, int k, int64_t n, int64_t rows) {
-  constexpr int N = Vec<T>::N, J = 8;
+                                                          float* __restrict__ dw, int k, int64_t n, int rows) {
+  constexpr int N = Vec<T>::N;
   __shared__ float part[8][J];
   const int64_t t = blockIdx.x;
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, warps = blockDim.x >> 5;
+  bool hole = false;                                   // a place without a slot among this CTA's k
+  for (int j = threadIdx.x; j < k; j += blockDim.x) hole |= order[t * k + j] < 0;
   for (int j0 = 0; j0 < k; j0 += J) {
-    int64_t at[J];
+    int at[J];
     float w[J], dot[J];
 #pragma unroll
     for (int j = 0; j < J; j++) {
       const bool in = j0 + j < k;
-      at[j] = in ? where[t * k + j0 + j] : -1;
+      at[j] = in ? __ldg(where + t * k + j0 + j) : -1;
       if (at[j] >= rows) at[j] = -1;
-      w[j] = in ? weights[t * k + j0 + j] : 0.0f;
+      w[j] = in ? __ldg(weights + t * k + j0 + j) : 0.0f;
       dot[j] = 0.0f;
     }
     for (int64_t c = threadIdx.x * N; c < n; c += blockDim.x * N) {
       float g[N], v[N], o[N];
-      load_vec<T, VEC>(dy + t * dy_stride, c, n).get(g);
+      const Vec<T> mine = load_vec<T, VEC>(dy + t * dy_stride, c, n);
       Vec<T> r[J];
 #pragma unroll
-      for (int j = 0; j < J; j++)
+      for (int j = 0; j < J; j++) {
+        r[j].raw = make_uint4(0, 0, 0, 0);
         if (at[j] >= 0) r[j] = load_vec<T, VEC>(z + at[j] * n, c, n);
+      }
+      mine.get(g);
 #pragma unroll
-      for (int j = 0; j < J; j++)
-        if (at[j] >= 0) {
-          r[j].get(v);
+      for (int j = 0; j < J; j++) {
+        r[j].get(v);
 #pragma unroll
-          for (int i = 0; i < N; i++) {
-            dot[j] = __fmaf_rn(g[i], v[i], dot[j]);
-            o[i] = __fmul_rn(w[j], g[i]);
-          }
-          Vec<T> q;
-          q.set(o);
-          store_vec<T, VEC>(dz + at[j] * n, c, n, q);
+        for (int i = 0; i < N; i++) {
+          if (at[j] >= 0) dot[j] = __fmaf_rn(g[i], v[i], dot[j]);
+          o[i] = __fmul_rn(w[j], g[i]);
         }
+        Vec<T> q;
+        q.set(o);
+        if (at[j] >= 0) store_vec<T, VEC>(dz + at[j] * n, c, n, q);
+      }
     }
 #pragma unroll
     for (int j = 0; j < J; j++) {
@@ -466,8 +519,9 @@ __global__ void __launch_bounds__(256) k_combine_backward(const T* __restrict__ 
       for (int i = 0; i < warps; i++) d = __fadd_rn(d, part[i][threadIdx.x]);
       dw[t * k + j0 + threadIdx.x] = d;
     }
-    __syncthreads();
+    if (j0 + J < k) __syncthreads();
   }
+  if (!__syncthreads_or(hole)) return;
   for (int j = 0; j < k; j++) {                        // the rows that no slot has
     if (order[t * k + j] >= 0) continue;
     Vec<T> zero;
@@ -509,6 +563,11 @@ int by_type(const char* who, int32_t type, F f) {
     default: return set_error(MXQ_ERR_VALUE, "%s: type %d", who, type);
   }
 }
+template <typename IN>
+int row_vec(const void* logits, int64_t stride, int E, int v) {
+  constexpr int N = 16 / sizeof(IN);
+  return v % N == 0 && E == 32 * v && stride % N == 0 && aligned16(logits);
+}
 template <int N>
 struct Int { static constexpr int value = N; };
 template <typename F>
@@ -532,6 +591,7 @@ extern "C" int mxq_route(const void* logits, int32_t type, int64_t stride, const
   return by_type("route", type, [&](auto zero) {
     using IN = decltype(zero);
     by_width(a.E, [&](auto v) {
+      a.vec = row_vec<IN>(logits, stride, a.E, decltype(v)::value);
       k_route<IN, decltype(v)::value><<<(unsigned)((T + 3) / 4), 128, 0, as_stream(stream)>>>(static_cast<const IN*>(logits), bias, weights,
                                                                                           experts, a);
     });
@@ -562,8 +622,8 @@ extern "C" int mxq_dispatch(const int32_t* experts_of, int64_t slots, int64_t ex
   // a CTA walks 4096 slots in four steps per warp; a cluster (at most 8 CTAs) shares more
   int ctas = 1;
   while (ctas < 8 && slots > 4096ll * ctas) ctas *= 2;
-  const int smem = (int)((kDispatchWarps + 1) * experts + 32) * 4;
-  if (int rc = allow_smem((const void*)k_dispatch, ((kDispatchWarps + 1) * kMostExperts + 32) * 4)) return rc;
+  const int smem = (int)((kDispatchWarps + 2) * experts + 32) * 4;
+  if (int rc = allow_smem((const void*)k_dispatch, ((kDispatchWarps + 2) * kMostExperts + 32) * 4)) return rc;
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3(ctas);
   cfg.blockDim = dim3(kDispatchWarps * 32);
@@ -613,9 +673,19 @@ extern "C" int mxq_combine_backward(const void* dy, int64_t dy_stride, const voi
     const bool vec = N % V == 0 && aligned16(z) && aligned16(dz) && aligned16(dy) && dy_stride % V == 0;
     const int64_t threads = (N + V - 1) / V;
     const int block = threads > 128 ? 256 : threads > 64 ? 128 : 64;
-    auto f = vec ? k_combine_backward<X, true> : k_combine_backward<X, false>;
-    f<<<(unsigned)T, block, 0, as_stream(stream)>>>(static_cast<const X*>(dy), dy_stride, static_cast<const X*>(z), weights, where, order,
-                                                    static_cast<X*>(dz), dw, (int)k, N, T * k);
+    auto go = [&](auto width) {
+      constexpr int J = decltype(width)::value;
+      auto f = vec ? k_combine_backward<X, true, J> : k_combine_backward<X, false, J>;
+      f<<<(unsigned)T, block, 0, as_stream(stream)>>>(static_cast<const X*>(dy), dy_stride, static_cast<const X*>(z), weights, where, order,
+                                                      static_cast<X*>(dz), dw, (int)k, N, (int)(T * k));
+    };
+    switch (k) {
+      case 1: go(Int<1>{}); break;
+      case 2: go(Int<2>{}); break;
+      case 3: case 4: go(Int<4>{}); break;
+      case 5: case 6: go(Int<6>{}); break;
+      default: go(Int<8>{});
+    }
     return MXQ_LAUNCH_CHECK("combine_backward");
   });
 }
