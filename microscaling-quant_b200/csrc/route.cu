@@ -356,9 +356,16 @@ __global__ void __launch_bounds__(kDispatchWarps * 32) k_dispatch(const int* __r
   if (rank == 0 && threadIdx.x == 0) offsets[E] = live;
   for (int64_t i = live + rank * (int64_t)blockDim.x + threadIdx.x; i < S; i += (int64_t)ctas * blockDim.x) order[i] = -1;
   __syncthreads();
+  const int bits = 32 - __clz(E - 1);                  // 0 for one expert
   auto place32 = [&](int64_t i, int x) {
     if (x < 0 || x >= E) x = -1;
-    const unsigned same = __match_any_sync(kAll, x);
+    // the lanes with this lane's expert: a ballot per bit (a match instruction takes longer)
+    unsigned same = __ballot_sync(kAll, x >= 0);
+    for (int bit = 0; bit < bits; bit++) {
+      const bool mine_set = x >> bit & 1;
+      const unsigned set = __ballot_sync(kAll, mine_set);
+      same &= mine_set ? set : ~set;
+    }
     const int place = x >= 0 ? start[x] + mine[x] + __popc(same & ((1u << lane) - 1u)) : -1;
     __syncwarp();
     if (x >= 0 && lane == __ffs(same) - 1) mine[x] += __popc(same);
@@ -464,7 +471,7 @@ __global__ void __launch_bounds__(256) k_combine(const T* __restrict__ z, const 
 // on their way together, and a thread's share of the dot products stays in registers and is added up over the CTA in a
 // fixed order.
 template <typename T, bool VEC, int J>
-__global__ void __launch_bounds__(256) k_combine_backward(const T* __restrict__ dy, int64_t dy_stride, const T* __restrict__ z,
+__global__ void __launch_bounds__(256, 3) k_combine_backward(const T* __restrict__ dy, int64_t dy_stride, const T* __restrict__ z,
                                                           const float* __restrict__ weights, const int* __restrict__ where,
                                                           const int* __restrict__ order, T* __restrict__ dz,
                                                           float* __restrict__ dw, int k, int64_t n, int rows) {
