@@ -269,8 +269,8 @@ int mxq_linear_packed(const uint8_t* x, const uint8_t* x_scales, int64_t x_pitch
                       void* stream);
 /* The same product by expert: rows offsets[e] .. offsets[e + 1] - 1 of y (experts + 1 non-decreasing offsets, the last
  * at most `slots`) are multiplied with expert e's N x K weights (w: experts x N x K, bias: experts x N). Row r of y takes
- * row r of x (per 0), or row order[r] / per (per > 0). Rows from the last offset on are not written. At most 1024
- * experts. */
+ * row r of x (per 0), or row order[r] / per (per > 0). Rows from the last offset on are not written; offsets
+ * outside [0, slots] and rows of x outside [0, x_rows) are cut to these. At most 1024 experts; x not FP4 if per > 0. */
 int mxq_experts_packed(const uint8_t* x, const uint8_t* x_scales, int64_t x_pitch, int64_t x_rows, const uint8_t* w,
                        const uint8_t* w_scales, int64_t w_pitch, int64_t experts, int64_t N, int64_t K,
                        const int32_t* offsets, const int32_t* order, int64_t slots, int64_t per,

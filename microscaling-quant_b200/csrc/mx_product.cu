@@ -1172,6 +1172,7 @@ int product(const char* who, Args& a, const Operand& x, const Operand& w, int64_
   const int fmtx = format_of(s->x_e, s->x_m), fmtw = format_of(s->w_e, s->w_m);
   if (int rc = check_operand(who, "x", x.codes, x.pitch, fmtx, K, &fx)) return rc;
   if (int rc = check_operand(who, "w", w.codes, w.pitch, fmtw, K, &fw)) return rc;
+  MXQ_REQUIRE(a.per == 0 || fmtx != kFmtE2M1, MXQ_ERR_UNSUPPORTED, "%s: rows of FP4 x cannot be gathered (mxq_lay_codes widens them)", who);
   MXQ_REQUIRE(s->activation >= kActNone && s->activation <= kActGeglu, MXQ_ERR_VALUE, "%s: activation %d", who, s->activation);
   MXQ_REQUIRE(s->out >= kOutF32 && s->out <= kOutPacked, MXQ_ERR_VALUE, "%s: output type %d", who, s->out);
   const bool gated = s->activation >= kActSwiglu;

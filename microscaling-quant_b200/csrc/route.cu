@@ -54,6 +54,10 @@ __device__ __forceinline__ uint32_t key_of(float f) {
 __device__ __forceinline__ float value_of(uint32_t key) {
   return __uint_as_float(key & 0x80000000u ? key & 0x7fffffffu : ~key);
 }
+// the key of a group's two largest, whose sum may pass the type's lowest value: that is still a group to choose
+__device__ __forceinline__ uint32_t key_of_pair(uint32_t best, uint32_t second) {
+  return key_of(fmaxf(__fadd_rn(value_of(best), value_of(second)), -3.402823466e38f));
+}
 __device__ __forceinline__ float sigmoid(float x) { return __frcp_rn(__fadd_rn(1.0f, expf(-x))); }
 __device__ __forceinline__ bool is_nan(float x) { return x != x; }
 
@@ -136,7 +140,7 @@ __global__ void __launch_bounds__(128) k_route(const IN* __restrict__ logits, co
 #pragma unroll
       for (int i = 0; i < V; i++) merge2(best, second, key[i], 0u);
       for (int d = 1; d < width; d <<= 1) merge2(best, second, __shfl_xor_sync(kAll, best, d), __shfl_xor_sync(kAll, second, d));
-      if (a.top2 && second) best = key_of(__fadd_rn(value_of(best), value_of(second)));
+      if (a.top2 && second) best = key_of_pair(best, second);
       const int g = lane / width;
       int ahead = 0;                                   // groups that come before this lane's
       for (int o = 0; o < a.groups; o++) {
@@ -157,7 +161,7 @@ __global__ void __launch_bounds__(128) k_route(const IN* __restrict__ logits, co
           merge2(best, second, in ? key[i] : 0u, 0u);
         }
         for (int d = 1; d < 32; d <<= 1) merge2(best, second, __shfl_xor_sync(kAll, best, d), __shfl_xor_sync(kAll, second, d));
-        if (a.top2 && second) best = key_of(__fadd_rn(value_of(best), value_of(second)));
+        if (a.top2 && second) best = key_of_pair(best, second);
         if (lane == g) mine = best;
       }
       unsigned kept = 0u;

@@ -81,15 +81,15 @@ def _pair(v, f: Format, who: str, what: str):
     return codes, scales, shape, K
 
 
-def _laid(codes: torch.Tensor, scales: torch.Tensor, shape, f: Format, K: int, dev):
+def _laid(codes: torch.Tensor, scales: torch.Tensor, shape, f: Format, K: int, dev, gathered: bool = False):
     """The operand as the kernels read it, (codes, scales, bytes from row to row, e, m): as it is where its rows allow
-    it, else laid out as 8-bit codes."""
+    it, else laid out as 8-bit codes. FP4 rows that are gathered one by one are laid out too."""
     codes, scales = _here(codes, dev), _here(scales, dev)
     bits = 1 + f.e + f.m
     if bits == 8:
         if K % 16 == 0 and codes.data_ptr() % 16 == 0:
             return codes, scales, K, f.e, f.m
-    elif bits == 4 and K % 128 == 0 and codes.data_ptr() % 32 == 0:
+    elif bits == 4 and not gathered and K % 128 == 0 and codes.data_ptr() % 32 == 0:
         return codes, scales, K // 2, f.e, f.m
     rows = codes.numel() // shape[-1]
     pitch = -(-K // 16) * 16
@@ -111,7 +111,7 @@ def lay_packed(w: Pair, fmt: Union[str, Format]) -> Tuple[Pair, str]:
     return (_lib.back(wide, codes.device), scales), "MXFP8_E4M3"
 
 
-def _x_operand(x, x_fmt, who: str, w: torch.Tensor):
+def _x_operand(x, x_fmt, who: str, w: torch.Tensor, gathered: bool = False):
     """(operand, leading shape, K, device, home) of x, a pair or a float tensor that is packed here."""
     f = _format(x_fmt, who)
     if isinstance(x, torch.Tensor):
@@ -140,7 +140,7 @@ def _x_operand(x, x_fmt, who: str, w: torch.Tensor):
         return (codes, scales, pitch, e, m), shape[:-1], K, dev, x.device
     codes, scales, shape, K = _pair(x, f, who, "x")
     dev = codes.device if codes.is_cuda else _lib.device_for(codes, w)
-    return _laid(codes, scales, shape, f, K, dev), shape[:-1], K, dev, codes.device
+    return _laid(codes, scales, shape, f, K, dev, gathered), shape[:-1], K, dev, codes.device
 
 
 def _make_spec(x_e, x_m, w_e, w_m, act, out, out_e, out_m):
@@ -261,7 +261,7 @@ def experts_packed(x: Union[Pair, torch.Tensor], w: Pair, fmt: Union[str, Format
     if bias is not None and tuple(bias.shape) != (E, N):
         raise ValueError(f"{who}: bias must have shape {(E, N)}, got {tuple(bias.shape)}")
     _ready()
-    (xc, xs, xp, xe, xm), lead, Kx, dev, home = _x_operand(x, x_fmt, who, wc)
+    (xc, xs, xp, xe, xm), lead, Kx, dev, home = _x_operand(x, x_fmt, who, wc, gather)
     if Kx != K:
         raise ValueError(f"{who}: x has {Kx} values per row and w {K}")
     if len(lead) != 1:
