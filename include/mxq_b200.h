@@ -334,6 +334,12 @@ int mxq_wait_status_word(uint32_t** out);
  * word and the device counter rise by one per 32 x 256 tile. cols a multiple of 32, V and P 16-byte aligned. */
 int mxq_testing_wait_timeout(const float* V, float* P, float* X, int64_t rows, int64_t cols, uint32_t wait_rounds,
                              void* stream);
+/* No reference counterpart; for tests of the timeout path only: mxq_linear_packed of E4M3 operands (M x K and N x K, K a
+ * multiple of 16, float32 y) whose stages expect bytes that never come, with waits of wait_cycles (1..2^22) clock cycles:
+ * the first wait for a stage runs out after its loads have landed, every role leaves, y comes out NaN and the wait-status
+ * word and the device counter rise by one at least. */
+int mxq_testing_product_timeout(const uint8_t* x, const uint8_t* x_scales, int64_t M, const uint8_t* w,
+                                const uint8_t* w_scales, int64_t N, int64_t K, float* y, int64_t wait_cycles, void* stream);
 
 #ifdef __cplusplus
 }

@@ -45,6 +45,7 @@ struct Args {
   int act, otype, ofmt;
   int vec_out;                 // y's (and the residual's) rows take 16-byte accesses
   unsigned* status;
+  int64_t wait_cycles;
 };
 
 // ------------------------------------------------------------------------------------------ epilogue values
@@ -166,8 +167,8 @@ struct ScaleRows {
 // step j of the four that v holds, into the ring's next stage
 template <int G>
 __device__ __forceinline__ bool store_scales(const uint4 (&v)[4 * G], int j, const Args& a, uint8_t* area, int pitch, uint64_t* ready,
-                                             uint64_t* empty, Ring& ring, int stages, volatile int* abort) {
-  if (!tc::wait_warp(&empty[ring.stage], ring.phase ^ 1u, abort, a.status)) return false;
+                                             uint64_t* empty, Ring& ring, int stages, const tc::Guard& guard) {
+  if (!tc::wait_warp(&empty[ring.stage], ring.phase ^ 1u, guard)) return false;
   uint8_t* to = area + (size_t)ring.stage * pitch + (threadIdx.x & 31) * 16;
   auto word = [j](const uint4& q) { return j == 0 ? q.x : j == 1 ? q.y : j == 2 ? q.z : q.w; };
 #pragma unroll
@@ -182,8 +183,8 @@ __device__ __forceinline__ bool store_scales(const uint4 (&v)[4 * G], int j, con
 // that its thread has under way, and the loader has the next loads under way. far: the full barriers' shared::cluster
 // address where they are in another CTA, else 0.
 __device__ __forceinline__ bool forward_scales(const Args& a, uint64_t* ready, uint64_t* full, uint32_t far, Ring& ring, int stages,
-                                               volatile int* abort) {
-  if (!tc::wait_warp(&ready[ring.stage], ring.phase, abort, a.status)) return false;
+                                               const tc::Guard& guard) {
+  if (!tc::wait_warp(&ready[ring.stage], ring.phase, guard)) return false;
   if (tc::elect()) {
     fence_proxy_async();
     if (far) tc::mbar_arrive_remote(far + 8u * ring.stage);
@@ -486,7 +487,7 @@ __global__ void __launch_bounds__(128 + 32 * kWriters, 1) __cluster_dims__(2, 1,
   uint8_t* passes = scales + kStages * kStageScales;
   TileShared& sh = *reinterpret_cast<TileShared*>(passes + kWriters * kPassBytes);
   const Table tab(&sh + 1, a.experts);
-  volatile int* abort = &sh.abort;
+  const tc::Guard guard = {&sh.abort, a.status, a.wait_cycles};
   const int warp = __shfl_sync(~0u, threadIdx.x >> 5, 0), lane = threadIdx.x & 31;
   constexpr int kCols = GATED ? 128 : 256;             // columns of y per tile
   const int col_tiles = (a.width + kCols - 1) / kCols;
@@ -533,7 +534,7 @@ __global__ void __launch_bounds__(128 + 32 * kWriters, 1) __cluster_dims__(2, 1,
       if (a.per > 0) rows = make_int4(x_row(a, t, r0), x_row(a, t, r0 + 1), x_row(a, t, r0 + 2), x_row(a, t, r0 + 3));
       const int w0 = t.expert * a.n + t.col * kCols + (rank ? second : 0);
       for (int kb = 0; kb < a.kblocks; kb++) {
-        ok = tc::wait_warp(&sh.empty[ring.stage], ring.phase ^ 1u, abort, a.status);
+        ok = tc::wait_warp(&sh.empty[ring.stage], ring.phase ^ 1u, guard);
         if (!ok) break;
         uint8_t* to = codes + ring.stage * kStageBytes;
         const uint32_t bar = full + 8u * ring.stage;
@@ -551,7 +552,7 @@ __global__ void __launch_bounds__(128 + 32 * kWriters, 1) __cluster_dims__(2, 1,
     if (!ok && lane == 0)                              // the loads under way land before the CTA leaves
       for (int s = 0; s < kStages && s < sent; s++) {
         ring.stage = ring.stage ? ring.stage - 1 : (ring.phase ^= 1u, kStages - 1);
-        tc::settle(&sh.full[ring.stage], ring.phase);
+        tc::settle(&sh.full[ring.stage], ring.phase, guard);
       }
   } else if (warp == 1) {
     if (rank == 0) {
@@ -559,11 +560,11 @@ __global__ void __launch_bounds__(128 + 32 * kWriters, 1) __cluster_dims__(2, 1,
       bool ok = true;
       int done = 0;
       for (int i = pair; ok && i < tiles; i += pairs, done++) {
-        if (done) ok = tc::wait_warp(&sh.acc_free, (done - 1) & 1, abort, a.status);
+        if (done) ok = tc::wait_warp(&sh.acc_free, (done - 1) & 1, guard);
         if (!ok) break;
         const uint32_t acc = tmem + (done & 1 ? 192 : 0);
         for (int kb = 0; kb < a.kblocks; kb++) {
-          ok = tc::wait_warp(&sh.full[ring.stage], ring.phase, abort, a.status);
+          ok = tc::wait_warp(&sh.full[ring.stage], ring.phase, guard);
           if (!ok) break;
           tc::fence_after();
           const uint32_t at = smem_addr(codes + ring.stage * kStageBytes);
@@ -585,7 +586,7 @@ __global__ void __launch_bounds__(128 + 32 * kWriters, 1) __cluster_dims__(2, 1,
       }
       if (!ok && tc::elect()) {
         tc::commit<true>(&sh.last);
-        tc::settle(&sh.last, 0);
+        tc::settle(&sh.last, 0, guard);
       }
     }
   } else if (warp == 2) {
@@ -621,7 +622,7 @@ __global__ void __launch_bounds__(128 + 32 * kWriters, 1) __cluster_dims__(2, 1,
       if (more) rows.load(nxt, g, a);
 #pragma unroll
       for (int j = 0; j < 4; j++)
-        if (j < steps && ok) ok = store_scales<3>(now, j, a, scales, kStageScales, sh.ready, sh.empty, ring, kStages, abort);
+        if (j < steps && ok) ok = store_scales<3>(now, j, a, scales, kStageScales, sh.ready, sh.empty, ring, kStages, guard);
 #pragma unroll
       for (int j = 0; j < 12; j++) now[j] = nxt[j];
     }
@@ -629,7 +630,7 @@ __global__ void __launch_bounds__(128 + 32 * kWriters, 1) __cluster_dims__(2, 1,
     Ring ring;
     bool ok = true;
     for (int i = pair; ok && i < tiles; i += pairs)
-      for (int kb = 0; kb < a.kblocks && ok; kb++) ok = forward_scales(a, sh.ready, sh.full, rank ? full : 0u, ring, kStages, abort);
+      for (int kb = 0; kb < a.kblocks && ok; kb++) ok = forward_scales(a, sh.ready, sh.full, rank ? full : 0u, ring, kStages, guard);
   } else {
     Tiles list;
     int done = 0;
@@ -665,7 +666,7 @@ __global__ void __launch_bounds__(128 + 32 * kWriters, 1) __cluster_dims__(2, 1,
       };
       fetch(t.col * kCols + unit_of(0) * 64);
       fetch_bias(t.col * kCols + unit_of(0) * 64);
-      const bool ok = tc::wait(&sh.acc_full, done & 1, abort, a.status);
+      const bool ok = tc::wait(&sh.acc_full, done & 1, guard);
       __syncwarp();
       tc::fence_after();
       // the second warps' word that they are through with the tile before; the first warps give theirs below
@@ -868,7 +869,7 @@ __global__ void __launch_bounds__(128, 2) k_mx_rows(const __grid_constant__ CUte
   uint8_t* scales = codes + S::kDepth * S::kStageCodes;
   RowsShared& sh = *reinterpret_cast<RowsShared*>(scales + S::kDepth * S::kStageScales);
   const Table tab(&sh + 1, a.experts);
-  volatile int* abort = &sh.abort;
+  const tc::Guard guard = {&sh.abort, a.status, a.wait_cycles};
   const int warp = __shfl_sync(~0u, threadIdx.x >> 5, 0), lane = threadIdx.x & 31;
   constexpr int kCols = GATED ? 64 : 128;              // columns of y per tile
   const int col_tiles = (a.width + kCols - 1) / kCols;
@@ -912,7 +913,7 @@ __global__ void __launch_bounds__(128, 2) k_mx_rows(const __grid_constant__ CUte
       rows = make_int4(x_row(a, t, 4 * lane), x_row(a, t, 4 * lane + 1), x_row(a, t, 4 * lane + 2), x_row(a, t, 4 * lane + 3));
     const int w0 = t.expert * a.n + t.col * kCols;
     for (int kb = k0; kb < k1; kb++) {
-      ok = tc::wait_warp(&sh.empty[ring.stage], ring.phase ^ 1u, abort, a.status);
+      ok = tc::wait_warp(&sh.empty[ring.stage], ring.phase ^ 1u, guard);
       if (!ok) break;
       uint8_t* to = codes + ring.stage * S::kStageCodes;
       uint64_t* bar = &sh.full[ring.stage];
@@ -930,13 +931,13 @@ __global__ void __launch_bounds__(128, 2) k_mx_rows(const __grid_constant__ CUte
     if (!ok && lane == 0)
       for (int s = 0; s < S::kDepth && s < sent; s++) {
         ring.stage = ring.stage ? ring.stage - 1 : (ring.phase ^= 1u, S::kDepth - 1);
-        tc::settle(&sh.full[ring.stage], ring.phase);
+        tc::settle(&sh.full[ring.stage], ring.phase, guard);
       }
   } else if (busy && warp == 1) {
     Ring ring;
     bool ok = true;
     for (int kb = k0; kb < k1; kb++) {
-      ok = tc::wait_warp(&sh.full[ring.stage], ring.phase, abort, a.status);
+      ok = tc::wait_warp(&sh.full[ring.stage], ring.phase, guard);
       if (!ok) break;
       tc::fence_after();
       const uint32_t at = smem_addr(codes + ring.stage * S::kStageCodes);
@@ -957,7 +958,7 @@ __global__ void __launch_bounds__(128, 2) k_mx_rows(const __grid_constant__ CUte
     }
     if (!ok && tc::elect()) {
       tc::commit<false>(&sh.last);
-      tc::settle(&sh.last, 0);
+      tc::settle(&sh.last, 0, guard);
     }
   } else if (busy && warp == 2) {
     ScaleRows<2> rows;                                 // w's 128 rows; x's, the last repeated up to 128
@@ -978,21 +979,21 @@ __global__ void __launch_bounds__(128, 2) k_mx_rows(const __grid_constant__ CUte
 #pragma unroll
       for (int j = 0; j < 4; j++)
         if (g * 4 + j >= k0 && g * 4 + j < k1 && ok)
-          ok = store_scales<2>(now, j, a, scales, S::kStageScales, sh.ready, sh.empty, ring, S::kDepth, abort);
+          ok = store_scales<2>(now, j, a, scales, S::kStageScales, sh.ready, sh.empty, ring, S::kDepth, guard);
 #pragma unroll
       for (int i = 0; i < 8; i++) now[i] = nxt[i];
     }
   } else if (busy) {
     Ring ring;
     bool ok = true;
-    for (int kb = k0; kb < k1 && ok; kb++) ok = forward_scales(a, sh.ready, sh.full, 0u, ring, S::kDepth, abort);
+    for (int kb = k0; kb < k1 && ok; kb++) ok = forward_scales(a, sh.ready, sh.full, 0u, ring, S::kDepth, guard);
   }
   __syncwarp();
 
   // partial sums, [row of x][feature], over the codes' stages, which are all consumed
   float* part = reinterpret_cast<float*>(codes);
   if (work) {
-    const bool ok = !busy || tc::wait(&sh.acc_full, 0, abort, a.status);
+    const bool ok = !busy || tc::wait(&sh.acc_full, 0, guard);
     __syncwarp();
     tc::fence_after();
     const uint32_t acc = tmem + ((uint32_t)(warp * 32) << 16);
@@ -1204,6 +1205,8 @@ int product(const char* who, Args& a, const Operand& x, const Operand& w, int64_
   if (a.rows == 0 || a.width == 0) return MXQ_OK;
   a.status = wait_status_word();
   if (!a.status) return MXQ_ERR_CUDA;
+  if (a.wait_cycles == 0) a.wait_cycles = tc::kWaitCycles;
+  else a.xbytes += 16;                                 // the test of the waits: bytes that never come
   return gated ? launch<true>(a, x, w, K, fx, fw, st) : launch<false>(a, x, w, K, fx, fw, st);
 }
 
@@ -1238,6 +1241,22 @@ extern "C" int mxq_linear_packed(const uint8_t* x, const uint8_t* x_scales, int6
   a.out_scales = out_scales;
   return product("linear_packed", a, {x, M, x_pitch, spec->x_e + spec->x_m == 3}, {w, N, w_pitch, spec->w_e + spec->w_m == 3}, K,
                  spec, as_stream(stream));
+}
+
+extern "C" int mxq_testing_product_timeout(const uint8_t* x, const uint8_t* x_scales, int64_t M, const uint8_t* w,
+                                           const uint8_t* w_scales, int64_t N, int64_t K, float* y, int64_t wait_cycles,
+                                           void* stream) {
+  if (int rc = check_sizes("testing_product_timeout", M, N, K, 1)) return rc;
+  MXQ_REQUIRE(wait_cycles >= 1 && wait_cycles <= (1 << 22), MXQ_ERR_VALUE, "testing_product_timeout: wait_cycles must be in [1, 2^22]");
+  const mxq_product_spec spec = {4, 3, 4, 3, MXQ_ACT_NONE, MXQ_OUT_F32, 0, 0};
+  Args a = {};
+  a.sx = x_scales;
+  a.sw = w_scales;
+  a.rows = a.xrows = (int)M;
+  a.n = (int)N;
+  a.out = y;
+  a.wait_cycles = wait_cycles;
+  return product("testing_product_timeout", a, {x, M, K, false}, {w, N, K, false}, K, &spec, as_stream(stream));
 }
 
 extern "C" int mxq_experts_packed(const uint8_t* x, const uint8_t* x_scales, int64_t x_pitch, int64_t x_rows, const uint8_t* w,

@@ -18,32 +18,37 @@ constexpr long long kWaitCycles = 4000000000ll;
 
 __device__ __forceinline__ bool try_wait(uint64_t* bar, unsigned parity) { return mbar_try_wait_rounds(bar, parity, 1); }
 
+// What bounds a CTA's waits: its word in shared memory, the library's status word, the limit.
+struct Guard {
+  volatile int* abort;
+  unsigned* status;
+  long long cycles;
+};
 // false: gave up (this wait ran out, or another role's did)
-__device__ __forceinline__ bool wait(uint64_t* bar, unsigned parity, volatile int* abort, unsigned* status_word) {
+__device__ __forceinline__ bool wait(uint64_t* bar, unsigned parity, const Guard& g) {
   if (try_wait(bar, parity) || try_wait(bar, parity)) return true;
   const long long begin = clock64();
   do {
     if (try_wait(bar, parity) || try_wait(bar, parity)) return true;
-    if (*abort) return false;
-  } while (clock64() - begin < kWaitCycles);
-  *abort = 1;
-  note_wait_timeout(status_word);
+    if (*g.abort) return false;
+  } while (clock64() - begin < g.cycles);
+  *g.abort = 1;
+  note_wait_timeout(g.status);
   return false;
 }
 // the same for what a role that gave up has in flight towards shared memory or TMEM, without the abort word
-__device__ __forceinline__ void settle(uint64_t* bar, unsigned parity) {
+__device__ __forceinline__ void settle(uint64_t* bar, unsigned parity, const Guard& g) {
   const long long begin = clock64();
-  while (!try_wait(bar, parity) && clock64() - begin < kWaitCycles / 20) {
+  while (!try_wait(bar, parity) && clock64() - begin < g.cycles / 16) {
   }
 }
 
 __device__ __forceinline__ void mbar_arrive(uint64_t* bar) {
   asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];\n" ::"r"(smem_addr(bar)) : "memory");
 }
-
 // wait() by a whole warp: the answer is the same in every lane, and the compiler knows it
-__device__ __forceinline__ bool wait_warp(uint64_t* bar, unsigned parity, volatile int* abort, unsigned* status_word) {
-  return __all_sync(0xffffffffu, wait(bar, parity, abort, status_word));
+__device__ __forceinline__ bool wait_warp(uint64_t* bar, unsigned parity, const Guard& g) {
+  return __all_sync(0xffffffffu, wait(bar, parity, g));
 }
 // one lane of a converged warp. The operands of what it issues have to be warp-uniform for the compiler (no lane index
 // in them, no branch on one around them): tcgen05 and TMA instructions take uniform registers, and from a branch on

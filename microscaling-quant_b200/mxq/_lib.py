@@ -109,6 +109,7 @@ _SIGS = {
     "mxq_combine_backward": [P, I64, P, I32, P, P, P, P, P, I64, I64, I64, P],
     "mxq_device_timeouts": [P],
     "mxq_wait_status_word": [P],
+    "mxq_testing_product_timeout": [P, P, I64, P, P, I64, I64, P, I64, P],
     "mxq_testing_wait_timeout": [P, P, P, I64, I64, ctypes.c_uint32, P],
 }
 
