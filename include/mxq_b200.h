@@ -256,25 +256,31 @@ typedef struct mxq_product_spec {
   int32_t x_e, x_m, w_e, w_m;   /* element formats of the codes */
   int32_t activation, out;      /* MXQ_ACT_*, MXQ_OUT_* */
   int32_t out_e, out_m;         /* MXQ_OUT_PACKED: the element format of the output's codes */
+  int32_t x_type;               /* 0: x is codes; 1 + MXQ_OUT_F32 / BF16 / F16: x is such values, packed to (x_e, x_m) first */
 } mxq_product_spec;
 /* y[M, F] = act(x w^T + bias) (* up) + residual with x M x K and w N x K; F = N, or N / 2 for a gated activation. Sums in
  * float32. bias: N float32 or NULL. residual: y's type, rows residual_stride elements apart, or NULL (not with a packed
  * output). A packed output's scale is 2^(floor(log2 amax) - emax) per 32 columns, codes rounded to nearest even and
- * saturated; a block with an Inf or a NaN gets the scale 0xFF and zero codes. Codes must be 8-bit (E4M3, E5M2) with base
- * and pitch multiples of 16 bytes, or FP4 with base and pitch multiples of 32 bytes and K a multiple of 128
- * (mxq_lay_codes brings any others to that). */
-int mxq_linear_packed(const uint8_t* x, const uint8_t* x_scales, int64_t x_pitch, int64_t M, const uint8_t* w,
+ * saturated; a block with an Inf or a NaN gets the scale 0xFF and zero codes. Codes of x and w may have any MX format,
+ * pitch (bytes from row to row; of float x: elements) and alignment. 8-bit codes (E4M3, E5M2) with base and pitch multiples
+ * of 16 bytes, and FP4 codes with base and pitch multiples of 32 bytes and K a multiple of 128, are read as they are; other
+ * codes, and float x, are laid out in `workspace` first (mxq_product_workspace bytes, 16-byte aligned; none when 0). */
+int64_t mxq_product_workspace(const void* x, int64_t x_pitch, int64_t x_rows, const uint8_t* w, int64_t w_pitch,
+                              int64_t w_rows, int64_t K, int32_t gathered, const mxq_product_spec* spec);
+int mxq_linear_packed(const void* x, const uint8_t* x_scales, int64_t x_pitch, int64_t M, const uint8_t* w,
                       const uint8_t* w_scales, int64_t w_pitch, int64_t N, int64_t K, const mxq_product_spec* spec,
                       const float* bias, const void* residual, int64_t residual_stride, void* out, uint8_t* out_scales,
-                      void* stream);
+                      void* workspace, int64_t workspace_bytes, void* stream);
 /* The same product by expert: rows offsets[e] .. offsets[e + 1] - 1 of y (experts + 1 non-decreasing offsets, the last
  * at most `slots`) are multiplied with expert e's N x K weights (w: experts x N x K, bias: experts x N). Row r of y takes
  * row r of x (per 0), or row order[r] / per (per > 0). Rows from the last offset on are not written; offsets
- * outside [0, slots] and rows of x outside [0, x_rows) are cut to these. At most 1024 experts; x not FP4 if per > 0. */
-int mxq_experts_packed(const uint8_t* x, const uint8_t* x_scales, int64_t x_pitch, int64_t x_rows, const uint8_t* w,
+ * outside [0, slots] and rows of x outside [0, x_rows) are cut to these. At most 1024 experts. gathered
+ * (mxq_product_workspace): per > 0. */
+int mxq_experts_packed(const void* x, const uint8_t* x_scales, int64_t x_pitch, int64_t x_rows, const uint8_t* w,
                        const uint8_t* w_scales, int64_t w_pitch, int64_t experts, int64_t N, int64_t K,
                        const int32_t* offsets, const int32_t* order, int64_t slots, int64_t per,
-                       const mxq_product_spec* spec, const float* bias, void* out, uint8_t* out_scales, void* stream);
+                       const mxq_product_spec* spec, const float* bias, void* out, uint8_t* out_scales, void* workspace,
+                       int64_t workspace_bytes, void* stream);
 /* rows x K codes of any MX element format (in_pitch bytes from row to row) as 8-bit codes at out_pitch: E4M3 and E5M2
  * copied, FP6 and FP4 as the E4M3 codes of the same values. */
 int mxq_lay_codes(const uint8_t* codes, int64_t in_pitch, uint8_t* out, int64_t out_pitch, int64_t rows, int64_t K,

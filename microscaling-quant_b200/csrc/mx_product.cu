@@ -1153,27 +1153,59 @@ int launch(Args& a, const Operand& x, const Operand& w, int64_t K, int fx, int f
 
 bool aligned(const void* p, int64_t n) { return reinterpret_cast<uintptr_t>(p) % (uintptr_t)n == 0; }
 
-int check_operand(const char* who, const char* what, const void* codes, int64_t pitch, int fmt, int64_t K, int* mma) {
-  MXQ_REQUIRE(fmt == kFmtE4M3 || fmt == kFmtE5M2 || fmt == kFmtE2M1, MXQ_ERR_UNSUPPORTED,
-              "%s: %s must be 8-bit or FP4 codes (mxq_lay_codes widens the others)", who, what);
-  if (fmt == kFmtE2M1) {
-    MXQ_REQUIRE(aligned(codes, 32) && pitch % 32 == 0 && K % 128 == 0 && pitch * 2 >= K, MXQ_ERR_VALUE,
-                "%s: FP4 %s needs a 32-byte aligned base and pitch and K a multiple of 128", who, what);
-    *mma = tc::kE2M1;
-  } else {
-    MXQ_REQUIRE(aligned(codes, 16) && pitch % 16 == 0 && pitch >= K, MXQ_ERR_VALUE,
-                "%s: %s needs a 16-byte aligned base and pitch", who, what);
-    *mma = fmt == kFmtE4M3 ? tc::kE4M3 : tc::kE5M2;
+// An operand as a caller has it: codes of a format (pitch in bytes) or, type > 0, floats of type - 1 (pitch in elements)
+struct Given {
+  const void* data;
+  const uint8_t* scales;
+  int64_t rows, pitch;
+  int fmt, type;
+};
+int mma_format(int fmt) { return fmt == kFmtE4M3 ? tc::kE4M3 : fmt == kFmtE5M2 ? tc::kE5M2 : tc::kE2M1; }
+int64_t codes_pitch(int64_t K) { return up_div(K, 16) * 16; }
+// whether the tensor maps take the codes as they are; rows that are gathered one by one must be 8-bit codes
+bool direct(const Given& o, int64_t K, bool gathered) {
+  if (o.type > 0) return false;
+  if (o.fmt == kFmtE4M3 || o.fmt == kFmtE5M2) return aligned(o.data, 16) && o.pitch % 16 == 0;
+  return o.fmt == kFmtE2M1 && !gathered && aligned(o.data, 32) && o.pitch % 32 == 0 && K % 128 == 0;
+}
+int64_t room(const Given& o, int64_t K, bool gathered) {
+  if (direct(o, K, gathered)) return 0;
+  return up_div(o.rows * codes_pitch(K) + (o.type > 0 ? o.rows * up_div(K, 32) : 0), 128) * 128;
+}
+// The operand as the kernels read it, laid out in `at` (room() bytes) where need be
+int lay(const char* who, const char* what, const Given& o, int64_t K, bool gathered, uint8_t* at, Operand* out, const uint8_t** scales,
+        int* fmt, cudaStream_t st) {
+  *scales = o.scales;
+  *fmt = o.fmt;
+  if (direct(o, K, gathered)) {
+    *out = {static_cast<const uint8_t*>(o.data), o.rows, o.pitch, o.fmt == kFmtE2M1};
+    return MXQ_OK;
   }
+  const int64_t pitch = codes_pitch(K);
+  int e, m;
+  exponent_mantissa(o.fmt, &e, &m);
+  *out = {at, o.rows, pitch, false};
+  if (o.fmt != kFmtE5M2) *fmt = kFmtE4M3;
+  if (o.type == 0) return mxq_lay_codes(static_cast<const uint8_t*>(o.data), o.pitch, at, pitch, o.rows, K, e, m, st);
+  uint8_t* sc = at + o.rows * pitch;
+  *scales = sc;
+  return mxq_pack_rows(o.data, o.type - 1, o.pitch, at, pitch, sc, o.rows, K, e, m, st);
+}
+
+int check_operand(const char* who, const char* what, const Given& o, int64_t K) {
+  MXQ_REQUIRE(o.fmt != kFmtNone, MXQ_ERR_VALUE, "%s: %s has no MX element format", who, what);
+  MXQ_REQUIRE(o.type >= 0 && o.type <= 1 + kOutF16, MXQ_ERR_VALUE, "%s: type %d of %s", who, o.type, what);
+  MXQ_REQUIRE(o.fmt != kFmtE2M1 || K % 2 == 0 || o.type > 0, MXQ_ERR_VALUE, "%s: FP4 codes of %s pair up, K is %lld", who, what, (long long)K);
+  const int64_t least = o.type > 0 || o.fmt != kFmtE2M1 ? K : K / 2;
+  MXQ_REQUIRE(o.rows <= 1 || o.pitch >= least, MXQ_ERR_VALUE, "%s: rows of %s are %lld apart and K is %lld", who, what, (long long)o.pitch,
+              (long long)K);
   return MXQ_OK;
 }
 
-int product(const char* who, Args& a, const Operand& x, const Operand& w, int64_t K, const mxq_product_spec* s, cudaStream_t st) {
-  int fx = 0, fw = 0;
-  const int fmtx = format_of(s->x_e, s->x_m), fmtw = format_of(s->w_e, s->w_m);
-  if (int rc = check_operand(who, "x", x.codes, x.pitch, fmtx, K, &fx)) return rc;
-  if (int rc = check_operand(who, "w", w.codes, w.pitch, fmtw, K, &fw)) return rc;
-  MXQ_REQUIRE(a.per == 0 || fmtx != kFmtE2M1, MXQ_ERR_UNSUPPORTED, "%s: rows of FP4 x cannot be gathered (mxq_lay_codes widens them)", who);
+int product(const char* who, Args& a, const Given& gx, const Given& gw, int64_t K, const mxq_product_spec* s, void* workspace,
+            int64_t workspace_bytes, cudaStream_t st) {
+  if (int rc = check_operand(who, "x", gx, K)) return rc;
+  if (int rc = check_operand(who, "w", gw, K)) return rc;
   MXQ_REQUIRE(s->activation >= kActNone && s->activation <= kActGeglu, MXQ_ERR_VALUE, "%s: activation %d", who, s->activation);
   MXQ_REQUIRE(s->out >= kOutF32 && s->out <= kOutPacked, MXQ_ERR_VALUE, "%s: output type %d", who, s->out);
   const bool gated = s->activation >= kActSwiglu;
@@ -1196,15 +1228,24 @@ int product(const char* who, Args& a, const Operand& x, const Operand& w, int64_
   const int size = s->out == kOutF32 ? 4 : s->out == kOutPacked ? 1 : 2;
   a.vec_out = a.out_pitch * size % 16 == 0 && aligned(a.out, 16) &&
               (a.residual == nullptr || (a.residual_stride * size % 16 == 0 && aligned(a.residual, 16)));
+  const int64_t need = room(gx, K, a.per > 0) + room(gw, K, false);
+  MXQ_REQUIRE(a.rows == 0 || a.width == 0 || need == 0 || (workspace != nullptr && aligned(workspace, 16) && workspace_bytes >= need),
+              MXQ_ERR_VALUE, "%s: needs a workspace of %lld bytes, 16-byte aligned", who, (long long)need);
+  if (a.rows == 0 || a.width == 0) return MXQ_OK;
+  a.status = wait_status_word();
+  if (!a.status) return MXQ_ERR_CUDA;
+  Operand x, w;
+  int fmtx, fmtw;
+  uint8_t* at = static_cast<uint8_t*>(workspace);
+  if (int rc = lay(who, "x", gx, K, a.per > 0, at, &x, &a.sx, &fmtx, st)) return rc;
+  if (int rc = lay(who, "w", gw, K, false, at + room(gx, K, a.per > 0), &w, &a.sw, &fmtw, st)) return rc;
+  const int fx = mma_format(fmtx), fw = mma_format(fmtw);
   a.nb = (int)up_div(K, 32);
   a.kblocks = (int)up_div(K, 128);
   a.vec = a.nb % 16 == 0 && aligned(a.sx, 16) && aligned(a.sw, 16) ? 16 : a.nb % 4 == 0 && aligned(a.sx, 4) && aligned(a.sw, 4) ? 4 : 1;
   // a load of FP4 codes counts the bytes read, half of those that it fills
   a.xbytes = fmtx == kFmtE2M1 ? 64 : 128;
   a.wbytes = fmtw == kFmtE2M1 ? 64 : 128;
-  if (a.rows == 0 || a.width == 0) return MXQ_OK;
-  a.status = wait_status_word();
-  if (!a.status) return MXQ_ERR_CUDA;
   if (a.wait_cycles == 0) a.wait_cycles = tc::kWaitCycles;
   else a.xbytes += 16;                                 // the test of the waits: bytes that never come
   return gated ? launch<true>(a, x, w, K, fx, fw, st) : launch<false>(a, x, w, K, fx, fw, st);
@@ -1223,15 +1264,20 @@ namespace mxq {
 unsigned product_wait_timeouts() { return read_wait_timeouts(); }
 }  // namespace mxq
 
-extern "C" int mxq_linear_packed(const uint8_t* x, const uint8_t* x_scales, int64_t x_pitch, int64_t M, const uint8_t* w,
+extern "C" int64_t mxq_product_workspace(const void* x, int64_t x_pitch, int64_t x_rows, const uint8_t* w, int64_t w_pitch, int64_t w_rows,
+                                         int64_t K, int32_t gathered, const mxq_product_spec* s) {
+  if (s == nullptr || K < 1 || x_rows < 0 || w_rows < 0) return -1;
+  return room({x, nullptr, x_rows, x_pitch, format_of(s->x_e, s->x_m), s->x_type}, K, gathered != 0) +
+         room({w, nullptr, w_rows, w_pitch, format_of(s->w_e, s->w_m), 0}, K, false);
+}
+
+extern "C" int mxq_linear_packed(const void* x, const uint8_t* x_scales, int64_t x_pitch, int64_t M, const uint8_t* w,
                                  const uint8_t* w_scales, int64_t w_pitch, int64_t N, int64_t K, const mxq_product_spec* spec,
                                  const float* bias, const void* residual, int64_t residual_stride, void* out,
-                                 uint8_t* out_scales, void* stream) {
+                                 uint8_t* out_scales, void* workspace, int64_t workspace_bytes, void* stream) {
   MXQ_REQUIRE(spec != nullptr, MXQ_ERR_VALUE, "linear_packed: no spec");
   if (int rc = check_sizes("linear_packed", M, N, K, 1)) return rc;
   Args a = {};
-  a.sx = x_scales;
-  a.sw = w_scales;
   a.rows = a.xrows = (int)M;
   a.n = (int)N;
   a.bias = bias;
@@ -1239,8 +1285,8 @@ extern "C" int mxq_linear_packed(const uint8_t* x, const uint8_t* x_scales, int6
   a.residual_stride = residual_stride;
   a.out = out;
   a.out_scales = out_scales;
-  return product("linear_packed", a, {x, M, x_pitch, spec->x_e + spec->x_m == 3}, {w, N, w_pitch, spec->w_e + spec->w_m == 3}, K,
-                 spec, as_stream(stream));
+  return product("linear_packed", a, {x, x_scales, M, x_pitch, format_of(spec->x_e, spec->x_m), spec->x_type},
+                 {w, w_scales, N, w_pitch, format_of(spec->w_e, spec->w_m), 0}, K, spec, workspace, workspace_bytes, as_stream(stream));
 }
 
 extern "C" int mxq_testing_product_timeout(const uint8_t* x, const uint8_t* x_scales, int64_t M, const uint8_t* w,
@@ -1248,22 +1294,21 @@ extern "C" int mxq_testing_product_timeout(const uint8_t* x, const uint8_t* x_sc
                                            void* stream) {
   if (int rc = check_sizes("testing_product_timeout", M, N, K, 1)) return rc;
   MXQ_REQUIRE(wait_cycles >= 1 && wait_cycles <= (1 << 22), MXQ_ERR_VALUE, "testing_product_timeout: wait_cycles must be in [1, 2^22]");
-  const mxq_product_spec spec = {4, 3, 4, 3, MXQ_ACT_NONE, MXQ_OUT_F32, 0, 0};
+  const mxq_product_spec spec = {4, 3, 4, 3, MXQ_ACT_NONE, MXQ_OUT_F32, 0, 0, 0};
   Args a = {};
-  a.sx = x_scales;
-  a.sw = w_scales;
   a.rows = a.xrows = (int)M;
   a.n = (int)N;
   a.out = y;
   a.wait_cycles = wait_cycles;
-  return product("testing_product_timeout", a, {x, M, K, false}, {w, N, K, false}, K, &spec, as_stream(stream));
+  return product("testing_product_timeout", a, {x, x_scales, M, K, kFmtE4M3, 0}, {w, w_scales, N, K, kFmtE4M3, 0}, K, &spec, nullptr, 0,
+                 as_stream(stream));
 }
 
-extern "C" int mxq_experts_packed(const uint8_t* x, const uint8_t* x_scales, int64_t x_pitch, int64_t x_rows, const uint8_t* w,
+extern "C" int mxq_experts_packed(const void* x, const uint8_t* x_scales, int64_t x_pitch, int64_t x_rows, const uint8_t* w,
                                   const uint8_t* w_scales, int64_t w_pitch, int64_t experts, int64_t N, int64_t K,
                                   const int32_t* offsets, const int32_t* order, int64_t slots, int64_t per,
                                   const mxq_product_spec* spec, const float* bias, void* out, uint8_t* out_scales,
-                                  void* stream) {
+                                  void* workspace, int64_t workspace_bytes, void* stream) {
   MXQ_REQUIRE(spec != nullptr, MXQ_ERR_VALUE, "experts_packed: no spec");
   if (int rc = check_sizes("experts_packed", slots, N, K, experts)) return rc;
   MXQ_REQUIRE(experts <= kMostExperts, MXQ_ERR_UNSUPPORTED, "experts_packed: at most %d experts, got %lld", kMostExperts,
@@ -1272,8 +1317,6 @@ extern "C" int mxq_experts_packed(const uint8_t* x, const uint8_t* x_scales, int
               MXQ_ERR_VALUE, "experts_packed: %lld rows of x do not serve %lld slots, %lld per row", (long long)x_rows,
               (long long)slots, (long long)per);
   Args a = {};
-  a.sx = x_scales;
-  a.sw = w_scales;
   a.offsets = offsets;
   a.order = order;
   a.experts = (int)experts;
@@ -1284,6 +1327,7 @@ extern "C" int mxq_experts_packed(const uint8_t* x, const uint8_t* x_scales, int
   a.bias = bias;
   a.out = out;
   a.out_scales = out_scales;
-  return product("experts_packed", a, {x, x_rows, x_pitch, spec->x_e + spec->x_m == 3},
-                 {w, experts * N, w_pitch, spec->w_e + spec->w_m == 3}, K, spec, as_stream(stream));
+  return product("experts_packed", a, {x, x_scales, x_rows, x_pitch, format_of(spec->x_e, spec->x_m), spec->x_type},
+                 {w, w_scales, experts * N, w_pitch, format_of(spec->w_e, spec->w_m), 0}, K, spec, workspace, workspace_bytes,
+                 as_stream(stream));
 }

@@ -45,7 +45,7 @@ class MxqAnchorSpec(ctypes.Structure):
 
 class MxqProductSpec(ctypes.Structure):
     _fields_ = [("x_e", I32), ("x_m", I32), ("w_e", I32), ("w_m", I32), ("activation", I32), ("out", I32),
-                ("out_e", I32), ("out_m", I32)]
+                ("out_e", I32), ("out_m", I32), ("x_type", I32)]
 
 
 class MxqRouteSpec(ctypes.Structure):
@@ -97,9 +97,10 @@ _SIGS = {
     "mxq_lut_decode": [P, P, I64, I32, I32, P, P],
     "mxq_lut_finder": [P, P, P, I64, I64, I32, I32, I32, P, P],
     "mxq_lut_format_tables": [I32, I32, P, P, P, P],
-    "mxq_linear_packed": [P, P, I64, I64, P, P, I64, I64, I64, ctypes.POINTER(MxqProductSpec), P, P, I64, P, P, P],
+    "mxq_linear_packed": [P, P, I64, I64, P, P, I64, I64, I64, ctypes.POINTER(MxqProductSpec), P, P, I64, P, P, P, I64,
+                          P],
     "mxq_experts_packed": [P, P, I64, I64, P, P, I64, I64, I64, I64, P, P, I64, I64, ctypes.POINTER(MxqProductSpec), P, P,
-                           P, P],
+                           P, P, I64, P],
     "mxq_lay_codes": [P, I64, P, I64, I64, I64, I32, I32, P],
     "mxq_pack_rows": [P, I32, I64, P, I64, P, I64, I64, I32, I32, P],
     "mxq_route": [P, I32, I64, P, P, P, I64, I64, I64, ctypes.POINTER(MxqRouteSpec), P],
@@ -130,6 +131,8 @@ def lib():
                     f.restype = I32
                 L.mxq_block_lut_workspace.argtypes = [I64, I64, I32, I32]
                 L.mxq_block_lut_workspace.restype = I64
+                L.mxq_product_workspace.argtypes = [P, I64, I64, P, I64, I64, I64, I32, ctypes.POINTER(MxqProductSpec)]
+                L.mxq_product_workspace.restype = I64
                 L.mxq_last_error.restype = ctypes.c_char_p
                 L.mxq_version.restype = ctypes.c_char_p
                 _lib = L

@@ -81,21 +81,11 @@ def _pair(v, f: Format, who: str, what: str):
     return codes, scales, shape, K
 
 
-def _laid(codes: torch.Tensor, scales: torch.Tensor, shape, f: Format, K: int, dev, gathered: bool = False):
-    """The operand as the kernels read it, (codes, scales, bytes from row to row, e, m): as it is where its rows allow
-    it, else laid out as 8-bit codes. FP4 rows that are gathered one by one are laid out too."""
-    codes, scales = _here(codes, dev), _here(scales, dev)
-    bits = 1 + f.e + f.m
-    if bits == 8:
-        if K % 16 == 0 and codes.data_ptr() % 16 == 0:
-            return codes, scales, K, f.e, f.m
-    elif bits == 4 and not gathered and K % 128 == 0 and codes.data_ptr() % 32 == 0:
-        return codes, scales, K // 2, f.e, f.m
-    rows = codes.numel() // shape[-1]
-    pitch = -(-K // 16) * 16
-    wide = torch.empty(*shape[:-1], pitch, dtype=torch.uint8, device=dev)
-    _lib.run("mxq_lay_codes", dev, codes.data_ptr(), shape[-1], wide.data_ptr(), pitch, rows, K, f.e, f.m)
-    return (wide, scales, pitch, f.e, f.m) if bits == 8 else (wide, scales, pitch, 4, 3)
+def _direct(at: int, f: Format, K: int, gathered: bool = False) -> bool:
+    """Whether the kernels read contiguous codes at address `at` as they are (else the call lays them out first)."""
+    if f.e + f.m == 7:
+        return K % 16 == 0 and at % 16 == 0
+    return f.e + f.m == 3 and not gathered and K % 128 == 0 and at % 32 == 0
 
 
 def lay_packed(w: Pair, fmt: Union[str, Format]) -> Tuple[Pair, str]:
@@ -104,15 +94,20 @@ def lay_packed(w: Pair, fmt: Union[str, Format]) -> Tuple[Pair, str]:
     kept so (the pair has no room between its rows) and come back unchanged."""
     f = _format(fmt, "lay_packed")
     codes, scales, shape, K = _pair(w, f, "lay_packed", "w")
-    bits = 1 + f.e + f.m
-    if bits == 8 or K % 16 or (bits == 4 and K % 128 == 0):
+    if f.e + f.m == 7 or K % 16 or (f.e + f.m == 3 and K % 128 == 0):
         return (codes, scales), f.name
-    wide = _laid(codes, scales, shape, f, K, _lib.device_for(codes))[0]
+    dev = _lib.device_for(codes)
+    c = _here(codes, dev)
+    wide = torch.empty(*shape[:-1], K, dtype=torch.uint8, device=dev)
+    rows = c.numel() // shape[-1]
+    if rows:
+        _lib.run("mxq_lay_codes", dev, c.data_ptr(), shape[-1], wide.data_ptr(), K, rows, K, f.e, f.m)
     return (_lib.back(wide, codes.device), scales), "MXFP8_E4M3"
 
 
 def _x_operand(x, x_fmt, who: str, w: torch.Tensor, gathered: bool = False):
-    """(operand, leading shape, K, device, home) of x, a pair or a float tensor that is packed here."""
+    """(data, scales or None, pitch, type, format, bytes of workspace, leading shape, K, device, home) of x: a pair, or a
+    float tensor that the call packs."""
     f = _format(x_fmt, who)
     if isinstance(x, torch.Tensor):
         kind = FLOATS.get(x.dtype)
@@ -131,23 +126,26 @@ def _x_operand(x, x_fmt, who: str, w: torch.Tensor, gathered: bool = False):
         if v.stride(1) != 1 or (rows > 1 and stride < K):
             v = v.detach().contiguous()
             stride = K
-        pitch = -(-K // 16) * 16
-        codes = torch.empty(rows, pitch, dtype=torch.uint8, device=dev)
-        scales = torch.empty(rows, -(-K // BLOCK), dtype=torch.uint8, device=dev)
-        _lib.run("mxq_pack_rows", dev, v.data_ptr(), kind, stride, codes.data_ptr(), pitch, scales.data_ptr(), rows, K, f.e,
-                 f.m)
-        e, m = (f.e, f.m) if f.e + f.m == 7 else (4, 3)
-        return (codes, scales, pitch, e, m), shape[:-1], K, dev, x.device
+        room = rows * (-(-K // 16) * 16 + -(-K // BLOCK)) + 128
+        return v, None, stride, 1 + kind, f, room, shape[:-1], K, dev, x.device
     codes, scales, shape, K = _pair(x, f, who, "x")
     dev = codes.device if codes.is_cuda else _lib.device_for(codes, w)
-    return _laid(codes, scales, shape, f, K, dev, gathered), shape[:-1], K, dev, codes.device
+    c, s = _here(codes, dev), _here(scales, dev)
+    room = 0 if _direct(c.data_ptr(), f, K, gathered) else c.numel() // shape[-1] * (-(-K // 16) * 16) + 128
+    return c, s, shape[-1], 0, f, room, shape[:-1], K, dev, codes.device
 
 
-def _make_spec(x_e, x_m, w_e, w_m, act, out, out_e, out_m):
-    return _lib.MxqProductSpec(x_e, x_m, w_e, w_m, act, out, out_e, out_m)
+def _make_spec(x_e, x_m, w_e, w_m, act, out, out_e, out_m, x_type):
+    return _lib.MxqProductSpec(x_e, x_m, w_e, w_m, act, out, out_e, out_m, x_type)
 
 
 _spec = _lib.cached(_make_spec)
+
+
+def _w_operand(wc, ws, shape, f: Format, K: int, dev):
+    """(codes, scales, bytes of workspace) of w on dev."""
+    c, s = _here(wc, dev), _here(ws, dev)
+    return c, s, 0 if _direct(c.data_ptr(), f, K) else c.numel() // shape[-1] * (-(-K // 16) * 16) + 128
 
 
 def _plan_output(out, activation, N: int, who: str):
@@ -204,7 +202,7 @@ def linear_packed(x: Union[Pair, torch.Tensor], w: Pair, fmt: Union[str, Format]
     if bias is not None and tuple(bias.shape) != (N,):
         raise ValueError(f"{who}: bias must have shape {(N,)}, got {tuple(bias.shape)}")
     _ready()
-    (xc, xs, xp, xe, xm), lead, Kx, dev, home = _x_operand(x, x_fmt, who, wc)
+    xc, xs, xp, xt, fx, room, lead, Kx, dev, home = _x_operand(x, x_fmt, who, wc)
     if Kx != K:
         raise ValueError(f"{who}: x has {Kx} values per row and w {K}")
     y, ys = _outputs(lead, out, fo, F, dev)
@@ -227,11 +225,13 @@ def linear_packed(x: Union[Pair, torch.Tensor], w: Pair, fmt: Union[str, Format]
     if M == 0 or N == 0:
         return _given(y, ys, dev, home)
     b = None if bias is None else _lib.on(bias, dev)
-    wc, ws, wp, we, wm = _laid(wc, ws, wshape, fw, K, dev)
-    spec = _spec(xe, xm, we, wm, act, otype, fo.e if fo else 0, fo.m if fo else 0)
-    _lib.run("mxq_linear_packed", dev, xc.data_ptr(), xs.data_ptr(), xp, M, wc.data_ptr(), ws.data_ptr(), wp, N, K,
+    wc, ws, more = _w_operand(wc, ws, wshape, fw, K, dev)
+    room += more
+    space = torch.empty(room, dtype=torch.uint8, device=dev) if room else None
+    spec = _spec(fx.e, fx.m, fw.e, fw.m, act, otype, fo.e if fo else 0, fo.m if fo else 0, xt)
+    _lib.run("mxq_linear_packed", dev, xc.data_ptr(), None if xs is None else xs.data_ptr(), xp, M, wc.data_ptr(), ws.data_ptr(), wshape[-1], N, K,
              ctypes.byref(spec), None if b is None else b.data_ptr(), r_at, r_stride, y.data_ptr(),
-             None if ys is None else ys.data_ptr())
+             None if ys is None else ys.data_ptr(), None if space is None else space.data_ptr(), room)
     return _given(y, ys, dev, home)
 
 
@@ -261,7 +261,7 @@ def experts_packed(x: Union[Pair, torch.Tensor], w: Pair, fmt: Union[str, Format
     if bias is not None and tuple(bias.shape) != (E, N):
         raise ValueError(f"{who}: bias must have shape {(E, N)}, got {tuple(bias.shape)}")
     _ready()
-    (xc, xs, xp, xe, xm), lead, Kx, dev, home = _x_operand(x, x_fmt, who, wc, gather)
+    xc, xs, xp, xt, fx, room, lead, Kx, dev, home = _x_operand(x, x_fmt, who, wc, gather)
     if Kx != K:
         raise ValueError(f"{who}: x has {Kx} values per row and w {K}")
     if len(lead) != 1:
@@ -280,9 +280,11 @@ def experts_packed(x: Union[Pair, torch.Tensor], w: Pair, fmt: Union[str, Format
         return _given(y, ys, dev, home)
     offsets, order = _index(offsets, dev, who, "offsets"), _index(order, dev, who, "order")
     b = None if bias is None else _lib.on(bias, dev)
-    wc, ws, wp, we, wm = _laid(wc, ws, wshape, fw, K, dev)
-    spec = _spec(xe, xm, we, wm, act, otype, fo.e if fo else 0, fo.m if fo else 0)
-    _lib.run("mxq_experts_packed", dev, xc.data_ptr(), xs.data_ptr(), xp, rows, wc.data_ptr(), ws.data_ptr(), wp, E, N, K,
+    wc, ws, more = _w_operand(wc, ws, wshape, fw, K, dev)
+    room += more
+    space = torch.empty(room, dtype=torch.uint8, device=dev) if room else None
+    spec = _spec(fx.e, fx.m, fw.e, fw.m, act, otype, fo.e if fo else 0, fo.m if fo else 0, xt)
+    _lib.run("mxq_experts_packed", dev, xc.data_ptr(), None if xs is None else xs.data_ptr(), xp, rows, wc.data_ptr(), ws.data_ptr(), wshape[-1], E, N, K,
              offsets.data_ptr(), order.data_ptr(), slots, per, ctypes.byref(spec), None if b is None else b.data_ptr(),
-             y.data_ptr(), None if ys is None else ys.data_ptr())
+             y.data_ptr(), None if ys is None else ys.data_ptr(), None if space is None else space.data_ptr(), room)
     return _given(y, ys, dev, home)

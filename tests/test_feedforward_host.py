@@ -31,18 +31,22 @@ def test_c_abi_refuses_first():
     none = None
 
     def linear(M=4, N=4, K=64, x_pitch=64, w_pitch=64, x=64, **kw):
-        s = dict(x_e=4, x_m=3, w_e=4, w_m=3, activation=0, out=0, out_e=0, out_m=0) | kw
+        s = dict(x_e=4, x_m=3, w_e=4, w_m=3, activation=0, out=0, out_e=0, out_m=0, x_type=0) | kw
         return L.mxq_linear_packed(x, none, x_pitch, M, 64, none, w_pitch, N, K, ctypes.byref(_lib.MxqProductSpec(**s)), none, none, 0,
-                                   none, none, none)
+                                   none, none, none, 0, none)
     for text, rc, call in (
             (b"no spec", _lib.ERR_VALUE, lambda: L.mxq_linear_packed(*[none] * 2, 0, 0, *[none] * 2, 0, 0, 0, none, *[none] * 2, 0,
-                                                                     *[none] * 3)),
+                                                                     *[none] * 3, 0, none)),
             (b"bad sizes", _lib.ERR_VALUE, lambda: linear(K=0)),
             (b"bad sizes", _lib.ERR_VALUE, lambda: linear(M=-1)),
-            (b"x must be 8-bit", _lib.ERR_UNSUPPORTED, lambda: linear(x_e=2, x_m=3)),
-            (b"16-byte aligned", _lib.ERR_VALUE, lambda: linear(x_pitch=72, K=72)),
-            (b"16-byte aligned", _lib.ERR_VALUE, lambda: linear(x=8)),
-            (b"FP4 w needs", _lib.ERR_VALUE, lambda: linear(w_e=2, w_m=1, w_pitch=32)),
+            (b"x has no MX element", _lib.ERR_VALUE, lambda: linear(x_e=3, x_m=3)),
+            (b"type 5 of x", _lib.ERR_VALUE, lambda: linear(x_type=5)),
+            (b"rows of w are 63 apart", _lib.ERR_VALUE, lambda: linear(w_pitch=63)),
+            (b"pair up", _lib.ERR_VALUE, lambda: linear(w_e=2, w_m=1, K=63)),
+            (b"a workspace of 384 bytes", _lib.ERR_VALUE, lambda: linear(x_pitch=74, w_pitch=80, K=72)),
+            (b"a workspace of 256 bytes", _lib.ERR_VALUE, lambda: linear(x=8)),
+            (b"a workspace of 256 bytes", _lib.ERR_VALUE, lambda: linear(w_e=2, w_m=3)),
+            (b"a workspace of 384 bytes", _lib.ERR_VALUE, lambda: linear(x_type=2)),
             (b"activation", _lib.ERR_VALUE, lambda: linear(activation=9)),
             (b"output type", _lib.ERR_VALUE, lambda: linear(out=4)),
             (b"even number", _lib.ERR_VALUE, lambda: linear(N=5, activation=5)),
@@ -50,13 +54,15 @@ def test_c_abi_refuses_first():
             (b"needs scales", _lib.ERR_VALUE, lambda: linear(out=3, out_e=4, out_m=3))):
         assert call() == rc and text in L.mxq_last_error(), (text, L.mxq_last_error())
     assert linear(M=0) == _lib.OK                             # nothing to do, no CUDA call
-    spec = _lib.MxqProductSpec(4, 3, 4, 3, 0, 0, 0, 0)
+    spec = _lib.MxqProductSpec(4, 3, 4, 3, 0, 0, 0, 0, 0)
 
-    def experts(E=2, slots=4, rows=2, per=2, K=64, spec=spec):
-        return L.mxq_experts_packed(64, none, 64, rows, 64, none, 64, E, 4, K, none, none, slots, per, ctypes.byref(spec), none, none,
-                                    none, none)
-    assert experts(K=128, spec=_lib.MxqProductSpec(2, 1, 2, 1, 0, 0, 0, 0)) == _lib.ERR_UNSUPPORTED
-    assert b"cannot be gathered" in L.mxq_last_error()
+    def experts(E=2, slots=4, rows=2, per=2):
+        return L.mxq_experts_packed(64, none, 64, rows, 64, none, 64, E, 4, 64, none, none, slots, per, ctypes.byref(spec), none, none,
+                                    none, none, 0, none)
+    fp4 = _lib.MxqProductSpec(2, 1, 2, 1, 0, 0, 0, 0, 0)
+    assert L.mxq_product_workspace(64, 64, 10, 64, 64, 10, 128, 0, ctypes.byref(fp4)) == 0
+    assert L.mxq_product_workspace(64, 64, 10, 64, 64, 10, 128, 1, ctypes.byref(fp4)) == 1280      # gathered rows are widened
+    assert L.mxq_product_workspace(64, 64, 10, 64, 64, 10, 128, 1, none) == -1
     assert experts(E=1025) == _lib.ERR_UNSUPPORTED and b"1024 experts" in L.mxq_last_error()
     assert experts(rows=1) == _lib.ERR_VALUE and b"do not serve" in L.mxq_last_error()
     assert experts(slots=0) == _lib.OK
