@@ -510,8 +510,8 @@ __global__ void __launch_bounds__(128 + 32 * kWriters, 1) __cluster_dims__(2, 1,
     tc::prefetch_map(&mw);
     tc::prefetch_map(&mx);
   }
-  if (warp == 1) tc::tmem_alloc<true>(&sh.tmem, 512);
   tc::wait_for_prior_grid();
+  if (warp == 1) tc::tmem_alloc<true>(&sh.tmem, 512);
   if (warp == 2 && a.experts) count_tiles(tab, a, 256, col_tiles);
   tc::fence_before();
   cluster.sync();
@@ -891,8 +891,8 @@ __global__ void __launch_bounds__(128, 2) k_mx_rows(const __grid_constant__ CUte
     tc::prefetch_map(&mw);
     tc::prefetch_map(&mx);
   }
-  if (warp == 1) tc::tmem_alloc<false>(&sh.tmem, S::kTmem);
   tc::wait_for_prior_grid();
+  if (warp == 1) tc::tmem_alloc<false>(&sh.tmem, S::kTmem);
   if (warp == 2 && a.experts) count_tiles(tab, a, BN, col_tiles);
   tc::fence_before();
   __syncthreads();
