@@ -45,18 +45,18 @@ __device__ __forceinline__ float warp_max(float v) {
   return v;
 }
 
-// An order-preserving key of a choice value; 0 (below every other) for -Inf and NaN, which are never chosen; -0 as +0.
-__device__ __forceinline__ uint32_t key_of(float f) {
+// An order-preserving key of a choice value; 0 (below every other) for -Inf and NaN, which are never chosen, and where
+// `live` is false; -0 as +0.
+__device__ __forceinline__ uint32_t key_if(bool live, float f) {
   const uint32_t b = __float_as_uint(__fadd_rn(f, 0.0f));
-  if ((b & 0x7fffffffu) > 0x7f800000u || b == 0xff800000u) return 0u;
-  return b & 0x80000000u ? ~b : b | 0x80000000u;
+  return live && f > -INFINITY ? b ^ ((uint32_t)((int32_t)b >> 31) | 0x80000000u) : 0u;
 }
 __device__ __forceinline__ float value_of(uint32_t key) {
   return __uint_as_float(key & 0x80000000u ? key & 0x7fffffffu : ~key);
 }
 // the key of a group's two largest, whose sum may pass the type's lowest value: that is still a group to choose
 __device__ __forceinline__ uint32_t key_of_pair(uint32_t best, uint32_t second) {
-  return key_of(fmaxf(__fadd_rn(value_of(best), value_of(second)), -3.402823466e38f));
+  return key_if(true, fmaxf(__fadd_rn(value_of(best), value_of(second)), -3.402823466e38f));
 }
 __device__ __forceinline__ float sigmoid(float x) { return __frcp_rn(__fadd_rn(1.0f, expf(-x))); }
 __device__ __forceinline__ bool is_nan(float x) { return x != x; }
@@ -64,7 +64,7 @@ __device__ __forceinline__ bool is_nan(float x) { return x != x; }
 struct RouteArgs {
   int64_t stride;
   int T, E, k, sigmoid, groups, keep, top2, renormalize;
-  int vec;                     // every lane's values are whole 16-byte pieces of the row, and there
+  int vec, vec_bias;           // every lane's values are whole 16-byte pieces of the row (the biases), and there
   float scale;
 };
 
@@ -93,45 +93,54 @@ __device__ __forceinline__ void merge2(uint32_t& a, uint32_t& b, uint32_t c, uin
 }
 
 // A warp per token, V neighbouring experts per lane (lane V on), so that the lowest lane holds the lowest experts and a
-// tie is the first lane of a ballot. The k largest are taken one after the other: the lanes' best by one warp reduction,
-// and the lane that had it looks for its next. Groups whose runs are whole lanes, a power of two of them (every usual
-// shape), are ranked by shuffles, all at once; others one by one.
+// tie is the first lane of a ballot. The k largest are taken one after the other: the lanes' best by one warp reduction, and
+// only the lane that had it finds which of its own it was. The chosen scores are made again from the logits at the end,
+// by lane j for the j-th. Groups whose runs are whole lanes, a power of two of them (every usual shape), are ranked by
+// shuffles, all at once; others one by one.
+//
+// Bound by issue: 8192 tokens of 256 experts (float32, 8 groups, k = 8) read 8 MB, 1.3 us at the copy's rate.
 template <typename IN, int V>
 __global__ void __launch_bounds__(128) k_route(const IN* __restrict__ logits, const float* __restrict__ bias,
                                                float* __restrict__ weights, int* __restrict__ experts, RouteArgs a) {
   const int lane = threadIdx.x & 31, e0 = lane * V;
   const int64_t t = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 5);
   if (t >= a.T) return;
-  float l[V], s[V];
+  float l[V];
   load_row<IN, V>(logits + t * a.stride, e0, a.E, a.vec, l);
   bool bad = false;
-#pragma unroll
-  for (int i = 0; i < V; i++) bad |= is_nan(l[i]);
-  bad = __any_sync(kAll, bad);
   float top = -INFINITY, sum = 1.0f;
-  if (!a.sigmoid) {
 #pragma unroll
-    for (int i = 0; i < V; i++) top = fmaxf(top, l[i]);
+  for (int i = 0; i < V; i++) {
+    bad |= is_nan(l[i]);
+    top = fmaxf(top, l[i]);
+  }
+  bad = __any_sync(kAll, bad);
+  uint32_t key[V];
+  if (!a.sigmoid) {
     top = warp_max(top);
     sum = 0.0f;
+    float s[V];
 #pragma unroll
     for (int i = 0; i < V; i++) {
-      s[i] = l[i] == -INFINITY || is_nan(l[i]) ? 0.0f : expf(__fsub_rn(l[i], top));
+      s[i] = l[i] > -INFINITY ? expf(__fsub_rn(l[i], top)) : 0.0f;
       sum = __fadd_rn(sum, s[i]);
     }
     sum = warp_sum(sum);
-  } else {
-#pragma unroll
-    for (int i = 0; i < V; i++) s[i] = sigmoid(l[i]);
-  }
-  uint32_t key[V];
-#pragma unroll
-  for (int i = 0; i < V; i++) {
-    key[i] = key_of(l[i]);
     if (bias) {
-      if (!a.sigmoid) s[i] = __fdiv_rn(s[i], sum);
-      key[i] = key[i] ? key_of(__fadd_rn(s[i], e0 + i < a.E ? __ldg(bias + e0 + i) : 0.0f)) : 0u;
+      float b[V];
+      load_row<float, V>(bias, e0, a.E, a.vec_bias, b);
+#pragma unroll
+      for (int i = 0; i < V; i++) key[i] = key_if(l[i] > -INFINITY, __fadd_rn(__fdiv_rn(s[i], sum), b[i]));
     }
+  } else if (bias) {
+    float b[V];
+    load_row<float, V>(bias, e0, a.E, a.vec_bias, b);
+#pragma unroll
+    for (int i = 0; i < V; i++) key[i] = key_if(l[i] > -INFINITY, __fadd_rn(sigmoid(l[i]), b[i]));
+  }
+  if (!bias) {
+#pragma unroll
+    for (int i = 0; i < V; i++) key[i] = key_if(true, l[i]);
   }
   if (a.groups > 1) {
     const int run = a.E / a.groups, width = run / V;
@@ -177,41 +186,40 @@ __global__ void __launch_bounds__(128) k_route(const IN* __restrict__ logits, co
         if (e0 + i < a.E && !(kept >> ((e0 + i) / run) & 1u)) key[i] = 0u;
     }
   }
-  uint32_t best = 0u;                                  // this lane's best, its place among the V, its score
-  int at = 0;
-  float sc = 0.0f;
-  auto look = [&] {
-    best = 0u;
+  auto largest = [&] {
+    uint32_t m = key[0];
 #pragma unroll
-    for (int i = 0; i < V; i++)
-      if (key[i] > best) {
-        best = key[i];
-        at = i;
-        sc = s[i];
-      }
+    for (int i = 1; i < V; i++) m = max(m, key[i]);
+    return m;
   };
-  look();
+  uint32_t best = largest();
   int chosen = -1;                                     // lane j: the j-th choice
-  float w = 0.0f;
   for (int j = 0; j < a.k; j++) {
     const uint32_t m = __reduce_max_sync(kAll, best);
     if (!m) break;
     const int win = __ffs(__ballot_sync(kAll, best == m)) - 1;
-    const int e = __shfl_sync(kAll, e0 + at, win);
-    const float v = __shfl_sync(kAll, sc, win);
-    if (lane == j) {
-      chosen = e;
-      w = v;
-    }
-    if (lane == win) {
+    int e = 0;
+    if (lane == win) {                                 // its first value that is m goes
+      bool found = false;
 #pragma unroll
-      for (int i = 0; i < V; i++)
-        if (i == at) key[i] = 0u;
-      look();
+      for (int i = 0; i < V; i++) {
+        const bool here = key[i] == m && !found;
+        found |= here;
+        if (here) {
+          e = e0 + i;
+          key[i] = 0u;
+        }
+      }
+      best = largest();
     }
+    e = __shfl_sync(kAll, e, win);
+    if (lane == j) chosen = e;
   }
-  if (!a.sigmoid && !bias) w = __fdiv_rn(w, sum);
-  if (chosen < 0) w = 0.0f;
+  float w = 0.0f;
+  if (chosen >= 0) {
+    const float x = to_float<IN>(logits[t * a.stride + chosen]);
+    w = a.sigmoid ? sigmoid(x) : __fdiv_rn(expf(__fsub_rn(x, top)), sum);
+  }
   if (a.renormalize) w = __fdiv_rn(w, __fadd_rn(warp_sum(w), kEps));
   w = bad ? __uint_as_float(0x7fc00000u) : __fmul_rn(w, a.scale);
   if (lane < a.k) {
@@ -287,7 +295,7 @@ __global__ void __launch_bounds__(128) k_route_backward(const float* __restrict_
 // A stable counting sort in one launch. The slots are cut into a contiguous run per warp; each warp counts its run by
 // expert in shared memory, the counts are added up over the warps, the cluster's CTAs and the experts, and each warp
 // then walks its run again, 32 slots at a time in order, giving each slot the next place of its expert.
-constexpr int kDispatchWarps = 32;
+constexpr int kDispatchWarps = 16;
 
 __global__ void __launch_bounds__(kDispatchWarps * 32) k_dispatch(const int* __restrict__ ids, int64_t S, int E,
                                                                   int* __restrict__ offsets, int* __restrict__ order,
@@ -305,8 +313,8 @@ __global__ void __launch_bounds__(kDispatchWarps * 32) k_dispatch(const int* __r
   const int64_t runs = (int64_t)ctas * kDispatchWarps, run = ((S + runs - 1) / runs + 31) / 32 * 32;
   const int64_t begin = min(S, (rank * (int64_t)kDispatchWarps + warp) * run), end = min(S, begin + run);
   int* mine = count + warp * E;
-  // the run's first 256 slots stay in registers for the second walk
-  constexpr int kHeld = 8;
+  // the run's first 512 slots stay in registers for the second walk
+  constexpr int kHeld = 16;
   int held[kHeld];
 #pragma unroll
   for (int h = 0; h < kHeld; h++) held[h] = begin + h * 32 + lane < end ? ids[begin + h * 32 + lane] : -1;
@@ -319,26 +327,39 @@ __global__ void __launch_bounds__(kDispatchWarps * 32) k_dispatch(const int* __r
     if (e >= 0 && e < E) atomicAdd(mine + e, 1);
   }
   __syncthreads();
-  const int e = threadIdx.x;                           // a thread per expert: E <= 1024
-  int own = 0;
-  if (e < E) {
-#pragma unroll 16
-    for (int w = 0; w < kDispatchWarps; w++) {
-      const int c = count[w * E + e];
-      count[w * E + e] = own;
-      own += c;
+  // two experts per thread (E <= 1024)
+  constexpr int kPer = kMostExperts / (kDispatchWarps * 32);
+  int all[kPer], before[kPer];
+#pragma unroll
+  for (int p = 0; p < kPer; p++) {
+    const int e = threadIdx.x * kPer + p;
+    int own = 0;
+    if (e < E) {
+#pragma unroll
+      for (int w = 0; w < kDispatchWarps; w++) {
+        const int c = count[w * E + e];
+        count[w * E + e] = own;
+        own += c;
+      }
+      total[e] = own;
     }
-    total[e] = own;
   }
   cluster.sync();
-  int all = 0, before = 0;
-  if (e < E)
-    for (int c = 0; c < ctas; c++) {
-      const int v = cluster.map_shared_rank(total, c)[e];
-      if (c < rank) before += v;
-      all += v;
-    }
-  int scan = all;                                      // over the experts: warps, then the warps' sums
+  int scan = 0;
+#pragma unroll
+  for (int p = 0; p < kPer; p++) {
+    const int e = threadIdx.x * kPer + p;
+    all[p] = before[p] = 0;
+    if (e < E)
+      for (int c = 0; c < ctas; c++) {
+        const int v = cluster.map_shared_rank(total, c)[e];
+        if (c < rank) before[p] += v;
+        all[p] += v;
+      }
+    scan += all[p];
+  }
+  const int mine_all = scan;
+  // over the experts: threads, then the warps' sums
 #pragma unroll
   for (int d = 1; d < 32; d <<= 1) {
     const int up = __shfl_up_sync(kAll, scan, d);
@@ -347,15 +368,21 @@ __global__ void __launch_bounds__(kDispatchWarps * 32) k_dispatch(const int* __r
   if (lane == 31) sums[warp] = scan;
   __syncthreads();
   int head = 0, live = 0;
+#pragma unroll
   for (int w = 0; w < kDispatchWarps; w++) {
     const int v = sums[w];
     if (w < warp) head += v;
     live += v;
   }
-  const int first = head + scan - all;
-  if (e < E) {
-    if (rank == 0) offsets[e] = first;
-    start[e] = first + before;
+  int first = head + scan - mine_all;
+#pragma unroll
+  for (int p = 0; p < kPer; p++) {
+    const int e = threadIdx.x * kPer + p;
+    if (e < E) {
+      if (rank == 0) offsets[e] = first;
+      start[e] = first + before[p];
+    }
+    first += all[p];
   }
   if (rank == 0 && threadIdx.x == 0) offsets[E] = live;
   for (int64_t i = live + rank * (int64_t)blockDim.x + threadIdx.x; i < S; i += (int64_t)ctas * blockDim.x) order[i] = -1;
@@ -603,6 +630,7 @@ extern "C" int mxq_route(const void* logits, int32_t type, int64_t stride, const
     using IN = decltype(zero);
     by_width(a.E, [&](auto v) {
       a.vec = row_vec<IN>(logits, stride, a.E, decltype(v)::value);
+      a.vec_bias = row_vec<float>(bias, 0, a.E, decltype(v)::value);
       k_route<IN, decltype(v)::value><<<(unsigned)((T + 3) / 4), 128, 0, as_stream(stream)>>>(static_cast<const IN*>(logits), bias, weights,
                                                                                           experts, a);
     });
@@ -630,9 +658,9 @@ extern "C" int mxq_dispatch(const int32_t* experts_of, int64_t slots, int64_t ex
                             int32_t* where, void* stream) {
   MXQ_REQUIRE(slots >= 0 && slots < (1ll << 30) && experts >= 1 && experts <= kMostExperts, MXQ_ERR_VALUE,
               "dispatch: %lld slots, %lld experts (at most %d)", (long long)slots, (long long)experts, kMostExperts);
-  // a CTA walks 4096 slots in four steps per warp; a cluster (at most 8 CTAs) shares more
+  // a CTA walks 2048 slots in four steps per warp; a cluster (at most 8 CTAs) shares more
   int ctas = 1;
-  while (ctas < 8 && slots > 4096ll * ctas) ctas *= 2;
+  while (ctas < 8 && slots > 2048ll * ctas) ctas *= 2;
   const int smem = (int)((kDispatchWarps + 2) * experts + 32) * 4;
   if (int rc = allow_smem((const void*)k_dispatch, ((kDispatchWarps + 2) * kMostExperts + 32) * 4)) return rc;
   cudaLaunchConfig_t cfg = {};
