@@ -49,27 +49,39 @@ struct Args {
 };
 
 // ------------------------------------------------------------------------------------------ epilogue values
-// x / (1 + exp(t)) by the hardware's exp2 and reciprocal (a few ulp of float32, subnormal intermediates flushed): y is
-// rounded to 16 bits or fewer, or, as float32, already carries the sum's own error of that size.
+// A packed output turns an error of float32 into a whole step of the code where it meets a tie, so the epilogue keeps
+// float32's accuracy: the hardware's reciprocal is good to an ulp and its exp2 to two, and exp2 is given the rounding error
+// of its argument too.
+//
+// x / (1 + exp(t)). t below -100 adds nothing to 1, and from 88 on the reciprocal is 0: nothing is left of a finite x, and
+// -Inf gives NaN, as -Inf * 0 does.
 __device__ __forceinline__ float over_one_plus_exp(float x, float t) {
+  t = fminf(fmaxf(t, -100.0f), 88.0f);
+  const float hi = __fmul_rn(t, 1.4426950408889634f), lo = __fmaf_rn(t, 1.4426950408889634f, -hi);
   float e, r;
-  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(e) : "f"(__fmul_rn(t, 1.4426950408889634f)));
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(e) : "f"(hi));
+  e = __fmaf_rn(e, __fmul_rn(lo, 0.6931471805599453f), e);
   asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(__fadd_rn(1.0f, e)));
   return __fmul_rn(x, r);
 }
 __device__ __forceinline__ float silu(float x) { return over_one_plus_exp(x, -x); }
-// x Phi(x), Phi by Abramowitz and Stegun's 7.1.26 for erfc (absolute error 1.5e-7): for z = |x| / sqrt(2), t = 1 / (1 + 0.3275911 z),
-// erfc(z) = (a1 t + .. + a5 t^5) exp(-z^2), and Phi is half of that below zero and one minus half of it above. A dozen
-// instructions where erff takes about forty: the epilogue's code has to stay in the instruction cache.
+// x Phi(x). With z = |x| / sqrt(2) and t = 1 / (1 + z / 2), erfc(z) / 2 = t P(t) exp(-z^2), P a polynomial of degree 8 fitted
+// here to the smallest relative error on 0 <= z <= 9.4 (4.2e-8, by iterated weighted least squares on Chebyshev points);
+// Phi is that below zero and one minus that above. 17 instructions where erff takes about forty: the epilogue's code has
+// to stay in the instruction cache.
 __device__ __forceinline__ float gelu(float x) {
-  const float z = fabsf(x) * 0.70710678118654752f;
+  const float z = fminf(fabsf(x) * 0.70710678118654752f, 14.0f);       // exp(-196) is 0
   float t, e;
-  asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(t) : "f"(__fmaf_rn(0.3275911f, z, 1.0f)));
+  asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(t) : "f"(__fmaf_rn(0.5f, z, 1.0f)));
   asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(e) : "f"(__fmul_rn(z * z, -1.4426950408889634f)));
-  float h = __fmaf_rn(t, 0.5f * 1.061405429f, 0.5f * -1.453152027f);
-  h = __fmaf_rn(t, h, 0.5f * 1.421413741f);
-  h = __fmaf_rn(t, h, 0.5f * -0.284496736f);
-  h = __fmaf_rn(t, h, 0.5f * 0.254829592f);
+  float h = __fmaf_rn(t, -0.02942352555692196f, 0.14174368977546692f);
+  h = __fmaf_rn(t, h, -0.24246817827224731f);
+  h = __fmaf_rn(t, h, 0.13773120939731598f);
+  h = __fmaf_rn(t, h, -0.012409592978656292f);
+  h = __fmaf_rn(t, h, 0.10095827281475067f);
+  h = __fmaf_rn(t, h, 0.12165011465549469f);
+  h = __fmaf_rn(t, h, 0.14117400348186493f);
+  h = __fmaf_rn(t, h, 0.1410439908504486f);
   h = h * t * e;
   return x * (x < 0.0f ? h : 1.0f - h);
 }

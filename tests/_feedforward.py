@@ -68,7 +68,7 @@ def product64(x, w, bias=None, activation=None):
 
     The products of the codes are exact. Each of the K additions may lose 2^-23 of the largest partial sum, itself at
     most S = sum |x w|: K 2^-23 S. The activation passes that on with its slope and adds its own error: a few ulp of its
-    result and of its argument (2^-19 of each), and for gelu 1.5e-7 of the argument by the erfc formula."""
+    result and of its argument (2^-19 of each)."""
     K = x.shape[-1]
     z, S = x @ w.T, x.abs() @ w.abs().T
     dz = (K + 1) * 2.0 ** -23 * S
