@@ -266,7 +266,7 @@ typedef struct mxq_product_spec {
  * of 16 bytes, and FP4 codes with base and pitch multiples of 32 bytes and K a multiple of 128, are read as they are; other
  * codes, and float x, are laid out in `workspace` first (mxq_product_workspace bytes, 16-byte aligned; none when 0). */
 int64_t mxq_product_workspace(const void* x, int64_t x_pitch, int64_t x_rows, const uint8_t* w, int64_t w_pitch,
-                              int64_t w_rows, int64_t K, int32_t gathered, const mxq_product_spec* spec);
+                              int64_t w_rows, int64_t K, int64_t gathered_slots, const mxq_product_spec* spec);
 int mxq_linear_packed(const void* x, const uint8_t* x_scales, int64_t x_pitch, int64_t M, const uint8_t* w,
                       const uint8_t* w_scales, int64_t w_pitch, int64_t N, int64_t K, const mxq_product_spec* spec,
                       const float* bias, const void* residual, int64_t residual_stride, void* out, uint8_t* out_scales,
@@ -274,8 +274,9 @@ int mxq_linear_packed(const void* x, const uint8_t* x_scales, int64_t x_pitch, i
 /* The same product by expert: rows offsets[e] .. offsets[e + 1] - 1 of y (experts + 1 non-decreasing offsets, the last
  * at most `slots`) are multiplied with expert e's N x K weights (w: experts x N x K, bias: experts x N). Row r of y takes
  * row r of x (per 0), or row order[r] / per (per > 0). Rows from the last offset on are not written; offsets
- * outside [0, slots] and rows of x outside [0, x_rows) are cut to these. At most 1024 experts. gathered
- * (mxq_product_workspace): per > 0. */
+ * outside [0, slots] and rows of x outside [0, x_rows) are cut to these. At most 1024 experts.
+ * gathered_slots (mxq_product_workspace): slots if per > 0, else 0; the workspace may be without its share for up to 8 slots
+ * per expert. */
 int mxq_experts_packed(const void* x, const uint8_t* x_scales, int64_t x_pitch, int64_t x_rows, const uint8_t* w,
                        const uint8_t* w_scales, int64_t w_pitch, int64_t experts, int64_t N, int64_t K,
                        const int32_t* offsets, const int32_t* order, int64_t slots, int64_t per,

@@ -64,6 +64,25 @@ __global__ void __launch_bounds__(256) k_lay_codes(const uint8_t* __restrict__ i
   }
 }
 
+// A warp per row of the product: the codes and scale bytes of the row of x that its slot takes, side by side in the order
+// of the slots.
+__global__ void __launch_bounds__(256) k_gather_rows(const uint8_t* __restrict__ codes, const uint8_t* __restrict__ scales, int64_t pitch,
+                                                     const int* __restrict__ order, int per, int x_rows, int64_t slots, int nb,
+                                                     uint8_t* __restrict__ to_codes, uint8_t* __restrict__ to_scales) {
+  start_next_grid();
+  const int64_t r = ((int64_t)blockIdx.x * blockDim.x + threadIdx.x) >> 5;
+  const int lane = threadIdx.x & 31;
+  if (r >= slots) return;
+  const int slot = order[r];
+  if (slot < 0) return;                                // a place without a slot: nobody reads it
+  const int64_t from = min(slot / per, x_rows - 1);
+  const uint4* a = reinterpret_cast<const uint4*>(codes + from * pitch);
+  uint4* b = reinterpret_cast<uint4*>(to_codes + r * pitch);
+#pragma unroll 4
+  for (int64_t i = lane; i < pitch / 16; i += 32) b[i] = __ldg(a + i);
+  for (int i = lane; i < nb; i += 32) to_scales[r * nb + i] = __ldg(scales + from * nb + i);
+}
+
 template <typename T>
 __device__ __forceinline__ float to_float(T v);
 template <>
@@ -129,6 +148,14 @@ int pack_rows(const void* x, int64_t x_stride, uint8_t* codes, int64_t out_pitch
 }
 
 }  // namespace
+
+namespace mxq {
+int gather_rows(const uint8_t* codes, const uint8_t* scales, int64_t pitch, const int* order, int per, int x_rows, int64_t slots, int nb,
+                uint8_t* to_codes, uint8_t* to_scales, cudaStream_t st) {
+  k_gather_rows<<<(unsigned)((slots + 7) / 8), 256, 0, st>>>(codes, scales, pitch, order, per, x_rows, slots, nb, to_codes, to_scales);
+  return MXQ_LAUNCH_CHECK("gather_rows");
+}
+}  // namespace mxq
 
 extern "C" int mxq_lay_codes(const uint8_t* codes, int64_t in_pitch, uint8_t* out, int64_t out_pitch, int64_t rows, int64_t K,
                              int32_t e, int32_t m, void* stream) {

@@ -19,6 +19,11 @@
 namespace cg = cooperative_groups;
 using namespace mxq;
 
+namespace mxq {
+int gather_rows(const uint8_t* codes, const uint8_t* scales, int64_t pitch, const int* order, int per, int x_rows, int64_t slots, int nb,
+                uint8_t* to_codes, uint8_t* to_scales, cudaStream_t st);         // mx_layout.cu
+}
+
 namespace {
 
 enum { kActNone = 0, kActRelu, kActGelu, kActGeluTanh, kActSilu, kActSwiglu, kActGeglu };
@@ -541,9 +546,6 @@ __global__ void __launch_bounds__(128 + 32 * kWriters, 1) __cluster_dims__(2, 1,
     int sent = 0;
     for (int i = pair; ok && i < tiles; i += pairs) {
       const Tile t = list.next(i, pairs, tiles, a, tab, 256, col_tiles);
-      int4 rows = make_int4(0, 0, 0, 0);
-      const int r0 = rank * 128 + 4 * lane;
-      if (a.per > 0) rows = make_int4(x_row(a, t, r0), x_row(a, t, r0 + 1), x_row(a, t, r0 + 2), x_row(a, t, r0 + 3));
       const int w0 = t.expert * a.n + t.col * kCols + (rank ? second : 0);
       for (int kb = 0; kb < a.kblocks; kb++) {
         ok = tc::wait_warp(&sh.empty[ring.stage], ring.phase ^ 1u, guard);
@@ -552,11 +554,10 @@ __global__ void __launch_bounds__(128 + 32 * kWriters, 1) __cluster_dims__(2, 1,
         const uint32_t bar = full + 8u * ring.stage;
         if (tc::elect()) {
           if (rank == 0) mbar_expect_tx(&sh.full[ring.stage], 256 * (a.xbytes + a.wbytes));
-          if (a.per == 0) tc::tma_load_pair(to, &mx, kb * 128, t.row0 + rank * 128, bar);
+          tc::tma_load_pair(to, &mx, kb * 128, t.row0 + rank * 128, bar);
           tc::tma_load_pair(to + kTileBytes, &mw, kb * 128, w0, bar);
         }
         __syncwarp();
-        if (a.per > 0) tc::tma_gather4_pair(to + lane * 512, &mx, kb * 128, rows, bar);
         ring.next(kStages);
         sent++;
       }
@@ -1107,7 +1108,7 @@ int launch_rows(Args& a, const Operand& x, const Operand& w, int64_t K, int64_t 
 template <bool GATED, int OUT>
 int launch_tile(Args& a, const Operand& x, const Operand& w, int64_t K, int64_t tiles, int fx, int fw, cudaStream_t st) {
   CUtensorMap mx, mw;
-  if (int rc = map_of(&mx, x, K, a.per > 0 ? 1 : 128)) return rc;
+  if (int rc = map_of(&mx, x, K, 128)) return rc;
   if (int rc = map_of(&mw, w, K, 128)) return rc;
   a.idesc = tc::mma_desc(fx, fw, 256, 256);
   const int smem = kTileSmem + (a.experts ? table_bytes(a.experts) : 0);
@@ -1129,37 +1130,50 @@ int launch_tile(Args& a, const Operand& x, const Operand& w, int64_t K, int64_t 
 
 int64_t up_div(int64_t a, int64_t b) { return (a + b - 1) / b; }
 
-template <bool GATED>
-int launch(Args& a, const Operand& x, const Operand& w, int64_t K, int fx, int fw, cudaStream_t st) {
+// How a product is cut up: by k_mx_rows in tiles of bn rows with K split, or by k_mx_tile
+struct Cut {
+  bool few;
+  int bn, split;
+  int64_t tiles;
+};
+Cut cut_of(const Args& a, bool gated, int64_t kblocks) {
   // rows that share a tile of w: all of them, or an expert's share
   const int64_t share = a.experts ? up_div(a.rows, a.experts) : a.rows;
   const int64_t groups = a.experts ? (a.experts < a.rows ? a.experts : a.rows) : 1;
-  const int64_t cols = up_div(a.width, GATED ? 64 : 128);
+  const int64_t cols = up_div(a.width, gated ? 64 : 128);
+  Cut c;
   // Tiles of few rows: as many as there are; by expert several times the mean, since the longest expert's second tile would
   // read w again (64 experts of 2048 x 1024 with 8 rows each at random: 37 us with tiles of 16, 33 with 32 and 64).
-  const int bn = a.experts ? (share <= 2 ? 16 : share <= 8 ? 32 : 64) : share <= 16 ? 16 : share <= 32 ? 32 : 64;
-  const int64_t tiles = (a.experts ? a.rows / bn + groups : up_div(a.rows, bn)) * cols;
+  c.bn = a.experts ? (share <= 2 ? 16 : share <= 8 ? 32 : 64) : share <= 16 ? 16 : share <= 32 ? 32 : 64;
+  c.tiles = (a.experts ? a.rows / c.bn + groups : up_div(a.rows, c.bn)) * cols;
   // Which kernel, measured on E4M3: dense 4096 x 4096, M = 256: 15.9 us by few rows, 17.8 by many, M = 384: 19.7 and 18.7;
   // 2048 x 2048, M = 512: 13.2 and 13.1; 8192 x 2048, M = 128: 13.4 and 13.8, M = 256: 15.1 and 13.9. By expert, 64 experts
   // 2048 x 1024: 8 rows each 33 and 35, 12 rows 44 and 39; 8 experts 4096 x 2048, 32 rows: 16 and 23.
-  const bool few = a.experts ? share <= 8 || tiles <= 4 * sm_count() : tiles <= sm_count();
-  if (!few) {
-    const int64_t wide = up_div(a.width, GATED ? 128 : 256);
-    const int64_t big = (a.experts ? a.rows / 256 + groups : up_div(a.rows, 256)) * wide;
-    switch (a.otype) {
-      case kOutF32: return launch_tile<GATED, kOutF32>(a, x, w, K, big, fx, fw, st);
-      case kOutBf16: return launch_tile<GATED, kOutBf16>(a, x, w, K, big, fx, fw, st);
-      case kOutF16: return launch_tile<GATED, kOutF16>(a, x, w, K, big, fx, fw, st);
-      default: return launch_tile<GATED, kOutPacked>(a, x, w, K, big, fx, fw, st);
-    }
+  c.few = a.experts ? share <= 8 || c.tiles <= 4 * sm_count() : c.tiles <= sm_count();
+  c.split = 1;
+  if (!c.few) {
+    c.tiles = (a.experts ? a.rows / 256 + groups : up_div(a.rows, 256)) * up_div(a.width, gated ? 128 : 256);
+    return c;
   }
   // K split over a cluster while that gives every SM two CTAs at most and each CTA two steps at least
-  int split = 1;
-  while (split < 8 && tiles * split * 2 <= 2 * sm_count() && a.kblocks >= split * 4) split *= 2;
-  switch (bn) {
-    case 16: return launch_rows<16, GATED>(a, x, w, K, tiles, split, fx, fw, st);
-    case 32: return launch_rows<32, GATED>(a, x, w, K, tiles, split, fx, fw, st);
-    default: return launch_rows<64, GATED>(a, x, w, K, tiles, split, fx, fw, st);
+  while (c.split < 8 && c.tiles * c.split * 2 <= 2 * sm_count() && kblocks >= c.split * 4) c.split *= 2;
+  return c;
+}
+
+template <bool GATED>
+int launch(Args& a, const Cut& c, const Operand& x, const Operand& w, int64_t K, int fx, int fw, cudaStream_t st) {
+  if (!c.few) {
+    switch (a.otype) {
+      case kOutF32: return launch_tile<GATED, kOutF32>(a, x, w, K, c.tiles, fx, fw, st);
+      case kOutBf16: return launch_tile<GATED, kOutBf16>(a, x, w, K, c.tiles, fx, fw, st);
+      case kOutF16: return launch_tile<GATED, kOutF16>(a, x, w, K, c.tiles, fx, fw, st);
+      default: return launch_tile<GATED, kOutPacked>(a, x, w, K, c.tiles, fx, fw, st);
+    }
+  }
+  switch (c.bn) {
+    case 16: return launch_rows<16, GATED>(a, x, w, K, c.tiles, c.split, fx, fw, st);
+    case 32: return launch_rows<32, GATED>(a, x, w, K, c.tiles, c.split, fx, fw, st);
+    default: return launch_rows<64, GATED>(a, x, w, K, c.tiles, c.split, fx, fw, st);
   }
 }
 
@@ -1184,6 +1198,8 @@ int64_t room(const Given& o, int64_t K, bool gathered) {
   if (direct(o, K, gathered)) return 0;
   return up_div(o.rows * codes_pitch(K) + (o.type > 0 ? o.rows * up_div(K, 32) : 0), 128) * 128;
 }
+// rows in the plan's order, at any pitch that their codes may have
+int64_t sorted_room(int64_t rows, int64_t K) { return up_div(rows * (codes_pitch(K) + up_div(K, 32)), 128) * 128; }
 // The operand as the kernels read it, laid out in `at` (room() bytes) where need be
 int lay(const char* who, const char* what, const Given& o, int64_t K, bool gathered, uint8_t* at, Operand* out, const uint8_t** scales,
         int* fmt, cudaStream_t st) {
@@ -1240,7 +1256,14 @@ int product(const char* who, Args& a, const Given& gx, const Given& gw, int64_t 
   const int size = s->out == kOutF32 ? 4 : s->out == kOutPacked ? 1 : 2;
   a.vec_out = a.out_pitch * size % 16 == 0 && aligned(a.out, 16) &&
               (a.residual == nullptr || (a.residual_stride * size % 16 == 0 && aligned(a.residual, 16)));
-  const int64_t need = room(gx, K, a.per > 0) + room(gw, K, false);
+  a.kblocks = (int)up_div(K, 128);
+  const Cut cut = cut_of(a, gated, a.kblocks);
+  // Rows that the plan scatters are fetched one by one by k_mx_rows in tiles of up to 32 (tile::gather4: four rows an
+  // instruction, about 65 cycles each), and brought into the plan's order first for larger tiles: 64 experts 2048 x 2048, 384
+  // rows each: 330 us fetched, 154 sorted; 8 experts 4096 x 4096, 16 rows each: 36 and 31.
+  const bool sorted = a.per > 0 && (!cut.few || cut.bn > 32);
+  const int64_t room_x = room(gx, K, a.per > 0), room_w = room(gw, K, false), room_s = sorted ? sorted_room(a.rows, K) : 0;
+  const int64_t need = room_x + room_w + room_s;
   MXQ_REQUIRE(a.rows == 0 || a.width == 0 || need == 0 || (workspace != nullptr && aligned(workspace, 16) && workspace_bytes >= need),
               MXQ_ERR_VALUE, "%s: needs a workspace of %lld bytes, 16-byte aligned", who, (long long)need);
   if (a.rows == 0 || a.width == 0) return MXQ_OK;
@@ -1250,17 +1273,25 @@ int product(const char* who, Args& a, const Given& gx, const Given& gw, int64_t 
   int fmtx, fmtw;
   uint8_t* at = static_cast<uint8_t*>(workspace);
   if (int rc = lay(who, "x", gx, K, a.per > 0, at, &x, &a.sx, &fmtx, st)) return rc;
-  if (int rc = lay(who, "w", gw, K, false, at + room(gx, K, a.per > 0), &w, &a.sw, &fmtw, st)) return rc;
-  const int fx = mma_format(fmtx), fw = mma_format(fmtw);
+  if (int rc = lay(who, "w", gw, K, false, at + room_x, &w, &a.sw, &fmtw, st)) return rc;
   a.nb = (int)up_div(K, 32);
-  a.kblocks = (int)up_div(K, 128);
+  if (sorted) {
+    uint8_t* codes = at + room_x + room_w;
+    uint8_t* scales = codes + a.rows * x.pitch;
+    if (int rc = gather_rows(x.codes, a.sx, x.pitch, a.order, a.per, a.xrows, a.rows, a.nb, codes, scales, st)) return rc;
+    x = {codes, a.rows, x.pitch, false};
+    a.sx = scales;
+    a.xrows = a.rows;
+    a.per = 0;
+  }
+  const int fx = mma_format(fmtx), fw = mma_format(fmtw);
   a.vec = a.nb % 16 == 0 && aligned(a.sx, 16) && aligned(a.sw, 16) ? 16 : a.nb % 4 == 0 && aligned(a.sx, 4) && aligned(a.sw, 4) ? 4 : 1;
   // a load of FP4 codes counts the bytes read, half of those that it fills
   a.xbytes = fmtx == kFmtE2M1 ? 64 : 128;
   a.wbytes = fmtw == kFmtE2M1 ? 64 : 128;
   if (a.wait_cycles == 0) a.wait_cycles = tc::kWaitCycles;
   else a.xbytes += 16;                                 // the test of the waits: bytes that never come
-  return gated ? launch<true>(a, x, w, K, fx, fw, st) : launch<false>(a, x, w, K, fx, fw, st);
+  return gated ? launch<true>(a, cut, x, w, K, fx, fw, st) : launch<false>(a, cut, x, w, K, fx, fw, st);
 }
 
 int check_sizes(const char* who, int64_t rows, int64_t N, int64_t K, int64_t experts) {
@@ -1277,10 +1308,10 @@ unsigned product_wait_timeouts() { return read_wait_timeouts(); }
 }  // namespace mxq
 
 extern "C" int64_t mxq_product_workspace(const void* x, int64_t x_pitch, int64_t x_rows, const uint8_t* w, int64_t w_pitch, int64_t w_rows,
-                                         int64_t K, int32_t gathered, const mxq_product_spec* s) {
-  if (s == nullptr || K < 1 || x_rows < 0 || w_rows < 0) return -1;
-  return room({x, nullptr, x_rows, x_pitch, format_of(s->x_e, s->x_m), s->x_type}, K, gathered != 0) +
-         room({w, nullptr, w_rows, w_pitch, format_of(s->w_e, s->w_m), 0}, K, false);
+                                         int64_t K, int64_t gathered_slots, const mxq_product_spec* s) {
+  if (s == nullptr || K < 1 || x_rows < 0 || w_rows < 0 || gathered_slots < 0) return -1;
+  return room({x, nullptr, x_rows, x_pitch, format_of(s->x_e, s->x_m), s->x_type}, K, gathered_slots > 0) +
+         room({w, nullptr, w_rows, w_pitch, format_of(s->w_e, s->w_m), 0}, K, false) + (gathered_slots > 0 ? sorted_room(gathered_slots, K) : 0);
 }
 
 extern "C" int mxq_linear_packed(const void* x, const uint8_t* x_scales, int64_t x_pitch, int64_t M, const uint8_t* w,

@@ -202,13 +202,5 @@ __device__ __forceinline__ void tma_gather4(void* dst, const CUtensorMap* map, i
       "l"(map), "r"(x), "r"(rows.x), "r"(rows.y), "r"(rows.z), "r"(rows.w), "r"(smem_addr(bar))
       : "memory");
 }
-__device__ __forceinline__ void tma_gather4_pair(void* dst, const CUtensorMap* map, int x, int4 rows, uint32_t bar) {
-  asm volatile(
-      "cp.async.bulk.tensor.2d.cta_group::2.shared::cluster.global.tile::gather4.mbarrier::complete_tx::bytes [%0], [%1, {%2, "
-      "%3, %4, %5, %6}], [%7];\n" ::"r"(smem_addr(dst)),
-      "l"(map), "r"(x), "r"(rows.x), "r"(rows.y), "r"(rows.z), "r"(rows.w), "r"(bar)
-      : "memory");
-}
-
 }  // namespace tc
 }  // namespace mxq

@@ -131,7 +131,7 @@ def lib():
                     f.restype = I32
                 L.mxq_block_lut_workspace.argtypes = [I64, I64, I32, I32]
                 L.mxq_block_lut_workspace.restype = I64
-                L.mxq_product_workspace.argtypes = [P, I64, I64, P, I64, I64, I64, I32, ctypes.POINTER(MxqProductSpec)]
+                L.mxq_product_workspace.argtypes = [P, I64, I64, P, I64, I64, I64, I64, ctypes.POINTER(MxqProductSpec)]
                 L.mxq_product_workspace.restype = I64
                 L.mxq_last_error.restype = ctypes.c_char_p
                 L.mxq_version.restype = ctypes.c_char_p

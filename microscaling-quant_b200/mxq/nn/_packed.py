@@ -282,6 +282,8 @@ def experts_packed(x: Union[Pair, torch.Tensor], w: Pair, fmt: Union[str, Format
     b = None if bias is None else _lib.on(bias, dev)
     wc, ws, more = _w_operand(wc, ws, wshape, fw, K, dev)
     room += more
+    if gather and slots > 8 * E:                            # room for x's rows in the plan's order
+        room += slots * (-(-K // 16) * 16 + -(-K // BLOCK)) + 256
     space = torch.empty(room, dtype=torch.uint8, device=dev) if room else None
     spec = _spec(fx.e, fx.m, fw.e, fw.m, act, otype, fo.e if fo else 0, fo.m if fo else 0, xt)
     _lib.run("mxq_experts_packed", dev, xc.data_ptr(), None if xs is None else xs.data_ptr(), xp, rows, wc.data_ptr(), ws.data_ptr(), wshape[-1], E, N, K,

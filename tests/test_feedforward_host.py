@@ -61,7 +61,7 @@ def test_c_abi_refuses_first():
                                     none, none, 0, none)
     fp4 = _lib.MxqProductSpec(2, 1, 2, 1, 0, 0, 0, 0, 0)
     assert L.mxq_product_workspace(64, 64, 10, 64, 64, 10, 128, 0, ctypes.byref(fp4)) == 0
-    assert L.mxq_product_workspace(64, 64, 10, 64, 64, 10, 128, 1, ctypes.byref(fp4)) == 1280      # gathered rows are widened
+    assert L.mxq_product_workspace(64, 64, 10, 64, 64, 10, 128, 20, ctypes.byref(fp4)) == 1280 + 2688   # widened and in order
     assert L.mxq_product_workspace(64, 64, 10, 64, 64, 10, 128, 1, none) == -1
     assert experts(E=1025) == _lib.ERR_UNSUPPORTED and b"1024 experts" in L.mxq_last_error()
     assert experts(rows=1) == _lib.ERR_VALUE and b"do not serve" in L.mxq_last_error()
