@@ -1260,7 +1260,7 @@ int product(const char* who, Args& a, const Given& gx, const Given& gw, int64_t 
   const Cut cut = cut_of(a, gated, a.kblocks);
   // Rows that the plan scatters are fetched one by one by k_mx_rows in tiles of up to 32 (tile::gather4: four rows an
   // instruction, about 65 cycles each), and brought into the plan's order first for larger tiles: 64 experts 2048 x 2048, 384
-  // rows each: 330 us fetched, 154 sorted; 8 experts 4096 x 4096, 16 rows each: 36 and 31.
+  // rows each: 330 us fetched, 154 sorted; 8 experts 4096 x 4096, 16 rows each: 36 and 33.
   const bool sorted = a.per > 0 && (!cut.few || cut.bn > 32);
   const int64_t room_x = room(gx, K, a.per > 0), room_w = room(gw, K, false), room_s = sorted ? sorted_room(a.rows, K) : 0;
   const int64_t need = room_x + room_w + room_s;
