@@ -311,9 +311,11 @@ int mxq_route_backward(const float* grad, const void* logits, int32_t type, int6
                        void* grad_logits, int64_t T, int64_t E, int64_t k, const mxq_route_spec* spec, void* stream);
 /* The slots (token-major, T x k flattened) in the order of their experts, each expert's in their own order: offsets
  * (experts + 1), order[place] = slot, where[slot] = place. A slot whose expert is outside [0, experts) is left out: its
- * where is -1 and the last places of order are -1. At most 1024 experts. */
+ * where is -1 and the last places of order are -1. At most 1024 experts. workspace: mxq_dispatch_workspace bytes (0 up to 98304
+ * slots), 4-byte aligned. */
+int64_t mxq_dispatch_workspace(int64_t slots, int64_t experts);
 int mxq_dispatch(const int32_t* experts_of, int64_t slots, int64_t experts, int32_t* offsets, int32_t* order,
-                 int32_t* where, void* stream);
+                 int32_t* where, void* workspace, int64_t workspace_bytes, void* stream);
 /* y[t] = sum_j weights[t, j] z[where[t, j]] + residual[t], z slots x N, y T x N (one type); float32 sums in the order of
  * j. A slot with where -1 adds weights * 0. residual: rows residual_stride apart, or NULL. */
 int mxq_combine(const void* z, int32_t type, const float* weights, const int32_t* where, const void* residual,

@@ -92,59 +92,77 @@ __device__ __forceinline__ float to_float<__nv_bfloat16>(__nv_bfloat16 v) { retu
 template <>
 __device__ __forceinline__ float to_float<__half>(__half v) { return __half2float(v); }
 
-// Four lanes per block of 32: 8 values each, the block's largest |value| by two shuffles. VEC: 16-byte loads.
-template <typename T, bool VEC>
+// Two lanes per block of 32: 16 values each, the block's largest |value| by a shuffle. VEC: 16-byte loads. I: the index
+// type, 32 bits while the lanes are fewer than 2^31 (the division by the blocks of a row is what it is for).
+template <typename T, bool VEC, int FMT, typename I>
 __global__ void __launch_bounds__(256) k_pack_rows(const T* __restrict__ x, int64_t x_stride, uint8_t* __restrict__ codes,
-                                                   int64_t out_pitch, uint8_t* __restrict__ scales, int64_t rows, int64_t K, int fmt) {
+                                                   int64_t out_pitch, uint8_t* __restrict__ scales, int64_t rows, int64_t K) {
   start_next_grid();
-  const int64_t nb = (K + 31) / 32, n = rows * nb * 4, stride = (int64_t)gridDim.x * blockDim.x;
-  const int64_t n32 = (n + 31) / 32 * 32;              // whole warps stay for the shuffles
-  for (int64_t i = (int64_t)blockIdx.x * blockDim.x + threadIdx.x; i < n32; i += stride) {
-    const int64_t b = i >> 2, r = b / nb, c = (b - r * nb) * 32 + (i & 3) * 8;
-    float v[8];
-    uint32_t top = 0;
+  constexpr int N = 16;
+  const I nb = (I)((K + 31) / 32), n = (I)(rows * (int64_t)nb * 2), stride = (I)gridDim.x * blockDim.x;
+  const I whole = (n + 31) / 32 * 32;                  // whole warps stay for the shuffle
+  for (I i = (I)blockIdx.x * blockDim.x + threadIdx.x; i < whole; i += stride) {
+    const I b = i >> 1, r = b / nb;
+    const int64_t c = (int64_t)(b - r * nb) * 32 + (int)(i & 1) * N;
     const bool live = i < n;
-    if (VEC && live && c + 8 <= K) {
-      const uint4* from = reinterpret_cast<const uint4*>(x + r * x_stride + c);
-      T t[8];
+    const T* from = x + (int64_t)r * x_stride + c;
+    float v[N];
+    if (VEC && live && c + N <= K) {
+      uint4 t[sizeof(T)];
 #pragma unroll
-      for (int j = 0; j < (int)(sizeof(T) / 2); j++) reinterpret_cast<uint4*>(t)[j] = __ldg(from + j);
+      for (int j = 0; j < (int)sizeof(T); j++) t[j] = __ldg(reinterpret_cast<const uint4*>(from) + j);
 #pragma unroll
-      for (int j = 0; j < 8; j++) v[j] = to_float<T>(t[j]);
+      for (int j = 0; j < N; j++) v[j] = to_float<T>(reinterpret_cast<const T*>(t)[j]);
     } else {
 #pragma unroll
-      for (int j = 0; j < 8; j++) v[j] = live && c + j < K ? to_float<T>(x[r * x_stride + c + j]) : 0.0f;
+      for (int j = 0; j < N; j++) v[j] = live && c + j < K ? to_float<T>(from[j]) : 0.0f;
     }
+    uint32_t top = 0;
 #pragma unroll
-    for (int j = 0; j < 8; j++) top = max(top, __float_as_uint(v[j]) & 0x7fffffffu);
+    for (int j = 0; j < N; j++) top = max(top, __float_as_uint(v[j]) & 0x7fffffffu);
     top = max(top, __shfl_xor_sync(~0u, top, 1));
-    top = max(top, __shfl_xor_sync(~0u, top, 2));
-    const uint32_t sb = scale_byte(top, fmt);
+    const uint32_t sb = scale_byte(top, FMT);
     const float inv = scale_inverse(sb);
     uint32_t q[4];
 #pragma unroll
     for (int j = 0; j < 4; j++) {
-      q[j] = encode2(fmt, scaled(v[2 * j], inv), scaled(v[2 * j + 1], inv));
-      if (fmt > kFmtE5M2) q[j] = widen2(fmt, q[j]);
+      uint32_t h[2];
+#pragma unroll
+      for (int p = 0; p < 2; p++) {
+        h[p] = encode2(FMT, __fmul_rn(v[4 * j + 2 * p], inv), __fmul_rn(v[4 * j + 2 * p + 1], inv));
+        if (FMT > kFmtE5M2) h[p] = widen2(FMT, h[p]);
+      }
+      q[j] = sb == 255u ? 0u : h[0] | h[1] << 16;      // a block with an Inf or a NaN: its scale says so
     }
     if (!live) continue;
-    if ((i & 3) == 0) scales[b] = (uint8_t)sb;
-    if (c < out_pitch)                                 // the pitch is a multiple of 16, c of 8
-      *reinterpret_cast<uint2*>(codes + r * out_pitch + c) = make_uint2(q[0] | q[1] << 16, q[2] | q[3] << 16);
+    if ((i & 1) == 0) scales[b] = (uint8_t)sb;
+    if (c < out_pitch)                                 // the pitch is a multiple of 16, as c is
+      *reinterpret_cast<uint4*>(codes + (int64_t)r * out_pitch + c) = make_uint4(q[0], q[1], q[2], q[3]);
   }
 }
 
+template <typename T, int FMT>
+int pack_rows(const void* x, int64_t x_stride, uint8_t* codes, int64_t out_pitch, uint8_t* scales, int64_t rows, int64_t K,
+              cudaStream_t st) {
+  const int64_t n = rows * ((K + 31) / 32) * 2;
+  const unsigned grid = grid_for(n, 256, 16);
+  const bool vec = reinterpret_cast<uintptr_t>(x) % 16 == 0 && x_stride * (int64_t)sizeof(T) % 16 == 0;
+  const bool small = n < (1ll << 31) - (int64_t)grid * 256 - 64;
+  auto f = vec ? (small ? k_pack_rows<T, true, FMT, uint32_t> : k_pack_rows<T, true, FMT, int64_t>)
+               : (small ? k_pack_rows<T, false, FMT, uint32_t> : k_pack_rows<T, false, FMT, int64_t>);
+  f<<<grid, 256, 0, st>>>(static_cast<const T*>(x), x_stride, codes, out_pitch, scales, rows, K);
+  return MXQ_LAUNCH_CHECK("pack_rows");
+}
 template <typename T>
 int pack_rows(const void* x, int64_t x_stride, uint8_t* codes, int64_t out_pitch, uint8_t* scales, int64_t rows, int64_t K, int fmt,
               cudaStream_t st) {
-  const int64_t n = rows * ((K + 31) / 32) * 4;
-  const unsigned grid = grid_for(n, 256, 16);
-  const bool vec = reinterpret_cast<uintptr_t>(x) % 16 == 0 && x_stride * (int64_t)sizeof(T) % 16 == 0;
-  if (vec)
-    k_pack_rows<T, true><<<grid, 256, 0, st>>>(static_cast<const T*>(x), x_stride, codes, out_pitch, scales, rows, K, fmt);
-  else
-    k_pack_rows<T, false><<<grid, 256, 0, st>>>(static_cast<const T*>(x), x_stride, codes, out_pitch, scales, rows, K, fmt);
-  return MXQ_LAUNCH_CHECK("pack_rows");
+  switch (fmt) {
+    case kFmtE4M3: return pack_rows<T, kFmtE4M3>(x, x_stride, codes, out_pitch, scales, rows, K, st);
+    case kFmtE5M2: return pack_rows<T, kFmtE5M2>(x, x_stride, codes, out_pitch, scales, rows, K, st);
+    case kFmtE3M2: return pack_rows<T, kFmtE3M2>(x, x_stride, codes, out_pitch, scales, rows, K, st);
+    case kFmtE2M3: return pack_rows<T, kFmtE2M3>(x, x_stride, codes, out_pitch, scales, rows, K, st);
+    default: return pack_rows<T, kFmtE2M1>(x, x_stride, codes, out_pitch, scales, rows, K, st);
+  }
 }
 
 }  // namespace

@@ -105,7 +105,7 @@ _SIGS = {
     "mxq_pack_rows": [P, I32, I64, P, I64, P, I64, I64, I32, I32, P],
     "mxq_route": [P, I32, I64, P, P, P, I64, I64, I64, ctypes.POINTER(MxqRouteSpec), P],
     "mxq_route_backward": [P, P, I32, I64, P, P, I64, I64, I64, ctypes.POINTER(MxqRouteSpec), P],
-    "mxq_dispatch": [P, I64, I64, P, P, P, P],
+    "mxq_dispatch": [P, I64, I64, P, P, P, P, I64, P],
     "mxq_combine": [P, I32, P, P, P, I64, P, I64, I64, I64, P],
     "mxq_combine_backward": [P, I64, P, I32, P, P, P, P, P, I64, I64, I64, P],
     "mxq_device_timeouts": [P],
@@ -131,6 +131,8 @@ def lib():
                     f.restype = I32
                 L.mxq_block_lut_workspace.argtypes = [I64, I64, I32, I32]
                 L.mxq_block_lut_workspace.restype = I64
+                L.mxq_dispatch_workspace.argtypes = [I64, I64]
+                L.mxq_dispatch_workspace.restype = I64
                 L.mxq_product_workspace.argtypes = [P, I64, I64, P, I64, I64, I64, I64, ctypes.POINTER(MxqProductSpec)]
                 L.mxq_product_workspace.restype = I64
                 L.mxq_last_error.restype = ctypes.c_char_p

@@ -30,6 +30,8 @@ __all__ = ["route", "route_backward", "dispatch", "combine", "combine_backward"]
 
 SCORES = ("softmax", "sigmoid")
 GROUP_SCORES = ("max", "top2")
+#: slots up to which dispatch needs no workspace
+ONE_LAUNCH = 98304
 
 
 def _make_spec(score, groups, keep, top2, renormalize, scale):
@@ -141,7 +143,13 @@ def dispatch(experts: torch.Tensor, n_experts: int) -> Dispatch:
     offsets = torch.empty(n_experts + 1, dtype=torch.int32, device=dev)
     order = torch.empty(n, dtype=torch.int32, device=dev)
     where = torch.empty_like(e)
-    _lib.run("mxq_dispatch", dev, e.data_ptr(), n, n_experts, offsets.data_ptr(), order.data_ptr(), where.data_ptr())
+    room, space = 0, None
+    if n > ONE_LAUNCH:
+        with _lib.using(dev):                               # the size goes by the device's SMs
+            room = _lib.lib().mxq_dispatch_workspace(n, n_experts)
+        space = torch.empty(room, dtype=torch.uint8, device=dev)
+    _lib.run("mxq_dispatch", dev, e.data_ptr(), n, n_experts, offsets.data_ptr(), order.data_ptr(), where.data_ptr(),
+             None if space is None else space.data_ptr(), room)
     if home != dev:
         offsets, order, where = offsets.to(home), order.to(home), where.to(home)
     return Dispatch(offsets, order, where)

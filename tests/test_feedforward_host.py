@@ -74,8 +74,10 @@ def test_c_abi_refuses_first():
     for text, kw in ((b"experts", dict(E=1025)), (b"k must be", dict(k=9)), (b"score", dict(score=2)), (b"groups", dict(groups=3)),
                      (b"groups", dict(groups=2, keep=3))):
         assert route(**kw) == _lib.ERR_VALUE and text in L.mxq_last_error()
-    assert L.mxq_dispatch(none, -1, 4, none, none, none, none) == _lib.ERR_VALUE
-    assert L.mxq_dispatch(none, 4, 2000, none, none, none, none) == _lib.ERR_VALUE
+    assert L.mxq_dispatch(none, -1, 4, none, none, none, none, 0, none) == _lib.ERR_VALUE
+    assert L.mxq_dispatch(none, 4, 2000, none, none, none, none, 0, none) == _lib.ERR_VALUE
+    assert L.mxq_dispatch_workspace(98304, 8) == 0 and L.mxq_dispatch_workspace(98305, 8) == 148 * 8 * 4
+    assert L.mxq_dispatch(none, 98305, 8, none, none, none, none, 0, none) == _lib.ERR_VALUE and b"4736 bytes" in L.mxq_last_error()
     assert L.mxq_combine(none, 0, none, none, none, 0, none, 3, 0, 4, none) == _lib.ERR_VALUE
     assert L.mxq_combine(none, 7, none, none, none, 0, none, 3, 1, 4, none) == _lib.ERR_VALUE
     assert L.mxq_lay_codes(none, 8, 16, 24, 1, 8, 4, 3, none) == _lib.ERR_VALUE
