@@ -1,7 +1,8 @@
 /* mxq_b200 — C ABI of the B200 (sm_100a) implementation of mxq's quantize-and-emulated-matmul hot path.
  *
  * Every entry point replaces one function of the reference Python package (chloe-wong/microscaling-quant,
- * paths below are mxq/...:line) and computes bit-identical results on the device. Conventions:
+ * paths below are mxq/...:line) and computes bit-identical results on the device, except those that say they have no
+ * reference counterpart. Conventions:
  *   - all array arguments are DEVICE pointers to contiguous row-major data; sizes are element counts;
  *   - `stream` is a cudaStream_t (NULL = the legacy default stream); calls are asynchronous unless stated;
  *   - the return value is MXQ_OK (0) or an MXQ_ERR_* code; mxq_last_error() returns this thread's message;

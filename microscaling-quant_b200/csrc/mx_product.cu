@@ -9,7 +9,7 @@
 //
 // Two kernels share the operand staging:
 //   k_mx_tile  256 rows of x by 256 rows of w per pair of CTAs, persistent, for many rows: the operations bound it.
-//   k_mx_rows  128 rows of w by 16-128 rows of x per CTA, K split over a cluster, for few rows: reading w bounds it.
+//   k_mx_rows  128 rows of w by 16-64 rows of x per CTA, K split over a cluster, for few rows: reading w bounds it.
 #include "common.cuh"
 #include "mx_codes.cuh"
 #include "tc.cuh"
@@ -492,6 +492,12 @@ __device__ __forceinline__ void add_bias(float mine, float (&y)[32]) {
 // Warp 0 loads the codes, warp 1 of the pair's first CTA issues the products, warps 2 and 3 bring the scales, warps 4-11 write
 // y: two per lane quarter, each with units of 64 columns.
 //
+// Measured (E4M3, bf16 y): 8192 x 8192 x 8192 436 us in a burst (2.52 PFLOP/s), 505 us back to back at the 1250 MHz that the power
+// limit leaves. A step of 128 along K takes its products' 512 cycles once the ring is full; a tile then adds about 700
+// idle cycles (its last product, the shared columns' way out, the word to the next) and a launch 5700 before its first
+// product and the last tile's epilogue behind it. Short K shows the epilogue: 24576 rows by expert, 2048 x 1024: 85 us, 62
+// without it.
+//
 // TMEM (512 columns, the same in both CTAs): two accumulators of 256 that share 64 columns, [0, 256) and [192, 448), and
 // the stages' scale words in [448, 508). The epilogue of a tile drains the shared columns first and then lets the next
 // tile's products start, so three quarters of it run beside them.
@@ -871,6 +877,11 @@ __device__ __forceinline__ void write_four(const Args& a, float (&y)[4], int64_t
   }
 }
 
+// Here w's rows are the A operand (128 lanes of TMEM) and x's the B operand (16 to 64 columns), so that a tile costs what its
+// bytes of w cost. Measured, 16 rows by 16384 x 16384: E4M3 50 us (5.5 TB/s), FP4 34 us (4.2 TB/s: a stage holds half the
+// bytes, and the time from a stage's release to its next product is the same). 1 row by 8192 x 2048: 7.6 us, of which
+// the launch, the set-up and the cluster's two barriers are most.
+//
 // The cluster's CTAs each take a share of K; their partial sums meet in shared memory and are added in rank order (the
 // same sum on every run), each CTA finishing its share of the rows of x.
 template <int BN, bool GATED>

@@ -98,7 +98,8 @@ __device__ __forceinline__ void merge2(uint32_t& a, uint32_t& b, uint32_t c, uin
 // by lane j for the j-th. Groups whose runs are whole lanes, a power of two of them (every usual shape), are ranked by
 // shuffles, all at once; others one by one.
 //
-// Bound by issue: 8192 tokens of 256 experts (float32, 8 groups, k = 8) read 8 MB, 1.3 us at the copy's rate.
+// Bound by issue (about 1000 instructions a token): 8192 tokens of 256 experts (float32, bias, 8 groups, k = 8) take 12.5
+// us, their 9.4 MB 1.4 us at the copy's rate; 16 tokens 3.4 us.
 template <typename IN, int V>
 __global__ void __launch_bounds__(128) k_route(const IN* __restrict__ logits, const float* __restrict__ bias,
                                                float* __restrict__ weights, int* __restrict__ experts, RouteArgs a) {
@@ -229,7 +230,9 @@ __global__ void __launch_bounds__(128) k_route(const IN* __restrict__ logits, co
 }
 
 // A warp per token. Lane j holds choice j: g = grad scale, ds = (g - sum g s / S) / S when renormalized; softmax:
-// dl = p (ds - sum ds p), ds 0 where not chosen; sigmoid: dl = ds s (1 - s) at the chosen.
+// dl = p (ds - sum ds p), ds 0 where not chosen; sigmoid: dl = ds s (1 - s) at the chosen. The probabilities are made again
+// from the logits: reading k floats and E logits a token, writing E. 8191 tokens of 64 experts (bf16): 4.2 us, two of them
+// the launch.
 template <typename IN, int V>
 __global__ void __launch_bounds__(128) k_route_backward(const float* __restrict__ grad, const IN* __restrict__ logits,
                                                         const int* __restrict__ experts, IN* __restrict__ out, RouteArgs a) {
@@ -492,7 +495,8 @@ __device__ __forceinline__ void store_vec(T* row, int64_t c, int64_t n, const Ve
   }
 }
 
-// A CTA per token and stretch of columns, 16 bytes of y per thread; four of the experts' rows are on their way at once.
+// A CTA per token and stretch of columns, 16 bytes of y per thread; four of the experts' rows are on their way at once. Bound
+// by the bytes: 4096 tokens, k = 8, 4096 columns (bf16) 47 us, 6.4 TB/s; 24 tokens of 2048 columns 2.6 us, a launch.
 template <typename T, bool VEC>
 __global__ void __launch_bounds__(256) k_combine(const T* __restrict__ z, const float* __restrict__ weights,
                                                  const int* __restrict__ where, const T* __restrict__ residual,
@@ -538,7 +542,8 @@ __global__ void __launch_bounds__(256) k_combine(const T* __restrict__ z, const 
 
 // A CTA per token. J experts' rows (all of them up to 8) at a time: dy's piece is read once for them, their pieces of z are
 // on their way together, and a thread's share of the dot products stays in registers and is added up over the CTA in a
-// fixed order.
+// fixed order. Bound by the bytes: 4096 tokens, k = 6, 2048 columns (bf16) 36.7 us, 6.0 TB/s (49 us with two CTAs per SM; 65
+// with the tail's look at `order` one load after the other).
 template <typename T, bool VEC, int J>
 __global__ void __launch_bounds__(256, 3) k_combine_backward(const T* __restrict__ dy, int64_t dy_stride, const T* __restrict__ z,
                                                           const float* __restrict__ weights, const int* __restrict__ where,
