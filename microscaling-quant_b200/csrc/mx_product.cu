@@ -49,6 +49,7 @@ struct Args {
   int64_t out_pitch, out_nb;
   int act, otype, ofmt;
   int vec_out;                 // y's (and the residual's) rows take 16-byte accesses
+  int map_out;                 // k_mx_tile: whole staged rows of y leave by TMA
   unsigned* status;
   int64_t wait_cycles;
 };
@@ -495,20 +496,21 @@ __device__ __forceinline__ void add_bias(float mine, float (&y)[32]) {
 // Measured (E4M3, bf16 y): 8192 x 8192 x 8192 436 us in a burst (2.52 PFLOP/s), 505 us back to back at the 1250 MHz that the power
 // limit leaves. A step of 128 along K takes its products' 512 cycles once the ring is full; a tile then adds about 700
 // idle cycles (its last product, the shared columns' way out, the word to the next) and a launch 5700 before its first
-// product and the last tile's epilogue behind it. Short K shows the epilogue: 24576 rows by expert, 2048 x 1024: 85 us, 62
-// without it.
+// product and the last tile's epilogue behind it. Short K shows the epilogue: 24576 rows by expert, 2048 x 1024: 81 us (85 with
+// the staged rows written by the warps), 62 without it; 8192 x 8192 x 256 47 us.
 //
 // TMEM (512 columns, the same in both CTAs): two accumulators of 256 that share 64 columns, [0, 256) and [192, 448), and
 // the stages' scale words in [448, 508). The epilogue of a tile drains the shared columns first and then lets the next
 // tile's products start, so three quarters of it run beside them.
 template <bool GATED, int OUT>
 __global__ void __launch_bounds__(128 + 32 * kWriters, 1) __cluster_dims__(2, 1, 1)
-    k_mx_tile(const __grid_constant__ CUtensorMap mx, const __grid_constant__ CUtensorMap mw, const __grid_constant__ Args a) {
+    k_mx_tile(const __grid_constant__ CUtensorMap mx, const __grid_constant__ CUtensorMap mw, const __grid_constant__ CUtensorMap my,
+              const __grid_constant__ Args a) {
   extern __shared__ uint8_t raw[];
   uint8_t* codes = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(raw) + 1023) & ~(uintptr_t)1023);
-  uint8_t* scales = codes + kStages * kStageBytes;
-  uint8_t* passes = scales + kStages * kStageScales;
-  TileShared& sh = *reinterpret_cast<TileShared*>(passes + kWriters * kPassBytes);
+  uint8_t* passes = codes + kStages * kStageBytes;     // multiples of 1024 bytes, as the swizzle wants them
+  uint8_t* scales = passes + kWriters * kPassBytes;
+  TileShared& sh = *reinterpret_cast<TileShared*>(scales + kStages * kStageScales);
   const Table tab(&sh + 1, a.experts);
   const tc::Guard guard = {&sh.abort, a.status, a.wait_cycles};
   const int warp = __shfl_sync(~0u, threadIdx.x >> 5, 0), lane = threadIdx.x & 31;
@@ -659,6 +661,25 @@ __global__ void __launch_bounds__(128 + 32 * kWriters, 1) __cluster_dims__(2, 1,
     constexpr int kUnits = kCols / 64;
     constexpr int size = OUT == kOutF32 ? 4 : OUT == kOutPacked ? 1 : 2;
     const bool nib = OUT == kOutPacked && a.ofmt == kFmtE2M1;
+    // the stage's last rows have left it
+    auto stage_free = [&] {
+      if (lane == 0) tc::store_read();
+      __syncwarp();
+    };
+    // the staged rows from column col on: by TMA where they are whole (it leaves out what is beyond y; by expert the next
+    // expert's rows are), else by the warp
+    auto put = [&](int row, int rows, int col, int cols) {
+      if (a.map_out && (rows == 32 || a.experts == 0)) {
+        fence_proxy_async();
+        __syncwarp();
+        if (lane == 0) tc::tma_store(&my, col * size, row, stage);
+      } else {
+        __syncwarp();
+        put_rows<8>(stage, static_cast<uint8_t*>(a.out) + (row * a.out_pitch + col) * size, a.out_pitch * size, rows, cols * size, size,
+                    a.vec_out);
+      }
+      __syncwarp();
+    };
     for (int i = pair; i < tiles; i += pairs, done++) {
       const Tile t = list.next(i, pairs, tiles, a, tab, 256, col_tiles);
       const int row = t.row0 + rank * 128 + q * 32;    // the warp's first
@@ -667,8 +688,9 @@ __global__ void __launch_bounds__(128 + 32 * kWriters, 1) __cluster_dims__(2, 1,
       auto unit_of = [&](int u) { return ((done & 1 ? 0 : kUnits - 1) + 2 * u + set) % kUnits; };
       // the residual's columns from col on go to the stage while the products and the activation are at work
       auto fetch = [&](int col) {
-        if (a.residual && rows > 0 && col < a.width)
-          get_rows(stage, static_cast<const uint8_t*>(a.residual) + (row * a.residual_stride + col) * size, a.residual_stride * size,
+        if (!a.residual || rows <= 0 || col >= a.width) return;
+        if (a.map_out) stage_free();
+        get_rows(stage, static_cast<const uint8_t*>(a.residual) + (row * a.residual_stride + col) * size, a.residual_stride * size,
                    rows, min(128, (a.width - col) * size), size, a.vec_out);
       };
       // a unit's biases: column lane and column 32 + lane, of the gates and of the ups
@@ -746,16 +768,17 @@ __global__ void __launch_bounds__(128 + 32 * kWriters, 1) __cluster_dims__(2, 1,
               const uint32_t sb = stage_block(a.ofmt, y, stage, c, left);
               if (lane < rows) a.out_scales[(row + lane) * a.out_nb + (col >> 5)] = (uint8_t)sb;
             } else {
-              if (a.residual && (c == 0 || OUT == kOutF32)) {
-                asm volatile("cp.async.wait_all;\n" ::: "memory");
-                __syncwarp();
+              if (c == 0 || OUT == kOutF32) {
+                if (a.residual) {
+                  asm volatile("cp.async.wait_all;\n" ::: "memory");
+                  __syncwarp();
+                } else if (a.map_out) {
+                  stage_free();
+                }
               }
               stage_row<OUT>(a.residual != nullptr, y, stage, OUT == kOutF32 ? 0 : 4 * c);
               if (OUT == kOutF32) {                    // 32 columns fill the stage
-                __syncwarp();
-                put_rows<8>(stage, static_cast<uint8_t*>(a.out) + (row * a.out_pitch + col) * 4, a.out_pitch * 4, rows,
-                            min(32, left) * 4, 4, a.vec_out);
-                __syncwarp();
+                put(row, rows, col, min(32, left));
                 if (c == 0) fetch(col + 32);
               }
             }
@@ -765,17 +788,18 @@ __global__ void __launch_bounds__(128 + 32 * kWriters, 1) __cluster_dims__(2, 1,
         }
         if (OUT == kOutF32 || !live) continue;
         const int left = min(64, a.width - col0);
-        __syncwarp();
         if (OUT == kOutPacked) {
           uint8_t* out = static_cast<uint8_t*>(a.out) + row * a.out_pitch;
+          __syncwarp();
           if (nib) put_rows<2>(stage, out + (col0 >> 1), a.out_pitch, rows, left >> 1, 1, a.vec_out);
           else put_rows<4>(stage, out + col0, a.out_pitch, rows, left, 1, a.vec_out);
+          __syncwarp();
         } else {
-          put_rows<8>(stage, static_cast<uint8_t*>(a.out) + (row * a.out_pitch + col0) * 2, a.out_pitch * 2, rows, left * 2, 2, a.vec_out);
+          put(row, rows, col0, left);
         }
-        __syncwarp();
       }
     }
+    if (a.map_out && lane == 0) tc::store_done();
   }
   __syncwarp();
   tc::fence_before();
@@ -1118,9 +1142,15 @@ int launch_rows(Args& a, const Operand& x, const Operand& w, int64_t K, int64_t 
 
 template <bool GATED, int OUT>
 int launch_tile(Args& a, const Operand& x, const Operand& w, int64_t K, int64_t tiles, int fx, int fw, cudaStream_t st) {
-  CUtensorMap mx, mw;
+  CUtensorMap mx, mw, my;
   if (int rc = map_of(&mx, x, K, 128)) return rc;
   if (int rc = map_of(&mw, w, K, 128)) return rc;
+  // y as bytes, in the stage's rows of 128
+  const int size = OUT == kOutF32 ? 4 : 2;
+  a.map_out = OUT != kOutPacked && a.vec_out;
+  my = mx;
+  if (a.map_out)
+    if (int rc = encode_tmap_codes(&my, a.out, false, (uint64_t)a.rows, (uint64_t)a.width * size, (uint64_t)a.out_pitch * size, 32)) return rc;
   a.idesc = tc::mma_desc(fx, fw, 256, 256);
   const int smem = kTileSmem + (a.experts ? table_bytes(a.experts) : 0);
   auto f = k_mx_tile<GATED, OUT>;
@@ -1136,7 +1166,7 @@ int launch_tile(Args& a, const Operand& x, const Operand& w, int64_t K, int64_t 
   at[0].val.programmaticStreamSerializationAllowed = 1;
   cfg.attrs = at;
   cfg.numAttrs = 1;
-  return check_cuda(cudaLaunchKernelEx(&cfg, f, mx, mw, a), "product");
+  return check_cuda(cudaLaunchKernelEx(&cfg, f, mx, mw, my, a), "product");
 }
 
 int64_t up_div(int64_t a, int64_t b) { return (a + b - 1) / b; }

@@ -194,6 +194,15 @@ __device__ __forceinline__ void tma_load_pair(void* dst, const CUtensorMap* map,
       "l"(map), "r"(x), "r"(y), "r"(bar)
       : "memory");
 }
+// a box from shared memory to a tensor, under way when it returns; the thread's boxes are read; they are written
+__device__ __forceinline__ void tma_store(const CUtensorMap* map, int x, int y, const void* src) {
+  asm volatile("cp.async.bulk.tensor.2d.global.shared::cta.bulk_group [%0, {%1, %2}], [%3];\n cp.async.bulk.commit_group;\n" ::"l"(map),
+               "r"(x), "r"(y), "r"(smem_addr(src))
+               : "memory");
+}
+__device__ __forceinline__ void store_read() { asm volatile("cp.async.bulk.wait_group.read 0;\n" ::: "memory"); }
+__device__ __forceinline__ void store_done() { asm volatile("cp.async.bulk.wait_group 0;\n" ::: "memory"); }
+
 // four rows of a tensor, 128 bytes each, one after the other in shared memory
 __device__ __forceinline__ void tma_gather4(void* dst, const CUtensorMap* map, int x, int4 rows, uint64_t* bar) {
   asm volatile(
