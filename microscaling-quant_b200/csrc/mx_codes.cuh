@@ -1,5 +1,5 @@
-// The packed form's element codes made on the device from float32: the formats, a block's scale byte (floor(log2 amax) -
-// emax by the exponent field) and the rounding of two values to two codes by sm_100's conversions.
+// The packed form's element codes made on the device from float32: the formats, a block's scale byte (floor(log2
+// amax) - emax by the exponent field) and the rounding of two values to two codes by sm_100's conversions.
 #pragma once
 #include <stdint.h>
 
@@ -54,8 +54,8 @@ __device__ __forceinline__ uint32_t encode2(int fmt, float lo, float hi) {
   return q;
 }
 
-// two FP6 or FP4 codes (the first in the low byte) as the E4M3 codes of the same values, exactly: 8-bit E4M3 holds every
-// value of the smaller grids
+// two FP6 or FP4 codes (the first in the low byte) as the E4M3 codes of the same values, exactly: 8-bit E4M3 holds
+// every value of the smaller grids
 __device__ __forceinline__ uint32_t widen2(int fmt, uint32_t codes) {
   uint32_t h;
   const uint16_t c = (uint16_t)codes;

@@ -1,7 +1,7 @@
-// Operands of the packed products brought to the layout that the tensor maps take: codes of any MX format as 8-bit codes
-// at a pitch of 16 bytes (k_lay_codes), and float rows packed on the way in (k_pack_rows). Both read their input once and
-// write their output once; they are bound by those bytes. 8192 x 8192: packing float32 50 us (6.7 TB/s), bf16 33 us (6.1);
-// FP6 codes laid out 24 us (5.7), FP4 22 us (4.5), E4M3 rows of 8184 28 us (4.8).
+// Operands of the packed products brought to the layout that the tensor maps take: codes of any MX format as 8-bit
+// codes at a pitch of 16 bytes (k_lay_codes), and float rows packed on the way in (k_pack_rows). Both read their
+// input once and write their output once; they are bound by those bytes. 8192 x 8192: packing float32 50 us (6.7
+// TB/s), bf16 33 us (6.1); FP6 codes laid out 24 us (5.7), FP4 22 us (4.5), E4M3 rows of 8184 28 us (4.8).
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 
@@ -65,8 +65,8 @@ __global__ void __launch_bounds__(256) k_lay_codes(const uint8_t* __restrict__ i
   }
 }
 
-// A warp per row of the product: the codes and scale bytes of the row of x that its slot takes, side by side in the order
-// of the slots.
+// A warp per row of the product: the codes and scale bytes of the row of x that its slot takes, side by side in the
+// order of the slots.
 __global__ void __launch_bounds__(256) k_gather_rows(const uint8_t* __restrict__ codes, const uint8_t* __restrict__ scales, int64_t pitch,
                                                      const int* __restrict__ order, int per, int x_rows, int64_t slots, int nb,
                                                      uint8_t* __restrict__ to_codes, uint8_t* __restrict__ to_scales) {

@@ -1,6 +1,6 @@
 // Routing to experts and back: the router's choice and its gradient, the slots in the order of their experts, and the
-// weighted sum of the experts' rows with its gradients. All of it is bound by the bytes it reads and writes or, for a few
-// tokens, by latency; scores and sums are float32.
+// weighted sum of the experts' rows with its gradients. All of it is bound by the bytes it reads and writes or, for a
+// few tokens, by latency; scores and sums are float32.
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 
@@ -93,13 +93,13 @@ __device__ __forceinline__ void merge2(uint32_t& a, uint32_t& b, uint32_t c, uin
 }
 
 // A warp per token, V neighbouring experts per lane (lane V on), so that the lowest lane holds the lowest experts and a
-// tie is the first lane of a ballot. The k largest are taken one after the other: the lanes' best by one warp reduction, and
-// only the lane that had it finds which of its own it was. The chosen scores are made again from the logits at the end,
-// by lane j for the j-th. Groups whose runs are whole lanes, a power of two of them (every usual shape), are ranked by
-// shuffles, all at once; others one by one.
+// tie is the first lane of a ballot. The k largest are taken one after the other: the lanes' best by one warp
+// reduction, and only the lane that had it finds which of its own it was. The chosen scores are made again from the
+// logits at the end, by lane j for the j-th. Groups whose runs are whole lanes, a power of two of them (every usual
+// shape), are ranked by shuffles, all at once; others one by one.
 //
-// Bound by issue (about 1000 instructions a token): 8192 tokens of 256 experts (float32, bias, 8 groups, k = 8) take 12.5
-// us, their 9.4 MB 1.4 us at the copy's rate; 16 tokens 3.4 us.
+// Bound by issue (about 1000 instructions a token): 8192 tokens of 256 experts (float32, bias, 8 groups, k = 8) take
+// 12.5 us, their 9.4 MB 1.4 us at the copy's rate; 16 tokens 3.4 us.
 template <typename IN, int V>
 __global__ void __launch_bounds__(128) k_route(const IN* __restrict__ logits, const float* __restrict__ bias,
                                                float* __restrict__ weights, int* __restrict__ experts, RouteArgs a) {
@@ -149,7 +149,8 @@ __global__ void __launch_bounds__(128) k_route(const IN* __restrict__ logits, co
       uint32_t best = 0u, second = 0u;
 #pragma unroll
       for (int i = 0; i < V; i++) merge2(best, second, key[i], 0u);
-      for (int d = 1; d < width; d <<= 1) merge2(best, second, __shfl_xor_sync(kAll, best, d), __shfl_xor_sync(kAll, second, d));
+      for (int d = 1; d < width; d <<= 1)
+        merge2(best, second, __shfl_xor_sync(kAll, best, d), __shfl_xor_sync(kAll, second, d));
       if (a.top2 && second) best = key_of_pair(best, second);
       const int g = lane / width;
       int ahead = 0;                                   // groups that come before this lane's
@@ -170,7 +171,8 @@ __global__ void __launch_bounds__(128) k_route(const IN* __restrict__ logits, co
           const bool in = e0 + i >= g * run && e0 + i < (g + 1) * run;
           merge2(best, second, in ? key[i] : 0u, 0u);
         }
-        for (int d = 1; d < 32; d <<= 1) merge2(best, second, __shfl_xor_sync(kAll, best, d), __shfl_xor_sync(kAll, second, d));
+        for (int d = 1; d < 32; d <<= 1)
+          merge2(best, second, __shfl_xor_sync(kAll, best, d), __shfl_xor_sync(kAll, second, d));
         if (a.top2 && second) best = key_of_pair(best, second);
         if (lane == g) mine = best;
       }
@@ -230,9 +232,9 @@ __global__ void __launch_bounds__(128) k_route(const IN* __restrict__ logits, co
 }
 
 // A warp per token. Lane j holds choice j: g = grad scale, ds = (g - sum g s / S) / S when renormalized; softmax:
-// dl = p (ds - sum ds p), ds 0 where not chosen; sigmoid: dl = ds s (1 - s) at the chosen. The probabilities are made again
-// from the logits: reading k floats and E logits a token, writing E. 8191 tokens of 64 experts (bf16): 4.2 us, two of them
-// the launch.
+// dl = p (ds - sum ds p), ds 0 where not chosen; sigmoid: dl = ds s (1 - s) at the chosen. The probabilities are made
+// again from the logits: reading k floats and E logits a token, writing E. 8191 tokens of 64 experts (bf16): 4.2 us,
+// two of them the launch.
 template <typename IN, int V>
 __global__ void __launch_bounds__(128) k_route_backward(const float* __restrict__ grad, const IN* __restrict__ logits,
                                                         const int* __restrict__ experts, IN* __restrict__ out, RouteArgs a) {
@@ -295,15 +297,15 @@ __global__ void __launch_bounds__(128) k_route_backward(const float* __restrict_
 }
 
 // ----------------------------------------------------------------------------------------------- dispatch
-// A stable counting sort. The slots are cut into a contiguous run per warp; each warp counts its run by expert in shared
-// memory, the counts are added up over the warps, the CTAs and the experts, and each warp then walks its run again, 32
-// slots at a time in order, giving each slot the next place of its expert.
+// A stable counting sort. The slots are cut into a contiguous run per warp; each warp counts its run by expert in
+// shared memory, the counts are added up over the warps, the CTAs and the experts, and each warp then walks its run
+// again, 32 slots at a time in order, giving each slot the next place of its expert.
 //
-// The CTAs' counts meet in one of two ways. Up to kOneLaunch slots one cluster does it all and reads them through distributed
-// shared memory: one launch, no workspace (128 slots of 128 experts 4.7 us; 65536 slots of 256 experts 12.7, against 15.3 in
-// two launches). More slots go over the whole GPU, with a first launch that writes each CTA's counts to the workspace: on
-// eight SMs the scattered stores of `order` take the time (131072 slots: 23.5 us in one cluster, 18.6 in two launches;
-// 524288: 89 and 21).
+// The CTAs' counts meet in one of two ways. Up to kOneLaunch slots one cluster does it all and reads them through
+// distributed shared memory: one launch, no workspace (128 slots of 128 experts 4.7 us; 65536 slots of 256 experts
+// 12.7, against 15.3 in two launches). More slots go over the whole GPU, with a first launch that writes each CTA's
+// counts to the workspace: on eight SMs the scattered stores of `order` take the time (131072 slots: 23.5 us in one
+// cluster, 18.6 in two launches; 524288: 89 and 21).
 constexpr int kDispatchWarps = 16;
 constexpr int64_t kOneLaunch = 98304;
 
@@ -426,7 +428,8 @@ __global__ void __launch_bounds__(kDispatchWarps * 32) k_dispatch(const int* __r
     }
   }
   if (rank == 0 && threadIdx.x == 0) offsets[E] = live;
-  for (int64_t i = live + rank * (int64_t)blockDim.x + threadIdx.x; i < S; i += (int64_t)ctas * blockDim.x) order[i] = -1;
+  for (int64_t i = live + rank * (int64_t)blockDim.x + threadIdx.x; i < S; i += (int64_t)ctas * blockDim.x)
+    order[i] = -1;
   __syncthreads();
   const int bits = 32 - __clz(E - 1);                  // 0 for one expert
   auto place32 = [&](int64_t i, int x) {
@@ -495,8 +498,9 @@ __device__ __forceinline__ void store_vec(T* row, int64_t c, int64_t n, const Ve
   }
 }
 
-// A CTA per token and stretch of columns, 16 bytes of y per thread; four of the experts' rows are on their way at once. Bound
-// by the bytes: 4096 tokens, k = 8, 4096 columns (bf16) 47 us, 6.4 TB/s; 24 tokens of 2048 columns 2.6 us, a launch.
+// A CTA per token and stretch of columns, 16 bytes of y per thread; four of the experts' rows are on their way at
+// once. Bound by the bytes: 4096 tokens, k = 8, 4096 columns (bf16) 47 us, 6.4 TB/s; 24 tokens of 2048 columns 2.6
+// us, a launch.
 template <typename T, bool VEC>
 __global__ void __launch_bounds__(256) k_combine(const T* __restrict__ z, const float* __restrict__ weights,
                                                  const int* __restrict__ where, const T* __restrict__ residual,
@@ -540,10 +544,10 @@ __global__ void __launch_bounds__(256) k_combine(const T* __restrict__ z, const 
   store_vec<T, VEC>(y + t * n, c, n, o);
 }
 
-// A CTA per token. J experts' rows (all of them up to 8) at a time: dy's piece is read once for them, their pieces of z are
-// on their way together, and a thread's share of the dot products stays in registers and is added up over the CTA in a
-// fixed order. Bound by the bytes: 4096 tokens, k = 6, 2048 columns (bf16) 36.7 us, 6.0 TB/s (49 us with two CTAs per SM; 65
-// with the tail's look at `order` one load after the other).
+// A CTA per token. J experts' rows (all of them up to 8) at a time: dy's piece is read once for them, their pieces of
+// z are on their way together, and a thread's share of the dot products stays in registers and is added up over the
+// CTA in a fixed order. Bound by the bytes: 4096 tokens, k = 6, 2048 columns (bf16) 36.7 us, 6.0 TB/s (49 us with two
+// CTAs per SM; 65 with the tail's look at `order` one load after the other).
 template <typename T, bool VEC, int J>
 __global__ void __launch_bounds__(256, 3) k_combine_backward(const T* __restrict__ dy, int64_t dy_stride, const T* __restrict__ z,
                                                           const float* __restrict__ weights, const int* __restrict__ where,

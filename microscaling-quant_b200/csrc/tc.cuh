@@ -94,9 +94,9 @@ __device__ __forceinline__ void tmem_free(uint32_t addr, uint32_t cols) {
     asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;\n" ::"r"(addr), "r"(cols));
 }
 
-// Programmatic dependent launch: this kernel may have been launched while the one before it on the stream was still at work;
-// what that one (or any before it) wrote may be read after this. TMEM is allocated after it too: held while waiting, it
-// could be what a block of the kernel before still needs to go on.
+// Programmatic dependent launch: this kernel may have been launched while the one before it on the stream was still
+// at work; what that one (or any before it) wrote may be read after this. TMEM is allocated after it too: held while
+// waiting, it could be what a block of the kernel before still needs to go on.
 __device__ __forceinline__ void wait_for_prior_grid() { asm volatile("griddepcontrol.wait;\n" ::: "memory"); }
 __device__ __forceinline__ void prefetch_map(const CUtensorMap* map) {
   asm volatile("prefetch.tensormap [%0];\n" ::"l"(map) : "memory");
