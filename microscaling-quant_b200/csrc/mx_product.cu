@@ -542,6 +542,7 @@ __global__ void __launch_bounds__(128 + 32 * kWriters, 1) __cluster_dims__(2, 1,
   tc::fence_before();
   cluster.sync();
   tc::fence_after();
+  tc::start_next_grid();
   const uint32_t tmem = sh.tmem;
   const uint32_t full = tc::remote(sh.full, 0);
   const int tiles = tile_count(a, tab, 256, col_tiles);
@@ -949,6 +950,7 @@ __global__ void __launch_bounds__(128, 2) k_mx_rows(const __grid_constant__ CUte
   tc::fence_before();
   __syncthreads();
   tc::fence_after();
+  tc::start_next_grid();
   const uint32_t tmem = sh.tmem;
   Tile t;
   const bool work = (int)blockIdx.x / split < tile_count(a, tab, BN, col_tiles);  // the same for the whole cluster

@@ -205,6 +205,32 @@ def test_repeats():
             assert torch.equal(nn.linear_packed(x, w, "MXFP8_E4M3", out=torch.float32), y)
 
 
+@pytest.mark.parametrize("M", [8, 100, 600])
+def test_chained_calls(M):
+    """Calls that take one another's outputs, back to back: a product may be launched before the one before it has ended, and
+    reads nothing until then. The same bits as with the device waited for after every call."""
+    from mxq import nn
+    g = gen(37 + M)
+    x0 = torch.randn(M, 512, generator=g).to(DEV, torch.bfloat16)
+    ws = [random_pair((512, 512), fmt, g, DEV) for fmt in ("MXFP8_E4M3", "MXFP4", "MXFP6_E3M2")]
+    ws = [((c, s - 5), f) for (c, s), f in zip(ws, ("MXFP8_E4M3", "MXFP4", "MXFP6_E3M2"))]
+
+    def chain(wait):
+        x, seen = x0, []
+        for i in range(24):
+            w, fmt = ws[i % 3]
+            packed = nn.linear_packed(x, w, fmt, activation="silu", out="MXFP8_E4M3")    # floats or the pair before
+            if wait:
+                torch.cuda.synchronize()
+            x = nn.linear_packed(packed, w, fmt, residual=x0, out=torch.bfloat16) if i % 2 else packed
+            if wait:
+                torch.cuda.synchronize()
+            seen.append(packed[0])
+        return seen
+    for a, b in zip(chain(False), chain(True)):
+        assert torch.equal(a, b)
+
+
 def test_output_beyond_32_bits():
     """More than 2^31 values of y: the last rows and columns are where they belong."""
     from mxq import nn
