@@ -16,12 +16,6 @@ inline int format_of(int e, int m) {
   return kFmtNone;
 }
 
-inline void exponent_mantissa(int fmt, int* e, int* m) {
-  constexpr int kE[5] = {4, 5, 3, 2, 2}, kM[5] = {3, 2, 2, 3, 1};
-  *e = kE[fmt];
-  *m = kM[fmt];
-}
-
 __device__ __forceinline__ int emax_of(int fmt) { return fmt == kFmtE4M3 ? 8 : fmt == kFmtE5M2 ? 15 : fmt == kFmtE3M2 ? 4 : 2; }
 
 // The scale byte of a block whose largest |value| has these bits: floor(log2) - emax by the exponent field (a

@@ -7,6 +7,7 @@
 
 #include "common.cuh"
 #include "mx_codes.cuh"
+#include "mx_layout.cuh"
 
 using namespace mxq;
 
@@ -30,16 +31,17 @@ __device__ __forceinline__ uint32_t lay4(const uint8_t* in, int64_t c, int64_t K
   return widen2(fmt, w & 0xffffu) | widen2(fmt, w >> 16) << 16;
 }
 
-// a thread per 16 codes of the output; its place beyond K is written as zeros (the tensor map never reads it)
-__global__ void __launch_bounds__(256) k_lay_codes(const uint8_t* __restrict__ in, int64_t in_pitch, uint8_t* __restrict__ out,
-                                                   int64_t out_pitch, int64_t rows, int64_t K, int fmt, int vec) {
-  start_next_grid();
-  const int64_t per = out_pitch >> 4, n = rows * per, stride = (int64_t)gridDim.x * blockDim.x;
-  for (int64_t i = (int64_t)blockIdx.x * blockDim.x + threadIdx.x; i < n; i += stride) {
+// A thread per 16 codes of the output; its place beyond K is written as zeros (the tensor map never reads it). Then, for
+// scale rows that are brought to a pitch of 16 bytes too, a thread per 16 of their bytes: zeros beyond the row, which
+// the products do read.
+__device__ __forceinline__ void lay_codes(const LayJob& job, int64_t first, int64_t stride) {
+  const int64_t K = job.K, per = job.out_pitch >> 4, n = job.rows * per;
+  const int fmt = job.fmt;
+  for (int64_t i = first; i < n; i += stride) {
     const int64_t r = i / per, c = (i - r * per) << 4;
-    const uint8_t* row = in + r * in_pitch;
+    const uint8_t* row = job.codes + r * job.pitch;
     uint32_t w[4];
-    if (vec && c + 16 <= K) {                          // the row's words are aligned: 16 codes in one or two loads
+    if (job.vec && c + 16 <= K) {                      // the row's words are aligned: 16 codes in one or two loads
       if (fmt == kFmtE2M1) {
         const uint2 q = __ldg(reinterpret_cast<const uint2*>(row + (c >> 1)));
         w[0] = widen2(fmt, q.x & 255u) | widen2(fmt, (q.x >> 8) & 255u) << 16;
@@ -61,13 +63,35 @@ __global__ void __launch_bounds__(256) k_lay_codes(const uint8_t* __restrict__ i
 #pragma unroll
       for (int j = 0; j < 4; j++) w[j] = c + 4 * j < K ? lay4(row, c + 4 * j, K, fmt) : 0u;
     }
-    *reinterpret_cast<uint4*>(out + r * out_pitch + c) = make_uint4(w[0], w[1], w[2], w[3]);
+    *reinterpret_cast<uint4*>(job.to_codes + r * job.out_pitch + c) = make_uint4(w[0], w[1], w[2], w[3]);
   }
+  if (job.to_scales == nullptr) return;
+  const int nb = (int)((K + 31) / 32);
+  const int64_t groups = job.scales_pitch >> 4, m = job.rows * groups;
+  for (int64_t i = first; i < m; i += stride) {
+    const int64_t r = i / groups;
+    const int at = (int)(i - r * groups) << 4;
+    const uint8_t* row = job.scales + r * nb;
+    uint32_t w[4] = {0u, 0u, 0u, 0u};
+#pragma unroll
+    for (int j = 0; j < 16; j++)
+      if (at + j < nb) w[j >> 2] |= (uint32_t)__ldg(row + at + j) << (8 * (j & 3));
+    *reinterpret_cast<uint4*>(job.to_scales + r * job.scales_pitch + at) = make_uint4(w[0], w[1], w[2], w[3]);
+  }
+}
+
+// one or two operands in one launch: the blocks from `second` on take the other
+__global__ void __launch_bounds__(256) k_lay_codes(LayJob one, LayJob two, unsigned second) {
+  start_next_grid();
+  if (blockIdx.x < second)
+    lay_codes(one, (int64_t)blockIdx.x * blockDim.x + threadIdx.x, (int64_t)second * blockDim.x);
+  else
+    lay_codes(two, (int64_t)(blockIdx.x - second) * blockDim.x + threadIdx.x, (int64_t)(gridDim.x - second) * blockDim.x);
 }
 
 // A warp per row of the product: the codes and scale bytes of the row of x that its slot takes, side by side in the
 // order of the slots.
-__global__ void __launch_bounds__(256) k_gather_rows(const uint8_t* __restrict__ codes, const uint8_t* __restrict__ scales, int64_t pitch,
+__global__ void __launch_bounds__(256) k_gather_rows(const uint8_t* __restrict__ codes, const uint8_t* __restrict__ scales, int64_t pitch, int scales_pitch,
                                                      const int* __restrict__ order, int per, int x_rows, int64_t slots, int nb,
                                                      uint8_t* __restrict__ to_codes, uint8_t* __restrict__ to_scales) {
   start_next_grid();
@@ -81,7 +105,7 @@ __global__ void __launch_bounds__(256) k_gather_rows(const uint8_t* __restrict__
   uint4* b = reinterpret_cast<uint4*>(to_codes + r * pitch);
 #pragma unroll 4
   for (int64_t i = lane; i < pitch / 16; i += 32) b[i] = __ldg(a + i);
-  for (int i = lane; i < nb; i += 32) to_scales[r * nb + i] = __ldg(scales + from * nb + i);
+  for (int i = lane; i < nb; i += 32) to_scales[r * nb + i] = __ldg(scales + from * scales_pitch + i);
 }
 
 template <typename T>
@@ -97,7 +121,8 @@ __device__ __forceinline__ float to_float<__half>(__half v) { return __half2floa
 // type, 32 bits while the lanes are fewer than 2^31 (the division by the blocks of a row is what it is for).
 template <typename T, bool VEC, int FMT, typename I>
 __global__ void __launch_bounds__(256) k_pack_rows(const T* __restrict__ x, int64_t x_stride, uint8_t* __restrict__ codes,
-                                                   int64_t out_pitch, uint8_t* __restrict__ scales, int64_t rows, int64_t K) {
+                                                   int64_t out_pitch, uint8_t* __restrict__ scales, int64_t scales_pitch,
+                                                   int64_t rows, int64_t K) {
   start_next_grid();
   constexpr int N = 16;
   const I nb = (I)((K + 31) / 32), n = (I)(rows * (int64_t)nb * 2), stride = (I)gridDim.x * blockDim.x;
@@ -136,43 +161,69 @@ __global__ void __launch_bounds__(256) k_pack_rows(const T* __restrict__ x, int6
       q[j] = sb == 255u ? 0u : h[0] | h[1] << 16;      // a block with an Inf or a NaN: its scale says so
     }
     if (!live) continue;
-    if ((i & 1) == 0) scales[b] = (uint8_t)sb;
+    if ((i & 1) == 0) {
+      const int at = (int)(b - r * nb);
+      uint8_t* to = scales + (int64_t)r * scales_pitch;
+      to[at] = (uint8_t)sb;
+      if (at + 1 == (int)nb)                           // a pitch beyond the row is read as zeros
+        for (int64_t j = nb; j < scales_pitch; j++) to[j] = 0;
+    }
     if (c < out_pitch)                                 // the pitch is a multiple of 16, as c is
       *reinterpret_cast<uint4*>(codes + (int64_t)r * out_pitch + c) = make_uint4(q[0], q[1], q[2], q[3]);
   }
 }
 
 template <typename T, int FMT>
-int pack_rows(const void* x, int64_t x_stride, uint8_t* codes, int64_t out_pitch, uint8_t* scales, int64_t rows, int64_t K,
-              cudaStream_t st) {
+int pack_rows(const void* x, int64_t x_stride, uint8_t* codes, int64_t out_pitch, uint8_t* scales, int64_t scales_pitch, int64_t rows,
+              int64_t K, cudaStream_t st) {
   const int64_t n = rows * ((K + 31) / 32) * 2;
   const unsigned grid = grid_for(n, 256, 16);
   const bool vec = reinterpret_cast<uintptr_t>(x) % 16 == 0 && x_stride * (int64_t)sizeof(T) % 16 == 0;
   const bool small = n < (1ll << 31) - (int64_t)grid * 256 - 64;
   auto f = vec ? (small ? k_pack_rows<T, true, FMT, uint32_t> : k_pack_rows<T, true, FMT, int64_t>)
                : (small ? k_pack_rows<T, false, FMT, uint32_t> : k_pack_rows<T, false, FMT, int64_t>);
-  f<<<grid, 256, 0, st>>>(static_cast<const T*>(x), x_stride, codes, out_pitch, scales, rows, K);
+  f<<<grid, 256, 0, st>>>(static_cast<const T*>(x), x_stride, codes, out_pitch, scales, scales_pitch, rows, K);
   return MXQ_LAUNCH_CHECK("pack_rows");
 }
 template <typename T>
-int pack_rows(const void* x, int64_t x_stride, uint8_t* codes, int64_t out_pitch, uint8_t* scales, int64_t rows, int64_t K, int fmt,
-              cudaStream_t st) {
+int pack_rows(const void* x, int64_t x_stride, uint8_t* codes, int64_t out_pitch, uint8_t* scales, int64_t scales_pitch, int64_t rows,
+              int64_t K, int fmt, cudaStream_t st) {
   switch (fmt) {
-    case kFmtE4M3: return pack_rows<T, kFmtE4M3>(x, x_stride, codes, out_pitch, scales, rows, K, st);
-    case kFmtE5M2: return pack_rows<T, kFmtE5M2>(x, x_stride, codes, out_pitch, scales, rows, K, st);
-    case kFmtE3M2: return pack_rows<T, kFmtE3M2>(x, x_stride, codes, out_pitch, scales, rows, K, st);
-    case kFmtE2M3: return pack_rows<T, kFmtE2M3>(x, x_stride, codes, out_pitch, scales, rows, K, st);
-    default: return pack_rows<T, kFmtE2M1>(x, x_stride, codes, out_pitch, scales, rows, K, st);
+    case kFmtE4M3: return pack_rows<T, kFmtE4M3>(x, x_stride, codes, out_pitch, scales, scales_pitch, rows, K, st);
+    case kFmtE5M2: return pack_rows<T, kFmtE5M2>(x, x_stride, codes, out_pitch, scales, scales_pitch, rows, K, st);
+    case kFmtE3M2: return pack_rows<T, kFmtE3M2>(x, x_stride, codes, out_pitch, scales, scales_pitch, rows, K, st);
+    case kFmtE2M3: return pack_rows<T, kFmtE2M3>(x, x_stride, codes, out_pitch, scales, scales_pitch, rows, K, st);
+    default: return pack_rows<T, kFmtE2M1>(x, x_stride, codes, out_pitch, scales, scales_pitch, rows, K, st);
   }
 }
 
 }  // namespace
 
 namespace mxq {
-int gather_rows(const uint8_t* codes, const uint8_t* scales, int64_t pitch, const int* order, int per, int x_rows, int64_t slots, int nb,
-                uint8_t* to_codes, uint8_t* to_scales, cudaStream_t st) {
-  k_gather_rows<<<(unsigned)((slots + 7) / 8), 256, 0, st>>>(codes, scales, pitch, order, per, x_rows, slots, nb, to_codes, to_scales);
+int gather_rows(const uint8_t* codes, const uint8_t* scales, int64_t pitch, int scales_pitch, const int* order, int per, int x_rows,
+                int64_t slots, int nb, uint8_t* to_codes, uint8_t* to_scales, cudaStream_t st) {
+  k_gather_rows<<<(unsigned)((slots + 7) / 8), 256, 0, st>>>(codes, scales, pitch, scales_pitch, order, per, x_rows, slots, nb, to_codes, to_scales);
   return MXQ_LAUNCH_CHECK("gather_rows");
+}
+
+static unsigned lay_grid(const LayJob& j) {
+  return j.rows > 0 ? grid_for(j.rows * (j.out_pitch / 16), 256, 16) : 0u;     // a row has more codes than scales
+}
+int lay_rows(LayJob one, LayJob two, cudaStream_t st) {
+  const unsigned a = lay_grid(one), b = lay_grid(two);
+  if (a + b == 0) return MXQ_OK;
+  for (LayJob* j : {&one, &two}) j->vec = reinterpret_cast<uintptr_t>(j->codes) % 8 == 0 && j->pitch % 8 == 0;
+  k_lay_codes<<<a + b, 256, 0, st>>>(one, two, a);
+  return MXQ_LAUNCH_CHECK("lay_codes");
+}
+
+int pack_rows_to(const void* x, int type, int64_t x_stride, uint8_t* codes, int64_t out_pitch, uint8_t* scales, int64_t scales_pitch,
+                 int64_t rows, int64_t K, int fmt, cudaStream_t st) {
+  if (rows == 0) return MXQ_OK;
+  if (type == MXQ_OUT_F32) return pack_rows<float>(x, x_stride, codes, out_pitch, scales, scales_pitch, rows, K, fmt, st);
+  if (type == MXQ_OUT_BF16) return pack_rows<__nv_bfloat16>(x, x_stride, codes, out_pitch, scales, scales_pitch, rows, K, fmt, st);
+  if (type == MXQ_OUT_F16) return pack_rows<__half>(x, x_stride, codes, out_pitch, scales, scales_pitch, rows, K, fmt, st);
+  return set_error(MXQ_ERR_VALUE, "pack_rows: type %d", type);
 }
 }  // namespace mxq
 
@@ -183,10 +234,7 @@ extern "C" int mxq_lay_codes(const uint8_t* codes, int64_t in_pitch, uint8_t* ou
   MXQ_REQUIRE(rows >= 0 && K >= 1 && out_pitch >= K && out_pitch % 16 == 0 && reinterpret_cast<uintptr_t>(out) % 16 == 0,
               MXQ_ERR_VALUE, "lay_codes: rows %lld, K %lld, output pitch %lld", (long long)rows, (long long)K, (long long)out_pitch);
   MXQ_REQUIRE(fmt != kFmtE2M1 || K % 2 == 0, MXQ_ERR_VALUE, "lay_codes: FP4 codes pair up, K is %lld", (long long)K);
-  if (rows == 0) return MXQ_OK;
-  const int vec = reinterpret_cast<uintptr_t>(codes) % 8 == 0 && in_pitch % 8 == 0;
-  k_lay_codes<<<grid_for(rows * (out_pitch / 16), 256, 16), 256, 0, as_stream(stream)>>>(codes, in_pitch, out, out_pitch, rows, K, fmt, vec);
-  return MXQ_LAUNCH_CHECK("lay_codes");
+  return lay_rows({codes, in_pitch, out, out_pitch, rows, K, fmt, 0, nullptr, nullptr, 0}, {}, as_stream(stream));
 }
 
 extern "C" int mxq_pack_rows(const void* x, int32_t type, int64_t x_stride, uint8_t* codes, int64_t out_pitch, uint8_t* scales,
@@ -195,10 +243,5 @@ extern "C" int mxq_pack_rows(const void* x, int32_t type, int64_t x_stride, uint
   MXQ_REQUIRE(fmt != kFmtNone, MXQ_ERR_VALUE, "pack_rows: (e=%d, m=%d) is not an MX element format", e, m);
   MXQ_REQUIRE(rows >= 0 && K >= 1 && out_pitch >= K && out_pitch % 16 == 0 && reinterpret_cast<uintptr_t>(codes) % 16 == 0,
               MXQ_ERR_VALUE, "pack_rows: rows %lld, K %lld, output pitch %lld", (long long)rows, (long long)K, (long long)out_pitch);
-  if (rows == 0) return MXQ_OK;
-  cudaStream_t st = as_stream(stream);
-  if (type == MXQ_OUT_F32) return pack_rows<float>(x, x_stride, codes, out_pitch, scales, rows, K, fmt, st);
-  if (type == MXQ_OUT_BF16) return pack_rows<__nv_bfloat16>(x, x_stride, codes, out_pitch, scales, rows, K, fmt, st);
-  if (type == MXQ_OUT_F16) return pack_rows<__half>(x, x_stride, codes, out_pitch, scales, rows, K, fmt, st);
-  return set_error(MXQ_ERR_VALUE, "pack_rows: type %d", type);
+  return pack_rows_to(x, type, x_stride, codes, out_pitch, scales, (K + 31) / 32, rows, K, fmt, as_stream(stream));
 }

@@ -12,17 +12,13 @@
 //   k_mx_rows  128 rows of w by 16-64 rows of x per CTA, K split over a cluster, for few rows: reading w bounds it.
 #include "common.cuh"
 #include "mx_codes.cuh"
+#include "mx_layout.cuh"
 #include "tc.cuh"
 
 #include <cooperative_groups.h>
 
 namespace cg = cooperative_groups;
 using namespace mxq;
-
-namespace mxq {
-int gather_rows(const uint8_t* codes, const uint8_t* scales, int64_t pitch, const int* order, int per, int x_rows, int64_t slots, int nb,
-                uint8_t* to_codes, uint8_t* to_scales, cudaStream_t st);         // mx_layout.cu
-}
 
 namespace {
 
@@ -32,7 +28,8 @@ enum { kOutF32 = 0, kOutBf16, kOutF16, kOutPacked };
 struct Args {
   const uint8_t *sx, *sw;      // E8M0 bytes, nb per row
   int nb;
-  int vec;                     // scale bytes are read 16, 4 or 1 at a time (alignment and nb allow it)
+  int sx_pitch, sw_pitch;      // bytes between the rows of sx and sw; what is behind a row's nb is 0 or never read
+  int vec;                     // scale bytes are read 16, 4 or 1 at a time (alignment and the pitches allow it)
   const int32_t *offsets, *order;
   int experts;                 // 0: dense
   int per;                     // > 0: row r of the product is row order[r] / per of x
@@ -309,7 +306,7 @@ __device__ __forceinline__ int x_row(const Args& a, const Tile& t, int r) {
   return min(max(r, 0), a.xrows - 1);
 }
 __device__ __forceinline__ const uint8_t* w_scales(const Args& a, const Tile& t, int r) {
-  return a.sw + ((int64_t)t.expert * a.n + min(r, a.n - 1)) * a.nb;
+  return a.sw + ((int64_t)t.expert * a.n + min(r, a.n - 1)) * a.sw_pitch;
 }
 
 // ------------------------------------------------------------------------------------------------ many rows
@@ -627,7 +624,7 @@ __global__ void __launch_bounds__(128 + 32 * kWriters, 1) __cluster_dims__(2, 1,
 #pragma unroll
       for (int j = 0; j < 4; j++) {
         const int r = j * 32 + lane;
-        rows.row[j] = a.sx + (int64_t)x_row(a, t, rank * 128 + r) * a.nb;
+        rows.row[j] = a.sx + (int64_t)x_row(a, t, rank * 128 + r) * a.sx_pitch;
         rows.row[4 + j] = w_scales(a, t, t.col * kCols + r);
         rows.row[8 + j] = w_scales(a, t, t.col * kCols + r + second);
       }
@@ -1020,7 +1017,7 @@ __global__ void __launch_bounds__(128, 2) k_mx_rows(const __grid_constant__ CUte
     for (int j = 0; j < 4; j++) {
       const int r = j * 32 + lane;
       rows.row[j] = w_scales(a, t, t.col * kCols + (GATED && r >= 64 ? a.width + r - 64 : r));
-      rows.row[4 + j] = a.sx + (int64_t)x_row(a, t, r) * a.nb;
+      rows.row[4 + j] = a.sx + (int64_t)x_row(a, t, r) * a.sx_pitch;
     }
     Ring ring;
     uint4 now[8], nxt[8];
@@ -1244,30 +1241,41 @@ bool direct(const Given& o, int64_t K, bool gathered) {
   if (o.fmt == kFmtE4M3 || o.fmt == kFmtE5M2) return aligned(o.data, 16) && o.pitch % 16 == 0;
   return o.fmt == kFmtE2M1 && !gathered && aligned(o.data, 32) && o.pitch % 32 == 0 && K % 128 == 0;
 }
+// Scale rows of an operand that is laid out come to 16 bytes too where they are at odd bytes (63 of them a row, 777 x 1000:
+// the product takes 15 us instead of 18); rows of a word or less are one load either way.
+bool scales_at_odd_bytes(int64_t K) { return K > 128 && up_div(K, 32) % 4 != 0; }
+int64_t scales_pitch(int64_t K) { return scales_at_odd_bytes(K) ? up_div(K, 512) * 16 : up_div(K, 32); }
 int64_t room(const Given& o, int64_t K, bool gathered) {
   if (direct(o, K, gathered)) return 0;
-  return up_div(o.rows * codes_pitch(K) + (o.type > 0 ? o.rows * up_div(K, 32) : 0), 128) * 128;
+  const bool scales = o.type > 0 || scales_at_odd_bytes(K);
+  return up_div(o.rows * (codes_pitch(K) + (scales ? scales_pitch(K) : 0)), 128) * 128;
 }
 // rows in the plan's order, at any pitch that their codes may have
 int64_t sorted_room(int64_t rows, int64_t K) { return up_div(rows * (codes_pitch(K) + up_div(K, 32)), 128) * 128; }
-// The operand as the kernels read it, laid out in `at` (room() bytes) where need be
-int lay(const char* who, const char* what, const Given& o, int64_t K, bool gathered, uint8_t* at, Operand* out, const uint8_t** scales,
-        int* fmt, cudaStream_t st) {
+// The operand as the kernels read it, laid out in `at` (room() bytes) where need be: floats are packed by a launch here,
+// codes are left to the caller's `job`
+int lay(const Given& o, int64_t K, bool gathered, uint8_t* at, Operand* out, const uint8_t** scales, int* pitch_of_scales, int* fmt,
+        LayJob* job, cudaStream_t st) {
+  const bool odd = scales_at_odd_bytes(K);
+  *job = {};
   *scales = o.scales;
+  *pitch_of_scales = (int)up_div(K, 32);
   *fmt = o.fmt;
   if (direct(o, K, gathered)) {
     *out = {static_cast<const uint8_t*>(o.data), o.rows, o.pitch, o.fmt == kFmtE2M1};
     return MXQ_OK;
   }
   const int64_t pitch = codes_pitch(K);
-  int e, m;
-  exponent_mantissa(o.fmt, &e, &m);
   *out = {at, o.rows, pitch, false};
   if (o.fmt != kFmtE5M2) *fmt = kFmtE4M3;
-  if (o.type == 0) return mxq_lay_codes(static_cast<const uint8_t*>(o.data), o.pitch, at, pitch, o.rows, K, e, m, st);
   uint8_t* sc = at + o.rows * pitch;
-  *scales = sc;
-  return mxq_pack_rows(o.data, o.type - 1, o.pitch, at, pitch, sc, o.rows, K, e, m, st);
+  if (o.type > 0 || odd) {
+    *scales = sc;
+    *pitch_of_scales = (int)scales_pitch(K);
+  }
+  if (o.type > 0) return pack_rows_to(o.data, o.type - 1, o.pitch, at, pitch, sc, *pitch_of_scales, o.rows, K, o.fmt, st);
+  *job = {static_cast<const uint8_t*>(o.data), o.pitch, at, pitch, o.rows, K, o.fmt, 0, o.scales, odd ? sc : nullptr, *pitch_of_scales};
+  return MXQ_OK;
 }
 
 int check_operand(const char* who, const char* what, const Given& o, int64_t K) {
@@ -1322,21 +1330,25 @@ int product(const char* who, Args& a, const Given& gx, const Given& gw, int64_t 
   Operand x, w;
   int fmtx, fmtw;
   uint8_t* at = static_cast<uint8_t*>(workspace);
-  if (int rc = lay(who, "x", gx, K, a.per > 0, at, &x, &a.sx, &fmtx, st)) return rc;
-  if (int rc = lay(who, "w", gw, K, false, at + room_x, &w, &a.sw, &fmtw, st)) return rc;
+  LayJob lay_x, lay_w;
+  if (int rc = lay(gx, K, a.per > 0, at, &x, &a.sx, &a.sx_pitch, &fmtx, &lay_x, st)) return rc;
+  if (int rc = lay(gw, K, false, at + room_x, &w, &a.sw, &a.sw_pitch, &fmtw, &lay_w, st)) return rc;
+  if (int rc = lay_rows(lay_x, lay_w, st)) return rc;
   a.nb = (int)up_div(K, 32);
   if (sorted) {
     uint8_t* codes = at + room_x + room_w;
     uint8_t* scales = codes + a.rows * x.pitch;
-    if (int rc = gather_rows(x.codes, a.sx, x.pitch, a.order, a.per, a.xrows, a.rows, a.nb, codes, scales, st))
+    if (int rc = gather_rows(x.codes, a.sx, x.pitch, a.sx_pitch, a.order, a.per, a.xrows, a.rows, a.nb, codes, scales, st))
       return rc;
     x = {codes, a.rows, x.pitch, false};
     a.sx = scales;
+    a.sx_pitch = a.nb;
     a.xrows = a.rows;
     a.per = 0;
   }
   const int fx = mma_format(fmtx), fw = mma_format(fmtw);
-  a.vec = a.nb % 16 == 0 && aligned(a.sx, 16) && aligned(a.sw, 16) ? 16 : a.nb % 4 == 0 && aligned(a.sx, 4) && aligned(a.sw, 4) ? 4 : 1;
+  auto scales_by = [&](int n) { return a.sx_pitch % n == 0 && a.sw_pitch % n == 0 && aligned(a.sx, n) && aligned(a.sw, n); };
+  a.vec = scales_by(16) ? 16 : scales_by(4) ? 4 : 1;
   // a load of FP4 codes counts the bytes read, half of those that it fills
   a.xbytes = fmtx == kFmtE2M1 ? 64 : 128;
   a.wbytes = fmtw == kFmtE2M1 ? 64 : 128;

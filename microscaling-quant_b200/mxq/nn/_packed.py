@@ -88,6 +88,11 @@ def _direct(at: int, f: Format, K: int, gathered: bool = False) -> bool:
     return f.e + f.m == 3 and not gathered and K % 128 == 0 and at % 32 == 0
 
 
+def _room(rows: int, K: int) -> int:
+    """The bytes that laying out an operand takes at most: codes and scales at pitches of 16 bytes."""
+    return rows * ((K + 15 & -16) + (-(-K // BLOCK) + 15 & -16)) + 128
+
+
 def lay_packed(w: Pair, fmt: Union[str, Format]) -> Tuple[Pair, str]:
     """(w, fmt) such that the products read w as it is, once for weights that are kept: FP6 codes, and FP4 codes with K
     no multiple of 128, become the E4M3 codes of the same values. Rows that would not be multiples of 16 bytes cannot be
@@ -126,12 +131,12 @@ def _x_operand(x, x_fmt, who: str, w: torch.Tensor, gathered: bool = False):
         if v.stride(1) != 1 or (rows > 1 and stride < K):
             v = v.detach().contiguous()
             stride = K
-        room = rows * (-(-K // 16) * 16 + -(-K // BLOCK)) + 128
+        room = _room(rows, K)
         return v, None, stride, 1 + kind, f, room, shape[:-1], K, dev, x.device
     codes, scales, shape, K = _pair(x, f, who, "x")
     dev = codes.device if codes.is_cuda else _lib.device_for(codes, w)
     c, s = _here(codes, dev), _here(scales, dev)
-    room = 0 if _direct(c.data_ptr(), f, K, gathered) else c.numel() // shape[-1] * (-(-K // 16) * 16) + 128
+    room = 0 if _direct(c.data_ptr(), f, K, gathered) else _room(c.numel() // shape[-1], K)
     return c, s, shape[-1], 0, f, room, shape[:-1], K, dev, codes.device
 
 
@@ -145,7 +150,7 @@ _spec = _lib.cached(_make_spec)
 def _w_operand(wc, ws, shape, f: Format, K: int, dev):
     """(codes, scales, bytes of workspace) of w on dev."""
     c, s = _here(wc, dev), _here(ws, dev)
-    return c, s, 0 if _direct(c.data_ptr(), f, K) else c.numel() // shape[-1] * (-(-K // 16) * 16) + 128
+    return c, s, 0 if _direct(c.data_ptr(), f, K) else _room(c.numel() // shape[-1], K)
 
 
 def _plan_output(out, activation, N: int, who: str):

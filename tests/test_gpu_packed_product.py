@@ -231,6 +231,41 @@ def test_chained_calls(M):
         assert torch.equal(a, b)
 
 
+def test_laid_scales():
+    """Scale rows that are laid out with their codes: odd numbers of blocks, the workspace's bytes and the scales of the
+    next row all NaN's, one operand laid out or both, floats packed, rows of x in a plan's order."""
+    from mxq import nn
+    g = gen(31)
+    for K in (8, 40, 1000, 2008, 2009):
+        for M, N in ((1, 40), (70, 300), (600, 520)):
+            for xf, wf in (("MXFP8_E4M3", "MXFP8_E5M2"), ("MXFP6_E3M2", "MXFP8_E4M3"), ("MXFP8_E4M3", "MXFP6_E2M3")):
+                x, w = random_pair((M + 1, K), xf, g, DEV), random_pair((N + 1, K), wf, g, DEV)
+                x[1][M:] = 255
+                w[1][N:] = 255
+                part = (x[0][:M], x[1][:M]), (w[0][:N], w[1][:N])
+                torch.full((8 << 20,), 255, dtype=torch.uint8, device=DEV)               # what the allocator hands out next
+                check(part[0], xf, part[1], wf, what=f"{M} x {N} x {K} {xf} {wf}")
+            v = torch.randn(M, K, generator=g).to(DEV, torch.bfloat16)
+            torch.full((8 << 20,), 255, dtype=torch.uint8, device=DEV)
+            packed = nn.linear_packed(v, part[1], wf, x_fmt="MXFP8_E4M3", out=torch.float32)
+            assert torch.isfinite(packed).all()
+            aligned = torch.zeros(M, -(-K // 512) * 512, device=DEV, dtype=torch.bfloat16)     # the same values, nothing odd
+            aligned[:, :K] = v
+            wide = torch.zeros(N, aligned.shape[1], device=DEV, dtype=torch.uint8)
+            wide[:, :K] = part[1][0]
+            scales = torch.full((N, aligned.shape[1] // 32), 127, device=DEV, dtype=torch.uint8)
+            scales[:, :part[1][1].shape[1]] = part[1][1]
+            same = nn.linear_packed(aligned, (wide, scales), wf, x_fmt="MXFP8_E4M3", out=torch.float32)
+            S = product64(v.double().abs(), decode(part[1], wf).abs())[0]
+            # two sums of K values, the packed ones no more than twice the floats
+            assert_close(packed, same.double(), 2 * (K + 1) * 2.0 ** -23 * 2 * S, torch.float32, f"floats {M} x {N} x {K}")
+        for T in (6, 900):                               # few rows and many through a plan
+            experts = torch.randint(0, 5, (T, 3), generator=g).int()
+            x, w = random_pair((T, K), "MXFP8_E4M3", g, DEV), random_pair((5, 130, K), "MXFP6_E3M2", g, DEV)
+            torch.full((8 << 20,), 255, dtype=torch.uint8, device=DEV)
+            check_experts(x, "MXFP8_E4M3", w, "MXFP6_E3M2", experts, 5, True, what=f"plan {T} {K}")
+
+
 def test_output_beyond_32_bits():
     """More than 2^31 values of y: the last rows and columns are where they belong."""
     from mxq import nn
