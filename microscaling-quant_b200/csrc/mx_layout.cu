@@ -1,7 +1,8 @@
 // Operands of the packed products brought to the layout that the tensor maps take: codes of any MX format as 8-bit
 // codes at a pitch of 16 bytes (k_lay_codes), and float rows packed on the way in (k_pack_rows). Both read their
 // input once and write their output once; they are bound by those bytes. 8192 x 8192: packing float32 50 us (6.7
-// TB/s), bf16 33 us (6.1); FP6 codes laid out 24 us (5.7), FP4 22 us (4.5), E4M3 rows of 8184 28 us (4.8).
+// TB/s), bf16 33 us (6.1); FP6 codes laid out 22.5 us (6.0; 24 with 64-bit indexes), FP4 21 us (4.9; 24), E4M3 rows of 8184
+// 27 us (4.9; 28.5).
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 
@@ -33,15 +34,20 @@ __device__ __forceinline__ uint32_t lay4(const uint8_t* in, int64_t c, int64_t K
 
 // A thread per 16 codes of the output; its place beyond K is written as zeros (the tensor map never reads it). Then, for
 // scale rows that are brought to a pitch of 16 bytes too, a thread per 16 of their bytes: zeros beyond the row, which
-// the products do read.
-__device__ __forceinline__ void lay_codes(const LayJob& job, int64_t first, int64_t stride) {
-  const int64_t K = job.K, per = job.out_pitch >> 4, n = job.rows * per;
-  const int fmt = job.fmt;
-  for (int64_t i = first; i < n; i += stride) {
-    const int64_t r = i / per, c = (i - r * per) << 4;
-    const uint8_t* row = job.codes + r * job.pitch;
+// the products do read. I: the index type, 32 bits while the threads' work is less than 2^31 (for the division).
+template <typename I>
+__device__ __forceinline__ void lay_codes(const LayJob& job, I first, I stride) {
+  const int64_t K = job.K, pitch = job.pitch, out_pitch = job.out_pitch;
+  const I per = (I)(out_pitch >> 4), n = (I)job.rows * per;
+  const int fmt = job.fmt, vec = job.vec;
+  const uint8_t* __restrict__ codes = job.codes;
+  uint8_t* __restrict__ to_codes = job.to_codes;
+  for (I i = first; i < n; i += stride) {
+    const I at = i / per;
+    const int64_t r = at, c = (int64_t)(i - at * per) << 4;
+    const uint8_t* row = codes + r * pitch;
     uint32_t w[4];
-    if (job.vec && c + 16 <= K) {                      // the row's words are aligned: 16 codes in one or two loads
+    if (vec && c + 16 <= K) {                      // the row's words are aligned: 16 codes in one or two loads
       if (fmt == kFmtE2M1) {
         const uint2 q = __ldg(reinterpret_cast<const uint2*>(row + (c >> 1)));
         w[0] = widen2(fmt, q.x & 255u) | widen2(fmt, (q.x >> 8) & 255u) << 16;
@@ -63,14 +69,14 @@ __device__ __forceinline__ void lay_codes(const LayJob& job, int64_t first, int6
 #pragma unroll
       for (int j = 0; j < 4; j++) w[j] = c + 4 * j < K ? lay4(row, c + 4 * j, K, fmt) : 0u;
     }
-    *reinterpret_cast<uint4*>(job.to_codes + r * job.out_pitch + c) = make_uint4(w[0], w[1], w[2], w[3]);
+    *reinterpret_cast<uint4*>(to_codes + r * out_pitch + c) = make_uint4(w[0], w[1], w[2], w[3]);
   }
   if (job.to_scales == nullptr) return;
   const int nb = (int)((K + 31) / 32);
-  const int64_t groups = job.scales_pitch >> 4, m = job.rows * groups;
-  for (int64_t i = first; i < m; i += stride) {
+  const I groups = (I)(job.scales_pitch >> 4), m = (I)job.rows * groups;
+  for (I i = first; i < m; i += stride) {
     const int64_t r = i / groups;
-    const int at = (int)(i - r * groups) << 4;
+    const int at = (int)(i - (I)r * groups) << 4;
     const uint8_t* row = job.scales + r * nb;
     uint32_t w[4] = {0u, 0u, 0u, 0u};
 #pragma unroll
@@ -81,18 +87,19 @@ __device__ __forceinline__ void lay_codes(const LayJob& job, int64_t first, int6
 }
 
 // one or two operands in one launch: the blocks from `second` on take the other
+template <typename I>
 __global__ void __launch_bounds__(256) k_lay_codes(LayJob one, LayJob two, unsigned second) {
   start_next_grid();
   if (blockIdx.x < second)
-    lay_codes(one, (int64_t)blockIdx.x * blockDim.x + threadIdx.x, (int64_t)second * blockDim.x);
+    lay_codes<I>(one, (I)blockIdx.x * blockDim.x + threadIdx.x, (I)second * blockDim.x);
   else
-    lay_codes(two, (int64_t)(blockIdx.x - second) * blockDim.x + threadIdx.x, (int64_t)(gridDim.x - second) * blockDim.x);
+    lay_codes<I>(two, (I)(blockIdx.x - second) * blockDim.x + threadIdx.x, (I)(gridDim.x - second) * blockDim.x);
 }
 
 // A warp per row of the product: the codes and scale bytes of the row of x that its slot takes, side by side in the
 // order of the slots.
-__global__ void __launch_bounds__(256) k_gather_rows(const uint8_t* __restrict__ codes, const uint8_t* __restrict__ scales, int64_t pitch, int scales_pitch,
-                                                     const int* __restrict__ order, int per, int x_rows, int64_t slots, int nb,
+__global__ void __launch_bounds__(256) k_gather_rows(const uint8_t* __restrict__ codes, const uint8_t* __restrict__ scales, int64_t pitch,
+                                                     int scales_pitch, const int* __restrict__ order, int per, int x_rows, int64_t slots, int nb,
                                                      uint8_t* __restrict__ to_codes, uint8_t* __restrict__ to_scales) {
   start_next_grid();
   const int64_t r = ((int64_t)blockIdx.x * blockDim.x + threadIdx.x) >> 5;
@@ -162,11 +169,15 @@ __global__ void __launch_bounds__(256) k_pack_rows(const T* __restrict__ x, int6
     }
     if (!live) continue;
     if ((i & 1) == 0) {
-      const int at = (int)(b - r * nb);
-      uint8_t* to = scales + (int64_t)r * scales_pitch;
-      to[at] = (uint8_t)sb;
-      if (at + 1 == (int)nb)                           // a pitch beyond the row is read as zeros
-        for (int64_t j = nb; j < scales_pitch; j++) to[j] = 0;
+      if (scales_pitch == (int64_t)nb) {
+        scales[b] = (uint8_t)sb;
+      } else {                                         // a pitch beyond the row is read as zeros
+        const int at = (int)(b - r * nb);
+        uint8_t* to = scales + (int64_t)r * scales_pitch;
+        to[at] = (uint8_t)sb;
+        if (at + 1 == (int)nb)
+          for (int64_t j = nb; j < scales_pitch; j++) to[j] = 0;
+      }
     }
     if (c < out_pitch)                                 // the pitch is a multiple of 16, as c is
       *reinterpret_cast<uint4*>(codes + (int64_t)r * out_pitch + c) = make_uint4(q[0], q[1], q[2], q[3]);
@@ -202,7 +213,8 @@ int pack_rows(const void* x, int64_t x_stride, uint8_t* codes, int64_t out_pitch
 namespace mxq {
 int gather_rows(const uint8_t* codes, const uint8_t* scales, int64_t pitch, int scales_pitch, const int* order, int per, int x_rows,
                 int64_t slots, int nb, uint8_t* to_codes, uint8_t* to_scales, cudaStream_t st) {
-  k_gather_rows<<<(unsigned)((slots + 7) / 8), 256, 0, st>>>(codes, scales, pitch, scales_pitch, order, per, x_rows, slots, nb, to_codes, to_scales);
+  k_gather_rows<<<(unsigned)((slots + 7) / 8), 256, 0, st>>>(codes, scales, pitch, scales_pitch, order, per, x_rows, slots, nb, to_codes,
+                                                             to_scales);
   return MXQ_LAUNCH_CHECK("gather_rows");
 }
 
@@ -213,7 +225,9 @@ int lay_rows(LayJob one, LayJob two, cudaStream_t st) {
   const unsigned a = lay_grid(one), b = lay_grid(two);
   if (a + b == 0) return MXQ_OK;
   for (LayJob* j : {&one, &two}) j->vec = reinterpret_cast<uintptr_t>(j->codes) % 8 == 0 && j->pitch % 8 == 0;
-  k_lay_codes<<<a + b, 256, 0, st>>>(one, two, a);
+  const int64_t most = (one.rows * one.out_pitch > two.rows * two.out_pitch ? one.rows * one.out_pitch : two.rows * two.out_pitch) / 16;
+  auto f = most < (1ll << 31) - (int64_t)(a + b) * 256 ? k_lay_codes<uint32_t> : k_lay_codes<int64_t>;
+  f<<<a + b, 256, 0, st>>>(one, two, a);
   return MXQ_LAUNCH_CHECK("lay_codes");
 }
 
