@@ -97,10 +97,12 @@ __global__ void __launch_bounds__(256) k_lay_codes(LayJob one, LayJob two, unsig
 }
 
 // A warp per row of the product: the codes and scale bytes of the row of x that its slot takes, side by side in the
-// order of the slots.
+// order of the slots. x's rows may be any multiple of 16 bytes apart; of each only its K codes are read (the last row may end
+// the caller's memory), and they are written at a pitch of their own, zeros up to it.
 __global__ void __launch_bounds__(256) k_gather_rows(const uint8_t* __restrict__ codes, const uint8_t* __restrict__ scales, int64_t pitch,
-                                                     int scales_pitch, const int* __restrict__ order, int per, int x_rows, int64_t slots, int nb,
-                                                     uint8_t* __restrict__ to_codes, uint8_t* __restrict__ to_scales) {
+                                                     int scales_pitch, const int* __restrict__ order, int per, int x_rows, int64_t slots,
+                                                     int64_t K, int nb, uint8_t* __restrict__ to_codes, int64_t to_pitch,
+                                                     uint8_t* __restrict__ to_scales) {
   start_next_grid();
   const int64_t r = ((int64_t)blockIdx.x * blockDim.x + threadIdx.x) >> 5;
   const int lane = threadIdx.x & 31;
@@ -109,9 +111,13 @@ __global__ void __launch_bounds__(256) k_gather_rows(const uint8_t* __restrict__
   if (slot < 0) return;                                // a place without a slot: nobody reads it
   const int64_t from = min(slot / per, x_rows - 1);
   const uint4* a = reinterpret_cast<const uint4*>(codes + from * pitch);
-  uint4* b = reinterpret_cast<uint4*>(to_codes + r * pitch);
+  uint4* b = reinterpret_cast<uint4*>(to_codes + r * to_pitch);
 #pragma unroll 4
-  for (int64_t i = lane; i < pitch / 16; i += 32) b[i] = __ldg(a + i);
+  for (int64_t i = lane; i < K / 16; i += 32) b[i] = __ldg(a + i);
+  if (const int left = (int)(K % 16)) {                // the last piece, byte by byte
+    const int64_t at = K - left;
+    if (lane < 16) to_codes[r * to_pitch + at + lane] = lane < left ? __ldg(codes + from * pitch + at + lane) : (uint8_t)0;
+  }
   for (int i = lane; i < nb; i += 32) to_scales[r * nb + i] = __ldg(scales + from * scales_pitch + i);
 }
 
@@ -212,9 +218,9 @@ int pack_rows(const void* x, int64_t x_stride, uint8_t* codes, int64_t out_pitch
 
 namespace mxq {
 int gather_rows(const uint8_t* codes, const uint8_t* scales, int64_t pitch, int scales_pitch, const int* order, int per, int x_rows,
-                int64_t slots, int nb, uint8_t* to_codes, uint8_t* to_scales, cudaStream_t st) {
-  k_gather_rows<<<(unsigned)((slots + 7) / 8), 256, 0, st>>>(codes, scales, pitch, scales_pitch, order, per, x_rows, slots, nb, to_codes,
-                                                             to_scales);
+                int64_t slots, int64_t K, uint8_t* to_codes, int64_t to_pitch, uint8_t* to_scales, cudaStream_t st) {
+  k_gather_rows<<<(unsigned)((slots + 7) / 8), 256, 0, st>>>(codes, scales, pitch, scales_pitch, order, per, x_rows, slots, K,
+                                                             (int)((K + 31) / 32), to_codes, to_pitch, to_scales);
   return MXQ_LAUNCH_CHECK("gather_rows");
 }
 

@@ -25,8 +25,9 @@ int lay_rows(LayJob one, LayJob two, cudaStream_t st);
 int pack_rows_to(const void* x, int type, int64_t x_stride, uint8_t* codes, int64_t out_pitch, uint8_t* scales, int64_t scales_pitch,
                  int64_t rows, int64_t K, int fmt, cudaStream_t st);
 
-// The rows of x that the slots of a plan take, in the plan's order; nb scale bytes a row.
+// The rows of x that the slots of a plan take, in the plan's order: K codes of each to a pitch of their own (a multiple of 16
+// and at least K; zeros up to the next multiple of 16), ceil(K / 32) scale bytes side by side.
 int gather_rows(const uint8_t* codes, const uint8_t* scales, int64_t pitch, int scales_pitch, const int* order, int per, int x_rows,
-                int64_t slots, int nb, uint8_t* to_codes, uint8_t* to_scales, cudaStream_t st);
+                int64_t slots, int64_t K, uint8_t* to_codes, int64_t to_pitch, uint8_t* to_scales, cudaStream_t st);
 
 }  // namespace mxq

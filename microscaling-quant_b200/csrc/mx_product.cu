@@ -1250,7 +1250,7 @@ int64_t room(const Given& o, int64_t K, bool gathered) {
   const bool scales = o.type > 0 || scales_at_odd_bytes(K);
   return up_div(o.rows * (codes_pitch(K) + (scales ? scales_pitch(K) : 0)), 128) * 128;
 }
-// rows in the plan's order, at any pitch that their codes may have
+// rows in the plan's order: their codes at codes_pitch(K), whatever the pitch of x, then their scales
 int64_t sorted_room(int64_t rows, int64_t K) { return up_div(rows * (codes_pitch(K) + up_div(K, 32)), 128) * 128; }
 // The operand as the kernels read it, laid out in `at` (room() bytes) where need be: floats are packed by a launch here,
 // codes are left to the caller's `job`
@@ -1337,10 +1337,10 @@ int product(const char* who, Args& a, const Given& gx, const Given& gw, int64_t 
   a.nb = (int)up_div(K, 32);
   if (sorted) {
     uint8_t* codes = at + room_x + room_w;
-    uint8_t* scales = codes + a.rows * x.pitch;
-    if (int rc = gather_rows(x.codes, a.sx, x.pitch, a.sx_pitch, a.order, a.per, a.xrows, a.rows, a.nb, codes, scales, st))
-      return rc;
-    x = {codes, a.rows, x.pitch, false};
+    const int64_t pitch = codes_pitch(K);
+    uint8_t* scales = codes + a.rows * pitch;
+    if (int rc = gather_rows(x.codes, a.sx, x.pitch, a.sx_pitch, a.order, a.per, a.xrows, a.rows, K, codes, pitch, scales, st)) return rc;
+    x = {codes, a.rows, pitch, false};
     a.sx = scales;
     a.sx_pitch = a.nb;
     a.xrows = a.rows;
