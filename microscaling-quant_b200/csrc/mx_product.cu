@@ -693,7 +693,7 @@ __global__ void __launch_bounds__(128 + 32 * kWriters, 1) __cluster_dims__(2, 1,
         if (!a.residual || rows <= 0 || col >= a.width) return;
         if (a.map_out) stage_free();
         get_rows(stage, static_cast<const uint8_t*>(a.residual) + (row * a.residual_stride + col) * size, a.residual_stride * size,
-                   rows, min(128, (a.width - col) * size), size, a.vec_out);
+                   rows, min(128 / size, a.width - col) * size, size, a.vec_out);
       };
       // a unit's biases: column lane and column 32 + lane, of the gates and of the ups
       const float* bias = a.bias ? a.bias + (int64_t)t.expert * a.n : nullptr;
@@ -1148,9 +1148,9 @@ int launch_tile(Args& a, const Operand& x, const Operand& w, int64_t K, int64_t 
   CUtensorMap mx, mw, my;
   if (int rc = map_of(&mx, x, K, 128)) return rc;
   if (int rc = map_of(&mw, w, K, 128)) return rc;
-  // y as bytes, in the stage's rows of 128
+  // y as bytes, in the stage's rows of 128; a tile's first byte in its row is a 32-bit coordinate
   const int size = OUT == kOutF32 ? 4 : 2;
-  a.map_out = OUT != kOutPacked && a.vec_out;
+  a.map_out = OUT != kOutPacked && a.vec_out && (int64_t)a.width * size < (1ll << 31);
   my = mx;
   if (a.map_out)
     if (int rc = encode_tmap_codes(&my, a.out, false, (uint64_t)a.rows, (uint64_t)a.width * size, (uint64_t)a.out_pitch * size, 32)) return rc;

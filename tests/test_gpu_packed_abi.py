@@ -41,3 +41,24 @@ def test_pitched_rows_through_a_plan(K, pitch, T, k, E):
               _lib.stream(y.device))
     assert (space[need:] == 0xa5).all()
     assert torch.equal(y[:live], want[:live])
+
+
+@pytest.mark.parametrize("residual", [False, True])
+def test_rows_of_more_than_2_31_bytes(residual):
+    """Float32 rows of y whose bytes pass 32 bits: every column is where it belongs, the residual's too."""
+    from mxq import nn
+    M, N, K = 2, (1 << 29) + 320, 32
+    x = (torch.full((M, K), 0x38, dtype=torch.uint8, device=DEV), torch.full((M, 1), 127, dtype=torch.uint8, device=DEV))    # ones
+    w = (torch.zeros(N, K, dtype=torch.uint8, device=DEV), torch.full((N, 1), 127, dtype=torch.uint8, device=DEV))
+    at = torch.tensor([0, 77, 1 << 28, (1 << 29) - 1, 1 << 29, (1 << 29) + 33, N - 1], device=DEV)
+    w[0][at] = 0x38
+    r = torch.zeros(M, N, device=DEV) if residual else None
+    if residual:
+        r[1, at] = torch.arange(1, 8, dtype=torch.float32, device=DEV)
+        r[0, N - 65] = 5.0
+    y = nn.linear_packed(x, w, "MXFP8_E4M3", residual=r, out=torch.float32)
+    assert (y[0, at] == K).all()
+    assert torch.equal(y[1, at], K + torch.arange(1, 8, device=DEV) * float(residual))
+    assert int(y.count_nonzero()) == 14 + int(residual)
+    if residual:
+        assert y[0, N - 65] == 5.0
