@@ -713,7 +713,11 @@ __global__ void __launch_bounds__(128 + 32 * kWriters, 1) __cluster_dims__(2, 1,
       __syncwarp();
       tc::fence_after();
       // the second warps' word that they are through with the tile before; the first warps give theirs below
-      if (set == 1 && lane == 0) tc::mbar_arrive_remote(acc_free);
+      if (set == 1) {
+        tc::fence_before();                            // their loads of that tile come before the word
+        __syncwarp();
+        if (lane == 0) tc::mbar_arrive_remote(acc_free);
+      }
       const uint32_t acc = tmem + (done & 1 ? 192 : 0) + ((uint32_t)(q * 32) << 16);
 #pragma unroll 1
       for (int u = 0; u < kUnits / 2; u++) {
