@@ -180,16 +180,21 @@ struct ScaleRows {
     for (int i = 0; i < 4 * G; i++) v[i] = load_scales(row[i], g, a.nb, a.vec);
   }
 };
-// step j of the four that v holds, into the ring's next stage
+// step j of the four that v holds, to its place in the layout
 template <int G>
-__device__ __forceinline__ bool store_scales(const uint4 (&v)[4 * G], int j, const Args& a, uint8_t* area, int pitch, uint64_t* ready,
-                                             uint64_t* empty, Ring& ring, int stages, const tc::Guard& guard) {
-  if (!tc::wait_warp(&empty[ring.stage], ring.phase ^ 1u, guard)) return false;
-  uint8_t* to = area + (size_t)ring.stage * pitch + (threadIdx.x & 31) * 16;
+__device__ __forceinline__ void put_words(const uint4 (&v)[4 * G], int j, uint8_t* to) {
   auto word = [j](const uint4& q) { return j == 0 ? q.x : j == 1 ? q.y : j == 2 ? q.z : q.w; };
 #pragma unroll
   for (int i = 0; i < G; i++)
-    *reinterpret_cast<uint4*>(to + 512 * i) = make_uint4(word(v[4 * i]), word(v[4 * i + 1]), word(v[4 * i + 2]), word(v[4 * i + 3]));
+    *reinterpret_cast<uint4*>(to + (threadIdx.x & 31) * 16 + 512 * i) =
+        make_uint4(word(v[4 * i]), word(v[4 * i + 1]), word(v[4 * i + 2]), word(v[4 * i + 3]));
+}
+// the same into the ring's next stage
+template <int G>
+__device__ __forceinline__ bool store_scales(const uint4 (&v)[4 * G], int j, const Args& a, uint8_t* area, int pitch, uint64_t* ready,
+                                             uint64_t* empty, Ring& ring, int stages, const tc::Guard& guard) {
+  if (!tc::wait_warp<false>(&empty[ring.stage], ring.phase ^ 1u, guard)) return false;
+  put_words<G>(v, j, area + (size_t)ring.stage * pitch);
   __syncwarp();
   if (tc::elect()) tc::mbar_arrive(&ready[ring.stage]);
   ring.next(stages);
@@ -197,10 +202,10 @@ __device__ __forceinline__ bool store_scales(const uint4 (&v)[4 * G], int j, con
 }
 // The words' way from the loader to the tensor core's view of shared memory, in a warp of its own: the fence waits
 // for all that its thread has under way, and the loader has the next loads under way. far: the full barriers'
-// shared::cluster address where they are in another CTA, else 0.
-__device__ __forceinline__ bool forward_scales(const Args& a, uint64_t* ready, uint64_t* full, uint32_t far, Ring& ring, int stages,
-                                               const tc::Guard& guard) {
-  if (!tc::wait_warp(&ready[ring.stage], ring.phase, guard)) return false;
+// shared::cluster address where they are in another CTA, else 0. Then the words are released to the cluster, which waits for
+// everything that the SM has under way, about 1900 cycles a time.
+__device__ __forceinline__ bool forward_scales(uint64_t* ready, uint64_t* full, uint32_t far, Ring& ring, int stages, const tc::Guard& guard) {
+  if (!tc::wait_warp<false>(&ready[ring.stage], ring.phase, guard)) return false;
   if (tc::elect()) {
     fence_proxy_async();
     if (far) tc::mbar_arrive_remote(far + 8u * ring.stage);
@@ -316,16 +321,22 @@ __device__ __forceinline__ const uint8_t* w_scales(const Args& a, const Tile& t,
 // 128; as a pair both are 128.
 constexpr int kStages = 5;
 constexpr int kStageBytes = 2 * kTileBytes;
-constexpr int kStageScales = 3 * 512;                  // x's 128 rows, all of w's 256
+// The scales come in groups of four steps (16 bytes of a row), in a ring of their own: the second CTA's words have to be
+// released to the cluster, and a release for every step (about 1900 cycles, against the 512 of its products) doubled
+// the kernel's time.
+constexpr int kGroups = 4;
+constexpr int kStepScales = 3 * 512;                   // x's 128 rows, all of w's 256
+constexpr int kGroupScales = 4 * kStepScales;
 constexpr int kWriters = 8;                            // epilogue warps
 constexpr int kPassBytes = 32 * 128;                   // what one of them stages: 32 rows of 128 bytes
 
 struct TileShared {
-  uint64_t full[kStages], empty[kStages], ready[kStages], acc_full, acc_free, last;
+  uint64_t full[kStages], empty[kStages], acc_full, acc_free, last;
+  uint64_t scales_ready[kGroups], scales_full[kGroups], scales_empty[kGroups];
   uint32_t tmem;
   int abort;
 };
-constexpr int kTileSmem = 1024 + kStages * (kStageBytes + kStageScales) + kWriters * kPassBytes + (int)sizeof(TileShared);
+constexpr int kTileSmem = 1024 + kStages * kStageBytes + kGroups * kGroupScales + kWriters * kPassBytes + (int)sizeof(TileShared);
 
 // place of 16-byte piece j of a staged row: neighbouring rows in other banks
 __device__ __forceinline__ uint8_t* piece(uint8_t* stage, int row, int j) { return stage + row * 128 + ((j ^ (row & 7)) << 4); }
@@ -488,8 +499,8 @@ __device__ __forceinline__ void add_bias(float mine, float (&y)[32]) {
   for (int j = 0; j < 32; j++) y[j] += __shfl_sync(~0u, mine, j);
 }
 
-// Warp 0 loads the codes, warp 1 of the pair's first CTA issues the products, warps 2 and 3 bring the scales, warps
-// 4-11 write y: two per lane quarter, each with units of 64 columns.
+// Warp 0 loads the codes, warp 1 of the pair's first CTA issues the products, warps 2 and 3 bring the scales (in the second
+// CTA warp 1 too), warps 4-11 write y: two per lane quarter, each with units of 64 columns.
 //
 // Measured (E4M3, bf16 y): 8192 x 8192 x 8192 436 us in a burst (2.52 PFLOP/s), 505 us back to back at the 1250 MHz
 // that the power limit leaves. A step of 128 along K takes its products' 512 cycles once the ring is full; a tile
@@ -508,7 +519,7 @@ __global__ void __launch_bounds__(128 + 32 * kWriters, 1) __cluster_dims__(2, 1,
   uint8_t* codes = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(raw) + 1023) & ~(uintptr_t)1023);
   uint8_t* passes = codes + kStages * kStageBytes;     // multiples of 1024 bytes, as the swizzle wants them
   uint8_t* scales = passes + kWriters * kPassBytes;
-  TileShared& sh = *reinterpret_cast<TileShared*>(scales + kStages * kStageScales);
+  TileShared& sh = *reinterpret_cast<TileShared*>(scales + kGroups * kGroupScales);
   const Table tab(&sh + 1, a.experts);
   const tc::Guard guard = {&sh.abort, a.status, a.wait_cycles};
   const int warp = __shfl_sync(~0u, threadIdx.x >> 5, 0), lane = threadIdx.x & 31;
@@ -519,9 +530,13 @@ __global__ void __launch_bounds__(128 + 32 * kWriters, 1) __cluster_dims__(2, 1,
 
   if (threadIdx.x == 0) {
     for (int i = 0; i < kStages; i++) {
-      mbar_init(&sh.full[i], 3);                       // the first CTA's: the codes' bytes, both CTAs' scales
+      mbar_init(&sh.full[i], 1);                       // the first CTA's: the codes' bytes, both CTAs'
       mbar_init(&sh.empty[i], 1);
-      mbar_init(&sh.ready[i], 1);
+    }
+    for (int i = 0; i < kGroups; i++) {
+      mbar_init(&sh.scales_ready[i], 1);
+      mbar_init(&sh.scales_full[i], 2);                // the first CTA's: both CTAs'
+      mbar_init(&sh.scales_empty[i], 1);
     }
     mbar_init(&sh.acc_full, 1);
     mbar_init(&sh.acc_free, 2 * kWriters);             // the first CTA's: both CTAs' epilogue warps
@@ -545,6 +560,18 @@ __global__ void __launch_bounds__(128 + 32 * kWriters, 1) __cluster_dims__(2, 1,
   const int tiles = tile_count(a, tab, 256, col_tiles);
   // the second half of a tile's w rows: the up projections, or the next 128 features
   const int second = GATED ? a.width : 128;
+  // groups of scales `from`, from + step, ... on their way to the tensor core; the second CTA's by two warps in turn, so that
+  // one's release passes beside the other's
+  auto forward = [&](int from, int step) {
+    const int per = (a.kblocks + 3) >> 2, groups = pair < tiles ? ((tiles - 1 - pair) / pairs + 1) * per : 0;
+    const uint32_t far = rank ? tc::remote(sh.scales_full, 0) : 0u;
+    Ring ring;
+    if (from) ring.next(kGroups);
+    for (int g = from; g < groups; g += step) {
+      if (!forward_scales(sh.scales_ready, sh.scales_full, far, ring, kGroups, guard)) break;
+      if (step == 2) ring.next(kGroups);
+    }
+  };
 
   if (warp == 0) {
     Ring ring;
@@ -555,7 +582,7 @@ __global__ void __launch_bounds__(128 + 32 * kWriters, 1) __cluster_dims__(2, 1,
       const Tile t = list.next(i, pairs, tiles, a, tab, 256, col_tiles);
       const int w0 = t.expert * a.n + t.col * kCols + (rank ? second : 0);
       for (int kb = 0; kb < a.kblocks; kb++) {
-        ok = tc::wait_warp(&sh.empty[ring.stage], ring.phase ^ 1u, guard);
+        ok = tc::wait_warp<true>(&sh.empty[ring.stage], ring.phase ^ 1u, guard);
         if (!ok) break;
         uint8_t* to = codes + ring.stage * kStageBytes;
         const uint32_t bar = full + 8u * ring.stage;
@@ -576,19 +603,21 @@ __global__ void __launch_bounds__(128 + 32 * kWriters, 1) __cluster_dims__(2, 1,
       }
   } else if (warp == 1) {
     if (rank == 0) {
-      Ring ring;
+      Ring ring, group;
       bool ok = true;
       int done = 0;
       for (int i = pair; ok && i < tiles; i += pairs, done++) {
-        if (done) ok = tc::wait_warp(&sh.acc_free, (done - 1) & 1, guard);
+        if (done) ok = tc::wait_warp<true>(&sh.acc_free, (done - 1) & 1, guard);
         if (!ok) break;
         const uint32_t acc = tmem + (done & 1 ? 192 : 0);
         for (int kb = 0; kb < a.kblocks; kb++) {
-          ok = tc::wait_warp(&sh.full[ring.stage], ring.phase, guard);
+          ok = ((kb & 3) || tc::wait_warp<true>(&sh.scales_full[group.stage], group.phase, guard)) &&
+               tc::wait_warp<true>(&sh.full[ring.stage], ring.phase, guard);
           if (!ok) break;
           tc::fence_after();
           const uint32_t at = smem_addr(codes + ring.stage * kStageBytes);
-          const uint32_t sc = smem_addr(scales + ring.stage * kStageScales);
+          const uint32_t sc = smem_addr(scales + group.stage * kGroupScales + (kb & 3) * kStepScales);
+          const bool last = kb == a.kblocks - 1;
           const uint32_t ts = tmem + 448 + ring.stage * 12;
           const uint64_t da = tc::operand_desc(at), db = tc::operand_desc(at + kTileBytes);
           if (tc::elect()) {
@@ -598,28 +627,31 @@ __global__ void __launch_bounds__(128 + 32 * kWriters, 1) __cluster_dims__(2, 1,
             for (int j = 0; j < 4; j++)                // 32 codes further: 2 units of 16 bytes
               tc::mma<true>(acc, da + 2 * j, db + 2 * j, tc::mma_desc_step(a.idesc, j), ts, ts + 4, kb > 0 || j > 0);
             tc::commit<true>(&sh.empty[ring.stage]);
-            if (kb == a.kblocks - 1) tc::commit<true>(&sh.acc_full);
+            if (last || (kb & 3) == 3) tc::commit<true>(&sh.scales_empty[group.stage]);
+            if (last) tc::commit<true>(&sh.acc_full);
           }
           __syncwarp();
           ring.next(kStages);
+          if (last || (kb & 3) == 3) group.next(kGroups);
         }
       }
       if (!ok && tc::elect()) {
         tc::commit<true>(&sh.last);
         tc::settle(&sh.last, 0, guard);
       }
+    } else {
+      forward(1, 2);
     }
   } else if (warp == 2) {
-    // x's 128 rows and w's 256. The next four steps' words are on their way while these are stored, over the ends of
-    // the tiles too.
-    const int groups = (a.kblocks + 3) >> 2;
+    // x's 128 rows and w's 256. A group's words are on their way while the groups before them wait for their turn, over the
+    // ends of the tiles too.
+    const int per = (a.kblocks + 3) >> 2;
     ScaleRows<3> rows;
-    uint4 now[12], nxt[12];
+    uint4 v[12];
     Ring ring;
     Tiles list;
-    int i = pair, g = 0;
-    auto aim = [&] {                                   // the rows of tile i
-      if (i >= tiles) return false;
+    bool ok = true;
+    for (int i = pair; ok && i < tiles; i += pairs) {
       const Tile t = list.next(i, pairs, tiles, a, tab, 256, col_tiles);
 #pragma unroll
       for (int j = 0; j < 4; j++) {
@@ -628,31 +660,20 @@ __global__ void __launch_bounds__(128 + 32 * kWriters, 1) __cluster_dims__(2, 1,
         rows.row[4 + j] = w_scales(a, t, t.col * kCols + r);
         rows.row[8 + j] = w_scales(a, t, t.col * kCols + r + second);
       }
-      return true;
-    };
-    bool more = aim(), ok = true;
-    if (more) rows.load(now, 0, a);
-    while (more && ok) {
-      const int steps = min(4, a.kblocks - 4 * g);
-      if (++g == groups) {
-        g = 0;
-        i += pairs;
-        more = aim();
+      for (int g = 0; g < per; g++) {
+        rows.load(v, g, a);
+        ok = tc::wait_warp<true>(&sh.scales_empty[ring.stage], ring.phase ^ 1u, guard);
+        if (!ok) break;
+#pragma unroll
+        for (int j = 0; j < 4; j++)
+          if (4 * g + j < a.kblocks) put_words<3>(v, j, scales + ring.stage * kGroupScales + j * kStepScales);
+        __syncwarp();
+        if (tc::elect()) tc::mbar_arrive(&sh.scales_ready[ring.stage]);
+        ring.next(kGroups);
       }
-      if (more) rows.load(nxt, g, a);
-#pragma unroll
-      for (int j = 0; j < 4; j++)
-        if (j < steps && ok)
-          ok = store_scales<3>(now, j, a, scales, kStageScales, sh.ready, sh.empty, ring, kStages, guard);
-#pragma unroll
-      for (int j = 0; j < 12; j++) now[j] = nxt[j];
     }
   } else if (warp == 3) {
-    Ring ring;
-    bool ok = true;
-    for (int i = pair; ok && i < tiles; i += pairs)
-      for (int kb = 0; kb < a.kblocks && ok; kb++)
-        ok = forward_scales(a, sh.ready, sh.full, rank ? full : 0u, ring, kStages, guard);
+    forward(0, rank ? 2 : 1);
   } else {
     Tiles list;
     int done = 0;
@@ -709,14 +730,14 @@ __global__ void __launch_bounds__(128 + 32 * kWriters, 1) __cluster_dims__(2, 1,
       };
       fetch(t.col * kCols + unit_of(0) * 64);
       fetch_bias(t.col * kCols + unit_of(0) * 64);
-      const bool ok = tc::wait(&sh.acc_full, done & 1, guard);
+      const bool ok = tc::wait<true>(&sh.acc_full, done & 1, guard);
       __syncwarp();
       tc::fence_after();
       // the second warps' word that they are through with the tile before; the first warps give theirs below
       if (set == 1) {
         tc::fence_before();                            // their loads of that tile come before the word
         __syncwarp();
-        if (lane == 0) tc::mbar_arrive_remote(acc_free);
+        if (lane == 0) tc::mbar_word_remote(acc_free);
       }
       const uint32_t acc = tmem + (done & 1 ? 192 : 0) + ((uint32_t)(q * 32) << 16);
 #pragma unroll 1
@@ -736,7 +757,7 @@ __global__ void __launch_bounds__(128 + 32 * kWriters, 1) __cluster_dims__(2, 1,
         if (set == 0 && u == 0) {                      // the next tile's products may start
           tc::fence_before();
           __syncwarp();
-          if (lane == 0) tc::mbar_arrive_remote(acc_free);
+          if (lane == 0) tc::mbar_word_remote(acc_free);
         }
         // One body for both halves, not unrolled: straight-line code for 64 columns ran from the instruction cache's
         // second level, at 4 to 5 cycles an instruction.
@@ -968,7 +989,7 @@ __global__ void __launch_bounds__(128, 2) k_mx_rows(const __grid_constant__ CUte
       rows = make_int4(x_row(a, t, 4 * lane), x_row(a, t, 4 * lane + 1), x_row(a, t, 4 * lane + 2), x_row(a, t, 4 * lane + 3));
     const int w0 = t.expert * a.n + t.col * kCols;
     for (int kb = k0; kb < k1; kb++) {
-      ok = tc::wait_warp(&sh.empty[ring.stage], ring.phase ^ 1u, guard);
+      ok = tc::wait_warp<false>(&sh.empty[ring.stage], ring.phase ^ 1u, guard);
       if (!ok) break;
       uint8_t* to = codes + ring.stage * S::kStageCodes;
       uint64_t* bar = &sh.full[ring.stage];
@@ -992,7 +1013,7 @@ __global__ void __launch_bounds__(128, 2) k_mx_rows(const __grid_constant__ CUte
     Ring ring;
     bool ok = true;
     for (int kb = k0; kb < k1; kb++) {
-      ok = tc::wait_warp(&sh.full[ring.stage], ring.phase, guard);
+      ok = tc::wait_warp<false>(&sh.full[ring.stage], ring.phase, guard);
       if (!ok) break;
       tc::fence_after();
       const uint32_t at = smem_addr(codes + ring.stage * S::kStageCodes);
@@ -1041,14 +1062,14 @@ __global__ void __launch_bounds__(128, 2) k_mx_rows(const __grid_constant__ CUte
   } else if (busy) {
     Ring ring;
     bool ok = true;
-    for (int kb = k0; kb < k1 && ok; kb++) ok = forward_scales(a, sh.ready, sh.full, 0u, ring, S::kDepth, guard);
+    for (int kb = k0; kb < k1 && ok; kb++) ok = forward_scales(sh.ready, sh.full, 0u, ring, S::kDepth, guard);
   }
   __syncwarp();
 
   // partial sums, [row of x][feature], over the codes' stages, which are all consumed
   float* part = reinterpret_cast<float*>(codes);
   if (work) {
-    const bool ok = !busy || tc::wait(&sh.acc_full, 0, guard);
+    const bool ok = !busy || tc::wait<false>(&sh.acc_full, 0, guard);
     __syncwarp();
     tc::fence_after();
     const uint32_t acc = tmem + ((uint32_t)(warp * 32) << 16);

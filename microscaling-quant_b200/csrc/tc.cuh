@@ -16,7 +16,18 @@ namespace tc {
 // how many cycles a wait may take, about two seconds: a correct one takes microseconds
 constexpr long long kWaitCycles = 4000000000ll;
 
-__device__ __forceinline__ bool try_wait(uint64_t* bar, unsigned parity) { return mbar_try_wait_rounds(bar, parity, 1); }
+// PAIR: what the barrier's arrivals in the other CTA of the pair released is seen by this thread too
+template <bool PAIR>
+__device__ __forceinline__ bool try_wait(uint64_t* bar, unsigned parity) {
+  if (!PAIR) return mbar_try_wait_rounds(bar, parity, 1);
+  unsigned done;
+  asm volatile(
+      "{\n .reg .pred p;\n mbarrier.try_wait.parity.acquire.cluster.shared::cta.b64 p, [%1], %2;\n selp.u32 %0, 1, 0, p;\n}\n"
+      : "=r"(done)
+      : "r"(smem_addr(bar)), "r"(parity)
+      : "memory");
+  return done;
+}
 
 // What bounds a CTA's waits: its word in shared memory, the library's status word, the limit.
 struct Guard {
@@ -25,11 +36,12 @@ struct Guard {
   long long cycles;
 };
 // false: gave up (this wait ran out, or another role's did)
+template <bool PAIR>
 __device__ __forceinline__ bool wait(uint64_t* bar, unsigned parity, const Guard& g) {
-  if (try_wait(bar, parity) || try_wait(bar, parity)) return true;
+  if (try_wait<PAIR>(bar, parity) || try_wait<PAIR>(bar, parity)) return true;
   const long long begin = clock64();
   do {
-    if (try_wait(bar, parity) || try_wait(bar, parity)) return true;
+    if (try_wait<PAIR>(bar, parity) || try_wait<PAIR>(bar, parity)) return true;
     if (*g.abort) return false;
   } while (clock64() - begin < g.cycles);
   *g.abort = 1;
@@ -39,7 +51,7 @@ __device__ __forceinline__ bool wait(uint64_t* bar, unsigned parity, const Guard
 // the same for what a role that gave up has in flight towards shared memory or TMEM, without the abort word
 __device__ __forceinline__ void settle(uint64_t* bar, unsigned parity, const Guard& g) {
   const long long begin = clock64();
-  while (!try_wait(bar, parity) && clock64() - begin < g.cycles / 16) {
+  while (!try_wait<false>(bar, parity) && clock64() - begin < g.cycles / 16) {
   }
 }
 
@@ -47,8 +59,9 @@ __device__ __forceinline__ void mbar_arrive(uint64_t* bar) {
   asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];\n" ::"r"(smem_addr(bar)) : "memory");
 }
 // wait() by a whole warp: the answer is the same in every lane, and the compiler knows it
+template <bool PAIR>
 __device__ __forceinline__ bool wait_warp(uint64_t* bar, unsigned parity, const Guard& g) {
-  return __all_sync(0xffffffffu, wait(bar, parity, g));
+  return __all_sync(0xffffffffu, wait<PAIR>(bar, parity, g));
 }
 // one lane of a converged warp. The operands of what it issues have to be warp-uniform for the compiler (no lane index
 // in them, no branch on one around them): tcgen05 and TMA instructions take uniform registers, and from a branch on
@@ -59,17 +72,20 @@ __device__ __forceinline__ bool elect() {
   return yes;
 }
 
-// the same barrier in CTA `rank` of the cluster, and an arrival there
+// the same barrier in CTA `rank` of the cluster
 __device__ __forceinline__ uint32_t remote(const void* p, uint32_t rank) {
   uint32_t r;
   asm volatile("mapa.shared::cluster.u32 %0, %1, %2;\n" : "=r"(r) : "r"(smem_addr(p)), "r"(rank));
   return r;
 }
-// Its release reaches this CTA's threads only: what the other CTA's tensor core is to read has to be in shared memory
-// before (fence_proxy_async ends when it is). A release for the cluster here waits for everything that the SM has under
-// way, measured 1900 cycles a time.
+// an arrival there that releases what this thread has written or been told of to the cluster
 __device__ __forceinline__ void mbar_arrive_remote(uint32_t bar) {
-  asm volatile("mbarrier.arrive.shared::cluster.b64 _, [%0];\n" ::"r"(bar) : "memory");
+  asm volatile("mbarrier.arrive.release.cluster.shared::cluster.b64 _, [%0];\n" ::"r"(bar) : "memory");
+}
+// The same word without a release: for what tcgen05.fence::before_thread_sync orders (loads from TMEM that are done), nothing
+// in memory.
+__device__ __forceinline__ void mbar_word_remote(uint32_t bar) {
+  asm volatile("mbarrier.arrive.relaxed.cluster.shared::cluster.b64 _, [%0];\n" ::"r"(bar) : "memory");
 }
 
 __device__ __forceinline__ void fence_before() { asm volatile("tcgen05.fence::before_thread_sync;\n" ::: "memory"); }
