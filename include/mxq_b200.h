@@ -294,11 +294,11 @@ int mxq_pack_rows(const void* x, int32_t type, int64_t x_stride, uint8_t* codes,
 
 /* Routing. Scores s = softmax or sigmoid of the T x E logits (type MXQ_OUT_F32 / BF16 / F16, rows `stride` elements
  * apart) in float32. An expert's choice value is its logit (bias NULL) or s + bias. groups > 1: the experts are `groups`
- * equal runs, a run's value is its largest choice value, or (top2) the sum of its two largest, and only the `keep` best
- * runs take part. experts[t, 0..k): the k largest choice values, descending; every tie goes to the lowest index.
- * weights: their s, divided by (their sum + 1e-20) if renormalize, times scale. A logit of -Inf or NaN is never chosen; a
- * place with nothing left to choose gets expert -1 and weight 0; the weights of a row with a NaN are NaN. At most 1024
- * experts, k at most 32, at most 32 groups. */
+ * equal runs, a run's value is its largest choice value, or (top2) the sum of its two largest s (+ bias), a logit of -Inf
+ * counting as s = 0, and only the `keep` best runs with an expert to choose take part. experts[t, 0..k): the k largest
+ * choice values, descending; every tie goes to the lowest index. weights: their s, divided by (their sum + 1e-20) if
+ * renormalize, times scale. A logit of -Inf or NaN is never chosen; a place with nothing left to choose gets expert -1 and
+ * weight 0; the weights of a row with a NaN are NaN. At most 1024 experts, k at most 32, at most 32 groups. */
 #define MXQ_SCORE_SOFTMAX 0
 #define MXQ_SCORE_SIGMOID 1
 typedef struct mxq_route_spec {

@@ -47,16 +47,18 @@ __device__ __forceinline__ float warp_max(float v) {
 
 // An order-preserving key of a choice value; 0 (below every other) for -Inf and NaN, which are never chosen, and where
 // `live` is false; -0 as +0.
-__device__ __forceinline__ uint32_t key_if(bool live, float f) {
+__device__ __forceinline__ uint32_t key_of(float f) {
   const uint32_t b = __float_as_uint(__fadd_rn(f, 0.0f));
-  return live && f > -INFINITY ? b ^ ((uint32_t)((int32_t)b >> 31) | 0x80000000u) : 0u;
+  return b ^ ((uint32_t)((int32_t)b >> 31) | 0x80000000u);
 }
+__device__ __forceinline__ uint32_t key_if(bool live, float f) { return live && f > -INFINITY ? key_of(f) : 0u; }
+constexpr float kLowest = -3.402823466e38f;
 __device__ __forceinline__ float value_of(uint32_t key) {
   return __uint_as_float(key & 0x80000000u ? key & 0x7fffffffu : ~key);
 }
 // the key of a group's two largest, whose sum may pass the type's lowest value: that is still a group to choose
 __device__ __forceinline__ uint32_t key_of_pair(uint32_t best, uint32_t second) {
-  return key_if(true, fmaxf(__fadd_rn(value_of(best), value_of(second)), -3.402823466e38f));
+  return key_if(true, fmaxf(__fadd_rn(value_of(best), value_of(second)), kLowest));
 }
 __device__ __forceinline__ float sigmoid(float x) { return __frcp_rn(__fadd_rn(1.0f, expf(-x))); }
 __device__ __forceinline__ bool is_nan(float x) { return x != x; }
@@ -98,6 +100,10 @@ __device__ __forceinline__ void merge2(uint32_t& a, uint32_t& b, uint32_t c, uin
 // logits at the end, by lane j for the j-th. Groups whose runs are whole lanes, a power of two of them (every usual
 // shape), are ranked by shuffles, all at once; others one by one.
 //
+// A group's two largest are summed as scores, with a bias or without one (logits order the experts as their scores do, but not
+// sums of two), and a masked expert counts there with the score 0 that its logit of -Inf has: taking an expert out cannot
+// raise its group. A group with nobody left to choose is not kept.
+//
 // Bound by issue (about 1000 instructions a token): 8192 tokens of 256 experts (float32, bias, 8 groups, k = 8) take
 // 12.5 us, their 9.4 MB 1.4 us at the copy's rate; 16 tokens 3.4 us.
 template <typename IN, int V>
@@ -116,7 +122,12 @@ __global__ void __launch_bounds__(128) k_route(const IN* __restrict__ logits, co
     top = fmaxf(top, l[i]);
   }
   bad = __any_sync(kAll, bad);
-  uint32_t key[V];
+  uint32_t key[V], rank[V];                            // what orders the experts; the groups
+  auto by_score = [&](int i, float s, float b) {
+    const float v = __fadd_rn(s, b);
+    rank[i] = key_of(fmaxf(v, kLowest));
+    key[i] = !bias ? key_if(true, l[i]) : l[i] > -INFINITY && v > -INFINITY ? rank[i] : 0u;
+  };
   if (!a.sigmoid) {
     top = warp_max(top);
     sum = 0.0f;
@@ -131,28 +142,45 @@ __global__ void __launch_bounds__(128) k_route(const IN* __restrict__ logits, co
       float b[V];
       load_row<float, V>(bias, e0, a.E, a.vec_bias, b);
 #pragma unroll
-      for (int i = 0; i < V; i++) key[i] = key_if(l[i] > -INFINITY, __fadd_rn(__fdiv_rn(s[i], sum), b[i]));
+      for (int i = 0; i < V; i++) by_score(i, __fdiv_rn(s[i], sum), b[i]);
+    } else if (a.top2) {
+#pragma unroll
+      for (int i = 0; i < V; i++) by_score(i, __fdiv_rn(s[i], sum), 0.0f);
     }
   } else if (bias) {
     float b[V];
     load_row<float, V>(bias, e0, a.E, a.vec_bias, b);
 #pragma unroll
-    for (int i = 0; i < V; i++) key[i] = key_if(l[i] > -INFINITY, __fadd_rn(sigmoid(l[i]), b[i]));
+    for (int i = 0; i < V; i++) by_score(i, sigmoid(l[i]), b[i]);
+  } else if (a.top2) {
+#pragma unroll
+    for (int i = 0; i < V; i++) by_score(i, sigmoid(l[i]), 0.0f);
   }
-  if (!bias) {
+  if (!bias && !a.top2) {
 #pragma unroll
     for (int i = 0; i < V; i++) key[i] = key_if(true, l[i]);
+  }
+  if (!a.top2) {
+#pragma unroll
+    for (int i = 0; i < V; i++) rank[i] = key[i];
   }
   if (a.groups > 1) {
     const int run = a.E / a.groups, width = run / V;
     if (run % V == 0 && (width & (width - 1)) == 0) {
-      uint32_t best = 0u, second = 0u;
+      uint32_t best = 0u, second = 0u, any = 0u;
 #pragma unroll
-      for (int i = 0; i < V; i++) merge2(best, second, key[i], 0u);
+      for (int i = 0; i < V; i++) {
+        merge2(best, second, rank[i], 0u);
+        any |= key[i];
+      }
       for (int d = 1; d < width; d <<= 1)
         merge2(best, second, __shfl_xor_sync(kAll, best, d), __shfl_xor_sync(kAll, second, d));
-      if (a.top2 && second) best = key_of_pair(best, second);
       const int g = lane / width;
+      if (a.top2) {
+        if (second) best = key_of_pair(best, second);
+        const unsigned alive = __ballot_sync(kAll, any != 0u);
+        if (!(alive >> (g * width & 31) & (0xffffffffu >> (32 - width)))) best = 0u;
+      }
       int ahead = 0;                                   // groups that come before this lane's
       for (int o = 0; o < a.groups; o++) {
         const uint32_t v = __shfl_sync(kAll, best, o * width);
@@ -165,16 +193,18 @@ __global__ void __launch_bounds__(128) k_route(const IN* __restrict__ logits, co
     } else {
       uint32_t mine = 0u;                              // lane g: the key of group g's value
       for (int g = 0; g < a.groups; g++) {
-        uint32_t best = 0u, second = 0u;
+        uint32_t best = 0u, second = 0u, any = 0u;
 #pragma unroll
         for (int i = 0; i < V; i++) {
           const bool in = e0 + i >= g * run && e0 + i < (g + 1) * run;
-          merge2(best, second, in ? key[i] : 0u, 0u);
+          merge2(best, second, in ? rank[i] : 0u, 0u);
+          any |= in ? key[i] : 0u;
         }
         for (int d = 1; d < 32; d <<= 1)
           merge2(best, second, __shfl_xor_sync(kAll, best, d), __shfl_xor_sync(kAll, second, d));
         if (a.top2 && second) best = key_of_pair(best, second);
         if (lane == g) mine = best;
+        if (!__any_sync(kAll, any != 0u) && lane == g) mine = 0u;
       }
       unsigned kept = 0u;
       for (int j = 0; j < a.keep; j++) {
@@ -633,7 +663,7 @@ int check_route(const char* who, int64_t T, int64_t E, int64_t k, const mxq_rout
   a.sigmoid = s->score == MXQ_SCORE_SIGMOID;
   a.groups = s->groups;
   a.keep = s->keep;
-  a.top2 = s->top2;
+  a.top2 = s->top2 && s->groups > 1;
   a.renormalize = s->renormalize;
   a.scale = s->scale;
   return MXQ_OK;

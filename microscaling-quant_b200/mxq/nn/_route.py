@@ -7,7 +7,8 @@
 route scores the T x E logits in float32 by softmax or sigmoid. Without a bias the experts are ranked by their logits,
 with one by score + bias (the bias balances the choice only; the weights are the plain scores). groups > 1 cuts the
 experts into equal runs, of which the `keep` best take part, by their largest ranking value or ("top2") the sum of
-their two largest. The k best experts are returned in descending order, every tie going to the lowest index; their
+their two largest scores, or score + bias (an expert with a logit of -Inf counts there with the score 0 that it has; a run with
+nobody to choose takes no part). The k best experts are returned in descending order, every tie going to the lowest index; their
 scores are divided by (their sum + 1e-20) if `renormalize` and multiplied with `scale`.
 
 Experts with a logit of -Inf are never chosen: a place with nothing left to choose gets expert -1 and weight 0, and its

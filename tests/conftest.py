@@ -16,6 +16,20 @@ def pytest_configure(config):
     config.addinivalue_line("markers", "gpu: needs a CUDA device (B200); run with -m gpu")
 
 
+#: Tests that hold a value that was found wrong and is no longer returned; they stand as they were written and are expected to fail.
+#: test_groups: without a bias its helper sums the two largest *logits* of a group, which ranks [10, -5] (scores 1.0000 and 0.0067)
+#: before [2, 2] (0.8808 each); groups are ranked by the sum of scores (test_gpu_route_groups.py has the same shapes and more).
+WRONG_VALUES = {f"test_gpu_route.py::test_groups[{case}]" for case in (
+    "8-4-2-softmax", "64-8-3-softmax", "64-8-3-sigmoid", "256-8-4-softmax", "96-4-1-softmax", "40-5-2-softmax", "40-5-2-sigmoid",
+    "128-32-7-softmax", "128-32-7-sigmoid", "1024-16-4-softmax", "1024-16-4-sigmoid")}
+
+
+def pytest_collection_modifyitems(items):
+    for item in items:
+        if item.nodeid.split("/")[-1] in WRONG_VALUES:
+            item.add_marker(pytest.mark.xfail(strict=True, raises=AssertionError, reason="sums logits where scores are meant"))
+
+
 @pytest.fixture(scope="session")
 def oracle():
     import oracle as o
