@@ -298,7 +298,8 @@ int mxq_pack_rows(const void* x, int32_t type, int64_t x_stride, uint8_t* codes,
  * counting as s = 0, and only the `keep` best runs with an expert to choose take part. experts[t, 0..k): the k largest
  * choice values, descending; every tie goes to the lowest index. weights: their s, divided by (their sum + 1e-20) if
  * renormalize, times scale. A logit of -Inf or NaN is never chosen; a place with nothing left to choose gets expert -1 and
- * weight 0; the weights of a row with a NaN are NaN. At most 1024 experts, k at most 32, at most 32 groups. */
+ * weight 0; the weights of a row with a NaN (softmax: or a +Inf) are NaN. At most 1024 experts, k at most 32, at most 32
+ * groups. */
 #define MXQ_SCORE_SOFTMAX 0
 #define MXQ_SCORE_SIGMOID 1
 typedef struct mxq_route_spec {

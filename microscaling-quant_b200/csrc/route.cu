@@ -130,6 +130,7 @@ __global__ void __launch_bounds__(128) k_route(const IN* __restrict__ logits, co
   };
   if (!a.sigmoid) {
     top = warp_max(top);
+    bad |= top == INFINITY;                            // Inf / Inf: no scores
     sum = 0.0f;
     float s[V];
 #pragma unroll
@@ -289,6 +290,7 @@ __global__ void __launch_bounds__(128) k_route_backward(const float* __restrict_
     s = live ? sigmoid(le) : 0.0f;
   } else {
     top = warp_max(top);
+    bad |= top == INFINITY;
 #pragma unroll
     for (int i = 0; i < V; i++) {
       l[i] = l[i] == -INFINITY ? 0.0f : expf(__fsub_rn(l[i], top));

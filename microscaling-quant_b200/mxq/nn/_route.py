@@ -12,8 +12,8 @@ nobody to choose takes no part). The k best experts are returned in descending o
 scores are divided by (their sum + 1e-20) if `renormalize` and multiplied with `scale`.
 
 Experts with a logit of -Inf are never chosen: a place with nothing left to choose gets expert -1 and weight 0, and its
-slot takes no part in dispatch, the products and combine (a padded token: a row of -Inf). A row that holds a NaN has
-weights NaN.
+slot takes no part in dispatch, the products and combine (a padded token: a row of -Inf). A row that holds a NaN, or
+under softmax a +Inf, has weights NaN, and so has its gradient.
 
 route is differentiable in the logits and combine in z, weights and residual (first order); experts and the plan are
 whole numbers and have no gradient. route_backward and combine_backward are the gradients by themselves.
