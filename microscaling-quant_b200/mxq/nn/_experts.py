@@ -6,7 +6,8 @@
 
 forward: the plan of the slots, the gated up-projection with x packed and read through the plan and its output packed
 again, the down-projection, the weighted sum. The weights are packed once by block.ocp (`fmt`), activations to `act_fmt`
-in each call. Differentiable in `weights` and `residual` (a router tuned against the packed experts); x and the experts
+in each call. The packed weights are the layer's state: state_dict has their codes and scales, and their formats, which a layer
+that loads them takes over. Differentiable in `weights` and `residual` (a router tuned against the packed experts); x and the experts
 themselves have no gradient.
 """
 from typing import Optional, Union
@@ -15,7 +16,7 @@ import torch
 from torch import nn
 
 from ..block import ocp
-from ..element_quant.formats import Format, get
+from ..element_quant.formats import FORMATS, Format, get
 from ._packed import GATED, experts_packed, lay_packed
 from ._route import combine, dispatch
 
@@ -38,9 +39,17 @@ class MXExperts(nn.Module):
         self.act_fmt, self.activation = get(act_fmt).name, activation
         for name, w in (("up", gate_up), ("down", down)):
             (codes, scales), self_fmt = lay_packed(ocp.quantize_packed(w.detach().float(), fmt, axis=-1), fmt)
-            self.register_buffer(f"{name}_codes", codes, persistent=False)
-            self.register_buffer(f"{name}_scales", scales, persistent=False)
+            self.register_buffer(f"{name}_codes", codes)
+            self.register_buffer(f"{name}_scales", scales)
             setattr(self, f"{name}_fmt", self_fmt)
+
+    def get_extra_state(self) -> torch.Tensor:
+        """(exponent, mantissa) bits of the up and the down weights' codes: a tensor, as all of a state_dict."""
+        return torch.tensor([(FORMATS[f].e, FORMATS[f].m) for f in (self.up_fmt, self.down_fmt)], dtype=torch.uint8)
+
+    def set_extra_state(self, state: torch.Tensor):
+        names = {(f.e, f.m): f.name for f in FORMATS.values()}
+        self.up_fmt, self.down_fmt = (names[tuple(em)] for em in state.tolist())
 
     def forward(self, x: torch.Tensor, weights: torch.Tensor, experts: torch.Tensor,
                 residual: Optional[torch.Tensor] = None) -> torch.Tensor:
