@@ -179,6 +179,19 @@ def on(t, device, dtype=torch.float32):
     return t.detach().to(device=device, dtype=dtype).contiguous()
 
 
+def tracked(*args):
+    """Whether autograd has to see a call on these (anything but tensors is passed over): one requires a gradient, or carries a
+    forward-mode tangent."""
+    level = torch.autograd.forward_ad._current_level
+    if level < 0 and not torch.is_grad_enabled():
+        return False
+    for t in args:
+        if isinstance(t, torch.Tensor) and (t.requires_grad and torch.is_grad_enabled() or
+                                            level >= 0 and torch.autograd.forward_ad.unpack_dual(t).tangent is not None):
+            return True
+    return False
+
+
 def ptr(t):
     return ctypes.c_void_p(t.data_ptr()) if t is not None else ctypes.c_void_p(0)
 

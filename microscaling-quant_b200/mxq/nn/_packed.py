@@ -1,4 +1,5 @@
-"""Products of packed MX operands on the tensor cores, dense and by expert (no reference counterpart). Inference only.
+"""Products of packed MX operands on the tensor cores, dense and by expert (no reference counterpart). Inference only: of their
+arguments the residual alone has a gradient (the result's); one that reaches a float x or a bias raises in backward.
 
     y = linear_packed(x, w, "MXFP8_E4M3", bias=b, activation="silu", residual=r)       ... x K, N x K -> ... x F
     z = experts_packed(x, w, "MXFP8_E4M3", plan, activation="swiglu", out="MXFP8_E4M3")
@@ -192,11 +193,35 @@ def _ready():
         _lib.wait_word()
 
 
+class _Product(torch.autograd.Function):
+    """A product whose float arguments are part of a graph."""
+    @staticmethod
+    def forward(ctx, who, call, x, bias, residual):
+        ctx.who, ctx.home = who, None if residual is None else residual.device
+        return call()
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, dy):
+        for i, what in ((2, "x"), (3, "bias")):
+            if ctx.needs_input_grad[i]:
+                raise RuntimeError(f"{ctx.who} is inference only: it has no gradient for {what}; detach it, or call under "
+                                   "torch.no_grad()")
+        return None, None, None, None, dy.to(ctx.home)
+
+
 def linear_packed(x: Union[Pair, torch.Tensor], w: Pair, fmt: Union[str, Format], x_fmt: Union[str, Format] = "MXFP8_E4M3",
                   bias: Optional[torch.Tensor] = None, activation: Optional[str] = None,
                   residual: Optional[torch.Tensor] = None, out: Union[torch.dtype, str] = torch.bfloat16):
     """y = act(x wᵀ + bias) [* up] + residual. x: (... x K) packed to x_fmt (a pair) or floats; w: an N x K pair of
     `fmt`; bias: N values; residual: y's shape and dtype. Returns y (... x F) of dtype `out`, or its (codes, scales)."""
+    if isinstance(out, torch.dtype) and _lib.tracked(x, bias, residual):
+        return _Product.apply("linear_packed", lambda: _linear(x, w, fmt, x_fmt, bias, activation, residual, out),
+                              x if isinstance(x, torch.Tensor) else None, bias, residual)
+    return _linear(x, w, fmt, x_fmt, bias, activation, residual, out)
+
+
+def _linear(x, w, fmt, x_fmt, bias, activation, residual, out):
     who = "linear_packed"
     fw = _format(fmt, who)
     wc, ws, wshape, K = _pair(w, fw, who, "w")
@@ -253,6 +278,13 @@ def experts_packed(x: Union[Pair, torch.Tensor], w: Pair, fmt: Union[str, Format
     weights. w: an E x N x K pair; bias: E x N. x: T x K, a row per token, read through the plan (gather), or
     slots x K in the plan's order (not gather). Returns slots x F in the plan's order; the rows of places without a slot
     (from offsets[-1] on) are not written."""
+    if isinstance(out, torch.dtype) and _lib.tracked(x, bias):
+        return _Product.apply("experts_packed", lambda: _experts(x, w, fmt, plan, gather, x_fmt, bias, activation, out),
+                              x if isinstance(x, torch.Tensor) else None, bias, None)
+    return _experts(x, w, fmt, plan, gather, x_fmt, bias, activation, out)
+
+
+def _experts(x, w, fmt, plan, gather, x_fmt, bias, activation, out):
     who = "experts_packed"
     fw = _format(fmt, who)
     wc, ws, wshape, K = _pair(w, fw, who, "w")
