@@ -16,7 +16,7 @@ slot takes no part in dispatch, the products and combine (a padded token: a row 
 under softmax a +Inf, has weights NaN, and so has its gradient.
 
 route is differentiable in the logits and combine in z, weights and residual (first order); experts and the plan are
-whole numbers and have no gradient. route_backward and combine_backward are the gradients by themselves.
+whole numbers and have no gradient; forward-mode tangents raise. route_backward and combine_backward are the gradients by themselves.
 """
 from typing import Optional, Tuple
 
@@ -109,7 +109,7 @@ def route(logits: torch.Tensor, k: int, score: str = "softmax", bias: Optional[t
     _, E = _route_args("route", logits, k, score, groups, keep, group_score)
     if bias is not None and tuple(bias.shape) != (E,):
         raise ValueError(f"route: bias must have shape {(E,)}, got {tuple(bias.shape)}")
-    if logits.requires_grad and torch.is_grad_enabled():
+    if _lib.tracked(logits):
         return _Route.apply(logits, k, score, bias, groups, keep, group_score, renormalize, scale)
     return _route(logits, k, score, bias, groups, keep, group_score, renormalize, scale)
 
@@ -206,8 +206,7 @@ def combine(z: torch.Tensor, weights: torch.Tensor, plan: Dispatch, residual: Op
     if residual is not None and (tuple(residual.shape) != (T, N) or residual.dtype != z.dtype):
         raise ValueError(f"combine: residual must be {z.dtype} of shape {(T, N)}, got {residual.dtype} "
                          f"{tuple(residual.shape)}")
-    if torch.is_grad_enabled() and (z.requires_grad or weights.requires_grad or
-                                    (residual is not None and residual.requires_grad)):
+    if _lib.tracked(z, weights, residual):
         return _Combine.apply(z, weights, *plan, residual)
     return _combine(z, weights, plan.where, residual)
 

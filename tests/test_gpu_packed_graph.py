@@ -82,3 +82,14 @@ def test_forward_mode_raises():
         raises_forward((lambda: nn.linear_packed(dual(x), w, "MXFP8_E4M3"), lambda: nn.linear_packed(x, w, "MXFP8_E4M3", bias=dual(bias)),
                         lambda: nn.linear_packed(x, w, "MXFP8_E4M3", residual=dual(r))))
         assert torch.equal(nn.linear_packed(x, w, "MXFP8_E4M3"), want)                      # no tangent: as ever
+
+
+def test_forward_mode_raises_in_routing():
+    from mxq import nn
+    logits = torch.randn(4, 8, device=DEV)
+    weights, experts = nn.route(logits, 2)
+    plan, z = nn.dispatch(experts, 8), torch.randn(8, 16, device=DEV)
+    with forward_ad.dual_level():
+        raises_forward((lambda: nn.route(dual(logits), 2), lambda: nn.combine(dual(z), weights, plan),
+                        lambda: nn.combine(z, dual(weights), plan), lambda: nn.combine(z, weights, plan, residual=dual(z[:4]))))
+        assert torch.equal(nn.route(logits, 2)[0], weights)
