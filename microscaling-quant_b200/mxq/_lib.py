@@ -13,6 +13,7 @@ import os
 import threading
 
 import torch
+from torch.autograd import forward_ad as _forward_ad
 
 HERE = os.path.dirname(os.path.abspath(__file__))
 LIB_PATH = os.path.join(HERE, "_lib", "libmxq_b200.so")
@@ -179,17 +180,19 @@ def on(t, device, dtype=torch.float32):
     return t.detach().to(device=device, dtype=dtype).contiguous()
 
 
+_Tensor = torch.Tensor
+
+
 def tracked(*args):
     """Whether autograd has to see a call on these (anything but tensors is passed over): one requires a gradient, or carries a
     forward-mode tangent."""
-    level = torch.autograd.forward_ad._current_level
-    if level < 0 and not torch.is_grad_enabled():
+    if _forward_ad._current_level < 0:
+        for t in args:
+            if isinstance(t, _Tensor) and t.requires_grad:
+                return torch.is_grad_enabled()
         return False
-    for t in args:
-        if isinstance(t, torch.Tensor) and (t.requires_grad and torch.is_grad_enabled() or
-                                            level >= 0 and torch.autograd.forward_ad.unpack_dual(t).tangent is not None):
-            return True
-    return False
+    return any(isinstance(t, _Tensor) and (t.requires_grad and torch.is_grad_enabled() or
+                                           _forward_ad.unpack_dual(t).tangent is not None) for t in args)
 
 
 def ptr(t):
