@@ -360,6 +360,8 @@ struct TileShared {
 };
 constexpr int kTileSmem = 1024 + kStages * kStageBytes + kGroups * kGroupScales + kWriters * kPassBytes + (int)sizeof(TileShared);
 
+static_assert(kTileSmem + table_bytes(kMostExperts) <= 227 * 1024, "shared memory of a CTA");
+
 // place of 16-byte piece j of a staged row: neighbouring rows in other banks
 __device__ __forceinline__ uint8_t* piece(uint8_t* stage, int row, int j) { return stage + row * 128 + ((j ^ (row & 7)) << 4); }
 

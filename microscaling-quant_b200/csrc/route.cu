@@ -798,7 +798,7 @@ extern "C" int mxq_combine(const void* z, int32_t type, const float* weights, co
     constexpr int V = Vec<X>::N;
     const bool vec = N % V == 0 && aligned16(z) && aligned16(y) && (!residual || (aligned16(residual) && residual_stride % V == 0));
     const int64_t threads = (N + V - 1) / V;
-    const int block = threads >= 256 ? 256 : threads > 128 ? 256 : threads > 64 ? 128 : 64;
+    const int block = threads > 128 ? 256 : threads > 64 ? 128 : 64;
     const dim3 grid((unsigned)T, (unsigned)((threads + block - 1) / block));
     auto f = vec ? k_combine<X, true> : k_combine<X, false>;
     f<<<grid, block, 0, as_stream(stream)>>>(static_cast<const X*>(z), weights, where, static_cast<const X*>(residual), residual_stride,
