@@ -5,7 +5,9 @@
 //
 // x and w are row-major codes with blocks of 32 along K, as block.*.quantize_packed(axis=-1) writes them. sm_100's
 // tcgen05.mma kind::mxf8f6f4 multiplies them as they are: codes and E8M0 bytes go from memory to shared memory to the
-// tensor core, nothing is dequantized. The products are exact and the sums are held in float32 in TMEM.
+// tensor core, nothing is dequantized. The products are exact and the sums are held in float32 in TMEM; the instruction cuts
+// them toward zero where a float32 multiply-add rounds: 4096 x 8192 x 2048 is 1.2e-7 of the norm from 64 bits (a float32 matrix
+// product 6e-8), its sums 8e-8 smaller in the mean.
 //
 // Two kernels share the operand staging:
 //   k_mx_tile  256 rows of x by 256 rows of w per pair of CTAs, persistent, for many rows: the operations bound it.
@@ -526,11 +528,13 @@ __device__ __forceinline__ void add_bias(float mine, float (&y)[32]) {
 // Warp 0 loads the codes, warp 1 of the pair's first CTA issues the products, warps 2 and 3 bring the scales (in the second
 // CTA warp 1 too), warps 4-11 write y: two per lane quarter, each with units of 64 columns.
 //
-// Measured (E4M3, bf16 y): 8192 x 8192 x 8192 436 us in a burst (2.52 PFLOP/s), 505 us back to back at the 1250 MHz
-// that the power limit leaves. A step of 128 along K takes its products' 512 cycles once the ring is full; a tile
-// then adds about 700 idle cycles (its last product, the shared columns' way out, the word to the next) and a launch
-// 5700 before its first product and the last tile's epilogue behind it. Short K shows the epilogue: 24576 rows by
-// expert, 2048 x 1024: 81 us (85 with the staged rows written by the warps), 62 without it; 8192 x 8192 x 256 47 us.
+// Measured (E4M3, bf16 y): 8192 x 8192 x 8192 434 us in a burst (2.53 PFLOP/s; 391 on a GPU that the power limit slowed
+// less), 456 us back to back. Clock readings of the issuer, 4096 x 4096 x 4096, a pair's four tiles in 81500 cycles: 7900 to
+// the first product (set-up 1900, the first scales and codes 6000), 65500 the products (512 a step of 128), 3400 at the tiles'
+// ends (the shared columns' way out, the word to the next), 4700 in waits between; then the last tile's epilogue. The seven
+// gated tiles of 4096 x 8192 x 2048 with packed y take 87 to 97 thousand: products 57, start 8 to 10, ends 6 to 8; the
+// other 14 to 22 thousand have no cause yet. Short K shows the epilogue: 24576 rows by expert, 2048 x 1024: 81 us (85 with
+// the staged rows written by the warps), 62 without it; 8192 x 8192 x 256 46 to 54 us.
 //
 // TMEM (512 columns, the same in both CTAs): two accumulators of 256 that share 64 columns, [0, 256) and [192, 448),
 // and the stages' scale words in [448, 508). The epilogue of a tile drains the shared columns first and then lets the
@@ -1240,10 +1244,10 @@ Cut cut_of(const Args& a, bool gated, int64_t kblocks) {
   // 64).
   c.bn = a.experts ? (share <= 2 ? 16 : share <= 8 ? 32 : 64) : share <= 16 ? 16 : share <= 32 ? 32 : 64;
   c.tiles = (a.experts ? a.rows / c.bn + groups : up_div(a.rows, c.bn)) * cols;
-  // Which kernel, measured on E4M3: dense 4096 x 4096, M = 256: 15.9 us by few rows, 17.8 by many, M = 384: 19.7 and
-  // 18.7; 2048 x 2048, M = 512: 13.2 and 13.1; 8192 x 2048, M = 128: 13.4 and 13.8, M = 256: 15.1 and 13.9. By
-  // expert, 64 experts 2048 x 1024: 8 rows each 33 and 35, 12 rows 44 and 39; 8 experts 4096 x 2048, 32 rows: 16 and
-  // 23.
+  // Which kernel, measured on E4M3: dense 4096 x 4096, M = 256: 14.9 us by few rows, 16.9 by many, M = 384: 19.0 and
+  // 17.4; 2048 x 2048, M = 512: 12.4 and 12.4; 8192 x 2048, M = 128: 12.5 and 12.7, M = 256: 14.5 and 12.9. By
+  // expert, 64 experts 2048 x 1024: 1 row each 22 and 28, 4 rows 38 and 37, 8 rows 39 and 37, 12 rows 40 and 38; 2048 x
+  // 2048: 8 rows 59 and 66, 12 rows 60 and 66; 8 experts 4096 x 2048, 32 rows: 14 and 20.
   c.few = a.experts ? share <= 8 || c.tiles <= 4 * sm_count() : c.tiles <= sm_count();
   c.split = 1;
   if (!c.few) {

@@ -105,7 +105,7 @@ __device__ __forceinline__ void merge2(uint32_t& a, uint32_t& b, uint32_t c, uin
 // raise its group. A group with nobody left to choose is not kept.
 //
 // Bound by issue (about 1000 instructions a token): 8192 tokens of 256 experts (float32, bias, 8 groups, k = 8) take
-// 12.5 us, their 9.4 MB 1.4 us at the copy's rate; 16 tokens 3.4 us.
+// 12.6 us (11.9 without a bias), their 9.4 MB 1.4 us at the copy's rate; 16 tokens of 128 experts 3.7 us.
 template <typename IN, int V>
 __global__ void __launch_bounds__(128) k_route(const IN* __restrict__ logits, const float* __restrict__ bias,
                                                float* __restrict__ weights, int* __restrict__ experts, RouteArgs a) {
