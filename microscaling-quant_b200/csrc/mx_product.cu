@@ -1473,7 +1473,8 @@ extern "C" int mxq_experts_packed(const void* x, const uint8_t* x_scales, int64_
   if (int rc = check_sizes("experts_packed", slots, N, K, experts)) return rc;
   MXQ_REQUIRE(experts <= kMostExperts, MXQ_ERR_UNSUPPORTED, "experts_packed: at most %d experts, got %lld", kMostExperts,
               (long long)experts);
-  MXQ_REQUIRE(per >= 0 && per < (1ll << 30) && (slots == 0 || (x_rows >= 1 && x_rows < (1ll << 30) && (per == 0 ? x_rows >= slots : x_rows * per >= slots))),
+  MXQ_REQUIRE(per >= 0 && per < (1ll << 30) &&
+                  (slots == 0 || (x_rows >= 1 && x_rows < (1ll << 30) && (per == 0 ? x_rows >= slots : x_rows * per >= slots))),
               MXQ_ERR_VALUE, "experts_packed: %lld rows of x do not serve %lld slots, %lld per row", (long long)x_rows,
               (long long)slots, (long long)per);
   Args a = {};
